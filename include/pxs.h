@@ -378,6 +378,42 @@ int pxs_linear_gate_residual(int dtype, const void * x, int64_t rows, int cin,
 int pxs_linear_residual(int dtype, const void * x, int64_t rows, int cin, const void * weight,
                         const float * bias, int cout, float * residual, void * stream);
 
+/* ---- linears in 8-bit integers ----------------------------------------------------
+ * Next to pxs_linear, pxs_linear_residual and pxs_linear_gate_residual, for
+ * weights and activations held in 8 bits (no counterpart in the reference).
+ *
+ * pxs_quantize_rows_i8: each row of x ([rows, channels], row stride ld_x
+ * elements) to 8-bit integers q [rows, channels] and a scale, x ~ q * scale:
+ * scale = max|x| / 127 and q = rint(x * (127 / max|x|)), ties to even, in fp32
+ * with every step rounded.  A row whose largest magnitude is below 2^-100 gets
+ * scale 0 and zeros; a row holding an infinity or a NaN gets scale NaN and
+ * zeros, so that its products are NaN.  Weights [cout, cin] are quantized by
+ * the same call, once: their scales are per output channel. */
+int pxs_quantize_rows_i8(int dtype, const void * x, int64_t ld_x, int64_t rows, int channels,
+                         int8_t * q, float * scales, void * stream);
+
+/* y = act((x W^T) * x_scales[row] * w_scales[channel] + bias) in y_dtype, x
+ * [rows, cin] and weight [cout, cin] 8-bit integers, summed exactly in 32 bits
+ * (cin is at most 131071).  bias may be NULL; act is PXS_ACT_*.  A cin that is
+ * a multiple of 16, with 16-byte-aligned x and weight, takes the fastest
+ * kernels. */
+int pxs_linear_i8(const int8_t * x, const float * x_scales, int64_t rows, int cin,
+                  const int8_t * weight, const float * w_scales, const float * bias, int cout,
+                  int act, int y_dtype, void * y, void * stream);
+
+/* residual (fp32) += the 8-bit linear, as pxs_linear_residual. */
+int pxs_linear_i8_residual(const int8_t * x, const float * x_scales, int64_t rows, int cin,
+                           const int8_t * weight, const float * w_scales, const float * bias,
+                           int cout, float * residual, void * stream);
+
+/* residual (fp32) += gate * the 8-bit linear, as pxs_linear_gate_residual
+ * (gate_offset 0..5 * cout). */
+int pxs_linear_i8_gate_residual(const int8_t * x, const float * x_scales, int64_t rows, int cin,
+                                const int8_t * weight, const float * w_scales, const float * bias,
+                                int cout, const int32_t * coords, const float * block_mod,
+                                const float * time_mod, int gate_offset, float * residual,
+                                void * stream);
+
 /* ---- a10-a12: row-wise normalisation and position embedding ------------------- */
 
 /* sparse_layer_norm (src/sparse.cpp:490-534); gamma/beta both NULL or both set.
@@ -402,6 +438,32 @@ int pxs_mh_rms_norm(int dtype, const void * x, int64_t ld_x, int64_t rows, int h
 int pxs_rope(int dtype, const int32_t * coords, const void * x, int64_t ld_x, int64_t rows,
              int heads, int head_dim, float freq_min, float freq_base, void * y, int64_t ld_y,
              void * stream);
+
+/* Rotary positions of token sequences (pxs_rope turns by voxel coordinates; no
+ * counterpart in the reference).
+ *
+ * pxs_rope_frequencies, on the host: freq[i] (rotary_dim / 2 of them, radians
+ * per position) = base^(-2 i / rotary_dim), stretched for contexts `factor`
+ * times as long: f * (keep + (1 - keep) / factor), where keep = 0 if
+ * original_length is 0 (every position divided by the factor), and otherwise
+ * grows from 0 to 1 as the turns that f makes over the original length,
+ * original_length * f / (2 pi), grow from low_turns to high_turns.  factor 1
+ * leaves the frequencies as they are. */
+#define PXS_ROPE_INTERLEAVED 0 /* pairs (2 i, 2 i + 1) */
+#define PXS_ROPE_HALF 1        /* pairs (i, i + rotary_dim / 2) */
+int pxs_rope_frequencies(int rotary_dim, double base, double factor, double original_length,
+                         double low_turns, double high_turns, double * freq);
+
+/* Turns the first rotary_dim values of each head of x ([rows, heads *
+ * head_dim], row stride ld_x) by positions[row] * freq[i] and copies the rest
+ * to y; cos and sin are multiplied by magnitude (1 unless a stretched context
+ * asks for more).  positions (any int32) and freq are device arrays; angles are
+ * taken in 64 bits.  y may be x (with ld_y = ld_x), and must not overlap it
+ * otherwise; the heads of q and k in one packed projection are turned by one
+ * call.  head_dim is at most 1024. */
+int pxs_rope_positions(int dtype, const int32_t * positions, const double * freq, const void * x,
+                       int64_t ld_x, int64_t rows, int heads, int head_dim, int rotary_dim,
+                       int layout, float magnitude, void * y, int64_t ld_y, void * stream);
 
 /* Fused attention prologue: split qkv [rows, 3C] into q, k, v [rows, C],
  * applying the per-head RMS norm (q_gamma/k_gamma non-NULL) and then RoPE

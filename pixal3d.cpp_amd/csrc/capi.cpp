@@ -28,6 +28,14 @@ int fail_workspace(const char * what) noexcept {
     }
 }
 
+int fail_call(const char * who, const char * what) noexcept {
+    try {
+        return fail(PXS_ERR_ARG, std::string(who) + ": " + what);
+    } catch (...) {
+        return fail(PXS_ERR_ARG, std::string());
+    }
+}
+
 int check_hip(hipError_t status, const char * what) {
     if (status == hipSuccess) return PXS_OK;
     return fail(PXS_ERR_HIP, std::string(what) + ": " + hipGetErrorString(status));

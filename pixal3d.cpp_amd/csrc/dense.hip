@@ -41,6 +41,7 @@
 
 #include "pxs_common.h"
 #include "split3.h"
+#include "tiles.h"
 
 #include <algorithm>
 
@@ -77,23 +78,6 @@ template <typename T> __device__ __forceinline__ void select_group(DenseArgs & a
     a.w = g.w[blockIdx.y];
     a.bias = g.bias[blockIdx.y];
     a.y = static_cast<T *>(a.y) + static_cast<int64_t>(blockIdx.y) * a.m * a.n;
-}
-
-// Output tile (row tile, column tile) of logical tile t: groups of g row
-// tiles share their column tiles, and inside a group consecutive t walk the
-// rows, so the tiles one XCD runs at a time cover g row tiles x (32 / g)
-// column tiles of operands instead of one row tile x every column tile.
-__device__ __forceinline__ void tile_of(int t, int tiles_m, int tiles_n, int g, int & tm, int & tn) {
-    if (g <= 1) {
-        tm = t / tiles_n;
-        tn = t % tiles_n;
-        return;
-    }
-    const int per_group = g * tiles_n;
-    const int grp = t / per_group, in = t % per_group;
-    const int rows = min(g, tiles_m - grp * g);  // the last group may be short
-    tm = grp * g + in % rows;
-    tn = in / rows;
 }
 
 __device__ __align__(16) uint4 g_dense_zero[8];  // 128 zero bytes: K pieces past the end
@@ -255,27 +239,6 @@ __device__ __forceinline__ void dense_store_staged(const DenseArgs & a, const f3
         if (row < a.m && c < a.n)
             *reinterpret_cast<uint4 *>(static_cast<T *>(a.y) + row * a.n + c) = v;
     }
-}
-
-// Rows of KB = 128 bytes per K chunk in LDS: 8 pieces of 16 bytes,
-// XOR-swizzled by row so that the 16 rows one LDS cycle serves (64 banks of
-// 4 bytes) read 16 different bank groups.
-template <int KB> __device__ __forceinline__ int piece_swz(int row);
-template <> __device__ __forceinline__ int piece_swz<128>(int row) { return (row & 7) ^ ((row >> 3) & 1); }
-
-// Waits until at most min(later, MAX) stages of PER instructions each are in
-// flight (s_waitcnt's count is a constant, six bits of it vmcnt).
-template <int MAX, int PER>
-__device__ __forceinline__ void wait_stages(int later) {
-    constexpr int n = MAX * PER;
-    static_assert(n < 64, "vmcnt has six bits");
-    if constexpr (MAX > 0) {
-        if (later < MAX) {
-            wait_stages<MAX - 1, PER>(later);
-            return;
-        }
-    }
-    __builtin_amdgcn_s_waitcnt(0x0F70 | (n & 15) | ((n >> 4) << 14));
 }
 
 // NW waves in a WAVES_M x (NW / WAVES_M) grid, each owning a (BM / WAVES_M) x

@@ -15,6 +15,7 @@ namespace pxs {
 void set_error(const std::string & message);
 int fail(int code, const std::string & message) noexcept;
 int fail_workspace(const char * what) noexcept;
+int fail_call(const char * who, const char * what) noexcept;  // PXS_ERR_ARG, "who: what"
 int check_hip(hipError_t status, const char * what);
 int check_launch(const char * what);
 

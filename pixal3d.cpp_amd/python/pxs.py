@@ -21,6 +21,7 @@ PXS_OK, PXS_ERR_ARG, PXS_ERR_HIP, PXS_ERR_DATA = 0, 1, 2, 3
 PXS_F32, PXS_BF16 = 0, 1
 PXS_ATTN_NOALLOC_MAX_SEGMENTS = 65536
 ACT_NONE, ACT_GELU_TANH, ACT_SILU = 0, 1, 2
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 
 VALIDATION_MESSAGES = {
     4: "sparse coordinate is outside its shape",
@@ -50,6 +51,13 @@ _SIGS = {
     "pxs_subm_conv3d": (_i32, [_i32, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp]),
     "pxs_subm_conv3d_grid": (_i32, [_i32, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32,
                                     _i32, _vp, C.c_uint32, _vp, _vp]),
+    "pxs_quantize_rows_i8": (_i32, [_i32, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "pxs_linear_i8": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
+    "pxs_linear_i8_residual": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp]),
+    "pxs_linear_i8_gate_residual": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i32,
+                                           _vp, _vp]),
+    "pxs_rope_frequencies": (_i32, [_i32] + [C.c_double] * 5 + [C.POINTER(C.c_double)]),
+    "pxs_rope_positions": (_i32, [_i32, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _f, _vp, _i64, _vp]),
     "pxs_status_reset": (_i32, [_vp, _vp]),
     "pxs_check_finite": (_i32, [_i32, _vp, _i64, _i32, _i64, _vp, _vp]),
     "pxs_value_stats_workspace_bytes": (C.c_size_t, [_i64]),
@@ -278,6 +286,17 @@ def _ptr(t):
     if t is None:
         return None
     return C.c_void_p(t if isinstance(t, int) else t.data_ptr())
+
+
+def _unit_stride(t, what):
+    """t must be [rows, columns] with columns next to one another and rows that do not overlap."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise PxsError(f"{what} must be rows of contiguous columns")
+
+
+def _expect(t, dtype, shape, what):
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise PxsError(f"{what} must be contiguous {dtype} {list(shape)}")
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -674,6 +693,64 @@ class Pxs:
                     "pxs_linear_gate_residual")
         return residual
 
+    # -- 8-bit linears ------------------------------------------------------------------
+    def quantize_rows(self, x, out=None, scales=None):
+        """pxs_quantize_rows_i8 -> (int8 [rows, channels], fp32 scales [rows]); x may be a
+        column slice (rows of any stride)."""
+        rows, channels = x.shape
+        _unit_stride(x, "quantize_rows: x")
+        q = torch.empty((rows, channels), dtype=torch.int8, device=x.device) if out is None else out
+        scales = torch.empty(rows, dtype=torch.float32, device=x.device) if scales is None else scales
+        _expect(q, torch.int8, (rows, channels), "quantize_rows: out")
+        _expect(scales, torch.float32, (rows,), "quantize_rows: scales")
+        self._check(self.lib.pxs_quantize_rows_i8(_dtype_code(x), _ptr(x), x.stride(0), rows, channels,
+                                                  _ptr(q), _ptr(scales), self.stream()),
+                    "pxs_quantize_rows_i8")
+        return q, scales
+
+    @staticmethod
+    def _i8_operands(x, x_scales, weight, w_scales, bias, what):
+        rows, cin = x.shape
+        cout = weight.shape[0]
+        _expect(x, torch.int8, (rows, cin), what + ": x")
+        _expect(weight, torch.int8, (cout, cin), what + ": weight")
+        _expect(x_scales, torch.float32, (rows,), what + ": x_scales")
+        _expect(w_scales, torch.float32, (cout,), what + ": w_scales")
+        if bias is not None:
+            _expect(bias, torch.float32, (cout,), what + ": bias")
+        return rows, cin, cout
+
+    def linear_i8(self, x, x_scales, weight, w_scales, bias=None, act=ACT_NONE, dtype=torch.bfloat16, out=None):
+        """pxs_linear_i8: act(x W^T * x_scales * w_scales + bias) in `dtype` (or out's)."""
+        rows, cin, cout = self._i8_operands(x, x_scales, weight, w_scales, bias, "linear_i8")
+        y = torch.empty((rows, cout), dtype=dtype, device=x.device) if out is None else out
+        _expect(y, y.dtype, (rows, cout), "linear_i8: out")
+        self._check(self.lib.pxs_linear_i8(_ptr(x), _ptr(x_scales), rows, cin, _ptr(weight), _ptr(w_scales),
+                                           _ptr(bias), cout, act, _dtype_code(y), _ptr(y), self.stream()),
+                    "pxs_linear_i8")
+        return y
+
+    def linear_i8_residual(self, x, x_scales, weight, w_scales, bias, residual):
+        """pxs_linear_i8_residual: residual (fp32) += the 8-bit linear."""
+        rows, cin, cout = self._i8_operands(x, x_scales, weight, w_scales, bias, "linear_i8_residual")
+        _expect(residual, torch.float32, (rows, cout), "linear_i8_residual: residual")
+        self._check(self.lib.pxs_linear_i8_residual(_ptr(x), _ptr(x_scales), rows, cin, _ptr(weight),
+                                                    _ptr(w_scales), _ptr(bias), cout, _ptr(residual),
+                                                    self.stream()),
+                    "pxs_linear_i8_residual")
+        return residual
+
+    def linear_i8_gate_residual(self, x, x_scales, weight, w_scales, bias, coords, block_mod, time_mod,
+                                gate_offset, residual):
+        """pxs_linear_i8_gate_residual: residual (fp32) += gate * the 8-bit linear."""
+        rows, cin, cout = self._i8_operands(x, x_scales, weight, w_scales, bias, "linear_i8_gate_residual")
+        _expect(residual, torch.float32, (rows, cout), "linear_i8_gate_residual: residual")
+        self._check(self.lib.pxs_linear_i8_gate_residual(
+            _ptr(x), _ptr(x_scales), rows, cin, _ptr(weight), _ptr(w_scales), _ptr(bias), cout, _ptr(coords),
+            _ptr(block_mod), _ptr(time_mod), gate_offset, _ptr(residual), self.stream()),
+            "pxs_linear_i8_gate_residual")
+        return residual
+
     # -- row-wise ---------------------------------------------------------------------
     def layer_norm(self, x, eps, gamma=None, beta=None, out_dtype=None):
         out_dtype = out_dtype or x.dtype
@@ -708,6 +785,31 @@ class Pxs:
                                       x.shape[0], heads, head_dim, freq_min, freq_base, _ptr(y),
                                       y.stride(0), self.stream()),
                     "pxs_rope")
+        return y
+
+    def rope_frequencies(self, rotary_dim, base=10000.0, factor=1.0, original_length=0.0, low_turns=1.0,
+                         high_turns=32.0, device="cuda"):
+        """pxs_rope_frequencies -> float64 [rotary_dim / 2] on the device."""
+        freq = (C.c_double * max(rotary_dim // 2, 1))()
+        self._check(self.lib.pxs_rope_frequencies(rotary_dim, base, factor, original_length, low_turns,
+                                                  high_turns, freq), "pxs_rope_frequencies")
+        return torch.tensor(list(freq), dtype=torch.float64, device=device)
+
+    def rope_positions(self, x, positions, freq, heads, head_dim, layout=ROPE_HALF, magnitude=1.0, out=None):
+        """pxs_rope_positions: the first 2 * len(freq) values of each head of x turned by
+        positions[row] * freq; out may be x."""
+        rows = x.shape[0]
+        _unit_stride(x, "rope_positions: x")
+        y = torch.empty((rows, heads * head_dim), dtype=x.dtype, device=x.device) if out is None else out
+        _unit_stride(y, "rope_positions: out")
+        if x.shape[1] != heads * head_dim or y.shape != x.shape or y.dtype != x.dtype:
+            raise PxsError("rope_positions: x and out must be [rows, heads * head_dim] of one dtype")
+        _expect(positions, torch.int32, (rows,), "rope_positions: positions")
+        _expect(freq, torch.float64, (freq.numel(),), "rope_positions: freq")
+        self._check(self.lib.pxs_rope_positions(_dtype_code(x), _ptr(positions), _ptr(freq), _ptr(x), x.stride(0),
+                                                rows, heads, head_dim, 2 * freq.numel(), layout, magnitude,
+                                                _ptr(y), y.stride(0), self.stream()),
+                    "pxs_rope_positions")
         return y
 
     def qkv_prepare(self, qkv, heads, head_dim, q_gamma=None, k_gamma=None, coords=None,
