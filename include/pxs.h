@@ -525,6 +525,40 @@ int pxs_varlen_attention_noalloc(int dtype, const void * q, int64_t ld_q, const 
                                  const int32_t * row_map, int heads, int head_dim, int value_dim,
                                  float scale, void * o, int64_t ld_o, void * stream);
 
+/* pxs_varlen_attention with scores that are capped, biased by distance and
+ * masked, for token sequences (no counterpart in the reference).  Queries of
+ * segment s, rows [cu_q[s], cu_q[s+1]), attend to keys [cu_k[s], cu_k[s+1]) and
+ * to no other segment's (the documents of a packed batch are its segments).
+ *   Heads: q and o have heads * head_dim columns, k and v kv_heads * head_dim;
+ *     query heads h share key/value head h / (heads / kv_heads).  heads is a
+ *     multiple of kv_heads, head_dim 1..256.
+ *   Positions: key j of a segment is at position j, query i at i + (keys -
+ *     queries) of its segment: the queries are the last positions, as new tokens
+ *     (one or many) over a cache of the ones before are.
+ *   Scores: scale * q.k; then cap * tanh(score / cap) if cap > 0; then minus
+ *     slopes[head] * |distance of the positions| if slopes (device fp32 [heads])
+ *     is set.
+ *   Mask: causal = 1 hides keys after a query's position, except those below
+ *     prefix[s] (device int64 [nseg], may be NULL), which all queries of the
+ *     segment see.  What hidden keys and values hold does not matter, NaN
+ *     included.  A query that sees no key gets zeros.
+ * Row strides ld_* are in elements.  total_q = cu_q[nseg] and total_k =
+ * cu_k[nseg], both below 2^31; rows of q and o behind the last segment are
+ * neither read nor written.  bf16 rows of 16-byte pieces with head_dim 64 or 128
+ * take the fastest kernels.  The result depends on the whole call's sizes in its
+ * last bits (the keys of few rows are split and joined in a fixed order); the
+ * same call gives the same bits.
+ * workspace: pxs_attention_scores_workspace_bytes of the same sizes; calls that
+ * may overlap need one each. */
+size_t pxs_attention_scores_workspace_bytes(int nseg, int64_t total_q, int64_t total_k, int heads,
+                                            int kv_heads, int head_dim);
+int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const void * k,
+                                int64_t ld_k, const void * v, int64_t ld_v, const int64_t * cu_q,
+                                const int64_t * cu_k, int nseg, int64_t total_q, int64_t total_k,
+                                int heads, int kv_heads, int head_dim, float scale, float cap,
+                                const float * slopes, int causal, const int64_t * prefix, void * o,
+                                int64_t ld_o, void * workspace, void * stream);
+
 /* Per-batch cu_seqlens from the batch column (src/sparse.cpp:731-737):
  * cu (device int64[batch_size + 1]). */
 int pxs_batch_cu_seqlens(const int32_t * coords, int64_t n, int batch_size, int64_t * cu,

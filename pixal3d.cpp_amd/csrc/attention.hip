@@ -15,6 +15,7 @@
 //   fp32: v_mfma_f32_32x32x2_f32   (64 + 64 per wave per tile)
 // head_dim and value_dim up to 64 (zero padded to 64 inside the kernel).
 
+#include "attn_common.h"
 #include "pxs_common.h"
 #include "scan.h"
 #include "split3.h"
@@ -27,7 +28,6 @@ namespace pxs {
 namespace {
 
 constexpr int kKeys = 64;  // keys per tile
-constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void wait_vmcnt0() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
@@ -60,24 +60,6 @@ __device__ __forceinline__ int64_t remap_xcd64(int64_t bid, int64_t blocks) {
     const int64_t q = blocks / 8, rem = blocks % 8;
     const int64_t xcd = bid % 8, slot = bid / 8;
     return (xcd < rem) ? xcd * (q + 1) + slot : rem * (q + 1) + (xcd - rem) * q + slot;
-}
-
-// The segment owning query tile t: the largest s with tile_start[s] <= t
-// (tile_start is non-decreasing; empty segments repeat a value).  The wave
-// samples 64 evenly spaced entries per round and keeps the last interval whose
-// start is <= t, so nseg <= 64 takes one dependent load and nseg <= 4096 two.
-__device__ __forceinline__ int find_segment(const int64_t * __restrict__ tile_start, int nseg,
-                                            int64_t t, int lane) {
-    int lo = 0, len = nseg;
-    while (len > 1) {
-        const int stride = (len + 63) >> 6;
-        const int off = lane * stride;
-        const bool le = off < len && tile_start[lo + off] <= t;
-        const int cnt = __popcll(__ballot(le));  // >= 1: tile_start[lo] <= t
-        lo += (cnt - 1) * stride;
-        len = min(stride, len - (cnt - 1) * stride);
-    }
-    return __builtin_amdgcn_readfirstlane(lo);
 }
 
 // Mean segment length (queries per segment, from the host-known total and
@@ -398,29 +380,12 @@ flash_attn_kernel(AttnArgs a) {
 
 __device__ __align__(16) uint4 g_attn_zero[8];
 
-__device__ __forceinline__ int kswz(int row) { return (row & 7) ^ ((row >> 3) & 1); }
-__device__ __forceinline__ int vswz(int row) { return (2 * (row & 3)) ^ ((row >> 2) & 1); }
-
-typedef short v4i16 __attribute__((ext_vector_type(4)));
 
 // Scores are kept in the raw (unscaled) domain; p = exp2(s * c - m * c) with
 // c = scale * log2(e) costs one FMA and one exp per score.  The running max m
 // is only raised when a tile's max exceeds it by more than kLazyLog2 / c
 // (p <= 2^kLazyLog2 meanwhile), so the O rescale runs on few tiles.
 constexpr float kLazyLog2 = 8.0f;
-
-__device__ __forceinline__ float lane_pair_max(float v) {
-    // max over lanes l and l ^ 32 (v_permlane32_swap exchanges the halves).
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v),
-                                                     false, false);
-    return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-}
-
-__device__ __forceinline__ float lane_pair_sum(float v) {
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v),
-                                                     false, false);
-    return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-}
 
 // Software-pipelined bf16 kernel (head_dim 64).  Each wave owns 32 queries.
 // Iteration j of the key loop issues 16 MFMAs that do not depend on tile j's

@@ -58,6 +58,9 @@ _SIGS = {
                                            _vp, _vp]),
     "pxs_rope_frequencies": (_i32, [_i32] + [C.c_double] * 5 + [C.POINTER(C.c_double)]),
     "pxs_rope_positions": (_i32, [_i32, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _f, _vp, _i64, _vp]),
+    "pxs_attention_scores_workspace_bytes": (C.c_size_t, [_i32, _i64, _i64, _i32, _i32, _i32]),
+    "pxs_varlen_attention_scores": (_i32, [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _i64,
+                                           _i32, _i32, _i32, _f, _f, _vp, _i32, _vp, _vp, _i64, _vp, _vp]),
     "pxs_status_reset": (_i32, [_vp, _vp]),
     "pxs_check_finite": (_i32, [_i32, _vp, _i64, _i32, _i64, _vp, _vp]),
     "pxs_value_stats_workspace_bytes": (C.c_size_t, [_i64]),
@@ -292,6 +295,11 @@ def _unit_stride(t, what):
     """t must be [rows, columns] with columns next to one another and rows that do not overlap."""
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         raise PxsError(f"{what} must be rows of contiguous columns")
+
+
+def _ld(t):
+    """Row stride of a tensor that _unit_stride accepted (a lone row has none of its own)."""
+    return max(t.stride(0), t.shape[1])
 
 
 def _expect(t, dtype, shape, what):
@@ -703,7 +711,7 @@ class Pxs:
         scales = torch.empty(rows, dtype=torch.float32, device=x.device) if scales is None else scales
         _expect(q, torch.int8, (rows, channels), "quantize_rows: out")
         _expect(scales, torch.float32, (rows,), "quantize_rows: scales")
-        self._check(self.lib.pxs_quantize_rows_i8(_dtype_code(x), _ptr(x), x.stride(0), rows, channels,
+        self._check(self.lib.pxs_quantize_rows_i8(_dtype_code(x), _ptr(x), _ld(x), rows, channels,
                                                   _ptr(q), _ptr(scales), self.stream()),
                     "pxs_quantize_rows_i8")
         return q, scales
@@ -806,9 +814,9 @@ class Pxs:
             raise PxsError("rope_positions: x and out must be [rows, heads * head_dim] of one dtype")
         _expect(positions, torch.int32, (rows,), "rope_positions: positions")
         _expect(freq, torch.float64, (freq.numel(),), "rope_positions: freq")
-        self._check(self.lib.pxs_rope_positions(_dtype_code(x), _ptr(positions), _ptr(freq), _ptr(x), x.stride(0),
+        self._check(self.lib.pxs_rope_positions(_dtype_code(x), _ptr(positions), _ptr(freq), _ptr(x), _ld(x),
                                                 rows, heads, head_dim, 2 * freq.numel(), layout, magnitude,
-                                                _ptr(y), y.stride(0), self.stream()),
+                                                _ptr(y), _ld(y), self.stream()),
                     "pxs_rope_positions")
         return y
 
@@ -868,6 +876,39 @@ class Pxs:
         return o
 
     # -- compositions ----------------------------------------------------------------------
+    def attention_scores_workspace(self, nseg, total_q, total_k, heads, kv_heads, head_dim, device="cuda"):
+        """A workspace for varlen_attention_scores calls of up to these sizes."""
+        return self._ws(self.lib.pxs_attention_scores_workspace_bytes(nseg, total_q, total_k, heads, kv_heads,
+                                                                      head_dim), device)
+
+    def varlen_attention_scores(self, q, k, v, cu_q, cu_k, heads, kv_heads, head_dim, scale, cap=0.0, slopes=None,
+                                causal=False, prefix=None, out=None, workspace=None):
+        """pxs_varlen_attention_scores: q [*, heads * head_dim], k and v [*, kv_heads * head_dim]
+        (rows of any stride), cu_q and cu_k int64 [segments + 1]."""
+        nseg, total_q, total_k = cu_q.numel() - 1, q.shape[0], k.shape[0]
+        o = torch.empty((total_q, heads * head_dim), dtype=q.dtype, device=q.device) if out is None else out
+        for t, columns, what in ((q, heads, "q"), (k, kv_heads, "k"), (v, kv_heads, "v"), (o, heads, "out")):
+            _unit_stride(t, "varlen_attention_scores: " + what)
+            if t.shape[1] != columns * head_dim or t.dtype != q.dtype:
+                raise PxsError(f"varlen_attention_scores: {what} must be [rows, {columns * head_dim}] {q.dtype}")
+        if v.shape[0] != total_k or o.shape[0] != total_q:
+            raise PxsError("varlen_attention_scores: k and v, q and out must have the same rows")
+        _expect(cu_q, torch.int64, (nseg + 1,), "varlen_attention_scores: cu_q")
+        _expect(cu_k, torch.int64, (nseg + 1,), "varlen_attention_scores: cu_k")
+        if slopes is not None:
+            _expect(slopes, torch.float32, (heads,), "varlen_attention_scores: slopes")
+        if prefix is not None:
+            _expect(prefix, torch.int64, (nseg,), "varlen_attention_scores: prefix")
+        need = self.lib.pxs_attention_scores_workspace_bytes(nseg, total_q, total_k, heads, kv_heads, head_dim)
+        ws = self._ws(need, q.device) if workspace is None else workspace
+        if ws.numel() * ws.element_size() < need:
+            raise PxsError(f"varlen_attention_scores: workspace of {need} bytes needed")
+        self._check(self.lib.pxs_varlen_attention_scores(
+            _dtype_code(q), _ptr(q), _ld(q), _ptr(k), _ld(k), _ptr(v), _ld(v), _ptr(cu_q), _ptr(cu_k),
+            nseg, total_q, total_k, heads, kv_heads, head_dim, scale, cap, _ptr(slopes), int(causal),
+            _ptr(prefix), _ptr(o), _ld(o), _ptr(ws), self.stream()), "pxs_varlen_attention_scores")
+        return o
+
     def transformer_block(self, cfg: BlockConfig, weights: BlockWeights, coords, batch_size, cu,
                           hidden, time_mod, context, ctx_offsets, projected=None, dtype=None):
         """pxs_transformer_block: hidden (fp32 [rows, C]) is updated in place."""

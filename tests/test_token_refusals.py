@@ -102,3 +102,28 @@ def test_rope_frequencies_refusals(lib, args, text):
 
 def test_rope_frequencies_null(lib):
     refused(lib, lib.pxs_rope_frequencies(64, 1e4, 1.0, 0.0, 0.0, 0.0, None), "null pointer")
+
+
+SCORES = dict(dtype=0, q=P, ld_q=256, k=P, ld_k=128, v=P, ld_v=128, cu_q=P, cu_k=P, nseg=2, total_q=10, total_k=20,
+              heads=4, kv=2, d=64, scale=0.125, cap=0.0, slopes=None, causal=1, prefix=None, o=P, ld_o=256, ws=P,
+              stream=None)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=5), "bad dtype"), (dict(heads=5), "multiple of kv_heads"), (dict(kv=0), "multiple of kv_heads"),
+    (dict(heads=131072, kv=1), "65535"), (dict(d=0), "head_dim"), (dict(d=257), "head_dim"), (dict(scale=0.0), "scale"),
+    (dict(scale=math.nan), "scale"), (dict(cap=-1.0), "cap"), (dict(cap=math.inf), "cap"), (dict(cap=1e-44), "out of range"),
+    (dict(causal=2), "causal"), (dict(causal=0, prefix=P), "prefix"), (dict(nseg=-1), "row counts"),
+    (dict(total_q=-1), "row counts"), (dict(total_k=2 ** 31), "row counts"), (dict(ld_q=255), "row stride"),
+    (dict(ld_k=127), "row stride"), (dict(ld_v=127), "row stride"), (dict(ld_o=255), "row stride"),
+    (dict(q=None), "null pointer"), (dict(k=None), "null pointer"), (dict(v=None), "null pointer"),
+    (dict(o=None), "null pointer"), (dict(cu_q=None), "null pointer"), (dict(cu_k=None), "null pointer"),
+    (dict(ws=None), "null pointer"), (dict(ws=C.c_void_p(4104)), "256-byte aligned"),
+    (dict(total_q=2 ** 31 - 1, heads=65535, kv=65535, ld_q=2 ** 23, ld_k=2 ** 23, ld_v=2 ** 23, ld_o=2 ** 23), "grid too large")])
+def test_attention_scores_refusals(lib, change, text):
+    refused(lib, lib.pxs_varlen_attention_scores(*{**SCORES, **change}.values()), text)
+
+
+def test_attention_scores_of_nothing(lib):
+    for change in (dict(nseg=0), dict(total_q=0)):
+        assert lib.pxs_varlen_attention_scores(*{**SCORES, **change}.values()) == pxs.PXS_OK
