@@ -23,8 +23,8 @@
 #include "attn_common.h"
 
 #include <algorithm>
-#include <atomic>
 #include <cmath>
+#include <type_traits>
 
 namespace pxs {
 namespace {
@@ -38,7 +38,8 @@ struct ScoreArgs {
     const int64_t * cu_k;
     int nseg;
     int64_t total_q;
-    const int64_t * tile_start;  // [nseg + 1] row tiles before each segment; null: at most 64 segments
+    const int64_t * tile_start;  // [nseg + 1] items before each segment; null: at most 64 segments
+    int chunk;                   // keys of an item of a segment with one row tile; 0: not cut
     int heads, kv_heads, group, d;
     float scale_log2;            // scale * log2(e), or with a cap scale / cap
     float cap_log2;              // cap * log2(e); 0: no cap
@@ -50,8 +51,8 @@ struct ScoreArgs {
     int vec;                     // rows of q, k and v in whole 16-byte pieces
     int64_t tiles;               // row tiles launched (bound)
     int splits;
-    float * part;                // [splits][total_q][heads][d] unnormalised outputs
-    float2 * part_ml;            // [splits][total_q][heads] maxima (log2 units) and sums
+    float * part;                // [partial rows][d] unnormalised outputs
+    float2 * part_ml;            // [partial rows] maxima (log2 units) and sums
 };
 
 // A workgroup's rows: a tile of a segment and key/value head, and the keys that its rows see.
@@ -64,40 +65,81 @@ struct Rows {
     int64_t rows;         // of the segment: nq * group
     int64_t shift;        // position of query i: i + shift
     int64_t prefix;
+    int chunk, chunks;    // of the segment's keys; 0 of 1 where they are not cut
 };
 
-// Row tile t of `rows_per_tile` rows (a power of two); false past the last.
-__device__ __forceinline__ bool locate_rows(const ScoreArgs & a, int64_t t, int rows_per_tile, int lane, Rows & w) {
-    const int shift = 31 - __clz(rows_per_tile);
-    int64_t first;
-    if (a.tile_start) {
-        if (t >= a.tile_start[a.nseg]) return false;
-        w.seg = find_segment(a.tile_start, a.nseg, t, lane);
-        first = a.tile_start[w.seg];
-    } else {
-        int64_t tiles = 0;
-        if (lane < a.nseg)
-            tiles = ((a.cu_q[lane + 1] - a.cu_q[lane]) * a.group + rows_per_tile - 1) >> shift;
-        int64_t end = tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int64_t below = __shfl_up(end, d, 64);
-            if (lane >= d) end += below;
-        }
-        const uint64_t before = __ballot(lane < a.nseg && end <= t);  // segments that end at or before t
-        w.seg = __popcll(before);
-        if (w.seg >= a.nseg) return false;
-        first = __shfl(end - tiles, w.seg, 64);
-    }
-    w.seg = __builtin_amdgcn_readfirstlane(w.seg);
+// Items of a segment: its row tiles, or where it has one and a.chunk is set the chunks of its keys.
+__device__ __forceinline__ int64_t segment_items(int64_t nq, int64_t nk, int group, int rows_per_tile, int chunk) {
+    const int64_t rows = nq * group;
+    if (rows <= 0) return 0;
+    if (chunk > 0 && rows <= rows_per_tile) return max((nk + chunk - 1) / chunk, int64_t(1));
+    return (rows + rows_per_tile - 1) / rows_per_tile;
+}
+
+// Segment w.seg's part of w, item i of its items.
+__device__ __forceinline__ void segment_rows(const ScoreArgs & a, int i, int rows_per_tile, Rows & w) {
     w.q0 = a.cu_q[w.seg];
     w.k0 = a.cu_k[w.seg];
     w.nq = a.cu_q[w.seg + 1] - w.q0;
     w.nk = a.cu_k[w.seg + 1] - w.k0;
     w.rows = w.nq * a.group;
-    w.row0 = (t - first) * rows_per_tile;
     w.shift = w.nk - w.nq;
     w.prefix = a.causal && a.prefix ? a.prefix[w.seg] : 0;
+    const bool cut = a.chunk > 0 && w.rows <= rows_per_tile;
+    w.row0 = cut ? 0 : static_cast<int64_t>(i) * rows_per_tile;
+    w.chunk = cut ? i : 0;
+    w.chunks = cut ? static_cast<int>((w.nk + a.chunk - 1) / a.chunk) : 1;
+}
+
+// The items of up to 64 segments, a segment a lane: end[lane] = items of the segments up to its own.
+__device__ __forceinline__ int64_t lane_items(const ScoreArgs & a, int rows_per_tile, int lane, int64_t & end) {
+    int64_t items = 0;
+    if (lane < a.nseg)
+        items = segment_items(a.cu_q[lane + 1] - a.cu_q[lane], a.cu_k[lane + 1] - a.cu_k[lane], a.group, rows_per_tile,
+                              a.chunk);
+    end = items;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int64_t below = __shfl_up(end, d, 64);
+        if (lane >= d) end += below;
+    }
+    return items;
+}
+
+// Item t; false past the last.
+__device__ __forceinline__ bool locate_rows(const ScoreArgs & a, int64_t t, int rows_per_tile, int lane, Rows & w) {
+    int64_t first;
+    int seg;
+    if (a.tile_start) {
+        if (t >= a.tile_start[a.nseg]) return false;
+        seg = find_segment(a.tile_start, a.nseg, t, lane);
+        first = a.tile_start[seg];
+    } else {
+        int64_t end;
+        const int64_t items = lane_items(a, rows_per_tile, lane, end);
+        seg = __popcll(__ballot(lane < a.nseg && end <= t));  // segments that end at or before t
+        if (seg >= a.nseg) return false;
+        first = __shfl(end - items, seg, 64);
+    }
+    w.seg = __builtin_amdgcn_readfirstlane(seg);
+    segment_rows(a, __builtin_amdgcn_readfirstlane(static_cast<int>(t - first)), rows_per_tile, w);
+    return true;
+}
+
+// Query qi of the call: its segment, and the first of the segment's items; false for a row of no segment.
+__device__ __forceinline__ bool locate_query(const ScoreArgs & a, int64_t qi, int rows_per_tile, int lane, Rows & w,
+                                             int64_t & item) {
+    if (qi < a.cu_q[0] || qi >= a.cu_q[a.nseg]) return false;
+    const int seg = find_segment(a.cu_q, a.nseg, qi, lane);
+    if (a.tile_start) {
+        item = a.tile_start[seg];
+    } else {
+        int64_t end;
+        const int64_t items = lane_items(a, rows_per_tile, lane, end);
+        item = __shfl(end - items, seg, 64);
+    }
+    w.seg = seg;
+    segment_rows(a, 0, rows_per_tile, w);
     return true;
 }
 
@@ -138,7 +180,7 @@ __device__ __forceinline__ bool is_finite_bits(float v) { return (__float_as_uin
 // times a weight of zero is NaN.  One wave per row; lane l holds dims l, l + 64, ...
 template <typename T, int NC>
 __device__ void row_alone(const ScoreArgs & a, const Rows & w, int64_t row, int64_t key0, int64_t key1, int lane,
-                          int64_t slot_split) {
+                          bool partial, int64_t slot) {
     const int64_t i = row / a.group;
     const int head = w.kv * a.group + static_cast<int>(row % a.group);
     const T * q = static_cast<const T *>(a.q) + (w.q0 + i) * a.ldq + static_cast<int64_t>(head) * a.d;
@@ -170,16 +212,20 @@ __device__ void row_alone(const ScoreArgs & a, const Rows & w, int64_t row, int6
             if (lane + 64 * c < a.d) acc[c] = acc[c] * keep + p * load_f32(v + j * a.ldv + lane + 64 * c);
         m = up;
     }
-    const int64_t slot = (slot_split * a.total_q + w.q0 + i) * a.heads + head;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a NaN sum stays NaN)
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int dim = lane + 64 * c;
         if (dim >= a.d) continue;
-        if (a.splits > 1) a.part[slot * a.d + dim] = acc[c];
+        if (partial) a.part[slot * a.d + dim] = acc[c];
         else store_f32(static_cast<T *>(a.o) + (w.q0 + i) * a.ldo + static_cast<int64_t>(head) * a.d + dim, acc[c] * inv);
     }
-    if (a.splits > 1 && lane == 0) a.part_ml[slot] = make_float2(m, l);
+    if (partial && lane == 0) a.part_ml[slot] = make_float2(m, l);
+}
+
+// Partial row of a (query, head) in split `split` of a call whose keys are split alike for all rows.
+__device__ __forceinline__ int64_t split_slot(const ScoreArgs & a, const Rows & w, int split, int64_t row) {
+    return (static_cast<int64_t>(split) * a.total_q + w.q0 + row / a.group) * a.heads + w.kv * a.group + row % a.group;
 }
 
 // Any dtype, head size up to DP, stride and alignment.  Four waves of 32 rows
@@ -363,11 +409,12 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
     if (again) {
         for (int i = 0; i < 32; ++i)
             if (wave_row0 + i < w.rows)
-                row_alone<T, DP / 64>(a, w, wave_row0 + i, kt_first * kKeys, kt_last * kKeys, lane, split);
+                row_alone<T, DP / 64>(a, w, wave_row0 + i, kt_first * kKeys, kt_last * kKeys, lane, a.splits > 1,
+                                      split_slot(a, w, split, wave_row0 + i));
         return;
     }
     if (!live) return;
-    const int64_t slot = (static_cast<int64_t>(split) * a.total_q + w.q0 + qi) * a.heads + head;
+    const int64_t slot = split_slot(a, w, split, row);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T * o = static_cast<T *>(a.o) + (w.q0 + qi) * a.ldo + static_cast<int64_t>(head) * a.d;
     if (a.splits > 1 && h == 0) a.part_ml[slot] = make_float2(m, l);
@@ -380,6 +427,641 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
             if (a.splits > 1) a.part[slot * a.d + dim] = oacc[dt][e];
             else store_f32(o + dim, oacc[dt][e] * inv);
         }
+}
+
+// ---- bf16, head size 64 or 128 -----------------------------------------------------
+// Tiles of kKeys keys, 8 KB of K and 8 KB of V, go from HBM to LDS by DMA, rows of
+// DH / 64 halves of 128 bytes; V is read transposed from LDS (ds_read_b64_tr_b16).
+// 16 matrix instructions a tile and wave, as many for S as for O.
+
+__device__ __align__(16) uint4 g_score_zero[8];  // what keys past a segment's end are read as
+
+constexpr int kCap = 1, kBias = 2;  // MODE bits: scores are capped, biased
+
+template <int DH> struct Fast {
+    static constexpr int KT = DH == 64 ? 2 : 1;   // 32-key sub-tiles of a tile
+    static constexpr int kKeys = 32 * KT;
+    static constexpr int kHalves = DH / 64;
+    static constexpr int kHalfBytes = kKeys * 128;
+    static constexpr int kTileBytes = kHalves * kHalfBytes;  // 8 KB
+    static constexpr int kUnits = kTileBytes / 1024;         // DMA instructions of a K or V tile (8 rows of a half)
+    static constexpr int NST = DH / 16, NDT = DH / 32;
+    typedef f32x16 Scores[KT];
+    typedef bf16x8 Weights[KT][2];
+    typedef f32x16 Out[NDT];
+};
+
+// One row's constants of the map from a product q . k to a weight's exponent:
+//   z = raw * mul + add                              (no cap)
+//   z = add + top / (1 + 2^(raw * mul))              (cap: cap tanh(x) = cap - 2 cap / (1 + e^2x))
+//   with a bias, add - slope * |behind - key|.
+struct RowScore {
+    float mul, top, slope;
+};
+
+template <int MODE>
+__device__ __forceinline__ RowScore row_score(const ScoreArgs & a, int head) {
+    RowScore s;
+    s.mul = MODE & kCap ? 2.0f * kLog2e * a.scale_log2 : a.scale_log2;
+    s.top = -2.0f * a.cap_log2;
+    s.slope = MODE & kBias ? -kLog2e * a.slopes[head] : 0.0f;
+    return s;
+}
+
+// z - base of a product; key: behind - key is the distance.  add is cap_log2 - base, or -base.
+template <int MODE>
+__device__ __forceinline__ float score_of(const RowScore & s, float raw, float add, float away) {
+    float b = add;
+    if constexpr (MODE & kBias) b = __builtin_fmaf(s.slope, fabsf(away), add);
+    if constexpr (MODE & kCap)
+        return __builtin_fmaf(s.top, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw * s.mul)), b);
+    return __builtin_fmaf(raw, s.mul, b);
+}
+
+template <int DH>
+__device__ __forceinline__ void tile_qk(const char * kl, const bf16x8 (&qf)[Fast<DH>::NST],
+                                        typename Fast<DH>::Scores & s, int h, int r) {
+    using F = Fast<DH>;
+#pragma unroll
+    for (int kt = 0; kt < F::KT; ++kt) {
+        const int row = kt * 32 + r;
+#pragma unroll
+        for (int st = 0; st < F::NST; ++st) {
+            const bf16x8 kf = *reinterpret_cast<const bf16x8 *>(
+                kl + (st / 4) * F::kHalfBytes + row * 128 + (((4 * h + st % 4) ^ kswz(row)) << 4));
+            if (st == 0) s[kt] = f32x16{};
+            s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st], s[kt], 0, 0, 0);
+        }
+    }
+}
+
+template <int DH>
+__device__ __forceinline__ void tile_pv(const char * vl, const typename Fast<DH>::Weights & p,
+                                        typename Fast<DH>::Out & oacc, int lane) {
+    using F = Fast<DH>;
+    const int G = lane >> 4, jl = lane & 15;
+    const int key_off = 4 * (G >> 1) + (jl >> 2), dim_off = 16 * (G & 1) + 4 * (jl & 3);
+#pragma unroll
+    for (int kt = 0; kt < F::KT; ++kt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int ka = kt * 32 + 16 * u + key_off, kb = ka + 8;
+#pragma unroll
+            for (int dt = 0; dt < F::NDT; ++dt) {
+                const int dbyte = ((dt % 2) * 32 + dim_off) * 2, piece = dbyte >> 4, within = dbyte & 15;
+                const char * vh = vl + (dt / 2) * F::kHalfBytes;
+                const char * pa = vh + ka * 128 + ((piece ^ vswz(ka)) << 4) + within;
+                const char * pb = vh + kb * 128 + ((piece ^ vswz(kb)) << 4) + within;
+                const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                               (v4i16 __attribute__((address_space(3))) *)(pa)));
+                const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                               (v4i16 __attribute__((address_space(3))) *)(pb)));
+                oacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    __builtin_bit_cast(bf16x8, make_uint4(lo.x, lo.y, hi.x, hi.y)), p[kt][u], oacc[dt], 0, 0, 0);
+            }
+        }
+}
+
+// Key of register e of sub-tile kt, and its part beyond 4 h.
+__device__ __forceinline__ constexpr int key_of(int kt, int e) { return kt * 32 + 8 * (e >> 2) + (e & 3); }
+
+// The running state of a lane's row: base (the maximum that weights are relative
+// to) and this lane's half of their sum.
+struct RowState {
+    float base, sum;
+};
+
+// Weights of a tile relative to state.base: p = 2^(z - base), and their sum over this lane.
+// behind: the lane's query position minus the tile's first key and 4 h.
+template <int DH, int MODE>
+__device__ __forceinline__ float tile_weights(const RowScore & rs, float cap_log2, const typename Fast<DH>::Scores & s,
+                                              typename Fast<DH>::Weights & p, float base, float behind) {
+    const bf16x2 ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+    const float add = MODE & kCap ? cap_log2 - base : -base;
+    float sum = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < Fast<DH>::KT; ++kt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const int i = 8 * u + e;
+                bf16x2 pp;
+                pp[0] = static_cast<__bf16>(__builtin_amdgcn_exp2f(
+                    score_of<MODE>(rs, s[kt][i], add, behind - static_cast<float>(key_of(kt, i)))));
+                pp[1] = static_cast<__bf16>(__builtin_amdgcn_exp2f(
+                    score_of<MODE>(rs, s[kt][i + 1], add, behind - static_cast<float>(key_of(kt, i + 1)))));
+                p[kt][u][e] = pp[0];
+                p[kt][u][e + 1] = pp[1];
+                sum = __builtin_amdgcn_fdot2_f32_bf16(pp, ones, sum, false);  // of the rounded weights
+            }
+    return sum;
+}
+
+// The largest z of a tile over the row's two lanes.
+template <int DH, int MODE>
+__device__ __forceinline__ float tile_max(const RowScore & rs, float cap_log2, const typename Fast<DH>::Scores & s,
+                                          float behind) {
+    const float add = MODE & kCap ? cap_log2 : 0.0f;
+    float top = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < Fast<DH>::KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            top = fmaxf(top, score_of<MODE>(rs, s[kt][e], add, behind - static_cast<float>(key_of(kt, e))));
+    return lane_pair_max(top);
+}
+
+// The exact step of a tile: hidden keys (at or past `seen` of the tile's keys, less 4 h)
+// get weight 0, the base rises to the maximum and the output with it.
+template <int DH, int MODE>
+__device__ __forceinline__ void tile_exact(const RowScore & rs, float cap_log2, typename Fast<DH>::Scores & s,
+                                           typename Fast<DH>::Weights & p, typename Fast<DH>::Out & oacc,
+                                           RowState & st, float behind, int seen) {
+    using F = Fast<DH>;
+    const float add = MODE & kCap ? cap_log2 : 0.0f;
+    float top = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < F::KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float z = score_of<MODE>(rs, s[kt][e], add, behind - static_cast<float>(key_of(kt, e)));
+            s[kt][e] = key_of(kt, e) < seen ? z : -INFINITY;
+            top = fmaxf(top, s[kt][e]);
+        }
+    const float up = fmaxf(st.base, lane_pair_max(top));
+    const float base = up == -INFINITY ? 0.0f : up;  // nothing seen yet: every weight is 0
+    const float keep = __builtin_amdgcn_exp2f(st.base - base);
+    const bf16x2 ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+    float sum = st.sum * keep;
+#pragma unroll
+    for (int kt = 0; kt < F::KT; ++kt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                bf16x2 pp;
+                pp[0] = static_cast<__bf16>(__builtin_amdgcn_exp2f(s[kt][8 * u + e] - base));
+                pp[1] = static_cast<__bf16>(__builtin_amdgcn_exp2f(s[kt][8 * u + e + 1] - base));
+                p[kt][u][e] = pp[0];
+                p[kt][u][e + 1] = pp[1];
+                sum = __builtin_amdgcn_fdot2_f32_bf16(pp, ones, sum, false);
+            }
+    st.sum = sum;
+    st.base = up;
+#pragma unroll
+    for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[dt][e] *= keep;
+}
+
+// A tile's 2 * kUnits DMA instructions, those of index first, first + step, ...: K then V units.
+template <int DH>
+struct TileSource {
+    const char * k;      // the segment's first key, this head
+    const char * v;
+    int64_t ldk, ldv;    // bytes
+    int nk;
+    uint64_t zero;
+};
+
+template <int DH, int COUNT>
+__device__ __forceinline__ void tile_offsets(const TileSource<DH> & src, int first, int lane, uint32_t (&off)[COUNT]) {
+    using F = Fast<DH>;
+    const int lrow = lane >> 3, lslot = lane & 7;
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+        const int unit = first + j;
+        const bool is_v = unit >= F::kUnits;
+        const int half = unit % F::kUnits / (F::kKeys / 8), row = unit % (F::kKeys / 8) * 8 + lrow;
+        off[j] = static_cast<uint32_t>(row * (is_v ? src.ldv : src.ldk) + half * 128 +
+                                       (lslot ^ (is_v ? vswz(row) : kswz(row))) * 16);
+    }
+}
+
+// Units first .. first + COUNT - 1 of tile t into the slot at LDS offset `lds` (K, then V).
+template <int DH, int COUNT>
+__device__ __forceinline__ void tile_issue(const TileSource<DH> & src, int t, int first, const uint32_t (&off)[COUNT],
+                                           uint32_t lds, int lane) {
+    using F = Fast<DH>;
+    const int kt0 = t * F::kKeys;
+    const char * kb = src.k + static_cast<int64_t>(kt0) * src.ldk;
+    const char * vb = src.v + static_cast<int64_t>(kt0) * src.ldv;
+    const bool whole = kt0 + F::kKeys <= src.nk;
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+        const int unit = first + j;
+        const bool is_v = unit >= F::kUnits;
+        const uint32_t at = lds + unit * 1024;
+        if (whole) {
+            lds_dma16_sbase(is_v ? vb : kb, off[j], at);
+        } else {
+            const int row = unit % (F::kKeys / 8) * 8 + (lane >> 3);
+            const char * g = kt0 + row < src.nk ? (is_v ? vb : kb) + off[j] : reinterpret_cast<const char *>(src.zero);
+            lds_dma16(g, at);
+        }
+    }
+}
+
+// Whether this thread's share of a V tile (of `threads` threads) holds an infinity or a NaN.
+template <int DH>
+__device__ __forceinline__ bool tile_odd(const char * vl, int thread, int threads) {
+    bool odd = false;
+    for (int i = thread; i < Fast<DH>::kTileBytes / 16; i += threads) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(vl + i * 16);
+        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            odd |= (x[e] & 0x7F800000u) == 0x7F800000u || (x[e] & 0x7F80u) == 0x7F80u;
+    }
+    return odd;
+}
+
+template <int DH>
+__device__ __forceinline__ void load_q(const ScoreArgs & a, const Rows & w, int qi, int head, bool live, int h,
+                                       bf16x8 (&qf)[Fast<DH>::NST]) {
+    const uint16_t * q = static_cast<const uint16_t *>(a.q) + (w.q0 + qi) * a.ldq + static_cast<int64_t>(head) * DH;
+#pragma unroll
+    for (int st = 0; st < Fast<DH>::NST; ++st) {
+        uint4 u = make_uint4(0u, 0u, 0u, 0u);
+        if (live) u = *reinterpret_cast<const uint4 *>(q + (st / 4) * 64 + 32 * h + 8 * (st % 4));
+        qf[st] = __builtin_bit_cast(bf16x8, u);
+    }
+}
+
+template <int DH>
+__device__ __forceinline__ TileSource<DH> tile_source(const ScoreArgs & a, const Rows & w) {
+    TileSource<DH> s;
+    s.k = uniform_ptr(reinterpret_cast<const char *>(static_cast<const uint16_t *>(a.k) + w.k0 * a.ldk + static_cast<int64_t>(w.kv) * DH));
+    s.v = uniform_ptr(reinterpret_cast<const char *>(static_cast<const uint16_t *>(a.v) + w.k0 * a.ldv + static_cast<int64_t>(w.kv) * DH));
+    s.ldk = a.ldk * 2;
+    s.ldv = a.ldv * 2;
+    s.nk = static_cast<int>(w.nk);
+    s.zero = reinterpret_cast<uint64_t>(&g_score_zero[0]);
+    asm volatile("" : "+s"(s.zero));
+    return s;
+}
+
+// Many rows a segment: four waves of 32 rows share the key tiles, a ring of four
+// slots of K and V.  The keys are walked from the last that is seen to the first:
+// the tiles with hidden keys come first, each an exact step (maximum, weights, product),
+// then one exact step on whole keys, after which every row has a base that one of its
+// own scores set.  From there on tile j's step issues the products that do not depend on
+// its weights, O += V P of the tile before and S of the next, and takes its weights while
+// they run, without a maximum: a row's weights are redone with one where their sum passes
+// 2^40 (bf16 and fp32 hold 2^127).  With a bias that falls with the distance the nearest
+// keys come first, so that is rare.
+constexpr int kSlots = 4;
+constexpr float kSumLimit = 0x1p40f;
+
+template <int DH, int MODE>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) score_attn_rows_kernel(ScoreArgs a) {
+    using F = Fast<DH>;
+    constexpr int kMine = 2 * F::kUnits / 4;  // DMA instructions of a wave and tile
+    __shared__ __align__(16) char lds[kSlots * 2 * F::kTileBytes];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, r = lane & 31;
+    const int64_t t = a.tiles - 1 - blockIdx.x % a.tiles;
+    const int rest = static_cast<int>(blockIdx.x / a.tiles);
+    const int split = rest % a.splits;
+    Rows w;
+    w.kv = rest / a.splits;
+    if (!locate_rows(a, t, 128, lane, w)) return;
+    const int end = static_cast<int>(keys_end(a, w, w.row0 + 127));
+    const int all = (end + F::kKeys - 1) / F::kKeys;
+    const int first = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
+    const int last = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits) - 1;
+    const int n = last - first + 1;  // tiles, walked from `last` down: step i is tile last - i
+
+    const int64_t wave_row0 = w.row0 + wave * 32;
+    const bool live = wave_row0 + r < w.rows;
+    const int64_t row = live ? wave_row0 + r : w.rows - 1;
+    const int qi = static_cast<int>(row / a.group);
+    const int head = w.kv * a.group + static_cast<int>(row % a.group);
+    const RowScore rs = row_score<MODE>(a, head);
+    const float cap_log2 = a.cap_log2;
+    bf16x8 qf[F::NST];
+    load_q<DH>(a, w, qi, head, live, h, qf);
+    const int seen = static_cast<int>(keys_end(a, w, row)) - 4 * h;
+    const int pos = qi + static_cast<int>(w.shift) - 4 * h;
+    const int whole = static_cast<int>(keys_all(a, w, w.row0)) / F::kKeys;  // tiles below hold seen keys only
+    const int wave_end = wave_row0 < w.rows ? static_cast<int>(keys_end(a, w, wave_row0 + 31)) : 0;
+
+    const TileSource<DH> src = tile_source<DH>(a, w);
+    uint32_t off[kMine];
+    tile_offsets<DH>(src, wave * kMine, lane, off);
+    const uint32_t lds0 = lds_offset(&lds[0]);
+    auto slot = [](int i) { return (i % kSlots) * 2 * F::kTileBytes; };
+    auto issue = [&](int i) __attribute__((always_inline)) {
+        tile_issue<DH>(src, last - i, wave * kMine, off, lds0 + slot(i), lane);
+    };
+    auto k_of = [&](int i) { return lds + slot(i); };
+    auto v_of = [&](int i) { return lds + slot(i) + F::kTileBytes; };
+    auto behind = [&](int i) { return static_cast<float>(pos - (last - i) * F::kKeys); };
+
+    typename F::Out oacc;
+#pragma unroll
+    for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
+    RowState st{-INFINITY, 0.0f};
+    bool odd = false;
+    // Exact steps: tiles with hidden keys, and one of whole keys.
+    const int exact = min(n, max(last + 1 - whole, 0) + 1);
+    if (n > 0) issue(0);
+    if (n > 1) issue(1);
+    typename F::Scores s_a, s_b;
+    typename F::Weights p;
+    int i = 0;
+    for (; i < exact; ++i) {
+        if (i + 1 < n) wait_vmcnt(kMine);
+        else wait_vmcnt(0);
+        barrier_no_fence();
+        if (i + 2 < n) issue(i + 2);
+        const int tile = last - i;
+        if (tile >= whole) odd |= tile_odd<DH>(v_of(i), tid, 256);
+        if (tile * F::kKeys < wave_end) {
+            tile_qk<DH>(k_of(i), qf, s_a, h, r);
+            tile_exact<DH, MODE>(rs, cap_log2, s_a, p, oacc, st, behind(i), seen - tile * F::kKeys);
+            tile_pv<DH>(v_of(i), p, oacc, lane);
+        }
+    }
+    if (i < n) {
+        // Steps exact .. n - 1, one tile's products behind its weights.  Slot use: step i
+        // reads V of i - 1 and K of i + 1 while i + 2 lands.
+        auto weights = [&](int i, typename F::Scores & s) __attribute__((always_inline)) {
+            float sum = tile_weights<DH, MODE>(rs, cap_log2, s, p, st.base, behind(i));
+            if (__builtin_expect(__ballot(!(sum <= kSumLimit)) != 0, 0)) {
+                const float top = fmaxf(st.base, tile_max<DH, MODE>(rs, cap_log2, s, behind(i)));
+                const float up = top == -INFINITY ? 0.0f : top;  // scores of minus infinity, or NaN, only
+                const float keep = __builtin_amdgcn_exp2f(st.base - up);
+                st.base = up;
+                st.sum *= keep;
+#pragma unroll
+                for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) oacc[dt][e] *= keep;
+                sum = tile_weights<DH, MODE>(rs, cap_log2, s, p, st.base, behind(i));
+            }
+            st.sum += sum;
+        };
+        if (i + 1 < n) wait_vmcnt(kMine);
+        else wait_vmcnt(0);
+        barrier_no_fence();
+        tile_qk<DH>(k_of(i), qf, s_a, h, r);
+        // The first: no product before it.
+        if (i + 1 < n) {
+            wait_vmcnt(0);
+            barrier_no_fence();
+            if (i + 2 < n) issue(i + 2);
+            tile_qk<DH>(k_of(i + 1), qf, s_b, h, r);
+        }
+        weights(i, s_a);
+        ++i;
+        auto step = [&](typename F::Scores & now, typename F::Scores & next) __attribute__((always_inline)) {
+            wait_vmcnt(0);
+            barrier_no_fence();
+            if (i + 2 < n) issue(i + 2);
+            tile_pv<DH>(v_of(i - 1), p, oacc, lane);
+            tile_qk<DH>(k_of(i + 1), qf, next, h, r);
+            weights(i, now);
+            ++i;
+        };
+        while (i + 2 < n) {
+            step(s_b, s_a);
+            step(s_a, s_b);
+        }
+        if (i + 1 < n) {
+            step(s_b, s_a);
+#pragma unroll
+            for (int kt = 0; kt < F::KT; ++kt) s_b[kt] = s_a[kt];
+        }
+        tile_pv<DH>(v_of(i - 1), p, oacc, lane);
+        if (i < n) {
+            weights(i, s_b);
+            tile_pv<DH>(v_of(i), p, oacc, lane);
+        }
+    }
+    if (__syncthreads_or(odd)) {
+        for (int j = 0; j < 32; ++j)
+            if (wave_row0 + j < w.rows)
+                row_alone<uint16_t, DH / 64>(a, w, wave_row0 + j, static_cast<int64_t>(first) * F::kKeys,
+                                             static_cast<int64_t>(last + 1) * F::kKeys, lane, a.splits > 1,
+                                             split_slot(a, w, split, wave_row0 + j));
+        return;
+    }
+    const float sum = lane_pair_sum(st.sum);
+    if (!live) return;
+    const int64_t part = split_slot(a, w, split, row);
+    if (a.splits > 1) {
+        if (h == 0) a.part_ml[part] = make_float2(st.base, sum);
+        float * o = a.part + part * DH;
+#pragma unroll
+        for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<float4 *>(o + dt * 32 + 8 * g + 4 * h) =
+                    make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
+        return;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t * o = static_cast<uint16_t *>(a.o) + (w.q0 + qi) * a.ldo + static_cast<int64_t>(head) * DH;
+#pragma unroll
+    for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint2 *>(o + dt * 32 + 8 * g + 4 * h) =
+                make_uint2(pack_bf16x2(oacc[dt][4 * g] * inv, oacc[dt][4 * g + 1] * inv),
+                           pack_bf16x2(oacc[dt][4 * g + 2] * inv, oacc[dt][4 * g + 3] * inv));
+}
+
+// Few rows a segment (new tokens over caches): a workgroup has one tile of 32 rows
+// and a chunk of the segment's keys, its four waves every fourth key tile of it, each
+// through a ring of its own in LDS, with no barrier before the end, where the waves'
+// results are joined.  Bound by reading the keys and values once.
+//
+// Segments of up to 32 rows are cut into chunks of a.chunk keys, an item each; so long
+// and short caches of one call load the CUs alike.  Others have an item per 32 rows.
+constexpr int kFewRows = 32;
+
+template <int DH> constexpr int kFewStages = 2;
+template <int DH> constexpr int kFewWaveBytes = kFewStages<DH> * 2 * Fast<DH>::kTileBytes;
+template <int DH> constexpr int kFewBytes = 4 * kFewWaveBytes<DH> + 4 * 32 * 2 * static_cast<int>(sizeof(float));
+
+// A wave's own LDS reads are done, and none is moved over this.
+__device__ __forceinline__ void wave_reads_done() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
+
+template <int DH, int MODE>
+__global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
+    using F = Fast<DH>;
+    constexpr int kInstr = 2 * F::kUnits;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, r = lane & 31;
+    Rows w;
+    w.kv = static_cast<int>(blockIdx.x % a.kv_heads);
+    const int64_t item = blockIdx.x / a.kv_heads;
+    if (!locate_rows(a, item, kFewRows, lane, w)) return;
+    const bool live = w.row0 + r < w.rows;
+    const int64_t row = live ? w.row0 + r : w.rows - 1;
+    const int qi = static_cast<int>(row / a.group);
+    const int head = w.kv * a.group + static_cast<int>(row % a.group);
+    int first = 0, last = (static_cast<int>(keys_end(a, w, w.row0 + kFewRows - 1)) + F::kKeys - 1) / F::kKeys;
+    if (w.chunks > 1) {
+        first = w.chunk * (a.chunk / F::kKeys);
+        last = min(last, first + a.chunk / F::kKeys);
+    }
+    const RowScore rs = row_score<MODE>(a, head);
+    const float cap_log2 = a.cap_log2;
+    const TileSource<DH> src = tile_source<DH>(a, w);
+    char * ring = smem + wave * kFewWaveBytes<DH>;
+    const uint32_t lds0 = lds_offset(ring);
+    uint32_t off[kInstr];
+    tile_offsets<DH>(src, 0, lane, off);
+    const int n = last - first > wave ? (last - first - wave + 3) / 4 : 0;  // tiles first + wave + 4 i
+    auto tile = [&](int i) { return first + wave + 4 * i; };
+    auto slot = [](int i) { return i % kFewStages<DH> * 2 * F::kTileBytes; };
+    auto issue = [&](int i) __attribute__((always_inline)) {
+        tile_issue<DH>(src, tile(i), 0, off, lds0 + slot(i), lane);
+    };
+    if (n > 0) issue(0);
+    bf16x8 qf[F::NST];
+    load_q<DH>(a, w, qi, head, live, h, qf);
+    const int seen = static_cast<int>(keys_end(a, w, row)) - 4 * h;
+    const int pos = qi + static_cast<int>(w.shift) - 4 * h;
+    const int whole = static_cast<int>(keys_all(a, w, w.row0)) / F::kKeys;
+    typename F::Out oacc;
+#pragma unroll
+    for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
+    RowState st{-INFINITY, 0.0f};
+    bool odd = false;
+    if (n > 1) issue(1);
+    for (int i = 0; i < n; ++i) {
+        if (i + 1 < n) wait_vmcnt(kInstr);
+        else wait_vmcnt(0);
+        asm volatile("" ::: "memory");
+        const char * kl = ring + slot(i);
+        const char * vl = kl + F::kTileBytes;
+        if (tile(i) >= whole) odd |= tile_odd<DH>(vl, lane, 64);
+        typename F::Scores s;
+        typename F::Weights p;
+        tile_qk<DH>(kl, qf, s, h, r);
+        tile_exact<DH, MODE>(rs, cap_log2, s, p, oacc, st, static_cast<float>(pos - tile(i) * F::kKeys),
+                             seen - tile(i) * F::kKeys);
+        tile_pv<DH>(vl, p, oacc, lane);
+        wave_reads_done();
+        if (i + 2 < n) issue(i + 2);
+    }
+    const int64_t part = (item * a.kv_heads + w.kv) * kFewRows;  // this item's rows of partial results
+    if (__syncthreads_or(odd)) {
+        for (int j = wave; j < kFewRows; j += 4)
+            if (w.row0 + j < w.rows)
+                row_alone<uint16_t, DH / 64>(a, w, w.row0 + j, static_cast<int64_t>(first) * F::kKeys,
+                                             static_cast<int64_t>(last) * F::kKeys, lane, w.chunks > 1, part + j);
+        return;
+    }
+    // The waves' results: outputs in their own rings, bases and sums behind the rings.
+    float * mine = reinterpret_cast<float *>(ring);
+    float2 * ml = reinterpret_cast<float2 *>(smem + 4 * kFewWaveBytes<DH>);
+    const float sum = lane_pair_sum(st.sum);
+    if (h == 0) ml[wave * 32 + r] = make_float2(st.base, sum);
+#pragma unroll
+    for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float4 *>(mine + r * DH + dt * 32 + 8 * g + 4 * h) =
+                make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
+    __syncthreads();
+    const int jr = tid >> 3, jc = tid & 7;  // 8 threads a row
+    if (w.row0 + jr >= w.rows) return;
+    float base = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) base = fmaxf(base, ml[i * 32 + jr].x);
+    const float ref = base == -INFINITY ? 0.0f : base;
+    float total = 0.0f, f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = ml[i * 32 + jr];
+        f[i] = __builtin_amdgcn_exp2f(v.x - ref);
+        total += v.y * f[i];
+    }
+    const int token = static_cast<int>((w.row0 + jr) / a.group);
+    const int to_head = w.kv * a.group + static_cast<int>((w.row0 + jr) % a.group);
+    uint16_t * o = static_cast<uint16_t *>(a.o) + (w.q0 + token) * a.ldo + static_cast<int64_t>(to_head) * DH;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    if (w.chunks > 1 && jc == 0) a.part_ml[part + jr] = make_float2(base, total);
+#pragma unroll
+    for (int c = jc * 4; c < DH; c += 32) {
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem + i * kFewWaveBytes<DH>) + jr * DH + c);
+            v[0] += x.x * f[i]; v[1] += x.y * f[i]; v[2] += x.z * f[i]; v[3] += x.w * f[i];
+        }
+        if (w.chunks > 1)
+            *reinterpret_cast<float4 *>(a.part + (part + jr) * DH + c) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            *reinterpret_cast<uint2 *>(o + c) = make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+    }
+}
+
+// Joins the chunks of a (query, head): four waves, each every fourth chunk, then their
+// results in order.
+template <int DH>
+__global__ void __launch_bounds__(256) score_join_few_kernel(ScoreArgs a) {
+    constexpr int V = DH / 64;
+    __shared__ float2 ml[4];
+    __shared__ float acc_of[4][DH];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t qi = blockIdx.x / a.heads;
+    const int head = static_cast<int>(blockIdx.x % a.heads);
+    Rows w;
+    w.kv = head / a.group;
+    int64_t item;
+    if (!locate_query(a, qi, kFewRows, lane, w, item) || w.chunks <= 1) return;
+    const int64_t row = (qi - w.q0) * a.group + head % a.group;
+    const int64_t at = (item * a.kv_heads + w.kv) * kFewRows + row;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * kFewRows;
+    float m = -INFINITY, l = 0.0f, acc[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) acc[c] = 0.0f;
+#pragma unroll 8
+    for (int i = wave; i < w.chunks; i += 4) {
+        const float2 p = a.part_ml[at + i * step];
+        const float * o = a.part + (at + i * step) * DH + lane * V;
+        const float up = fmaxf(m, p.x), ref = up == -INFINITY ? 0.0f : up;
+        const float keep = __builtin_amdgcn_exp2f(m - ref), f = __builtin_amdgcn_exp2f(p.x - ref);
+        l = l * keep + p.y * f;
+#pragma unroll
+        for (int c = 0; c < V; ++c) acc[c] = acc[c] * keep + o[c] * f;
+        m = up;
+    }
+    if (lane == 0) ml[wave] = make_float2(m, l);
+#pragma unroll
+    for (int c = 0; c < V; ++c) acc_of[wave][lane * V + c] = acc[c];
+    __syncthreads();
+    if (wave != 0) return;
+    float base = -INFINITY, total = 0.0f, v[V];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) base = fmaxf(base, ml[i].x);
+    const float ref = base == -INFINITY ? 0.0f : base;
+#pragma unroll
+    for (int c = 0; c < V; ++c) v[c] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = __builtin_amdgcn_exp2f(ml[i].x - ref);
+        total += ml[i].y * f;
+#pragma unroll
+        for (int c = 0; c < V; ++c) v[c] += acc_of[i][lane * V + c] * f;
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    uint16_t * o = static_cast<uint16_t *>(a.o) + qi * a.ldo + static_cast<int64_t>(head) * DH + lane * V;
+#pragma unroll
+    for (int c = 0; c < V; ++c) o[c] = f32_to_bf16(v[c] * inv);
 }
 
 // Joins the splits of a row: one wave per (query, head), in the splits' order.
@@ -409,15 +1091,18 @@ __global__ void __launch_bounds__(256) score_join_kernel(ScoreArgs a) {
         if (lane + 64 * c < a.d) store_f32(o + lane + 64 * c, acc[c] * inv);
 }
 
-// tile_start[s] = row tiles of the segments before s, for more segments than a wave's lanes.
-__global__ void __launch_bounds__(1024) score_tiles_kernel(const int64_t * __restrict__ cu_q, int nseg, int group,
-                                                           int rows_per_tile, int64_t * __restrict__ tile_start) {
+// tile_start[s] = items of the segments before s, for more segments than a wave's lanes.
+__global__ void __launch_bounds__(1024) score_tiles_kernel(const int64_t * __restrict__ cu_q,
+                                                           const int64_t * __restrict__ cu_k, int nseg, int group,
+                                                           int rows_per_tile, int chunk,
+                                                           int64_t * __restrict__ tile_start) {
     __shared__ int64_t waves[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int64_t before = 0;
     for (int s0 = 0; s0 < nseg; s0 += 1024) {
         const int s = s0 + tid;
-        const int64_t tiles = s < nseg ? ((cu_q[s + 1] - cu_q[s]) * group + rows_per_tile - 1) / rows_per_tile : 0;
+        int64_t tiles = 0;
+        if (s < nseg) tiles = segment_items(cu_q[s + 1] - cu_q[s], cu_k[s + 1] - cu_k[s], group, rows_per_tile, chunk);
         int64_t sum = tiles;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -465,6 +1150,23 @@ int64_t split_rows(int64_t total_q, int64_t total_k, int heads) {
     return std::min(kSplitGrid * kRowTile, total_q > kSplitGrid * kRowTile ? kSplitGrid * kRowTile : total_q * heads * most);
 }
 
+// Few rows a segment: keys of a chunk, so that a call has about kFewItems of them.
+constexpr int64_t kFewItems = 1024;
+constexpr int64_t kFewKeys = 256;  // at least, and a multiple of
+int64_t few_chunk(int64_t total_k, int kv_heads) {
+    const int64_t keys = (total_k * kv_heads + kFewItems - 1) / kFewItems;
+    return std::max<int64_t>(1, (keys + kFewKeys - 1) / kFewKeys) * kFewKeys;
+}
+bool few_rows(int64_t total_q, int nseg, int group) { return total_q * group <= static_cast<int64_t>(kFewRows) * nseg; }
+int64_t few_items(int64_t total_q, int64_t total_k, int nseg, int kv_heads, int group) {
+    return total_q * group / kFewRows + total_k / few_chunk(total_k, kv_heads) + nseg + 1;
+}
+// Rows of partial results of any such call of up to these sizes: its queries' rows fill at
+// most nseg tiles, and total_k / chunk is at most both total_k / kFewKeys and kFewItems / kv_heads.
+int64_t few_part_rows(int64_t total_k, int nseg, int kv_heads) {
+    return ((2 * static_cast<int64_t>(nseg) + 1) * kv_heads + std::min(total_k / kFewKeys * kv_heads, kFewItems)) * kFewRows;
+}
+
 template <typename T, int DP>
 int launch_any(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
     constexpr int smem = AnyTile<T, DP>::kBytes;
@@ -479,13 +1181,43 @@ int launch_any(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
 }
 
 template <typename T>
-int run_scores(ScoreArgs a, int64_t blocks, hipStream_t s) {
-    int rc;
-    if (a.d <= 64) rc = launch_any<T, 64>(a, blocks, s);
-    else if (a.d <= 128) rc = launch_any<T, 128>(a, blocks, s);
-    else rc = launch_any<T, 256>(a, blocks, s);
-    if (rc || a.splits == 1) return rc;
-    hipLaunchKernelGGL(score_join_kernel<T>, dim3(grid_for(a.total_q * a.heads, 4)), dim3(256), 0, s, a);
+int run_any(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
+    if (a.d <= 64) return launch_any<T, 64>(a, blocks, s);
+    if (a.d <= 128) return launch_any<T, 128>(a, blocks, s);
+    return launch_any<T, 256>(a, blocks, s);
+}
+
+// kernel<mode of the call>
+template <typename F> int with_mode(const ScoreArgs & a, F && launch) {
+    if (a.cap_log2 > 0.0f) {
+        if (a.slopes) return launch(std::integral_constant<int, kCap | kBias>{});
+        return launch(std::integral_constant<int, kCap>{});
+    }
+    if (a.slopes) return launch(std::integral_constant<int, kBias>{});
+    return launch(std::integral_constant<int, 0>{});
+}
+
+template <int DH>
+int run_rows(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
+    return with_mode(a, [&](auto mode) {
+        hipLaunchKernelGGL((score_attn_rows_kernel<DH, decltype(mode)::value>), dim3(static_cast<unsigned>(blocks)),
+                           dim3(256), 0, s, a);
+        return check_launch("scored attention");
+    });
+}
+
+template <int DH>
+int run_few(const ScoreArgs & a, int64_t blocks, bool join, hipStream_t s) {
+    const int rc = with_mode(a, [&](auto mode) {
+        auto kernel = &score_attn_few_kernel<DH, decltype(mode)::value>;
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, kFewBytes<DH>);
+        if (e != hipSuccess) return check_hip(e, "hipFuncSetAttribute(score_attn_few)");
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), kFewBytes<DH>, s, a);
+        return check_launch("scored attention of few rows");
+    });
+    if (rc || !join) return rc;
+    hipLaunchKernelGGL(score_join_few_kernel<DH>, dim3(static_cast<unsigned>(a.total_q * a.heads)), dim3(256), 0, s, a);
     return check_launch("scored attention join");
 }
 
@@ -502,9 +1234,9 @@ extern "C" {
 
 size_t pxs_attention_scores_workspace_bytes(int nseg, int64_t total_q, int64_t total_k, int heads, int kv_heads,
                                             int head_dim) {
-    (void)kv_heads;
-    if (nseg <= 0 || total_q <= 0 || heads <= 0 || head_dim <= 0) return 256;
-    const size_t rows = static_cast<size_t>(split_rows(total_q, std::max<int64_t>(total_k, 0), heads));
+    if (nseg <= 0 || total_q <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 256;
+    total_k = std::max<int64_t>(total_k, 0);
+    const size_t rows = static_cast<size_t>(std::max(split_rows(total_q, total_k, heads), few_part_rows(total_k, nseg, kv_heads)));
     return round256((static_cast<size_t>(nseg) + 1) * sizeof(int64_t)) + round256(rows * sizeof(float2)) +
            round256(rows * head_dim * sizeof(float));
 }
@@ -547,24 +1279,47 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
     const int elem = dtype == PXS_BF16 ? 2 : 4;
     a.vec = rows_of_pieces(q, ld_q, head_dim, elem) && rows_of_pieces(k, ld_k, head_dim, elem) &&
             rows_of_pieces(v, ld_v, head_dim, elem);
-    a.tiles = row_tiles(total_q, nseg, a.group);
-    a.splits = score_splits(nseg, total_q, total_k, kv_heads, a.group);
-    const int64_t blocks = a.tiles * kv_heads * a.splits;
-    PXS_CHECK(blocks <= UINT32_MAX / 256, PXS_ERR_ARG, "attention grid too large");
+    // The fast kernels' 32-bit offsets within a key tile hold row strides below 2^24.
+    const bool fast = dtype == PXS_BF16 && (head_dim == 64 || head_dim == 128) && a.vec && ld_k < (1 << 24) &&
+                      ld_v < (1 << 24) && reinterpret_cast<uintptr_t>(o) % 8 == 0 && ld_o % 4 == 0;
+    const bool few = fast && few_rows(total_q, nseg, a.group);
+    a.splits = 1;
+    int64_t blocks, part_rows = 0;
+    if (few) {
+        a.chunk = static_cast<int>(few_chunk(total_k, kv_heads));
+        a.tiles = few_items(total_q, total_k, nseg, kv_heads, a.group);
+        blocks = a.tiles * kv_heads;
+        part_rows = blocks * kFewRows;
+    } else {
+        a.tiles = row_tiles(total_q, nseg, a.group);
+        a.splits = score_splits(nseg, total_q, total_k, kv_heads, a.group);
+        blocks = a.tiles * kv_heads * a.splits;
+        if (a.splits > 1) part_rows = a.splits * total_q * heads;
+    }
+    PXS_CHECK(blocks <= UINT32_MAX / 256 && (!few || total_q * heads <= UINT32_MAX / 256), PXS_ERR_ARG,
+              "attention grid too large");
     char * ws = static_cast<char *>(workspace);
     if (nseg > kWaveSegments) {
         a.tile_start = reinterpret_cast<int64_t *>(ws);
-        hipLaunchKernelGGL(score_tiles_kernel, dim3(1), dim3(1024), 0, s, cu_q, nseg, a.group, kRowTile,
-                           reinterpret_cast<int64_t *>(ws));
+        hipLaunchKernelGGL(score_tiles_kernel, dim3(1), dim3(1024), 0, s, cu_q, cu_k, nseg, a.group,
+                           few ? kFewRows : kRowTile, a.chunk, reinterpret_cast<int64_t *>(ws));
         if (int rc = check_launch("scored attention tiles")) return rc;
     }
-    if (a.splits > 1) {
-        const size_t rows = static_cast<size_t>(a.splits) * total_q * heads;
-        ws += round256((static_cast<size_t>(nseg) + 1) * sizeof(int64_t));
-        a.part_ml = reinterpret_cast<float2 *>(ws);
-        a.part = reinterpret_cast<float *>(ws + round256(rows * sizeof(float2)));
+    ws += round256((static_cast<size_t>(nseg) + 1) * sizeof(int64_t));
+    a.part_ml = reinterpret_cast<float2 *>(ws);
+    a.part = reinterpret_cast<float *>(ws + round256(static_cast<size_t>(part_rows) * sizeof(float2)));
+    if (few) {
+        const bool join = total_k > a.chunk;  // otherwise no segment is cut
+        return head_dim == 64 ? run_few<64>(a, blocks, join, s) : run_few<128>(a, blocks, join, s);
     }
-    return dtype == PXS_F32 ? run_scores<float>(a, blocks, s) : run_scores<uint16_t>(a, blocks, s);
+    int rc;
+    if (fast) rc = head_dim == 64 ? run_rows<64>(a, blocks, s) : run_rows<128>(a, blocks, s);
+    else rc = dtype == PXS_F32 ? run_any<float>(a, blocks, s) : run_any<uint16_t>(a, blocks, s);
+    if (rc || a.splits == 1) return rc;
+    const dim3 grid(grid_for(total_q * heads, 4));
+    if (dtype == PXS_F32) hipLaunchKernelGGL(score_join_kernel<float>, grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(score_join_kernel<uint16_t>, grid, dim3(256), 0, s, a);
+    return check_launch("scored attention join");
 }
 
 } // extern "C"
