@@ -1172,9 +1172,8 @@ int launch_any(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
     constexpr int smem = AnyTile<T, DP>::kBytes;
     auto kernel = &score_attn_any_kernel<T, DP>;
     if constexpr (smem > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != hipSuccess) return check_hip(e, "hipFuncSetAttribute(score_attn)");
+        static std::atomic<uint64_t> done{0};
+        if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), smem, done, "hipFuncSetAttribute(score_attn)")) return rc;
     }
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), smem, s, a);
     return check_launch("scored attention");
@@ -1210,9 +1209,8 @@ template <int DH>
 int run_few(const ScoreArgs & a, int64_t blocks, bool join, hipStream_t s) {
     const int rc = with_mode(a, [&](auto mode) {
         auto kernel = &score_attn_few_kernel<DH, decltype(mode)::value>;
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, kFewBytes<DH>);
-        if (e != hipSuccess) return check_hip(e, "hipFuncSetAttribute(score_attn_few)");
+        static std::atomic<uint64_t> done{0};
+        if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), kFewBytes<DH>, done, "hipFuncSetAttribute(score_attn_few)")) return rc;
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), kFewBytes<DH>, s, a);
         return check_launch("scored attention of few rows");
     });

@@ -712,9 +712,8 @@ int launch_i8_tiles(I8Args a, hipStream_t s) {
     if (int rc = check_i8_grid(blocks, NW * KG * 64)) return rc;
     auto kernel = &linear_i8_kernel<T, BM, BN, NW, WAVES_M, NSTAGE, KG, EPI>;
     if constexpr (smem > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != hipSuccess) return check_hip(e, "hipFuncSetAttribute(linear_i8)");
+        static std::atomic<uint64_t> done{0};
+        if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), smem, done, "hipFuncSetAttribute(linear_i8)")) return rc;
     }
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(NW * KG * 64), smem, s, a);
     return check_launch("8-bit linear");
@@ -727,9 +726,8 @@ int launch_i8_any(const I8Args & a, hipStream_t s) {
     if (int rc = check_i8_grid(blocks, NW * 64)) return rc;
     auto kernel = &linear_i8_any_kernel<T, BM, BN, NW, WAVES_M, EPI>;
     if constexpr (smem > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != hipSuccess) return check_hip(e, "hipFuncSetAttribute(linear_i8_any)");
+        static std::atomic<uint64_t> done{0};
+        if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), smem, done, "hipFuncSetAttribute(linear_i8_any)")) return rc;
     }
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(NW * 64), smem, s, a);
     return check_launch("8-bit linear");

@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <string>
@@ -156,6 +157,19 @@ int child_conv(const void * x, int64_t n, int channels, const void * weight, con
         if (reinterpret_cast<uintptr_t>(ws) % 256 != 0)                 \
             return ::pxs::fail_workspace(what);                         \
     } while (0)
+
+// Lets `kernel` use `bytes` of dynamic LDS (above 64 KB) on the current device, asked for once
+// per device: `done`, one word per kernel, has a bit for each of the first 64.
+inline int allow_lds(const void * kernel, int bytes, std::atomic<uint64_t> & done, const char * what) {
+    int dev = 0;
+    if (hipError_t e = hipGetDevice(&dev)) return check_hip(e, what);
+    const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return PXS_OK;
+    if (hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes))
+        return check_hip(e, what);
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return PXS_OK;
+}
 
 inline hipStream_t as_stream(void * s) { return static_cast<hipStream_t>(s); }
 

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from functools import lru_cache
 from pathlib import Path
 
 import numpy as np
@@ -273,6 +274,7 @@ class DecoderHParams(C.Structure):
                 ("num_blocks", C.c_int * PXS_DECODER_MAX_LEVELS)]
 
 
+@lru_cache(maxsize=None)
 def load_library(path: Path = LIB_PATH) -> C.CDLL:
     if not Path(path).exists():
         raise PxsError(f"{path} is not built (run __graft_entry__.build())")
@@ -286,15 +288,16 @@ def load_library(path: Path = LIB_PATH) -> C.CDLL:
 
 def _ptr(t):
     """A device pointer argument: a tensor, a raw address (int) or None."""
-    if t is None:
-        return None
-    return C.c_void_p(t if isinstance(t, int) else t.data_ptr())
+    return t if t is None or isinstance(t, int) else t.data_ptr()
 
 
-def _unit_stride(t, what):
-    """t must be [rows, columns] with columns next to one another and rows that do not overlap."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        raise PxsError(f"{what} must be rows of contiguous columns")
+def _unit_stride(t, what, dev):
+    """t must be [rows, columns] on device `dev`, columns next to one another, rows that do not overlap."""
+    if t.dim() == 2 and t.get_device() == dev:
+        (rows, columns), (row_stride, column_stride) = t.shape, t.stride()
+        if (column_stride == 1 or columns <= 1) and (row_stride >= columns or rows <= 1):
+            return
+    raise PxsError(f"{what} must be rows of contiguous columns on the current device")
 
 
 def _ld(t):
@@ -302,9 +305,13 @@ def _ld(t):
     return max(t.stride(0), t.shape[1])
 
 
-def _expect(t, dtype, shape, what):
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-        raise PxsError(f"{what} must be contiguous {dtype} {list(shape)}")
+def _expect(t, dtype, shape, what, dev):
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
+        raise PxsError(f"{what} must be contiguous {dtype} {list(shape)} on the current device")
+
+
+# torch's own accessor of the current stream's handle: building a Stream object takes 3 us.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -325,7 +332,9 @@ class Pxs:
     # -- plumbing ---------------------------------------------------------------
     @staticmethod
     def stream():
-        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        if _raw_stream is None:
+            return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(torch.cuda.current_device())
 
     def _check(self, rc: int, what: str):
         if rc != 0:
@@ -705,43 +714,49 @@ class Pxs:
     def quantize_rows(self, x, out=None, scales=None):
         """pxs_quantize_rows_i8 -> (int8 [rows, channels], fp32 scales [rows]); x may be a
         column slice (rows of any stride)."""
+        dev = torch.cuda.current_device()
+        _unit_stride(x, "quantize_rows: x", dev)
         rows, channels = x.shape
-        _unit_stride(x, "quantize_rows: x")
         q = torch.empty((rows, channels), dtype=torch.int8, device=x.device) if out is None else out
         scales = torch.empty(rows, dtype=torch.float32, device=x.device) if scales is None else scales
-        _expect(q, torch.int8, (rows, channels), "quantize_rows: out")
-        _expect(scales, torch.float32, (rows,), "quantize_rows: scales")
-        self._check(self.lib.pxs_quantize_rows_i8(_dtype_code(x), _ptr(x), _ld(x), rows, channels,
-                                                  _ptr(q), _ptr(scales), self.stream()),
+        _expect(q, torch.int8, (rows, channels), "quantize_rows: out", dev)
+        _expect(scales, torch.float32, (rows,), "quantize_rows: scales", dev)
+        self._check(self.lib.pxs_quantize_rows_i8(_dtype_code(x), x.data_ptr(), _ld(x), rows, channels,
+                                                  q.data_ptr(), scales.data_ptr(), self.stream()),
                     "pxs_quantize_rows_i8")
         return q, scales
 
     @staticmethod
-    def _i8_operands(x, x_scales, weight, w_scales, bias, what):
+    def _i8_operands(x, x_scales, weight, w_scales, bias, out, what):
+        dev = torch.cuda.current_device()
+        if x.dim() != 2 or weight.dim() != 2:
+            raise PxsError(f"{what}: x must be [rows, cin], weight [cout, cin]")
         rows, cin = x.shape
         cout = weight.shape[0]
-        _expect(x, torch.int8, (rows, cin), what + ": x")
-        _expect(weight, torch.int8, (cout, cin), what + ": weight")
-        _expect(x_scales, torch.float32, (rows,), what + ": x_scales")
-        _expect(w_scales, torch.float32, (cout,), what + ": w_scales")
+        _expect(x, torch.int8, (rows, cin), what + ": x", dev)
+        _expect(weight, torch.int8, (cout, cin), what + ": weight", dev)
+        _expect(x_scales, torch.float32, (rows,), what + ": x_scales", dev)
+        _expect(w_scales, torch.float32, (cout,), what + ": w_scales", dev)
         if bias is not None:
-            _expect(bias, torch.float32, (cout,), what + ": bias")
+            _expect(bias, torch.float32, (cout,), what + ": bias", dev)
+        _expect(out, out.dtype, (rows, cout), what + ": the output", dev)
         return rows, cin, cout
 
     def linear_i8(self, x, x_scales, weight, w_scales, bias=None, act=ACT_NONE, dtype=torch.bfloat16, out=None):
         """pxs_linear_i8: act(x W^T * x_scales * w_scales + bias) in `dtype` (or out's)."""
-        rows, cin, cout = self._i8_operands(x, x_scales, weight, w_scales, bias, "linear_i8")
-        y = torch.empty((rows, cout), dtype=dtype, device=x.device) if out is None else out
-        _expect(y, y.dtype, (rows, cout), "linear_i8: out")
-        self._check(self.lib.pxs_linear_i8(_ptr(x), _ptr(x_scales), rows, cin, _ptr(weight), _ptr(w_scales),
-                                           _ptr(bias), cout, act, _dtype_code(y), _ptr(y), self.stream()),
+        y = torch.empty((x.shape[0], weight.shape[0]), dtype=dtype, device=x.device) if out is None else out
+        rows, cin, cout = self._i8_operands(x, x_scales, weight, w_scales, bias, y, "linear_i8")
+        self._check(self.lib.pxs_linear_i8(x.data_ptr(), x_scales.data_ptr(), rows, cin, weight.data_ptr(),
+                                           w_scales.data_ptr(), _ptr(bias), cout, act, _dtype_code(y),
+                                           y.data_ptr(), self.stream()),
                     "pxs_linear_i8")
         return y
 
     def linear_i8_residual(self, x, x_scales, weight, w_scales, bias, residual):
         """pxs_linear_i8_residual: residual (fp32) += the 8-bit linear."""
-        rows, cin, cout = self._i8_operands(x, x_scales, weight, w_scales, bias, "linear_i8_residual")
-        _expect(residual, torch.float32, (rows, cout), "linear_i8_residual: residual")
+        rows, cin, cout = self._i8_operands(x, x_scales, weight, w_scales, bias, residual, "linear_i8_residual")
+        if residual.dtype != torch.float32:
+            raise PxsError("linear_i8_residual: residual must be float32")
         self._check(self.lib.pxs_linear_i8_residual(_ptr(x), _ptr(x_scales), rows, cin, _ptr(weight),
                                                     _ptr(w_scales), _ptr(bias), cout, _ptr(residual),
                                                     self.stream()),
@@ -750,9 +765,18 @@ class Pxs:
 
     def linear_i8_gate_residual(self, x, x_scales, weight, w_scales, bias, coords, block_mod, time_mod,
                                 gate_offset, residual):
-        """pxs_linear_i8_gate_residual: residual (fp32) += gate * the 8-bit linear."""
-        rows, cin, cout = self._i8_operands(x, x_scales, weight, w_scales, bias, "linear_i8_gate_residual")
-        _expect(residual, torch.float32, (rows, cout), "linear_i8_gate_residual: residual")
+        """pxs_linear_i8_gate_residual: residual (fp32) += gate * the 8-bit linear; block_mod [6 cout],
+        time_mod [batch, 6 cout], coords int32 [rows, 4]."""
+        what = "linear_i8_gate_residual"
+        rows, cin, cout = self._i8_operands(x, x_scales, weight, w_scales, bias, residual, what)
+        dev = torch.cuda.current_device()
+        if residual.dtype != torch.float32:
+            raise PxsError(what + ": residual must be float32")
+        _expect(coords, torch.int32, (rows, 4), what + ": coords", dev)
+        _expect(block_mod, torch.float32, block_mod.shape, what + ": block_mod", dev)
+        _expect(time_mod, torch.float32, time_mod.shape, what + ": time_mod", dev)
+        if block_mod.numel() != 6 * cout or time_mod.numel() % (6 * cout) != 0:
+            raise PxsError(what + ": block_mod must hold 6 * cout values, time_mod as many for each batch item")
         self._check(self.lib.pxs_linear_i8_gate_residual(
             _ptr(x), _ptr(x_scales), rows, cin, _ptr(weight), _ptr(w_scales), _ptr(bias), cout, _ptr(coords),
             _ptr(block_mod), _ptr(time_mod), gate_offset, _ptr(residual), self.stream()),
@@ -806,17 +830,19 @@ class Pxs:
     def rope_positions(self, x, positions, freq, heads, head_dim, layout=ROPE_HALF, magnitude=1.0, out=None):
         """pxs_rope_positions: the first 2 * len(freq) values of each head of x turned by
         positions[row] * freq; out may be x."""
+        dev = torch.cuda.current_device()
         rows = x.shape[0]
-        _unit_stride(x, "rope_positions: x")
         y = torch.empty((rows, heads * head_dim), dtype=x.dtype, device=x.device) if out is None else out
-        _unit_stride(y, "rope_positions: out")
+        _unit_stride(x, "rope_positions: x", dev)
+        _unit_stride(y, "rope_positions: out", dev)
         if x.shape[1] != heads * head_dim or y.shape != x.shape or y.dtype != x.dtype:
             raise PxsError("rope_positions: x and out must be [rows, heads * head_dim] of one dtype")
-        _expect(positions, torch.int32, (rows,), "rope_positions: positions")
-        _expect(freq, torch.float64, (freq.numel(),), "rope_positions: freq")
-        self._check(self.lib.pxs_rope_positions(_dtype_code(x), _ptr(positions), _ptr(freq), _ptr(x), _ld(x),
-                                                rows, heads, head_dim, 2 * freq.numel(), layout, magnitude,
-                                                _ptr(y), _ld(y), self.stream()),
+        pairs = freq.numel()
+        _expect(positions, torch.int32, (rows,), "rope_positions: positions", dev)
+        _expect(freq, torch.float64, (pairs,), "rope_positions: freq", dev)
+        self._check(self.lib.pxs_rope_positions(_dtype_code(x), positions.data_ptr(), freq.data_ptr(), x.data_ptr(),
+                                                _ld(x), rows, heads, head_dim, 2 * pairs, layout, magnitude,
+                                                y.data_ptr(), _ld(y), self.stream()),
                     "pxs_rope_positions")
         return y
 
@@ -885,28 +911,28 @@ class Pxs:
                                 causal=False, prefix=None, out=None, workspace=None):
         """pxs_varlen_attention_scores: q [*, heads * head_dim], k and v [*, kv_heads * head_dim]
         (rows of any stride), cu_q and cu_k int64 [segments + 1]."""
+        dev = torch.cuda.current_device()
         nseg, total_q, total_k = cu_q.numel() - 1, q.shape[0], k.shape[0]
         o = torch.empty((total_q, heads * head_dim), dtype=q.dtype, device=q.device) if out is None else out
-        for t, columns, what in ((q, heads, "q"), (k, kv_heads, "k"), (v, kv_heads, "v"), (o, heads, "out")):
-            _unit_stride(t, "varlen_attention_scores: " + what)
-            if t.shape[1] != columns * head_dim or t.dtype != q.dtype:
-                raise PxsError(f"varlen_attention_scores: {what} must be [rows, {columns * head_dim}] {q.dtype}")
-        if v.shape[0] != total_k or o.shape[0] != total_q:
-            raise PxsError("varlen_attention_scores: k and v, q and out must have the same rows")
-        _expect(cu_q, torch.int64, (nseg + 1,), "varlen_attention_scores: cu_q")
-        _expect(cu_k, torch.int64, (nseg + 1,), "varlen_attention_scores: cu_k")
+        for t, rows, columns, what in ((q, total_q, heads, "q"), (k, total_k, kv_heads, "k"),
+                                       (v, total_k, kv_heads, "v"), (o, total_q, heads, "out")):
+            _unit_stride(t, "varlen_attention_scores: " + what, dev)
+            if t.shape != (rows, columns * head_dim) or t.dtype != q.dtype:
+                raise PxsError(f"varlen_attention_scores: {what} must be {[rows, columns * head_dim]} {q.dtype}")
+        _expect(cu_q, torch.int64, (nseg + 1,), "varlen_attention_scores: cu_q", dev)
+        _expect(cu_k, torch.int64, (nseg + 1,), "varlen_attention_scores: cu_k", dev)
         if slopes is not None:
-            _expect(slopes, torch.float32, (heads,), "varlen_attention_scores: slopes")
+            _expect(slopes, torch.float32, (heads,), "varlen_attention_scores: slopes", dev)
         if prefix is not None:
-            _expect(prefix, torch.int64, (nseg,), "varlen_attention_scores: prefix")
+            _expect(prefix, torch.int64, (nseg,), "varlen_attention_scores: prefix", dev)
         need = self.lib.pxs_attention_scores_workspace_bytes(nseg, total_q, total_k, heads, kv_heads, head_dim)
         ws = self._ws(need, q.device) if workspace is None else workspace
-        if ws.numel() * ws.element_size() < need:
-            raise PxsError(f"varlen_attention_scores: workspace of {need} bytes needed")
+        if ws.numel() * ws.element_size() < need or ws.get_device() != dev:
+            raise PxsError(f"varlen_attention_scores: a workspace of {need} bytes on the current device needed")
         self._check(self.lib.pxs_varlen_attention_scores(
-            _dtype_code(q), _ptr(q), _ld(q), _ptr(k), _ld(k), _ptr(v), _ld(v), _ptr(cu_q), _ptr(cu_k),
-            nseg, total_q, total_k, heads, kv_heads, head_dim, scale, cap, _ptr(slopes), int(causal),
-            _ptr(prefix), _ptr(o), _ld(o), _ptr(ws), self.stream()), "pxs_varlen_attention_scores")
+            _dtype_code(q), q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), cu_q.data_ptr(),
+            cu_k.data_ptr(), nseg, total_q, total_k, heads, kv_heads, head_dim, scale, cap, _ptr(slopes), int(causal),
+            _ptr(prefix), o.data_ptr(), _ld(o), ws.data_ptr(), self.stream()), "pxs_varlen_attention_scores")
         return o
 
     def transformer_block(self, cfg: BlockConfig, weights: BlockWeights, coords, batch_size, cu,
