@@ -543,8 +543,8 @@ int pxs_varlen_attention_noalloc(int dtype, const void * q, int64_t ld_q, const 
  *     segment see.  What hidden keys and values hold does not matter, NaN
  *     included.  A query that sees no key gets zeros.
  * Row strides ld_* are in elements.  total_q = cu_q[nseg] and total_k =
- * cu_k[nseg], both below 2^31; rows of q and o behind the last segment are
- * neither read nor written.  bf16 rows of 16-byte pieces with head_dim 64 or 128
+ * cu_k[nseg], total_k and total_q * heads / kv_heads at most 2^31 - 1024; rows
+ * of q and o behind the last segment are neither read nor written.  bf16 rows of 16-byte pieces with head_dim 64 or 128
  * take the fastest kernels.  The result depends on the whole call's sizes in its
  * last bits (the keys of few rows are split and joined in a fixed order); the
  * same call gives the same bits.

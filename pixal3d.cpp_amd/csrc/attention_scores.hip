@@ -59,12 +59,12 @@ struct ScoreArgs {
 struct Rows {
     int seg;
     int kv;
-    int64_t q0, k0;       // the segment's first query and key
-    int64_t nq, nk;
-    int64_t row0;         // first row of the tile
-    int64_t rows;         // of the segment: nq * group
-    int64_t shift;        // position of query i: i + shift
-    int64_t prefix;
+    int q0, k0;           // the segment's first query and key
+    int nk;
+    int row0;             // first row of the tile
+    int rows;             // of the segment: queries * group
+    int shift;            // position of query i: i + shift
+    int prefix;           // keys that every row sees, 0..nk
     int chunk, chunks;    // of the segment's keys; 0 of 1 where they are not cut
 };
 
@@ -78,17 +78,17 @@ __device__ __forceinline__ int64_t segment_items(int64_t nq, int64_t nk, int gro
 
 // Segment w.seg's part of w, item i of its items.
 __device__ __forceinline__ void segment_rows(const ScoreArgs & a, int i, int rows_per_tile, Rows & w) {
-    w.q0 = a.cu_q[w.seg];
-    w.k0 = a.cu_k[w.seg];
-    w.nq = a.cu_q[w.seg + 1] - w.q0;
-    w.nk = a.cu_k[w.seg + 1] - w.k0;
-    w.rows = w.nq * a.group;
-    w.shift = w.nk - w.nq;
-    w.prefix = a.causal && a.prefix ? a.prefix[w.seg] : 0;
+    w.q0 = static_cast<int>(a.cu_q[w.seg]);
+    w.k0 = static_cast<int>(a.cu_k[w.seg]);
+    w.nk = static_cast<int>(a.cu_k[w.seg + 1]) - w.k0;
+    const int nq = static_cast<int>(a.cu_q[w.seg + 1]) - w.q0;
+    w.rows = nq * a.group;
+    w.shift = w.nk - nq;
+    w.prefix = a.causal && a.prefix ? static_cast<int>(max(min(a.prefix[w.seg], static_cast<int64_t>(w.nk)), int64_t(0))) : 0;
     const bool cut = a.chunk > 0 && w.rows <= rows_per_tile;
-    w.row0 = cut ? 0 : static_cast<int64_t>(i) * rows_per_tile;
+    w.row0 = cut ? 0 : i * rows_per_tile;
     w.chunk = cut ? i : 0;
-    w.chunks = cut ? static_cast<int>((w.nk + a.chunk - 1) / a.chunk) : 1;
+    w.chunks = !cut ? 1 : w.nk > 0 ? (w.nk - 1) / a.chunk + 1 : 0;
 }
 
 // The items of up to 64 segments, a segment a lane: end[lane] = items of the segments up to its own.
@@ -126,6 +126,70 @@ __device__ __forceinline__ bool locate_rows(const ScoreArgs & a, int64_t t, int 
     return true;
 }
 
+// Row tiles of a segment with `tiles` of them whose rows see fewer than x keys (they come first:
+// later rows see no fewer).
+__device__ __forceinline__ int tiles_below(int x, int nq, int nk, int prefix, int group, int tiles, int shift) {
+    if (x <= prefix || x <= 0) return 0;  // (keys seen are at least the prefix, up to nk)
+    if (x > nk) return tiles;
+    // the first tile with a row of query x - 1 - (nk - nq) or later
+    const int64_t query = static_cast<int64_t>(x) - 1 - (nk - nq);
+    return query <= 0 ? 0 : static_cast<int>(min(query * group >> shift, static_cast<int64_t>(tiles)));
+}
+
+// The t-th row tile of a call with a causal mask and 2 to 64 segments, those that see most keys
+// first: 64 classes of keys seen, counted by a lane each, then the tile within its class.  (In
+// the segments' order the last of a call's tiles may be its longest: prompts of 8192, 2903 and
+// 4739 tokens, 16 heads of 128, SORT_US us against 611.)
+__device__ __forceinline__ bool locate_sorted(const ScoreArgs & a, int t, int rows_per_tile, int lane, Rows & w) {
+    const int shift = 31 - __clz(rows_per_tile);
+    int nq = 0, nk = 0, prefix = 0, tiles = 0;
+    if (lane < a.nseg) {
+        nq = static_cast<int>(a.cu_q[lane + 1] - a.cu_q[lane]);
+        nk = static_cast<int>(a.cu_k[lane + 1] - a.cu_k[lane]);
+        prefix = a.prefix ? static_cast<int>(max(min(a.prefix[lane], static_cast<int64_t>(nk)), int64_t(0))) : 0;
+        tiles = static_cast<int>((static_cast<int64_t>(nq) * a.group + rows_per_tile - 1) >> shift);
+    }
+    int most = nk;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) most = max(most, __shfl_xor(most, d, 64));
+    const int unit = most / 64 + 1;  // most < 64 unit
+    int count = 0;                   // tiles that see at least lane * unit keys
+    for (int s = 0; s < a.nseg; ++s) {
+        const int of = __builtin_amdgcn_readlane(tiles, s);
+        count += of - tiles_below(lane * unit, __builtin_amdgcn_readlane(nq, s), __builtin_amdgcn_readlane(nk, s),
+                                  __builtin_amdgcn_readlane(prefix, s), a.group, of, shift);
+    }
+    const int cls = __popcll(__ballot(count > t)) - 1;
+    if (cls < 0) return false;
+    const int ahead = cls == 63 ? 0 : __builtin_amdgcn_readlane(count, cls + 1);
+    const int lo = tiles_below(cls * unit, nq, nk, prefix, a.group, tiles, shift);
+    const int hi = cls == 63 ? tiles : tiles_below((cls + 1) * unit, nq, nk, prefix, a.group, tiles, shift);
+    int end = hi - lo;  // the class's tiles of the segments up to this lane's
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int below = __shfl_up(end, d, 64);
+        if (lane >= d) end += below;
+    }
+    const int at = t - ahead;
+    const int seg = __popcll(__ballot(lane < a.nseg && end <= at));
+    w.seg = __builtin_amdgcn_readfirstlane(seg);
+    const int within = at - (__builtin_amdgcn_readlane(end, w.seg) - (__builtin_amdgcn_readlane(hi, w.seg) - __builtin_amdgcn_readlane(lo, w.seg)));
+    segment_rows(a, __builtin_amdgcn_readlane(hi, w.seg) - 1 - within, rows_per_tile, w);
+    return true;
+}
+
+// A workgroup's row tile and split: key/value heads next to one another, so that an XCD, which
+// takes every eighth workgroup, reads few of them; the longest tiles first.
+__device__ __forceinline__ bool locate_work(const ScoreArgs & a, int rows_per_tile, int lane, Rows & w, int & split) {
+    const int per = a.kv_heads * a.splits, rest = static_cast<int>(blockIdx.x % per);
+    const int64_t t = blockIdx.x / per;
+    w.kv = rest % a.kv_heads;
+    split = rest / a.kv_heads;
+    if (a.causal && !a.tile_start && a.nseg > 1)
+        return locate_sorted(a, static_cast<int>(t), rows_per_tile, lane, w);
+    return locate_rows(a, a.tiles - 1 - t, rows_per_tile, lane, w);
+}
+
 // Query qi of the call: its segment, and the first of the segment's items; false for a row of no segment.
 __device__ __forceinline__ bool locate_query(const ScoreArgs & a, int64_t qi, int rows_per_tile, int lane, Rows & w,
                                              int64_t & item) {
@@ -144,15 +208,14 @@ __device__ __forceinline__ bool locate_query(const ScoreArgs & a, int64_t qi, in
 }
 
 // One past the last key that any of the rows up to `row` (inclusive) sees.
-__device__ __forceinline__ int64_t keys_end(const ScoreArgs & a, const Rows & w, int64_t row) {
+__device__ __forceinline__ int keys_end(const ScoreArgs & a, const Rows & w, int row) {
     if (!a.causal) return w.nk;
-    const int64_t last = min(row, w.rows - 1) / a.group;
-    return min(w.nk, max(last + w.shift + 1, max(w.prefix, int64_t(0))));
+    return min(w.nk, max(min(row, w.rows - 1) / a.group + w.shift + 1, w.prefix));
 }
 // The keys that every row from `row` on sees: all below.
-__device__ __forceinline__ int64_t keys_all(const ScoreArgs & a, const Rows & w, int64_t row) {
+__device__ __forceinline__ int keys_all(const ScoreArgs & a, const Rows & w, int row) {
     if (!a.causal) return w.nk;
-    return min(w.nk, max(row / a.group + w.shift + 1, max(w.prefix, int64_t(0))));
+    return min(w.nk, max(row / a.group + w.shift + 1, w.prefix));
 }
 
 // A score in log2 units, from a product q . k and the key's distance behind the query.
@@ -179,10 +242,10 @@ __device__ __forceinline__ bool is_finite_bits(float v) { return (__float_as_uin
 // altogether: for tiles where an unseen key's value is infinite or NaN, which
 // times a weight of zero is NaN.  One wave per row; lane l holds dims l, l + 64, ...
 template <typename T, int NC>
-__device__ void row_alone(const ScoreArgs & a, const Rows & w, int64_t row, int64_t key0, int64_t key1, int lane,
-                          bool partial, int64_t slot) {
-    const int64_t i = row / a.group;
-    const int head = w.kv * a.group + static_cast<int>(row % a.group);
+__device__ void row_alone(const ScoreArgs & a, const Rows & w, int row, int key0, int key1, int lane, bool partial,
+                          int64_t slot) {
+    const int i = row / a.group;
+    const int head = w.kv * a.group + row % a.group;
     const T * q = static_cast<const T *>(a.q) + (w.q0 + i) * a.ldq + static_cast<int64_t>(head) * a.d;
     const T * k = static_cast<const T *>(a.k) + w.k0 * a.ldk + static_cast<int64_t>(w.kv) * a.d;
     const T * v = static_cast<const T *>(a.v) + w.k0 * a.ldv + static_cast<int64_t>(w.kv) * a.d;
@@ -194,7 +257,7 @@ __device__ void row_alone(const ScoreArgs & a, const Rows & w, int64_t row, int6
         acc[c] = 0.0f;
     }
     float m = -INFINITY, l = 0.0f;
-    const int64_t end = min(key1, keys_end(a, w, row));
+    const int end = min(key1, keys_end(a, w, row));
     for (int64_t j = key0; j < end; ++j) {
         float dot = 0.0f;
 #pragma unroll
@@ -224,8 +287,8 @@ __device__ void row_alone(const ScoreArgs & a, const Rows & w, int64_t row, int6
 }
 
 // Partial row of a (query, head) in split `split` of a call whose keys are split alike for all rows.
-__device__ __forceinline__ int64_t split_slot(const ScoreArgs & a, const Rows & w, int split, int64_t row) {
-    return (static_cast<int64_t>(split) * a.total_q + w.q0 + row / a.group) * a.heads + w.kv * a.group + row % a.group;
+__device__ __forceinline__ int64_t split_slot(const ScoreArgs & a, const Rows & w, int split, int row) {
+    return (split * a.total_q + w.q0 + row / a.group) * a.heads + w.kv * a.group + row % a.group;
 }
 
 // Any dtype, head size up to DP, stride and alignment.  Four waves of 32 rows
@@ -251,26 +314,23 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, r = lane & 31;
 
-    // The row tiles of a key/value head and split from the last, which sees most, to the first.
-    const int64_t t = a.tiles - 1 - blockIdx.x % a.tiles;
-    const int rest = static_cast<int>(blockIdx.x / a.tiles);
-    const int split = rest % a.splits;
     Rows w;
-    w.kv = rest / a.splits;
-    if (!locate_rows(a, t, 128, lane, w)) return;
-    const int64_t end = keys_end(a, w, w.row0 + 127);
-    const int64_t key_tiles = (end + kKeys - 1) / kKeys;
-    const int64_t kt_first = key_tiles * split / a.splits, kt_last = key_tiles * (split + 1) / a.splits;
+    int split;
+    if (!locate_work(a, 128, lane, w, split)) return;
+    const int end = keys_end(a, w, w.row0 + 127);
+    const int key_tiles = (end + kKeys - 1) / kKeys;
+    const int kt_first = static_cast<int>(static_cast<int64_t>(key_tiles) * split / a.splits);
+    const int kt_last = static_cast<int>(static_cast<int64_t>(key_tiles) * (split + 1) / a.splits);
 
     const T * k = static_cast<const T *>(a.k) + w.k0 * a.ldk + static_cast<int64_t>(w.kv) * a.d;
     const T * v = static_cast<const T *>(a.v) + w.k0 * a.ldv + static_cast<int64_t>(w.kv) * a.d;
 
     // This lane's row and its Q fragment (dims h DP/2 .. h DP/2 + DP/2 - 1).
-    const int64_t wave_row0 = w.row0 + wave * 32;
-    const int64_t row = wave_row0 + r;
+    const int wave_row0 = w.row0 + wave * 32;
+    const int row = wave_row0 + r;
     const bool live = row < w.rows;
-    const int64_t qi = (live ? row : 0) / a.group;
-    const int head = w.kv * a.group + static_cast<int>((live ? row : 0) % a.group);
+    const int qi = (live ? row : 0) / a.group;
+    const int head = w.kv * a.group + (live ? row : 0) % a.group;
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
     T qv[DP / 2];
 #pragma unroll
@@ -288,12 +348,12 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
     float m = -INFINITY, l = 0.0f;
-    const int64_t my_end = live ? keys_end(a, w, row) : 0;  // keys >= my_end are masked
-    const int64_t wave_all = keys_all(a, w, wave_row0);     // keys below are seen by all of the wave's rows
-    const int64_t tile_all = keys_all(a, w, w.row0);
+    const int my_end = live ? keys_end(a, w, row) : 0;  // keys >= my_end are masked
+    const int wave_all = keys_all(a, w, wave_row0);     // keys below are seen by all of the wave's rows
+    const int tile_all = keys_all(a, w, w.row0);
     bool again = false;
 
-    for (int64_t kt0 = kt_first * kKeys; kt0 < kt_last * kKeys; kt0 += kKeys) {
+    for (int kt0 = kt_first * kKeys; kt0 < kt_last * kKeys; kt0 += kKeys) {
         __syncthreads();
         bool odd = false;
         for (int c = tid; c < kKeys * kPieces; c += 256) {
@@ -302,8 +362,8 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
 #pragma unroll
             for (int e = 0; e < kVec; ++e) kk[e] = vv[e] = T(0);
             if (kt0 + key < w.nk) {
-                load_dims<T>(k + (kt0 + key) * a.ldk, piece * kVec, a.d, a.vec, kk);
-                load_dims<T>(v + (kt0 + key) * a.ldv, piece * kVec, a.d, a.vec, vv);
+                load_dims<T>(k + static_cast<int64_t>(kt0 + key) * a.ldk, piece * kVec, a.d, a.vec, kk);
+                load_dims<T>(v + static_cast<int64_t>(kt0 + key) * a.ldv, piece * kVec, a.d, a.vec, vv);
             }
             *reinterpret_cast<uint4 *>(k_lds + key * Tile::kKPitch + piece * 16) = *reinterpret_cast<const uint4 *>(kk);
 #pragma unroll
@@ -342,7 +402,7 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
         }
         // Register e of sub-tile kt holds key kt * 32 + 8 (e / 4) + 4 h + e % 4.
         const bool masked = kt0 + kKeys > wave_all || kt0 + kKeys > w.nk;
-        const int behind = static_cast<int>(qi + w.shift - kt0), seen = static_cast<int>(my_end - kt0);
+        const int behind = qi + w.shift - kt0, seen = my_end - kt0;
         float top = -INFINITY;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
@@ -696,7 +756,7 @@ __device__ __forceinline__ TileSource<DH> tile_source(const ScoreArgs & a, const
     s.v = uniform_ptr(reinterpret_cast<const char *>(static_cast<const uint16_t *>(a.v) + w.k0 * a.ldv + static_cast<int64_t>(w.kv) * DH));
     s.ldk = a.ldk * 2;
     s.ldv = a.ldv * 2;
-    s.nk = static_cast<int>(w.nk);
+    s.nk = w.nk;
     s.zero = reinterpret_cast<uint64_t>(&g_score_zero[0]);
     asm volatile("" : "+s"(s.zero));
     return s;
@@ -722,31 +782,28 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, r = lane & 31;
-    const int64_t t = a.tiles - 1 - blockIdx.x % a.tiles;
-    const int rest = static_cast<int>(blockIdx.x / a.tiles);
-    const int split = rest % a.splits;
     Rows w;
-    w.kv = rest / a.splits;
-    if (!locate_rows(a, t, 128, lane, w)) return;
-    const int end = static_cast<int>(keys_end(a, w, w.row0 + 127));
+    int split;
+    if (!locate_work(a, 128, lane, w, split)) return;
+    const int end = keys_end(a, w, w.row0 + 127);
     const int all = (end + F::kKeys - 1) / F::kKeys;
     const int first = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
     const int last = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits) - 1;
     const int n = last - first + 1;  // tiles, walked from `last` down: step i is tile last - i
 
-    const int64_t wave_row0 = w.row0 + wave * 32;
+    const int wave_row0 = w.row0 + wave * 32;
     const bool live = wave_row0 + r < w.rows;
-    const int64_t row = live ? wave_row0 + r : w.rows - 1;
-    const int qi = static_cast<int>(row / a.group);
-    const int head = w.kv * a.group + static_cast<int>(row % a.group);
+    const int row = live ? wave_row0 + r : w.rows - 1;
+    const int qi = row / a.group;
+    const int head = w.kv * a.group + row % a.group;
     const RowScore rs = row_score<MODE>(a, head);
     const float cap_log2 = a.cap_log2;
     bf16x8 qf[F::NST];
     load_q<DH>(a, w, qi, head, live, h, qf);
-    const int seen = static_cast<int>(keys_end(a, w, row)) - 4 * h;
-    const int pos = qi + static_cast<int>(w.shift) - 4 * h;
-    const int whole = static_cast<int>(keys_all(a, w, w.row0)) / F::kKeys;  // tiles below hold seen keys only
-    const int wave_end = wave_row0 < w.rows ? static_cast<int>(keys_end(a, w, wave_row0 + 31)) : 0;
+    const int seen = keys_end(a, w, row) - 4 * h;
+    const int pos = qi + w.shift - 4 * h;
+    const int whole = keys_all(a, w, w.row0) / F::kKeys;  // tiles below hold seen keys only
+    const int wave_end = wave_row0 < w.rows ? keys_end(a, w, wave_row0 + 31) : 0;
 
     const TileSource<DH> src = tile_source<DH>(a, w);
     uint32_t off[kMine];
@@ -844,9 +901,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
     if (__syncthreads_or(odd)) {
         for (int j = 0; j < 32; ++j)
             if (wave_row0 + j < w.rows)
-                row_alone<uint16_t, DH / 64>(a, w, wave_row0 + j, static_cast<int64_t>(first) * F::kKeys,
-                                             static_cast<int64_t>(last + 1) * F::kKeys, lane, a.splits > 1,
-                                             split_slot(a, w, split, wave_row0 + j));
+                row_alone<uint16_t, DH / 64>(a, w, wave_row0 + j, first * F::kKeys, (last + 1) * F::kKeys, lane,
+                                             a.splits > 1, split_slot(a, w, split, wave_row0 + j));
         return;
     }
     const float sum = lane_pair_sum(st.sum);
@@ -907,10 +963,10 @@ __global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
     const int64_t item = blockIdx.x / a.kv_heads;
     if (!locate_rows(a, item, kFewRows, lane, w)) return;
     const bool live = w.row0 + r < w.rows;
-    const int64_t row = live ? w.row0 + r : w.rows - 1;
-    const int qi = static_cast<int>(row / a.group);
-    const int head = w.kv * a.group + static_cast<int>(row % a.group);
-    int first = 0, last = (static_cast<int>(keys_end(a, w, w.row0 + kFewRows - 1)) + F::kKeys - 1) / F::kKeys;
+    const int row = live ? w.row0 + r : w.rows - 1;
+    const int qi = row / a.group;
+    const int head = w.kv * a.group + row % a.group;
+    int first = 0, last = (keys_end(a, w, w.row0 + kFewRows - 1) + F::kKeys - 1) / F::kKeys;
     if (w.chunks > 1) {
         first = w.chunk * (a.chunk / F::kKeys);
         last = min(last, first + a.chunk / F::kKeys);
@@ -931,9 +987,9 @@ __global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
     if (n > 0) issue(0);
     bf16x8 qf[F::NST];
     load_q<DH>(a, w, qi, head, live, h, qf);
-    const int seen = static_cast<int>(keys_end(a, w, row)) - 4 * h;
-    const int pos = qi + static_cast<int>(w.shift) - 4 * h;
-    const int whole = static_cast<int>(keys_all(a, w, w.row0)) / F::kKeys;
+    const int seen = keys_end(a, w, row) - 4 * h;
+    const int pos = qi + w.shift - 4 * h;
+    const int whole = keys_all(a, w, w.row0) / F::kKeys;
     typename F::Out oacc;
 #pragma unroll
     for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
@@ -960,8 +1016,8 @@ __global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
     if (__syncthreads_or(odd)) {
         for (int j = wave; j < kFewRows; j += 4)
             if (w.row0 + j < w.rows)
-                row_alone<uint16_t, DH / 64>(a, w, w.row0 + j, static_cast<int64_t>(first) * F::kKeys,
-                                             static_cast<int64_t>(last) * F::kKeys, lane, w.chunks > 1, part + j);
+                row_alone<uint16_t, DH / 64>(a, w, w.row0 + j, first * F::kKeys, last * F::kKeys, lane, w.chunks > 1,
+                                             part + j);
         return;
     }
     // The waves' results: outputs in their own rings, bases and sums behind the rings.
@@ -989,8 +1045,8 @@ __global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
         f[i] = __builtin_amdgcn_exp2f(v.x - ref);
         total += v.y * f[i];
     }
-    const int token = static_cast<int>((w.row0 + jr) / a.group);
-    const int to_head = w.kv * a.group + static_cast<int>((w.row0 + jr) % a.group);
+    const int token = (w.row0 + jr) / a.group;
+    const int to_head = w.kv * a.group + (w.row0 + jr) % a.group;
     uint16_t * o = static_cast<uint16_t *>(a.o) + (w.q0 + token) * a.ldo + static_cast<int64_t>(to_head) * DH;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     if (w.chunks > 1 && jc == 0) a.part_ml[part + jr] = make_float2(base, total);
@@ -1126,6 +1182,7 @@ __global__ void __launch_bounds__(1024) score_tiles_kernel(const int64_t * __res
 // ---- host -----------------------------------------------------------------------
 
 constexpr int kScoreMaxDim = 256;
+constexpr int64_t kScoreMaxRows = INT32_MAX - 1023;  // rows and keys are counted in 32 bits, a tile past their end
 constexpr int kWaveSegments = 64;   // segments that a wave's lanes hold; more take a table
 constexpr int kRowTile = 128;
 constexpr int64_t kSplitGrid = 512; // workgroups (two a CU) up to which a call's keys are split
@@ -1155,7 +1212,7 @@ constexpr int64_t kFewItems = 1024;
 constexpr int64_t kFewKeys = 256;  // at least, and a multiple of
 int64_t few_chunk(int64_t total_k, int kv_heads) {
     const int64_t keys = (total_k * kv_heads + kFewItems - 1) / kFewItems;
-    return std::max<int64_t>(1, (keys + kFewKeys - 1) / kFewKeys) * kFewKeys;
+    return std::min<int64_t>(std::max<int64_t>(1, (keys + kFewKeys - 1) / kFewKeys) * kFewKeys, 1 << 30);
 }
 bool few_rows(int64_t total_q, int nseg, int group) { return total_q * group <= static_cast<int64_t>(kFewRows) * nseg; }
 int64_t few_items(int64_t total_q, int64_t total_k, int nseg, int kv_heads, int group) {
@@ -1164,7 +1221,7 @@ int64_t few_items(int64_t total_q, int64_t total_k, int nseg, int kv_heads, int 
 // Rows of partial results of any such call of up to these sizes: its queries' rows fill at
 // most nseg tiles, and total_k / chunk is at most both total_k / kFewKeys and kFewItems / kv_heads.
 int64_t few_part_rows(int64_t total_k, int nseg, int kv_heads) {
-    return ((2 * static_cast<int64_t>(nseg) + 1) * kv_heads + std::min(total_k / kFewKeys * kv_heads, kFewItems)) * kFewRows;
+    return ((2 * static_cast<int64_t>(nseg) + 3) * kv_heads + std::min(total_k / kFewKeys * kv_heads, kFewItems)) * kFewRows;
 }
 
 template <typename T, int DP>
@@ -1258,8 +1315,9 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
     PXS_CHECK(causal || !prefix, PXS_ERR_ARG, "pxs_varlen_attention_scores: a prefix needs the causal mask");
     PXS_CHECK(std::isfinite(scale * kLog2e) && (cap == 0.0f || (std::isfinite(scale / cap) && std::isfinite(cap * kLog2e))),
               PXS_ERR_ARG, "pxs_varlen_attention_scores: scale and cap out of range");
-    PXS_CHECK(nseg >= 0 && total_q >= 0 && total_k >= 0 && total_q <= INT32_MAX && total_k <= INT32_MAX, PXS_ERR_ARG,
-              "pxs_varlen_attention_scores: row counts must be in 0..2^31 - 1");
+    PXS_CHECK(nseg >= 0 && total_q >= 0 && total_k >= 0 && total_q <= kScoreMaxRows / (heads / kv_heads) &&
+                  total_k <= kScoreMaxRows,
+              PXS_ERR_ARG, "pxs_varlen_attention_scores: row counts must be in 0..2^31 - 1024, as total_q * heads / kv_heads");
     const int64_t wq = static_cast<int64_t>(heads) * head_dim, wk = static_cast<int64_t>(kv_heads) * head_dim;
     PXS_CHECK(ld_q >= wq && ld_k >= wk && ld_v >= wk && ld_o >= wq, PXS_ERR_ARG,
               "pxs_varlen_attention_scores: row stride smaller than heads * head_dim");

@@ -114,12 +114,13 @@ SCORES = dict(dtype=0, q=P, ld_q=256, k=P, ld_k=128, v=P, ld_v=128, cu_q=P, cu_k
     (dict(heads=131072, kv=1), "65535"), (dict(d=0), "head_dim"), (dict(d=257), "head_dim"), (dict(scale=0.0), "scale"),
     (dict(scale=math.nan), "scale"), (dict(cap=-1.0), "cap"), (dict(cap=math.inf), "cap"), (dict(cap=1e-44), "out of range"),
     (dict(causal=2), "causal"), (dict(causal=0, prefix=P), "prefix"), (dict(nseg=-1), "row counts"),
-    (dict(total_q=-1), "row counts"), (dict(total_k=2 ** 31), "row counts"), (dict(ld_q=255), "row stride"),
+    (dict(total_q=-1), "row counts"), (dict(total_k=2 ** 31 - 1023), "row counts"),
+    (dict(total_q=2 ** 31 - 1024, heads=4, kv=2), "row counts"), (dict(ld_q=255), "row stride"),
     (dict(ld_k=127), "row stride"), (dict(ld_v=127), "row stride"), (dict(ld_o=255), "row stride"),
     (dict(q=None), "null pointer"), (dict(k=None), "null pointer"), (dict(v=None), "null pointer"),
     (dict(o=None), "null pointer"), (dict(cu_q=None), "null pointer"), (dict(cu_k=None), "null pointer"),
     (dict(ws=None), "null pointer"), (dict(ws=C.c_void_p(4104)), "256-byte aligned"),
-    (dict(total_q=2 ** 31 - 1, heads=65535, kv=65535, ld_q=2 ** 23, ld_k=2 ** 23, ld_v=2 ** 23, ld_o=2 ** 23), "grid too large")])
+    (dict(total_q=2 ** 31 - 1024, heads=65535, kv=65535, ld_q=2 ** 23, ld_k=2 ** 23, ld_v=2 ** 23, ld_o=2 ** 23), "grid too large")])
 def test_attention_scores_refusals(lib, change, text):
     refused(lib, lib.pxs_varlen_attention_scores(*{**SCORES, **change}.values()), text)
 
