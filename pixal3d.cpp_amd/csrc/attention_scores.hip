@@ -21,6 +21,7 @@
 // fp32, and a second launch joins them in order.
 
 #include "attn_common.h"
+#include "tiles.h"
 
 #include <algorithm>
 #include <cmath>
@@ -57,7 +58,6 @@ struct ScoreArgs {
 
 // A workgroup's rows: a tile of a segment and key/value head, and the keys that its rows see.
 struct Rows {
-    int seg;
     int kv;
     int q0, k0;           // the segment's first query and key
     int nk;
@@ -76,53 +76,68 @@ __device__ __forceinline__ int64_t segment_items(int64_t nq, int64_t nk, int gro
     return (rows + rows_per_tile - 1) / rows_per_tile;
 }
 
-// Segment w.seg's part of w, item i of its items.
-__device__ __forceinline__ void segment_rows(const ScoreArgs & a, int i, int rows_per_tile, Rows & w) {
-    w.q0 = static_cast<int>(a.cu_q[w.seg]);
-    w.k0 = static_cast<int>(a.cu_k[w.seg]);
-    w.nk = static_cast<int>(a.cu_k[w.seg + 1]) - w.k0;
-    const int nq = static_cast<int>(a.cu_q[w.seg + 1]) - w.q0;
-    w.rows = nq * a.group;
-    w.shift = w.nk - nq;
-    w.prefix = a.causal && a.prefix ? static_cast<int>(max(min(a.prefix[w.seg], static_cast<int64_t>(w.nk)), int64_t(0))) : 0;
+// A segment's first query and key, its queries, keys and prefix (0..keys).
+struct Segment {
+    int q0, k0, nq, nk, prefix;
+};
+__device__ __forceinline__ Segment load_segment(const ScoreArgs & a, int s) {
+    const int64_t q0 = a.cu_q[s], q1 = a.cu_q[s + 1], k0 = a.cu_k[s], k1 = a.cu_k[s + 1];
+    const int64_t prefix = a.causal && a.prefix ? a.prefix[s] : 0;
+    return {static_cast<int>(q0), static_cast<int>(k0), static_cast<int>(q1 - q0), static_cast<int>(k1 - k0),
+            static_cast<int>(max(min(prefix, k1 - k0), int64_t(0)))};
+}
+// The segment that lane `from` (the same in all lanes) holds.
+__device__ __forceinline__ Segment segment_of(const Segment & g, int from) {
+    return {__builtin_amdgcn_readlane(g.q0, from), __builtin_amdgcn_readlane(g.k0, from),
+            __builtin_amdgcn_readlane(g.nq, from), __builtin_amdgcn_readlane(g.nk, from),
+            __builtin_amdgcn_readlane(g.prefix, from)};
+}
+// Up to 64 segments, one a lane, read together (a segment's bounds are then no second wait).
+__device__ __forceinline__ Segment lane_segment(const ScoreArgs & a, int lane) {
+    Segment g{};
+    if (lane < a.nseg) g = load_segment(a, lane);
+    return g;
+}
+
+// Item i of a segment.
+__device__ __forceinline__ void segment_rows(const ScoreArgs & a, const Segment & g, int i, int rows_per_tile, Rows & w) {
+    w.q0 = g.q0;
+    w.k0 = g.k0;
+    w.nk = g.nk;
+    w.rows = g.nq * a.group;
+    w.shift = g.nk - g.nq;
+    w.prefix = g.prefix;
     const bool cut = a.chunk > 0 && w.rows <= rows_per_tile;
     w.row0 = cut ? 0 : i * rows_per_tile;
     w.chunk = cut ? i : 0;
-    w.chunks = !cut ? 1 : w.nk > 0 ? (w.nk - 1) / a.chunk + 1 : 0;
+    w.chunks = !cut ? 1 : g.nk > 0 ? (g.nk - 1) / a.chunk + 1 : 0;
 }
 
-// The items of up to 64 segments, a segment a lane: end[lane] = items of the segments up to its own.
-__device__ __forceinline__ int64_t lane_items(const ScoreArgs & a, int rows_per_tile, int lane, int64_t & end) {
-    int64_t items = 0;
-    if (lane < a.nseg)
-        items = segment_items(a.cu_q[lane + 1] - a.cu_q[lane], a.cu_k[lane + 1] - a.cu_k[lane], a.group, rows_per_tile,
-                              a.chunk);
-    end = items;
+// v summed over the lanes up to each.
+__device__ __forceinline__ int lane_sums(int v, int lane) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-        const int64_t below = __shfl_up(end, d, 64);
-        if (lane >= d) end += below;
+        const int below = __shfl_up(v, d, 64);
+        if (lane >= d) v += below;
     }
-    return items;
+    return v;
 }
 
 // Item t; false past the last.
-__device__ __forceinline__ bool locate_rows(const ScoreArgs & a, int64_t t, int rows_per_tile, int lane, Rows & w) {
-    int64_t first;
-    int seg;
+__device__ __forceinline__ bool locate_rows(const ScoreArgs & a, int t, int rows_per_tile, int lane, Rows & w) {
     if (a.tile_start) {
         if (t >= a.tile_start[a.nseg]) return false;
-        seg = find_segment(a.tile_start, a.nseg, t, lane);
-        first = a.tile_start[seg];
-    } else {
-        int64_t end;
-        const int64_t items = lane_items(a, rows_per_tile, lane, end);
-        seg = __popcll(__ballot(lane < a.nseg && end <= t));  // segments that end at or before t
-        if (seg >= a.nseg) return false;
-        first = __shfl(end - items, seg, 64);
+        const int seg = __builtin_amdgcn_readfirstlane(find_segment(a.tile_start, a.nseg, t, lane));
+        segment_rows(a, load_segment(a, seg), __builtin_amdgcn_readfirstlane(static_cast<int>(t - a.tile_start[seg])),
+                     rows_per_tile, w);
+        return true;
     }
-    w.seg = __builtin_amdgcn_readfirstlane(seg);
-    segment_rows(a, __builtin_amdgcn_readfirstlane(static_cast<int>(t - first)), rows_per_tile, w);
+    const Segment g = lane_segment(a, lane);
+    const int items = static_cast<int>(segment_items(g.nq, g.nk, a.group, rows_per_tile, a.chunk));
+    const int end = lane_sums(items, lane);
+    const int seg = __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < a.nseg && end <= t)));  // those that end at or before t
+    if (seg >= a.nseg) return false;
+    segment_rows(a, segment_of(g, seg), t - __builtin_amdgcn_readlane(end - items, seg), rows_per_tile, w);
     return true;
 }
 
@@ -139,16 +154,12 @@ __device__ __forceinline__ int tiles_below(int x, int nq, int nk, int prefix, in
 // The t-th row tile of a call with a causal mask and 2 to 64 segments, those that see most keys
 // first: 64 classes of keys seen, counted by a lane each, then the tile within its class.  (In
 // the segments' order the last of a call's tiles may be its longest: prompts of 8192, 2903 and
-// 4739 tokens, 16 heads of 128, SORT_US us against 611.)
+// 4739 tokens, 16 heads of 128, 524 us against 611.)
 __device__ __forceinline__ bool locate_sorted(const ScoreArgs & a, int t, int rows_per_tile, int lane, Rows & w) {
     const int shift = 31 - __clz(rows_per_tile);
-    int nq = 0, nk = 0, prefix = 0, tiles = 0;
-    if (lane < a.nseg) {
-        nq = static_cast<int>(a.cu_q[lane + 1] - a.cu_q[lane]);
-        nk = static_cast<int>(a.cu_k[lane + 1] - a.cu_k[lane]);
-        prefix = a.prefix ? static_cast<int>(max(min(a.prefix[lane], static_cast<int64_t>(nk)), int64_t(0))) : 0;
-        tiles = static_cast<int>((static_cast<int64_t>(nq) * a.group + rows_per_tile - 1) >> shift);
-    }
+    const Segment g = lane_segment(a, lane);
+    const int nq = g.nq, nk = g.nk, prefix = g.prefix;
+    const int tiles = static_cast<int>((static_cast<int64_t>(nq) * a.group + rows_per_tile - 1) >> shift);
     int most = nk;
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) most = max(most, __shfl_xor(most, d, 64));
@@ -164,17 +175,11 @@ __device__ __forceinline__ bool locate_sorted(const ScoreArgs & a, int t, int ro
     const int ahead = cls == 63 ? 0 : __builtin_amdgcn_readlane(count, cls + 1);
     const int lo = tiles_below(cls * unit, nq, nk, prefix, a.group, tiles, shift);
     const int hi = cls == 63 ? tiles : tiles_below((cls + 1) * unit, nq, nk, prefix, a.group, tiles, shift);
-    int end = hi - lo;  // the class's tiles of the segments up to this lane's
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int below = __shfl_up(end, d, 64);
-        if (lane >= d) end += below;
-    }
+    const int end = lane_sums(hi - lo, lane);  // the class's tiles of the segments up to this lane's
     const int at = t - ahead;
-    const int seg = __popcll(__ballot(lane < a.nseg && end <= at));
-    w.seg = __builtin_amdgcn_readfirstlane(seg);
-    const int within = at - (__builtin_amdgcn_readlane(end, w.seg) - (__builtin_amdgcn_readlane(hi, w.seg) - __builtin_amdgcn_readlane(lo, w.seg)));
-    segment_rows(a, __builtin_amdgcn_readlane(hi, w.seg) - 1 - within, rows_per_tile, w);
+    const int seg = __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < a.nseg && end <= at)));
+    const int within = at - __builtin_amdgcn_readlane(end - (hi - lo), seg);
+    segment_rows(a, segment_of(g, seg), __builtin_amdgcn_readlane(hi, seg) - 1 - within, rows_per_tile, w);
     return true;
 }
 
@@ -182,28 +187,31 @@ __device__ __forceinline__ bool locate_sorted(const ScoreArgs & a, int t, int ro
 // takes every eighth workgroup, reads few of them; the longest tiles first.
 __device__ __forceinline__ bool locate_work(const ScoreArgs & a, int rows_per_tile, int lane, Rows & w, int & split) {
     const int per = a.kv_heads * a.splits, rest = static_cast<int>(blockIdx.x % per);
-    const int64_t t = blockIdx.x / per;
+    const int t = static_cast<int>(blockIdx.x / per);
     w.kv = rest % a.kv_heads;
     split = rest / a.kv_heads;
     if (a.causal && !a.tile_start && a.nseg > 1)
-        return locate_sorted(a, static_cast<int>(t), rows_per_tile, lane, w);
-    return locate_rows(a, a.tiles - 1 - t, rows_per_tile, lane, w);
+        return locate_sorted(a, t, rows_per_tile, lane, w);
+    return locate_rows(a, static_cast<int>(a.tiles) - 1 - t, rows_per_tile, lane, w);
 }
 
 // Query qi of the call: its segment, and the first of the segment's items; false for a row of no segment.
-__device__ __forceinline__ bool locate_query(const ScoreArgs & a, int64_t qi, int rows_per_tile, int lane, Rows & w,
-                                             int64_t & item) {
-    if (qi < a.cu_q[0] || qi >= a.cu_q[a.nseg]) return false;
-    const int seg = find_segment(a.cu_q, a.nseg, qi, lane);
+__device__ __forceinline__ bool locate_query(const ScoreArgs & a, int qi, int rows_per_tile, int lane, Rows & w, int & item) {
     if (a.tile_start) {
-        item = a.tile_start[seg];
-    } else {
-        int64_t end;
-        const int64_t items = lane_items(a, rows_per_tile, lane, end);
-        item = __shfl(end - items, seg, 64);
+        if (qi < a.cu_q[0] || qi >= a.cu_q[a.nseg]) return false;
+        const int seg = find_segment(a.cu_q, a.nseg, qi, lane);
+        item = static_cast<int>(a.tile_start[seg]);
+        segment_rows(a, load_segment(a, seg), 0, rows_per_tile, w);
+        return true;
     }
-    w.seg = seg;
-    segment_rows(a, 0, rows_per_tile, w);
+    const Segment g = lane_segment(a, lane);
+    const int items = static_cast<int>(segment_items(g.nq, g.nk, a.group, rows_per_tile, a.chunk));
+    const int end = lane_sums(items, lane);
+    const uint64_t mine = __ballot(lane < a.nseg && qi >= g.q0 && qi < g.q0 + g.nq);
+    if (mine == 0) return false;
+    const int seg = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<long long>(mine)) - 1);
+    item = __builtin_amdgcn_readlane(end - items, seg);
+    segment_rows(a, segment_of(g, seg), 0, rows_per_tile, w);
     return true;
 }
 
@@ -292,14 +300,19 @@ __device__ __forceinline__ int64_t split_slot(const ScoreArgs & a, const Rows & 
 }
 
 // Any dtype, head size up to DP, stride and alignment.  Four waves of 32 rows
-// share tiles of kKeys keys, staged through registers into LDS (V transposed).  As in
+// share tiles of kKeys keys, staged through registers into LDS.  As in
 // attention.hip a wave computes S^T = K Q^T, so that a lane owns one row and half of
-// its scores, and O^T += V^T P^T with P straight from those registers.
+// its scores, and O^T += V^T P^T with P straight from those registers.  bf16 reads four keys
+// of a dim at a time, so its V is staged transposed; fp32 reads one, 32 dims side by side, from V as
+// it lies.  Waves past the segment's rows only help to stage: a new token's tile
+// costs one wave's products.  fp32 is bound by v_mfma_f32_32x32x2_f32 (64 cycles, 153 TFLOP/s in a
+// large product here).
 template <typename T, int DP> struct AnyTile {
+    static constexpr bool kTransposed = sizeof(T) == 2;
     static constexpr int kKeys = DP == 64 ? 64 : 32;
     static constexpr int kKPitch = DP * static_cast<int>(sizeof(T)) + 16;
-    static constexpr int kVPitch = kKeys * static_cast<int>(sizeof(T)) + (sizeof(T) == 2 ? 8 : 16);
-    static constexpr int kBytes = kKeys * kKPitch + DP * kVPitch;
+    static constexpr int kVPitch = kTransposed ? kKeys * 2 + 8 : kKPitch;
+    static constexpr int kBytes = kKeys * kKPitch + (kTransposed ? DP : kKeys) * kVPitch;
 };
 
 template <typename T, int DP>
@@ -309,7 +322,7 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
     constexpr int kPieces = DP / kVec;  // 16-byte pieces of a padded row
     extern __shared__ __align__(16) char smem[];
     char * k_lds = smem;
-    char * vt_lds = smem + kKeys * Tile::kKPitch;
+    char * v_lds = smem + kKeys * Tile::kKPitch;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, r = lane & 31;
@@ -366,14 +379,18 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
                 load_dims<T>(v + static_cast<int64_t>(kt0 + key) * a.ldv, piece * kVec, a.d, a.vec, vv);
             }
             *reinterpret_cast<uint4 *>(k_lds + key * Tile::kKPitch + piece * 16) = *reinterpret_cast<const uint4 *>(kk);
+            if constexpr (!Tile::kTransposed)
+                *reinterpret_cast<uint4 *>(v_lds + key * Tile::kVPitch + piece * 16) = *reinterpret_cast<const uint4 *>(vv);
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
                 odd |= !is_finite_bits(load_f32(&vv[e]));
-                *reinterpret_cast<T *>(vt_lds + (piece * kVec + e) * Tile::kVPitch + key * static_cast<int>(sizeof(T))) = vv[e];
+                if constexpr (Tile::kTransposed)
+                    *reinterpret_cast<T *>(v_lds + (piece * kVec + e) * Tile::kVPitch + key * static_cast<int>(sizeof(T))) = vv[e];
             }
         }
         // A tile with keys that some row does not see, and values that are not finite.
         again |= __syncthreads_or(odd && min(kt0 + kKeys, w.nk) > tile_all);
+        if (wave_row0 >= w.rows) continue;
 
         f32x16 s[KT];
 #pragma unroll
@@ -444,7 +461,7 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
                     for (int e = 0; e < 8; ++e) p[e] = static_cast<__bf16>(s[kt][8 * u + e]);
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
-                        const char * vrow = vt_lds + (dt * 32 + r) * Tile::kVPitch;
+                        const char * vrow = v_lds + (dt * 32 + r) * Tile::kVPitch;
                         const int key = kt * 32 + 16 * u + 4 * h;
                         const uint2 lo = *reinterpret_cast<const uint2 *>(vrow + key * 2);
                         const uint2 hi = *reinterpret_cast<const uint2 *>(vrow + (key + 8) * 2);
@@ -454,15 +471,13 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int e = 0; e < 16; ++e) {
+                    const char * vrow = v_lds + (kt * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) * Tile::kVPitch + r * 4;
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const f32x4 vf = *reinterpret_cast<const f32x4 *>(vt_lds + (dt * 32 + r) * Tile::kVPitch +
-                                                                          (kt * 32 + 8 * i + 4 * h) * 4);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            oacc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[j], s[kt][4 * i + j], oacc[dt], 0, 0, 0);
-                    }
+                    for (int dt = 0; dt < DT; ++dt)
+                        oacc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float *>(vrow + dt * 128),
+                                                                        s[kt][e], oacc[dt], 0, 0, 0);
+                }
             }
         }
     }
@@ -489,7 +504,7 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
         }
 }
 
-// ---- bf16, head size 64 or 128 -----------------------------------------------------
+// ---- bf16, head sizes of whole 16-byte pieces up to 128 -----------------------------------------------------
 // Tiles of kKeys keys, 8 KB of K and 8 KB of V, go from HBM to LDS by DMA, rows of
 // DH / 64 halves of 128 bytes; V is read transposed from LDS (ds_read_b64_tr_b16).
 // 16 matrix instructions a tile and wave, as many for S as for O.
@@ -498,6 +513,8 @@ __device__ __align__(16) uint4 g_score_zero[8];  // what keys past a segment's e
 
 constexpr int kCap = 1, kBias = 2;  // MODE bits: scores are capped, biased
 
+// Head sizes that are multiples of 8 up to 128 run as the next of 64 and 128 (WHOLE false): the
+// missing pieces of a row come from a line of zeros.
 template <int DH> struct Fast {
     static constexpr int KT = DH == 64 ? 2 : 1;   // 32-key sub-tiles of a tile
     static constexpr int kKeys = 32 * KT;
@@ -683,24 +700,27 @@ struct TileSource {
     int64_t ldk, ldv;    // bytes
     int nk;
     uint64_t zero;
+    uint32_t lacks;      // bit j: instruction j's piece of this lane lies past the head
 };
 
 template <int DH, int COUNT>
-__device__ __forceinline__ void tile_offsets(const TileSource<DH> & src, int first, int lane, uint32_t (&off)[COUNT]) {
+__device__ __forceinline__ void tile_offsets(TileSource<DH> & src, int d, int first, int lane, uint32_t (&off)[COUNT]) {
     using F = Fast<DH>;
+    src.lacks = 0;
     const int lrow = lane >> 3, lslot = lane & 7;
 #pragma unroll
     for (int j = 0; j < COUNT; ++j) {
         const int unit = first + j;
         const bool is_v = unit >= F::kUnits;
         const int half = unit % F::kUnits / (F::kKeys / 8), row = unit % (F::kKeys / 8) * 8 + lrow;
-        off[j] = static_cast<uint32_t>(row * (is_v ? src.ldv : src.ldk) + half * 128 +
-                                       (lslot ^ (is_v ? vswz(row) : kswz(row))) * 16);
+        const int byte = half * 128 + (lslot ^ (is_v ? vswz(row) : kswz(row))) * 16;
+        off[j] = static_cast<uint32_t>(row * (is_v ? src.ldv : src.ldk) + byte);
+        src.lacks |= (byte >= 2 * d ? 1u : 0u) << j;
     }
 }
 
 // Units first .. first + COUNT - 1 of tile t into the slot at LDS offset `lds` (K, then V).
-template <int DH, int COUNT>
+template <int DH, bool WHOLE, int COUNT>
 __device__ __forceinline__ void tile_issue(const TileSource<DH> & src, int t, int first, const uint32_t (&off)[COUNT],
                                            uint32_t lds, int lane) {
     using F = Fast<DH>;
@@ -713,12 +733,12 @@ __device__ __forceinline__ void tile_issue(const TileSource<DH> & src, int t, in
         const int unit = first + j;
         const bool is_v = unit >= F::kUnits;
         const uint32_t at = lds + unit * 1024;
-        if (whole) {
+        if (WHOLE && whole) {
             lds_dma16_sbase(is_v ? vb : kb, off[j], at);
         } else {
             const int row = unit % (F::kKeys / 8) * 8 + (lane >> 3);
-            const char * g = kt0 + row < src.nk ? (is_v ? vb : kb) + off[j] : reinterpret_cast<const char *>(src.zero);
-            lds_dma16(g, at);
+            const bool in = kt0 + row < src.nk && (WHOLE || !(src.lacks >> j & 1u));
+            lds_dma16(in ? (is_v ? vb : kb) + off[j] : reinterpret_cast<const char *>(src.zero), at);
         }
     }
 }
@@ -740,11 +760,11 @@ __device__ __forceinline__ bool tile_odd(const char * vl, int thread, int thread
 template <int DH>
 __device__ __forceinline__ void load_q(const ScoreArgs & a, const Rows & w, int qi, int head, bool live, int h,
                                        bf16x8 (&qf)[Fast<DH>::NST]) {
-    const uint16_t * q = static_cast<const uint16_t *>(a.q) + (w.q0 + qi) * a.ldq + static_cast<int64_t>(head) * DH;
+    const uint16_t * q = static_cast<const uint16_t *>(a.q) + (w.q0 + qi) * a.ldq + static_cast<int64_t>(head) * a.d;
 #pragma unroll
     for (int st = 0; st < Fast<DH>::NST; ++st) {
         uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (live) u = *reinterpret_cast<const uint4 *>(q + (st / 4) * 64 + 32 * h + 8 * (st % 4));
+        if (live && (st / 4) * 64 + 32 * h + 8 * (st % 4) < a.d) u = *reinterpret_cast<const uint4 *>(q + (st / 4) * 64 + 32 * h + 8 * (st % 4));
         qf[st] = __builtin_bit_cast(bf16x8, u);
     }
 }
@@ -752,8 +772,8 @@ __device__ __forceinline__ void load_q(const ScoreArgs & a, const Rows & w, int 
 template <int DH>
 __device__ __forceinline__ TileSource<DH> tile_source(const ScoreArgs & a, const Rows & w) {
     TileSource<DH> s;
-    s.k = uniform_ptr(reinterpret_cast<const char *>(static_cast<const uint16_t *>(a.k) + w.k0 * a.ldk + static_cast<int64_t>(w.kv) * DH));
-    s.v = uniform_ptr(reinterpret_cast<const char *>(static_cast<const uint16_t *>(a.v) + w.k0 * a.ldv + static_cast<int64_t>(w.kv) * DH));
+    s.k = uniform_ptr(reinterpret_cast<const char *>(static_cast<const uint16_t *>(a.k) + w.k0 * a.ldk + static_cast<int64_t>(w.kv) * a.d));
+    s.v = uniform_ptr(reinterpret_cast<const char *>(static_cast<const uint16_t *>(a.v) + w.k0 * a.ldv + static_cast<int64_t>(w.kv) * a.d));
     s.ldk = a.ldk * 2;
     s.ldv = a.ldv * 2;
     s.nk = w.nk;
@@ -774,7 +794,7 @@ __device__ __forceinline__ TileSource<DH> tile_source(const ScoreArgs & a, const
 constexpr int kSlots = 4;
 constexpr float kSumLimit = 0x1p40f;
 
-template <int DH, int MODE>
+template <int DH, int MODE, bool WHOLE>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) score_attn_rows_kernel(ScoreArgs a) {
     using F = Fast<DH>;
     constexpr int kMine = 2 * F::kUnits / 4;  // DMA instructions of a wave and tile
@@ -805,13 +825,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
     const int whole = keys_all(a, w, w.row0) / F::kKeys;  // tiles below hold seen keys only
     const int wave_end = wave_row0 < w.rows ? keys_end(a, w, wave_row0 + 31) : 0;
 
-    const TileSource<DH> src = tile_source<DH>(a, w);
+    TileSource<DH> src = tile_source<DH>(a, w);
     uint32_t off[kMine];
-    tile_offsets<DH>(src, wave * kMine, lane, off);
+    tile_offsets<DH>(src, a.d, wave * kMine, lane, off);
     const uint32_t lds0 = lds_offset(&lds[0]);
     auto slot = [](int i) { return (i % kSlots) * 2 * F::kTileBytes; };
     auto issue = [&](int i) __attribute__((always_inline)) {
-        tile_issue<DH>(src, last - i, wave * kMine, off, lds0 + slot(i), lane);
+        tile_issue<DH, WHOLE>(src, last - i, wave * kMine, off, lds0 + slot(i), lane);
     };
     auto k_of = [&](int i) { return lds + slot(i); };
     auto v_of = [&](int i) { return lds + slot(i) + F::kTileBytes; };
@@ -910,38 +930,42 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
     const int64_t part = split_slot(a, w, split, row);
     if (a.splits > 1) {
         if (h == 0) a.part_ml[part] = make_float2(st.base, sum);
-        float * o = a.part + part * DH;
+        float * o = a.part + part * a.d;
 #pragma unroll
         for (int dt = 0; dt < F::NDT; ++dt)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<float4 *>(o + dt * 32 + 8 * g + 4 * h) =
-                    make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
+                if (WHOLE || dt * 32 + 8 * g + 4 * h < a.d)
+                    *reinterpret_cast<float4 *>(o + dt * 32 + 8 * g + 4 * h) =
+                        make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
         return;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint16_t * o = static_cast<uint16_t *>(a.o) + (w.q0 + qi) * a.ldo + static_cast<int64_t>(head) * DH;
+    uint16_t * o = static_cast<uint16_t *>(a.o) + (w.q0 + qi) * a.ldo + static_cast<int64_t>(head) * a.d;
 #pragma unroll
     for (int dt = 0; dt < F::NDT; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<uint2 *>(o + dt * 32 + 8 * g + 4 * h) =
-                make_uint2(pack_bf16x2(oacc[dt][4 * g] * inv, oacc[dt][4 * g + 1] * inv),
-                           pack_bf16x2(oacc[dt][4 * g + 2] * inv, oacc[dt][4 * g + 3] * inv));
+            if (WHOLE || dt * 32 + 8 * g + 4 * h < a.d)
+                *reinterpret_cast<uint2 *>(o + dt * 32 + 8 * g + 4 * h) =
+                    make_uint2(pack_bf16x2(oacc[dt][4 * g] * inv, oacc[dt][4 * g + 1] * inv),
+                               pack_bf16x2(oacc[dt][4 * g + 2] * inv, oacc[dt][4 * g + 3] * inv));
 }
 
 // Few rows a segment (new tokens over caches): a workgroup has one tile of 32 rows
-// and a chunk of the segment's keys, its four waves every fourth key tile of it, each
+// and a chunk of the segment's keys, its two waves every second key tile of it, each
 // through a ring of its own in LDS, with no barrier before the end, where the waves'
-// results are joined.  Bound by reading the keys and values once.
+// results are joined.  Bound by reading the keys and values once (4.9 TB/s, where a copy
+// reaches 4.85).  Two waves and two workgroups a CU: with four waves and one, the start and end
+// of a chunk were not hidden (158 us against 142 for eight tokens over 170,161 keys).
 //
 // Segments of up to 32 rows are cut into chunks of a.chunk keys, an item each; so long
 // and short caches of one call load the CUs alike.  Others have an item per 32 rows.
 constexpr int kFewRows = 32;
 
-template <int DH> constexpr int kFewStages = 2;
-template <int DH> constexpr int kFewWaveBytes = kFewStages<DH> * 2 * Fast<DH>::kTileBytes;
-template <int DH> constexpr int kFewBytes = 4 * kFewWaveBytes<DH> + 4 * 32 * 2 * static_cast<int>(sizeof(float));
+constexpr int kFewWaves = 2, kFewStages = 2;  // 64 KB of LDS: two workgroups a CU
+template <int DH> constexpr int kFewWaveBytes = kFewStages * 2 * Fast<DH>::kTileBytes;
+template <int DH> constexpr int kFewBytes = kFewWaves * kFewWaveBytes<DH> + kFewWaves * 32 * 2 * static_cast<int>(sizeof(float));
 
 // A wave's own LDS reads are done, and none is moved over this.
 __device__ __forceinline__ void wave_reads_done() {
@@ -950,8 +974,8 @@ __device__ __forceinline__ void wave_reads_done() {
     asm volatile("" ::: "memory");
 }
 
-template <int DH, int MODE>
-__global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
+template <int DH, int MODE, bool WHOLE>
+__global__ void __launch_bounds__(kFewWaves * 64) score_attn_few_kernel(ScoreArgs a) {
     using F = Fast<DH>;
     constexpr int kInstr = 2 * F::kUnits;
     extern __shared__ __align__(16) char smem[];
@@ -960,7 +984,7 @@ __global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
     const int h = lane >> 5, r = lane & 31;
     Rows w;
     w.kv = static_cast<int>(blockIdx.x % a.kv_heads);
-    const int64_t item = blockIdx.x / a.kv_heads;
+    const int item = static_cast<int>(blockIdx.x / a.kv_heads);
     if (!locate_rows(a, item, kFewRows, lane, w)) return;
     const bool live = w.row0 + r < w.rows;
     const int row = live ? w.row0 + r : w.rows - 1;
@@ -973,16 +997,16 @@ __global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
     }
     const RowScore rs = row_score<MODE>(a, head);
     const float cap_log2 = a.cap_log2;
-    const TileSource<DH> src = tile_source<DH>(a, w);
+    TileSource<DH> src = tile_source<DH>(a, w);
     char * ring = smem + wave * kFewWaveBytes<DH>;
     const uint32_t lds0 = lds_offset(ring);
     uint32_t off[kInstr];
-    tile_offsets<DH>(src, 0, lane, off);
-    const int n = last - first > wave ? (last - first - wave + 3) / 4 : 0;  // tiles first + wave + 4 i
-    auto tile = [&](int i) { return first + wave + 4 * i; };
-    auto slot = [](int i) { return i % kFewStages<DH> * 2 * F::kTileBytes; };
+    tile_offsets<DH>(src, a.d, 0, lane, off);
+    const int n = last - first > wave ? (last - first - wave + kFewWaves - 1) / kFewWaves : 0;
+    auto tile = [&](int i) { return first + wave + kFewWaves * i; };
+    auto slot = [](int i) { return i % kFewStages * 2 * F::kTileBytes; };
     auto issue = [&](int i) __attribute__((always_inline)) {
-        tile_issue<DH>(src, tile(i), 0, off, lds0 + slot(i), lane);
+        tile_issue<DH, WHOLE>(src, tile(i), 0, off, lds0 + slot(i), lane);
     };
     if (n > 0) issue(0);
     bf16x8 qf[F::NST];
@@ -995,10 +1019,11 @@ __global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
     for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
     RowState st{-INFINITY, 0.0f};
     bool odd = false;
-    if (n > 1) issue(1);
+#pragma unroll
+    for (int i = 1; i < kFewStages; ++i)
+        if (i < n) issue(i);
     for (int i = 0; i < n; ++i) {
-        if (i + 1 < n) wait_vmcnt(kInstr);
-        else wait_vmcnt(0);
+        wait_stages<kFewStages - 1, kInstr>(n - 1 - i);
         asm volatile("" ::: "memory");
         const char * kl = ring + slot(i);
         const char * vl = kl + F::kTileBytes;
@@ -1010,11 +1035,11 @@ __global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
                              seen - tile(i) * F::kKeys);
         tile_pv<DH>(vl, p, oacc, lane);
         wave_reads_done();
-        if (i + 2 < n) issue(i + 2);
+        if (i + kFewStages < n) issue(i + kFewStages);
     }
-    const int64_t part = (item * a.kv_heads + w.kv) * kFewRows;  // this item's rows of partial results
+    const int64_t part = (static_cast<int64_t>(item) * a.kv_heads + w.kv) * kFewRows;  // this item's rows of partial results
     if (__syncthreads_or(odd)) {
-        for (int j = wave; j < kFewRows; j += 4)
+        for (int j = wave; j < kFewRows; j += kFewWaves)
             if (w.row0 + j < w.rows)
                 row_alone<uint16_t, DH / 64>(a, w, w.row0 + j, first * F::kKeys, last * F::kKeys, lane, w.chunks > 1,
                                              part + j);
@@ -1022,7 +1047,7 @@ __global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
     }
     // The waves' results: outputs in their own rings, bases and sums behind the rings.
     float * mine = reinterpret_cast<float *>(ring);
-    float2 * ml = reinterpret_cast<float2 *>(smem + 4 * kFewWaveBytes<DH>);
+    float2 * ml = reinterpret_cast<float2 *>(smem + kFewWaves * kFewWaveBytes<DH>);
     const float sum = lane_pair_sum(st.sum);
     if (h == 0) ml[wave * 32 + r] = make_float2(st.base, sum);
 #pragma unroll
@@ -1032,63 +1057,71 @@ __global__ void __launch_bounds__(256) score_attn_few_kernel(ScoreArgs a) {
             *reinterpret_cast<float4 *>(mine + r * DH + dt * 32 + 8 * g + 4 * h) =
                 make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
     __syncthreads();
-    const int jr = tid >> 3, jc = tid & 7;  // 8 threads a row
-    if (w.row0 + jr >= w.rows) return;
-    float base = -INFINITY;
+    const int jc = tid & 7;  // 8 threads a row
 #pragma unroll
-    for (int i = 0; i < 4; ++i) base = fmaxf(base, ml[i * 32 + jr].x);
-    const float ref = base == -INFINITY ? 0.0f : base;
-    float total = 0.0f, f[4];
+    for (int jr = tid >> 3; jr < kFewRows; jr += kFewWaves * 8) {
+        if (w.row0 + jr >= w.rows) return;
+        float base = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 v = ml[i * 32 + jr];
-        f[i] = __builtin_amdgcn_exp2f(v.x - ref);
-        total += v.y * f[i];
-    }
-    const int token = (w.row0 + jr) / a.group;
-    const int to_head = w.kv * a.group + (w.row0 + jr) % a.group;
-    uint16_t * o = static_cast<uint16_t *>(a.o) + (w.q0 + token) * a.ldo + static_cast<int64_t>(to_head) * DH;
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    if (w.chunks > 1 && jc == 0) a.part_ml[part + jr] = make_float2(base, total);
+        for (int i = 0; i < kFewWaves; ++i) base = fmaxf(base, ml[i * 32 + jr].x);
+        const float ref = base == -INFINITY ? 0.0f : base;
+        float total = 0.0f, f[kFewWaves];
 #pragma unroll
-    for (int c = jc * 4; c < DH; c += 32) {
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem + i * kFewWaveBytes<DH>) + jr * DH + c);
-            v[0] += x.x * f[i]; v[1] += x.y * f[i]; v[2] += x.z * f[i]; v[3] += x.w * f[i];
+        for (int i = 0; i < kFewWaves; ++i) {
+            const float2 v = ml[i * 32 + jr];
+            f[i] = __builtin_amdgcn_exp2f(v.x - ref);
+            total += v.y * f[i];
         }
-        if (w.chunks > 1)
-            *reinterpret_cast<float4 *>(a.part + (part + jr) * DH + c) = make_float4(v[0], v[1], v[2], v[3]);
-        else
-            *reinterpret_cast<uint2 *>(o + c) = make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+        const int token = (w.row0 + jr) / a.group;
+        const int to_head = w.kv * a.group + (w.row0 + jr) % a.group;
+        uint16_t * o = static_cast<uint16_t *>(a.o) + (w.q0 + token) * a.ldo + static_cast<int64_t>(to_head) * a.d;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        if (w.chunks > 1 && jc == 0) a.part_ml[part + jr] = make_float2(base, total);
+#pragma unroll
+        for (int c = jc * 4; c < DH; c += 32) {
+            if (!WHOLE && c >= a.d) break;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < kFewWaves; ++i) {
+                const float4 x = *reinterpret_cast<const float4 *>(
+                    reinterpret_cast<const float *>(smem + i * kFewWaveBytes<DH>) + jr * DH + c);
+                v[0] += x.x * f[i]; v[1] += x.y * f[i]; v[2] += x.z * f[i]; v[3] += x.w * f[i];
+            }
+            if (w.chunks > 1)
+                *reinterpret_cast<float4 *>(a.part + (part + jr) * a.d + c) = make_float4(v[0], v[1], v[2], v[3]);
+            else
+                *reinterpret_cast<uint2 *>(o + c) =
+                    make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+        }
     }
 }
 
-// Joins the chunks of a (query, head): four waves, each every fourth chunk, then their
-// results in order.
+// Joins the chunks of a (query, head): eight groups of 32 lanes, each every eighth chunk, then
+// their results in order.  Lane l of a group has dims DH / 32 l on.
 template <int DH>
 __global__ void __launch_bounds__(256) score_join_few_kernel(ScoreArgs a) {
-    constexpr int V = DH / 64;
-    __shared__ float2 ml[4];
-    __shared__ float acc_of[4][DH];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t qi = blockIdx.x / a.heads;
+    constexpr int V = DH / 32, kGroups = 8;
+    typedef float vec __attribute__((ext_vector_type(V)));
+    __shared__ float2 ml[kGroups];
+    __shared__ float acc_of[kGroups][DH];
+    const int lane = threadIdx.x & 63, l32 = threadIdx.x & 31, grp = threadIdx.x >> 5;
+    const int qi = static_cast<int>(blockIdx.x / a.heads);
     const int head = static_cast<int>(blockIdx.x % a.heads);
     Rows w;
     w.kv = head / a.group;
-    int64_t item;
+    int item;
     if (!locate_query(a, qi, kFewRows, lane, w, item) || w.chunks <= 1) return;
-    const int64_t row = (qi - w.q0) * a.group + head % a.group;
-    const int64_t at = (item * a.kv_heads + w.kv) * kFewRows + row;
+    const int row = (qi - w.q0) * a.group + head % a.group;
+    const int64_t at = (static_cast<int64_t>(item) * a.kv_heads + w.kv) * kFewRows + row;
     const int64_t step = static_cast<int64_t>(a.kv_heads) * kFewRows;
-    float m = -INFINITY, l = 0.0f, acc[V];
-#pragma unroll
-    for (int c = 0; c < V; ++c) acc[c] = 0.0f;
-#pragma unroll 8
-    for (int i = wave; i < w.chunks; i += 4) {
+    const bool in = l32 * V < a.d;
+    float m = -INFINITY, l = 0.0f;
+    vec acc = {};
+#pragma unroll 4
+    for (int i = grp; i < w.chunks; i += kGroups) {
         const float2 p = a.part_ml[at + i * step];
-        const float * o = a.part + (at + i * step) * DH + lane * V;
+        vec o = {};
+        if (in) o = *reinterpret_cast<const vec *>(a.part + (at + i * step) * a.d + l32 * V);
         const float up = fmaxf(m, p.x), ref = up == -INFINITY ? 0.0f : up;
         const float keep = __builtin_amdgcn_exp2f(m - ref), f = __builtin_amdgcn_exp2f(p.x - ref);
         l = l * keep + p.y * f;
@@ -1096,28 +1129,23 @@ __global__ void __launch_bounds__(256) score_join_few_kernel(ScoreArgs a) {
         for (int c = 0; c < V; ++c) acc[c] = acc[c] * keep + o[c] * f;
         m = up;
     }
-    if (lane == 0) ml[wave] = make_float2(m, l);
-#pragma unroll
-    for (int c = 0; c < V; ++c) acc_of[wave][lane * V + c] = acc[c];
+    if (l32 == 0) ml[grp] = make_float2(m, l);
+    *reinterpret_cast<vec *>(&acc_of[grp][l32 * V]) = acc;
     __syncthreads();
-    if (wave != 0) return;
-    float base = -INFINITY, total = 0.0f, v[V];
+    const int dim = threadIdx.x;
+    if (dim >= a.d) return;
+    float base = -INFINITY, total = 0.0f, v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) base = fmaxf(base, ml[i].x);
+    for (int i = 0; i < kGroups; ++i) base = fmaxf(base, ml[i].x);
     const float ref = base == -INFINITY ? 0.0f : base;
 #pragma unroll
-    for (int c = 0; c < V; ++c) v[c] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kGroups; ++i) {
         const float f = __builtin_amdgcn_exp2f(ml[i].x - ref);
         total += ml[i].y * f;
-#pragma unroll
-        for (int c = 0; c < V; ++c) v[c] += acc_of[i][lane * V + c] * f;
+        v += acc_of[i][dim] * f;
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    uint16_t * o = static_cast<uint16_t *>(a.o) + qi * a.ldo + static_cast<int64_t>(head) * DH + lane * V;
-#pragma unroll
-    for (int c = 0; c < V; ++c) o[c] = f32_to_bf16(v[c] * inv);
+    static_cast<uint16_t *>(a.o)[qi * a.ldo + static_cast<int64_t>(head) * a.d + dim] = f32_to_bf16(v * inv);
 }
 
 // Joins the splits of a row: one wave per (query, head), in the splits' order.
@@ -1186,30 +1214,35 @@ constexpr int64_t kScoreMaxRows = INT32_MAX - 1023;  // rows and keys are counte
 constexpr int kWaveSegments = 64;   // segments that a wave's lanes hold; more take a table
 constexpr int kRowTile = 128;
 constexpr int64_t kSplitGrid = 512; // workgroups (two a CU) up to which a call's keys are split
+constexpr int64_t kSplitGridF32 = 1024;  // fp32: a workgroup keeps a CU's matrix cores busy, so finer
 constexpr int64_t kSplitKeys = 256; // keys that a split has at least, of the segments' mean
 
 int64_t row_tiles(int64_t total_q, int nseg, int group) { return total_q * group / kRowTile + nseg; }
 
 // Splits of the keys: as many as keep row tiles * key/value heads * splits within
 // kSplitGrid, and kSplitKeys keys each.
-int score_splits(int nseg, int64_t total_q, int64_t total_k, int kv_heads, int group) {
-    const int64_t fit = kSplitGrid / (row_tiles(total_q, nseg, group) * kv_heads);
+int score_splits(int64_t grid, int nseg, int64_t total_q, int64_t total_k, int kv_heads, int group) {
+    const int64_t fit = grid / (row_tiles(total_q, nseg, group) * kv_heads);
     return static_cast<int>(std::max<int64_t>(1, std::min(fit, total_k / nseg / kSplitKeys)));
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Rows of partial results at most: a split call has at most kSplitGrid workgroups of
+// Rows of partial results at most: a split call has at most kSplitGridF32 workgroups of
 // kRowTile rows, whatever its other sizes; so the size never falls as a call grows.
 int64_t split_rows(int64_t total_q, int64_t total_k, int heads) {
-    const int64_t most = std::max<int64_t>(1, std::min(kSplitGrid, total_k / kSplitKeys));
+    constexpr int64_t kGrid = kSplitGridF32, kMost = kGrid * kRowTile;
+    const int64_t most = std::max<int64_t>(1, std::min(kGrid, total_k / kSplitKeys));
     if (most == 1) return 0;
-    return std::min(kSplitGrid * kRowTile, total_q > kSplitGrid * kRowTile ? kSplitGrid * kRowTile : total_q * heads * most);
+    return std::min(kMost, total_q > kMost ? kMost : total_q * heads * most);
 }
 
-// Few rows a segment: keys of a chunk, so that a call has about kFewItems of them.
+// Few rows a segment: keys of a chunk, so that a call has about kFewItems items, two rounds of two
+// workgroups a CU.  Eight tokens over 170,161 keys, 8 key/value heads of 128: 142 us (4.9 TB/s) with
+// 1,024 items, 153 with 1,536, 157 with 768, 170 with 512; at least 128 keys, a tile or two for each
+// wave: one token over 1,501 keys, 16 heads of 64, 10.1 us against 11.6 with 256.
 constexpr int64_t kFewItems = 1024;
-constexpr int64_t kFewKeys = 256;  // at least, and a multiple of
+constexpr int64_t kFewKeys = 128;  // at least, and a multiple of
 int64_t few_chunk(int64_t total_k, int kv_heads) {
     const int64_t keys = (total_k * kv_heads + kFewItems - 1) / kFewItems;
     return std::min<int64_t>(std::max<int64_t>(1, (keys + kFewKeys - 1) / kFewKeys) * kFewKeys, 1 << 30);
@@ -1253,22 +1286,22 @@ template <typename F> int with_mode(const ScoreArgs & a, F && launch) {
     return launch(std::integral_constant<int, 0>{});
 }
 
-template <int DH>
+template <int DH, bool WHOLE>
 int run_rows(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
     return with_mode(a, [&](auto mode) {
-        hipLaunchKernelGGL((score_attn_rows_kernel<DH, decltype(mode)::value>), dim3(static_cast<unsigned>(blocks)),
+        hipLaunchKernelGGL((score_attn_rows_kernel<DH, decltype(mode)::value, WHOLE>), dim3(static_cast<unsigned>(blocks)),
                            dim3(256), 0, s, a);
         return check_launch("scored attention");
     });
 }
 
-template <int DH>
+template <int DH, bool WHOLE>
 int run_few(const ScoreArgs & a, int64_t blocks, bool join, hipStream_t s) {
     const int rc = with_mode(a, [&](auto mode) {
-        auto kernel = &score_attn_few_kernel<DH, decltype(mode)::value>;
+        auto kernel = &score_attn_few_kernel<DH, decltype(mode)::value, WHOLE>;
         static std::atomic<uint64_t> done{0};
         if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), kFewBytes<DH>, done, "hipFuncSetAttribute(score_attn_few)")) return rc;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), kFewBytes<DH>, s, a);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kFewWaves * 64), kFewBytes<DH>, s, a);
         return check_launch("scored attention of few rows");
     });
     if (rc || !join) return rc;
@@ -1336,7 +1369,7 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
     a.vec = rows_of_pieces(q, ld_q, head_dim, elem) && rows_of_pieces(k, ld_k, head_dim, elem) &&
             rows_of_pieces(v, ld_v, head_dim, elem);
     // The fast kernels' 32-bit offsets within a key tile hold row strides below 2^24.
-    const bool fast = dtype == PXS_BF16 && (head_dim == 64 || head_dim == 128) && a.vec && ld_k < (1 << 24) &&
+    const bool fast = dtype == PXS_BF16 && head_dim <= 128 && a.vec && ld_k < (1 << 24) &&
                       ld_v < (1 << 24) && reinterpret_cast<uintptr_t>(o) % 8 == 0 && ld_o % 4 == 0;
     const bool few = fast && few_rows(total_q, nseg, a.group);
     a.splits = 1;
@@ -1348,7 +1381,7 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
         part_rows = blocks * kFewRows;
     } else {
         a.tiles = row_tiles(total_q, nseg, a.group);
-        a.splits = score_splits(nseg, total_q, total_k, kv_heads, a.group);
+        a.splits = score_splits(dtype == PXS_F32 ? kSplitGridF32 : kSplitGrid, nseg, total_q, total_k, kv_heads, a.group);
         blocks = a.tiles * kv_heads * a.splits;
         if (a.splits > 1) part_rows = a.splits * total_q * heads;
     }
@@ -1366,10 +1399,14 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
     a.part = reinterpret_cast<float *>(ws + round256(static_cast<size_t>(part_rows) * sizeof(float2)));
     if (few) {
         const bool join = total_k > a.chunk;  // otherwise no segment is cut
-        return head_dim == 64 ? run_few<64>(a, blocks, join, s) : run_few<128>(a, blocks, join, s);
+        if (head_dim == 64) return run_few<64, true>(a, blocks, join, s);
+        if (head_dim == 128) return run_few<128, true>(a, blocks, join, s);
+        return head_dim < 64 ? run_few<64, false>(a, blocks, join, s) : run_few<128, false>(a, blocks, join, s);
     }
     int rc;
-    if (fast) rc = head_dim == 64 ? run_rows<64>(a, blocks, s) : run_rows<128>(a, blocks, s);
+    if (fast && head_dim == 64) rc = run_rows<64, true>(a, blocks, s);
+    else if (fast && head_dim == 128) rc = run_rows<128, true>(a, blocks, s);
+    else if (fast) rc = head_dim < 64 ? run_rows<64, false>(a, blocks, s) : run_rows<128, false>(a, blocks, s);
     else rc = dtype == PXS_F32 ? run_any<float>(a, blocks, s) : run_any<uint16_t>(a, blocks, s);
     if (rc || a.splits == 1) return rc;
     const dim3 grid(grid_for(total_q * heads, 4));

@@ -47,6 +47,33 @@ __device__ __forceinline__ float2 turn(int32_t position, double freq, float magn
     return make_float2(((q + 1) & 2) ? -cs * magnitude : cs * magnitude, (q & 2) ? -sn * magnitude : sn * magnitude);
 }
 
+// Every 256th (row, head, unit of a head) from the thread's own, without a division a step.
+struct UnitWalk {
+    int row, head, unit, heads, units, step_row, step_head, step_unit;
+    __device__ __forceinline__ UnitWalk(int h, int u) : heads(h), units(u) {
+        const int per_row = h * u, t = threadIdx.x;
+        row = t / per_row;
+        head = t % per_row / u;
+        unit = t % u;
+        step_row = 256 / per_row;
+        step_head = 256 % per_row / u;
+        step_unit = 256 % u;
+    }
+    __device__ __forceinline__ void next() {
+        unit += step_unit;
+        head += step_head;
+        row += step_row;
+        if (unit >= units) {
+            unit -= units;
+            ++head;
+        }
+        if (head >= heads) {
+            head -= heads;
+            ++row;
+        }
+    }
+};
+
 // One value pair or one value of the rest per thread: heads, widths, strides and
 // alignments of any kind.
 template <typename T, bool HALF>
@@ -63,11 +90,10 @@ __global__ void __launch_bounds__(256) rope_any_kernel(RopeArgs a) {
         for (int i = threadIdx.x; i < rows * pairs; i += 256)
             turns[i] = turn(a.positions[row0 + i / pairs], a.freq[i % pairs], a.magnitude);
         __syncthreads();
-        const int per_row = a.heads * units;
-        for (int i = threadIdx.x; i < rows * per_row; i += 256) {
-            const int r = i / per_row, head = i % per_row / units, u = i % units;
-            const T * xs = x + (row0 + r) * a.ldx + static_cast<int64_t>(head) * a.head_dim;
-            T * ys = y + (row0 + r) * a.ldy + static_cast<int64_t>(head) * a.head_dim;
+        for (UnitWalk at(a.heads, units); at.row < rows; at.next()) {
+            const int r = at.row, u = at.unit;
+            const T * xs = x + (row0 + r) * a.ldx + static_cast<int64_t>(at.head) * a.head_dim;
+            T * ys = y + (row0 + r) * a.ldy + static_cast<int64_t>(at.head) * a.head_dim;
             if (u < pairs) {
                 const int ia = HALF ? u : 2 * u, ib = HALF ? u + pairs : 2 * u + 1;
                 const float va = load_f32(xs + ia), vb = load_f32(xs + ib);
@@ -81,17 +107,90 @@ __global__ void __launch_bounds__(256) rope_any_kernel(RopeArgs a) {
     }
 }
 
+// Heads, halves and rests of whole vectors: V values (16 bytes) a lane and load.  The same
+// steps as above with a vector of pairs per unit; interleaved pairs lie inside a vector, those
+// of the half layout in two vectors rotary / 2 apart.  Bound by reading and writing the heads once:
+// 32,768 x 32 heads of 64 in bf16 44 us, 6.1 TB/s (92 us a value at a time).
+template <typename T, int V> struct RopeVec {
+    T v[V];
+};
+
+template <typename T, bool HALF>
+__global__ void __launch_bounds__(256) rope_vec_kernel(RopeArgs a) {
+    constexpr int V = 16 / static_cast<int>(sizeof(T));
+    using Vec = RopeVec<T, V>;
+    extern __shared__ float2 turns[];  // [rows of the block][rotary / 2]
+    const int pairs = a.rotary / 2;
+    const int turned = HALF ? pairs / V : a.rotary / V;  // units of a head that are turned
+    const int units = turned + (a.head_dim - a.rotary) / V;
+    const T * x = static_cast<const T *>(a.x);
+    T * y = static_cast<T *>(a.y);
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.rows_per_block; row0 < a.rows;
+         row0 += static_cast<int64_t>(gridDim.x) * a.rows_per_block) {
+        const int rows = static_cast<int>(min(static_cast<int64_t>(a.rows_per_block), a.rows - row0));
+        __syncthreads();  // the turns of the rows before have been read
+        for (int i = threadIdx.x; i < rows * pairs; i += 256)
+            turns[i] = turn(a.positions[row0 + i / pairs], a.freq[i % pairs], a.magnitude);
+        __syncthreads();
+        for (UnitWalk walk(a.heads, units); walk.row < rows; walk.next()) {
+            const int r = walk.row, u = walk.unit;
+            const int64_t col = static_cast<int64_t>(walk.head) * a.head_dim;
+            const T * xs = x + (row0 + r) * a.ldx + col;
+            T * ys = y + (row0 + r) * a.ldy + col;
+            const float2 * t = turns + r * pairs;
+            if (u >= turned) {
+                const int at = a.rotary + (u - turned) * V;
+                *reinterpret_cast<uint4 *>(ys + at) = *reinterpret_cast<const uint4 *>(xs + at);
+            } else if constexpr (HALF) {
+                const int at = u * V;
+                Vec va = *reinterpret_cast<const Vec *>(__builtin_assume_aligned(xs + at, 16));
+                Vec vb = *reinterpret_cast<const Vec *>(__builtin_assume_aligned(xs + at + pairs, 16));
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float p = load_f32(&va.v[e]), q = load_f32(&vb.v[e]);
+                    const float2 c = t[at + e];
+                    store_f32(&va.v[e], p * c.x - q * c.y);
+                    store_f32(&vb.v[e], p * c.y + q * c.x);
+                }
+                *reinterpret_cast<uint4 *>(ys + at) = __builtin_bit_cast(uint4, va);
+                *reinterpret_cast<uint4 *>(ys + at + pairs) = __builtin_bit_cast(uint4, vb);
+            } else {
+                const int at = u * V;
+                Vec va = *reinterpret_cast<const Vec *>(__builtin_assume_aligned(xs + at, 16));
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                    const float p = load_f32(&va.v[2 * e]), q = load_f32(&va.v[2 * e + 1]);
+                    const float2 c = t[at / 2 + e];
+                    store_f32(&va.v[2 * e], p * c.x - q * c.y);
+                    store_f32(&va.v[2 * e + 1], p * c.y + q * c.x);
+                }
+                *reinterpret_cast<uint4 *>(ys + at) = __builtin_bit_cast(uint4, va);
+            }
+        }
+    }
+}
+
 constexpr int kRopeMaxDim = 1024;
 
 template <typename T>
 int launch_rope(RopeArgs a, bool half, hipStream_t s) {
-    a.rows_per_block = 1;
+    constexpr int V = 16 / static_cast<int>(sizeof(T));
+    const bool vec = a.head_dim % V == 0 && a.rotary % (half ? 2 * V : V) == 0 && a.ldx % V == 0 && a.ldy % V == 0 &&
+                     reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
+    // Rows of a workgroup: about 4096 values (32,768 x 32 heads of 64, half layout: 44 us, with 2048
+    // 47, with 16,384 51), if that leaves two workgroups a CU.
+    const int64_t row = static_cast<int64_t>(a.heads) * a.head_dim;
+    a.rows_per_block = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, 4096 / row),
+                                                          std::max<int64_t>(1, a.rows / 512)));
+    a.rows_per_block = std::min(a.rows_per_block, 32);
     const int smem = a.rows_per_block * (a.rotary / 2) * static_cast<int>(sizeof(float2));
     const int64_t blocks = std::min<int64_t>((a.rows + a.rows_per_block - 1) / a.rows_per_block, 1 << 20);
     auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), smem, s, a);
     };
-    if (half) launch(rope_any_kernel<T, true>);
+    if (vec && half) launch(rope_vec_kernel<T, true>);
+    else if (vec) launch(rope_vec_kernel<T, false>);
+    else if (half) launch(rope_any_kernel<T, true>);
     else launch(rope_any_kernel<T, false>);
     return check_launch("rotary positions");
 }
