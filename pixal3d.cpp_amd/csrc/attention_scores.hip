@@ -316,7 +316,8 @@ template <typename T, int DP> struct AnyTile {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1)))
+score_attn_any_kernel(ScoreArgs a) {
     using Tile = AnyTile<T, DP>;
     constexpr int kVec = 16 / static_cast<int>(sizeof(T)), kKeys = Tile::kKeys, KT = kKeys / 32, DT = DP / 32;
     constexpr int kPieces = DP / kVec;  // 16-byte pieces of a padded row
@@ -366,30 +367,41 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
     const int tile_all = keys_all(a, w, w.row0);
     bool again = false;
 
+    // This thread's pieces of a K and a V tile, the next tile's loaded while one is multiplied.
+    constexpr int kMine = kKeys * kPieces / 256;
+    T kk[kMine][kVec], vv[kMine][kVec];
+    auto load = [&](int kt0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const int key = (tid + 256 * j) / kPieces, piece = (tid + 256 * j) % kPieces;
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) kk[j][e] = vv[j][e] = T(0);
+            if (kt0 + key < w.nk) {
+                load_dims<T>(k + static_cast<int64_t>(kt0 + key) * a.ldk, piece * kVec, a.d, a.vec, kk[j]);
+                load_dims<T>(v + static_cast<int64_t>(kt0 + key) * a.ldv, piece * kVec, a.d, a.vec, vv[j]);
+            }
+        }
+    };
+    if (kt_first < kt_last) load(kt_first * kKeys);
     for (int kt0 = kt_first * kKeys; kt0 < kt_last * kKeys; kt0 += kKeys) {
         __syncthreads();
         bool odd = false;
-        for (int c = tid; c < kKeys * kPieces; c += 256) {
-            const int key = c / kPieces, piece = c % kPieces;
-            T kk[kVec], vv[kVec];
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) kk[e] = vv[e] = T(0);
-            if (kt0 + key < w.nk) {
-                load_dims<T>(k + static_cast<int64_t>(kt0 + key) * a.ldk, piece * kVec, a.d, a.vec, kk);
-                load_dims<T>(v + static_cast<int64_t>(kt0 + key) * a.ldv, piece * kVec, a.d, a.vec, vv);
-            }
-            *reinterpret_cast<uint4 *>(k_lds + key * Tile::kKPitch + piece * 16) = *reinterpret_cast<const uint4 *>(kk);
+        for (int j = 0; j < kMine; ++j) {
+            const int key = (tid + 256 * j) / kPieces, piece = (tid + 256 * j) % kPieces;
+            *reinterpret_cast<uint4 *>(k_lds + key * Tile::kKPitch + piece * 16) = *reinterpret_cast<const uint4 *>(kk[j]);
             if constexpr (!Tile::kTransposed)
-                *reinterpret_cast<uint4 *>(v_lds + key * Tile::kVPitch + piece * 16) = *reinterpret_cast<const uint4 *>(vv);
+                *reinterpret_cast<uint4 *>(v_lds + key * Tile::kVPitch + piece * 16) = *reinterpret_cast<const uint4 *>(vv[j]);
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
-                odd |= !is_finite_bits(load_f32(&vv[e]));
+                odd |= !is_finite_bits(load_f32(&vv[j][e]));
                 if constexpr (Tile::kTransposed)
-                    *reinterpret_cast<T *>(v_lds + (piece * kVec + e) * Tile::kVPitch + key * static_cast<int>(sizeof(T))) = vv[e];
+                    *reinterpret_cast<T *>(v_lds + (piece * kVec + e) * Tile::kVPitch + key * static_cast<int>(sizeof(T))) = vv[j][e];
             }
         }
         // A tile with keys that some row does not see, and values that are not finite.
         again |= __syncthreads_or(odd && min(kt0 + kKeys, w.nk) > tile_all);
+        if (kt0 + kKeys < kt_last * kKeys) load(kt0 + kKeys);
         if (wave_row0 >= w.rows) continue;
 
         f32x16 s[KT];
@@ -421,26 +433,36 @@ __global__ void __launch_bounds__(256) score_attn_any_kernel(ScoreArgs a) {
         const bool masked = kt0 + kKeys > wave_all || kt0 + kKeys > w.nk;
         const int behind = qi + w.shift - kt0, seen = my_end - kt0;
         float top = -INFINITY;
+        if (a.cap_log2 > 0.0f || a.slopes || masked) {
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int key = kt * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-                float z = score_log2(a, s[kt][e], slope, static_cast<float>(behind - key));
-                if (masked && key >= seen) z = -INFINITY;
-                s[kt][e] = z;
-                top = fmaxf(top, z);
-            }
+                for (int e = 0; e < 16; ++e) {
+                    const int key = kt * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+                    float z = score_log2(a, s[kt][e], slope, static_cast<float>(behind - key));
+                    if (key >= seen) z = -INFINITY;
+                    s[kt][e] = z;
+                    top = fmaxf(top, z);
+                }
+        } else {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[kt][e] *= a.scale_log2;
+                    top = fmaxf(top, s[kt][e]);
+                }
+        }
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float up = fmaxf(m, top);
         const float base = up == -INFINITY ? 0.0f : up;  // nothing seen yet: every weight is 0
-        const float keep = exp2f(m - base);
+        const float keep = __builtin_amdgcn_exp2f(m - base);
         float sum = 0.0f;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const float p = exp2f(s[kt][e] - base);
+                const float p = __builtin_amdgcn_exp2f(s[kt][e] - base);  // (0 below 2^-126)
                 s[kt][e] = p;
                 sum += p;
             }
@@ -1148,31 +1170,41 @@ __global__ void __launch_bounds__(256) score_join_few_kernel(ScoreArgs a) {
     static_cast<uint16_t *>(a.o)[qi * a.ldo + static_cast<int64_t>(head) * a.d + dim] = f32_to_bf16(v * inv);
 }
 
-// Joins the splits of a row: one wave per (query, head), in the splits' order.
+// Joins the splits of a (query, head), in their order: a thread has four of its dims.
 template <typename T>
 __global__ void __launch_bounds__(256) score_join_kernel(ScoreArgs a) {
-    const int lane = threadIdx.x & 63;
+    const int quads = (a.d + 3) / 4;
     const int64_t rows = a.total_q * a.heads;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t row = i / quads;
+    const int dim = static_cast<int>(i % quads) * 4, dims = min(4, a.d - dim);
     if (row >= rows || row < a.cu_q[0] * a.heads || row >= a.cu_q[a.nseg] * a.heads) return;  // (rows of no segment)
-    float m = -INFINITY;
-    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, a.part_ml[i * rows + row].x);
-    const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < a.splits; ++i) {
-        const float2 ml = a.part_ml[i * rows + row];
-        if (ml.y == 0.0f) continue;  // saw nothing
-        const float f = exp2f(ml.x - base);
-        l += ml.y * f;
+    float m = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+        const int64_t at = s * rows + row;
+        const float2 ml = a.part_ml[at];
+        const float * o = a.part + at * a.d + dim;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (dims == 4) {
+            __builtin_memcpy(v, o, 16);
+        } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (lane + 64 * c < a.d) acc[c] += a.part[(i * rows + row) * a.d + lane + 64 * c] * f;
+            for (int c = 0; c < 4; ++c)
+                if (c < dims) v[c] = o[c];
+        }
+        const float up = fmaxf(m, ml.x), ref = up == -INFINITY ? 0.0f : up;
+        const float keep = exp2f(m - ref), f = exp2f(ml.x - ref);  // 0 for a split that saw nothing
+        l = l * keep + ml.y * f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] = acc[c] * keep + v[c] * f;
+        m = up;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T * o = static_cast<T *>(a.o) + row / a.heads * a.ldo + row % a.heads * a.d;
+    T * o = static_cast<T *>(a.o) + row / a.heads * a.ldo + row % a.heads * a.d + dim;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-        if (lane + 64 * c < a.d) store_f32(o + lane + 64 * c, acc[c] * inv);
+        if (c < dims) store_f32(o + c, acc[c] * inv);
 }
 
 // tile_start[s] = items of the segments before s, for more segments than a wave's lanes.
@@ -1409,7 +1441,7 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
     else if (fast) rc = head_dim < 64 ? run_rows<64, false>(a, blocks, s) : run_rows<128, false>(a, blocks, s);
     else rc = dtype == PXS_F32 ? run_any<float>(a, blocks, s) : run_any<uint16_t>(a, blocks, s);
     if (rc || a.splits == 1) return rc;
-    const dim3 grid(grid_for(total_q * heads, 4));
+    const dim3 grid(grid_for(total_q * heads * ((head_dim + 3) / 4), 256));
     if (dtype == PXS_F32) hipLaunchKernelGGL(score_join_kernel<float>, grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL(score_join_kernel<uint16_t>, grid, dim3(256), 0, s, a);
     return check_launch("scored attention join");
