@@ -533,7 +533,9 @@ score_attn_any_kernel(ScoreArgs a) {
 
 __device__ __align__(16) uint4 g_score_zero[8];  // what keys past a segment's end are read as
 
-constexpr int kCap = 1, kBias = 2;  // MODE bits: scores are capped, biased
+// MODE bits: scores are capped, biased, and of a biased call that its mask lets queries see only keys at
+// or before them in the tiles taken without a maximum.
+constexpr int kCap = 1, kBias = 2, kBehind = 4;
 
 // Head sizes that are multiples of 8 up to 128 run as the next of 64 and 128 (WHOLE false): the
 // missing pieces of a row come from a line of zeros.
@@ -632,11 +634,19 @@ struct RowState {
 
 // Weights of a tile relative to state.base: p = 2^(z - base), and their sum over this lane.
 // behind: the lane's query position minus the tile's first key and 4 h.
+// With kBehind the bias is a line over the keys, one operation a score and not two.
 template <int DH, int MODE>
 __device__ __forceinline__ float tile_weights(const RowScore & rs, float cap_log2, const typename Fast<DH>::Scores & s,
                                               typename Fast<DH>::Weights & p, float base, float behind) {
     const bf16x2 ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
     const float add = MODE & kCap ? cap_log2 - base : -base;
+    const float start = MODE & kBehind ? __builtin_fmaf(rs.slope, behind, add) : 0.0f;
+    auto weight = [&](int kt, int e) __attribute__((always_inline)) {
+        const float key = static_cast<float>(key_of(kt, e));
+        const float z = MODE & kBehind ? score_of<MODE & kCap>(rs, s[kt][e], __builtin_fmaf(rs.slope, -key, start), 0.0f)
+                                       : score_of<MODE>(rs, s[kt][e], add, behind - key);
+        return static_cast<__bf16>(__builtin_amdgcn_exp2f(z));
+    };
     float sum = 0.0f;
 #pragma unroll
     for (int kt = 0; kt < Fast<DH>::KT; ++kt)
@@ -646,10 +656,8 @@ __device__ __forceinline__ float tile_weights(const RowScore & rs, float cap_log
             for (int e = 0; e < 8; e += 2) {
                 const int i = 8 * u + e;
                 bf16x2 pp;
-                pp[0] = static_cast<__bf16>(__builtin_amdgcn_exp2f(
-                    score_of<MODE>(rs, s[kt][i], add, behind - static_cast<float>(key_of(kt, i)))));
-                pp[1] = static_cast<__bf16>(__builtin_amdgcn_exp2f(
-                    score_of<MODE>(rs, s[kt][i + 1], add, behind - static_cast<float>(key_of(kt, i + 1)))));
+                pp[0] = weight(kt, i);
+                pp[1] = weight(kt, i + 1);
                 p[kt][u][e] = pp[0];
                 p[kt][u][e + 1] = pp[1];
                 sum = __builtin_amdgcn_fdot2_f32_bf16(pp, ones, sum, false);  // of the rounded weights
@@ -844,7 +852,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
     load_q<DH>(a, w, qi, head, live, h, qf);
     const int seen = keys_end(a, w, row) - 4 * h;
     const int pos = qi + w.shift - 4 * h;
-    const int whole = keys_all(a, w, w.row0) / F::kKeys;  // tiles below hold seen keys only
+    // Tiles below hold seen keys only, and with kBehind none after a query.
+    const int first_pos = w.row0 / a.group + w.shift;
+    const int whole = max(MODE & kBehind ? min(keys_all(a, w, w.row0), first_pos + 1) : keys_all(a, w, w.row0), 0) / F::kKeys;
     const int wave_end = wave_row0 < w.rows ? keys_end(a, w, wave_row0 + 31) : 0;
 
     TileSource<DH> src = tile_source<DH>(a, w);
@@ -1309,7 +1319,11 @@ int run_any(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
 }
 
 // kernel<mode of the call>
-template <typename F> int with_mode(const ScoreArgs & a, F && launch) {
+template <bool BEHIND, typename F> int with_mode(const ScoreArgs & a, F && launch) {
+    if (BEHIND && a.slopes && a.causal) {
+        if (a.cap_log2 > 0.0f) return launch(std::integral_constant<int, kCap | kBias | kBehind>{});
+        return launch(std::integral_constant<int, kBias | kBehind>{});
+    }
     if (a.cap_log2 > 0.0f) {
         if (a.slopes) return launch(std::integral_constant<int, kCap | kBias>{});
         return launch(std::integral_constant<int, kCap>{});
@@ -1320,7 +1334,7 @@ template <typename F> int with_mode(const ScoreArgs & a, F && launch) {
 
 template <int DH, bool WHOLE>
 int run_rows(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
-    return with_mode(a, [&](auto mode) {
+    return with_mode<true>(a, [&](auto mode) {
         hipLaunchKernelGGL((score_attn_rows_kernel<DH, decltype(mode)::value, WHOLE>), dim3(static_cast<unsigned>(blocks)),
                            dim3(256), 0, s, a);
         return check_launch("scored attention");
@@ -1329,7 +1343,7 @@ int run_rows(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
 
 template <int DH, bool WHOLE>
 int run_few(const ScoreArgs & a, int64_t blocks, bool join, hipStream_t s) {
-    const int rc = with_mode(a, [&](auto mode) {
+    const int rc = with_mode<false>(a, [&](auto mode) {
         auto kernel = &score_attn_few_kernel<DH, decltype(mode)::value, WHOLE>;
         static std::atomic<uint64_t> done{0};
         if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), kFewBytes<DH>, done, "hipFuncSetAttribute(score_attn_few)")) return rc;
