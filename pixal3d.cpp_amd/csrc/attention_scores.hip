@@ -38,7 +38,7 @@ struct ScoreArgs {
     const int64_t * cu_q;
     const int64_t * cu_k;
     int nseg;
-    int64_t total_q;
+    int64_t total_q, total_k;
     const int64_t * tile_start;  // [nseg + 1] items before each segment; null: at most 64 segments
     int chunk;                   // keys of an item of a segment with one row tile; 0: not cut
     int heads, kv_heads, group, d;
@@ -80,11 +80,12 @@ __device__ __forceinline__ int64_t segment_items(int64_t nq, int64_t nk, int gro
 struct Segment {
     int q0, k0, nq, nk, prefix;
 };
+// (Bounds are kept within the call's rows, whatever cu_q and cu_k hold.)
 __device__ __forceinline__ Segment load_segment(const ScoreArgs & a, int s) {
-    const int64_t q0 = a.cu_q[s], q1 = a.cu_q[s + 1], k0 = a.cu_k[s], k1 = a.cu_k[s + 1];
-    const int64_t prefix = a.causal && a.prefix ? a.prefix[s] : 0;
-    return {static_cast<int>(q0), static_cast<int>(k0), static_cast<int>(q1 - q0), static_cast<int>(k1 - k0),
-            static_cast<int>(max(min(prefix, k1 - k0), int64_t(0)))};
+    auto within = [](int64_t v, int64_t lo, int64_t hi) { return static_cast<int>(max(min(v, hi), lo)); };
+    const int q0 = within(a.cu_q[s], 0, a.total_q), q1 = within(a.cu_q[s + 1], q0, a.total_q);
+    const int k0 = within(a.cu_k[s], 0, a.total_k), k1 = within(a.cu_k[s + 1], k0, a.total_k);
+    return {q0, k0, q1 - q0, k1 - k0, a.causal && a.prefix ? within(a.prefix[s], 0, k1 - k0) : 0};
 }
 // The segment that lane `from` (the same in all lanes) holds.
 __device__ __forceinline__ Segment segment_of(const Segment & g, int from) {
@@ -99,8 +100,8 @@ __device__ __forceinline__ Segment lane_segment(const ScoreArgs & a, int lane) {
     return g;
 }
 
-// Item i of a segment.
-__device__ __forceinline__ void segment_rows(const ScoreArgs & a, const Segment & g, int i, int rows_per_tile, Rows & w) {
+// Item i of a segment; false where it has no such rows.
+__device__ __forceinline__ bool segment_rows(const ScoreArgs & a, const Segment & g, int i, int rows_per_tile, Rows & w) {
     w.q0 = g.q0;
     w.k0 = g.k0;
     w.nk = g.nk;
@@ -111,6 +112,7 @@ __device__ __forceinline__ void segment_rows(const ScoreArgs & a, const Segment 
     w.row0 = cut ? 0 : i * rows_per_tile;
     w.chunk = cut ? i : 0;
     w.chunks = !cut ? 1 : g.nk > 0 ? (g.nk - 1) / a.chunk + 1 : 0;
+    return w.row0 < w.rows;
 }
 
 // v summed over the lanes up to each.
@@ -128,17 +130,15 @@ __device__ __forceinline__ bool locate_rows(const ScoreArgs & a, int t, int rows
     if (a.tile_start) {
         if (t >= a.tile_start[a.nseg]) return false;
         const int seg = __builtin_amdgcn_readfirstlane(find_segment(a.tile_start, a.nseg, t, lane));
-        segment_rows(a, load_segment(a, seg), __builtin_amdgcn_readfirstlane(static_cast<int>(t - a.tile_start[seg])),
-                     rows_per_tile, w);
-        return true;
+        return segment_rows(a, load_segment(a, seg), __builtin_amdgcn_readfirstlane(static_cast<int>(t - a.tile_start[seg])),
+                            rows_per_tile, w);
     }
     const Segment g = lane_segment(a, lane);
     const int items = static_cast<int>(segment_items(g.nq, g.nk, a.group, rows_per_tile, a.chunk));
     const int end = lane_sums(items, lane);
     const int seg = __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < a.nseg && end <= t)));  // those that end at or before t
     if (seg >= a.nseg) return false;
-    segment_rows(a, segment_of(g, seg), t - __builtin_amdgcn_readlane(end - items, seg), rows_per_tile, w);
-    return true;
+    return segment_rows(a, segment_of(g, seg), t - __builtin_amdgcn_readlane(end - items, seg), rows_per_tile, w);
 }
 
 // Row tiles of a segment with `tiles` of them whose rows see fewer than x keys (they come first:
@@ -179,8 +179,7 @@ __device__ __forceinline__ bool locate_sorted(const ScoreArgs & a, int t, int ro
     const int at = t - ahead;
     const int seg = __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < a.nseg && end <= at)));
     const int within = at - __builtin_amdgcn_readlane(end - (hi - lo), seg);
-    segment_rows(a, segment_of(g, seg), __builtin_amdgcn_readlane(hi, seg) - 1 - within, rows_per_tile, w);
-    return true;
+    return segment_rows(a, segment_of(g, seg), __builtin_amdgcn_readlane(hi, seg) - 1 - within, rows_per_tile, w);
 }
 
 // A workgroup's row tile and split: key/value heads next to one another, so that an XCD, which
@@ -201,8 +200,7 @@ __device__ __forceinline__ bool locate_query(const ScoreArgs & a, int qi, int ro
         if (qi < a.cu_q[0] || qi >= a.cu_q[a.nseg]) return false;
         const int seg = find_segment(a.cu_q, a.nseg, qi, lane);
         item = static_cast<int>(a.tile_start[seg]);
-        segment_rows(a, load_segment(a, seg), 0, rows_per_tile, w);
-        return true;
+        return segment_rows(a, load_segment(a, seg), 0, rows_per_tile, w);
     }
     const Segment g = lane_segment(a, lane);
     const int items = static_cast<int>(segment_items(g.nq, g.nk, a.group, rows_per_tile, a.chunk));
@@ -211,8 +209,7 @@ __device__ __forceinline__ bool locate_query(const ScoreArgs & a, int qi, int ro
     if (mine == 0) return false;
     const int seg = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<long long>(mine)) - 1);
     item = __builtin_amdgcn_readlane(end - items, seg);
-    segment_rows(a, segment_of(g, seg), 0, rows_per_tile, w);
-    return true;
+    return segment_rows(a, segment_of(g, seg), 0, rows_per_tile, w);
 }
 
 // One past the last key that any of the rows up to `row` (inclusive) sees.
@@ -1406,7 +1403,7 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
     hipStream_t s = as_stream(stream);
     ScoreArgs a{};
     a.q = q; a.k = k; a.v = v; a.ldq = ld_q; a.ldk = ld_k; a.ldv = ld_v;
-    a.cu_q = cu_q; a.cu_k = cu_k; a.nseg = nseg; a.total_q = total_q;
+    a.cu_q = cu_q; a.cu_k = cu_k; a.nseg = nseg; a.total_q = total_q; a.total_k = total_k;
     a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.d = head_dim;
     a.scale_log2 = cap > 0.0f ? scale / cap : scale * kLog2e;
     a.cap_log2 = cap * kLog2e;

@@ -736,6 +736,7 @@ int launch_i8_any(const I8Args & a, hipStream_t s) {
 template <typename T, int RB, int EPI>
 int launch_i8_few(const I8Args & a, hipStream_t s) {
     const dim3 grid(grid_for(a.n, 16), grid_for(a.m, 16 * RB));
+    if (int rc = check_i8_grid(grid.x, kFewWaves * 64)) return rc;
     hipLaunchKernelGGL((linear_i8_few_kernel<T, RB, EPI>), grid, dim3(kFewWaves * 64), 0, s, a);
     return check_launch("8-bit linear of few rows");
 }
