@@ -21,6 +21,7 @@
 // fp32, and a second launch joins them in order.
 
 #include "attn_common.h"
+#include "split3.h"
 #include "tiles.h"
 
 #include <algorithm>
@@ -299,35 +300,41 @@ __device__ __forceinline__ int64_t split_slot(const ScoreArgs & a, const Rows & 
 // Any dtype, head size up to DP, stride and alignment.  Four waves of 32 rows
 // share tiles of kKeys keys, staged through registers into LDS.  As in
 // attention.hip a wave computes S^T = K Q^T, so that a lane owns one row and half of
-// its scores, and O^T += V^T P^T with P straight from those registers.  bf16 reads four keys
-// of a dim at a time, so its V is staged transposed; fp32 reads one, 32 dims side by side, from V as
-// it lies.  Waves past the segment's rows only help to stage: a new token's tile
-// costs one wave's products.  fp32 is bound by v_mfma_f32_32x32x2_f32 (64 cycles, 153 TFLOP/s in a
-// large product here).
-template <typename T, int DP> struct AnyTile {
+// its scores, and O^T += V^T P^T with P straight from those registers.  Waves past the segment's
+// rows only help to stage: a new token's tile costs one wave's products.
+//
+// bf16: V is staged transposed, four keys of a dim a read.
+// fp32, SPLIT (heads up to 128): operands and weights split in three bf16 terms, six of their
+//   products (split3.h), 192 cycles where v_mfma_f32_32x32x2_f32 takes 512; K and V in three planes,
+//   laid out as the bf16 kernels' tiles are.  Bound by the vector instructions that split beside the
+//   matrix cores.  A workgroup that meets values the terms may not hold (above 2^50, not finite, or in V
+//   below 2^-110 and not zero) writes nothing and takes the next form.  (The scores' losses stay under
+//   128 x 2^50 x 2^-134 of the scale, at most 2^41.)  4,000 tokens, 16 heads of 64: SPLIT_US us against 644.
+// fp32 otherwise: v_mfma_f32_32x32x2_f32, V read as it lies, 32 dims of a key side by side.
+template <typename T, int DP, bool SPLIT> struct AnyTile {
     static constexpr bool kTransposed = sizeof(T) == 2;
     static constexpr int kKeys = DP == 64 ? 64 : 32;
+    static constexpr int kPlane = kKeys * DP * 2;  // SPLIT: one term of a K or V tile
     static constexpr int kKPitch = DP * static_cast<int>(sizeof(T)) + 16;
     static constexpr int kVPitch = kTransposed ? kKeys * 2 + 8 : kKPitch;
-    static constexpr int kBytes = kKeys * kKPitch + (kTransposed ? DP : kKeys) * kVPitch;
+    static constexpr int kBytes = SPLIT ? 6 * kPlane : kKeys * kKPitch + (kTransposed ? DP : kKeys) * kVPitch;
 };
+constexpr uint32_t kSplitHighBits = 177u << 23, kSplitWholeBits = 17u << 23;  // 2^50, 2^-110
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1)))
-score_attn_any_kernel(ScoreArgs a) {
-    using Tile = AnyTile<T, DP>;
+// One pass over the keys of a row tile's split; false where SPLIT does not hold its values.
+template <typename T, int DP, bool SPLIT>
+__device__ __forceinline__ bool any_pass(const ScoreArgs & a, const Rows & w, int split, char * smem) {
+    static_assert(!SPLIT || (sizeof(T) == 4 && DP <= 128), "the split is of fp32");
+    using Tile = AnyTile<T, DP, SPLIT>;
     constexpr int kVec = 16 / static_cast<int>(sizeof(T)), kKeys = Tile::kKeys, KT = kKeys / 32, DT = DP / 32;
     constexpr int kPieces = DP / kVec;  // 16-byte pieces of a padded row
-    extern __shared__ __align__(16) char smem[];
+    constexpr int NST = DP / 16, kHalf = kKeys * 128;
     char * k_lds = smem;
-    char * v_lds = smem + kKeys * Tile::kKPitch;
+    char * v_lds = smem + (SPLIT ? 3 * Tile::kPlane : kKeys * Tile::kKPitch);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, r = lane & 31;
 
-    Rows w;
-    int split;
-    if (!locate_work(a, 128, lane, w, split)) return;
     const int end = keys_end(a, w, w.row0 + 127);
     const int key_tiles = (end + kKeys - 1) / kKeys;
     const int kt_first = static_cast<int>(static_cast<int64_t>(key_tiles) * split / a.splits);
@@ -336,24 +343,46 @@ score_attn_any_kernel(ScoreArgs a) {
     const T * k = static_cast<const T *>(a.k) + w.k0 * a.ldk + static_cast<int64_t>(w.kv) * a.d;
     const T * v = static_cast<const T *>(a.v) + w.k0 * a.ldv + static_cast<int64_t>(w.kv) * a.d;
 
-    // This lane's row and its Q fragment (dims h DP/2 .. h DP/2 + DP/2 - 1).
+    // This lane's row and its Q fragment (dims h DP/2 .. h DP/2 + DP/2 - 1, or as the planes hold them).
     const int wave_row0 = w.row0 + wave * 32;
     const int row = wave_row0 + r;
     const bool live = row < w.rows;
     const int qi = (live ? row : 0) / a.group;
     const int head = w.kv * a.group + (live ? row : 0) % a.group;
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
-    T qv[DP / 2];
+    const T * q = static_cast<const T *>(a.q) + (w.q0 + qi) * a.ldq + static_cast<int64_t>(head) * a.d;
+    T qv[SPLIT ? 1 : DP / 2];
+    bf16x8 qf[SPLIT ? 3 : 1][SPLIT ? NST : 1];
+    uint32_t hi_bits = 0;  // the largest magnitude met
+    bool wild = false;
+    float unused = 0.0f;
+    if constexpr (SPLIT) {
 #pragma unroll
-    for (int c = 0; c < DP / 2 / kVec; ++c) {
-        T tmp[kVec];
+        for (int st = 0; st < NST; ++st) {
+            float f[2][4] = {};
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) tmp[e] = T(0);
-        if (live)
-            load_dims<T>(static_cast<const T *>(a.q) + (w.q0 + qi) * a.ldq + static_cast<int64_t>(head) * a.d,
-                         h * (DP / 2) + c * kVec, a.d, a.vec, tmp);
+            for (int i = 0; i < 2; ++i) {
+                if (live) load_dims<float>(q, (st / 4) * 64 + 32 * h + 8 * (st % 4) + 4 * i, a.d, a.vec, f[i]);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) qv[c * kVec + e] = tmp[e];
+                for (int e = 0; e < 4; ++e) hi_bits = max(hi_bits, __float_as_uint(f[i][e]) & 0x7FFFFFFFu);
+            }
+            uint2 lo4[3], hi4[3];
+            split4(make_float4(f[0][0], f[0][1], f[0][2], f[0][3]), lo4, unused);
+            split4(make_float4(f[1][0], f[1][1], f[1][2], f[1][3]), hi4, unused);
+#pragma unroll
+            for (int t = 0; t < 3; ++t)
+                qf[t][st] = __builtin_bit_cast(bf16x8, make_uint4(lo4[t].x, lo4[t].y, hi4[t].x, hi4[t].y));
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < DP / 2 / kVec; ++c) {
+            T tmp[kVec];
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) tmp[e] = T(0);
+            if (live) load_dims<T>(q, h * (DP / 2) + c * kVec, a.d, a.vec, tmp);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) qv[c * kVec + e] = tmp[e];
+        }
     }
     f32x16 oacc[DT];
 #pragma unroll
@@ -381,11 +410,30 @@ score_attn_any_kernel(ScoreArgs a) {
     };
     if (kt_first < kt_last) load(kt_first * kKeys);
     for (int kt0 = kt_first * kKeys; kt0 < kt_last * kKeys; kt0 += kKeys) {
-        __syncthreads();
+        barrier_no_fence();  // every wave has read the tile before
         bool odd = false;
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
             const int key = (tid + 256 * j) / kPieces, piece = (tid + 256 * j) % kPieces;
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t kb = __float_as_uint(kk[j][e]) & 0x7FFFFFFFu, vb = __float_as_uint(vv[j][e]) & 0x7FFFFFFFu;
+                    hi_bits = max(hi_bits, max(kb, vb));
+                    wild |= vb - 1u < kSplitWholeBits - 1u;
+                }
+                const int at = (piece >> 4) * kHalf + key * 128 + (piece & 1) * 8, p16 = (piece & 15) >> 1;
+                uint2 t[3];
+                split4(make_float4(kk[j][0], kk[j][1], kk[j][2], kk[j][3]), t, unused);
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    *reinterpret_cast<uint2 *>(k_lds + p * Tile::kPlane + at + ((p16 ^ kswz(key)) << 4)) = t[p];
+                split4(make_float4(vv[j][0], vv[j][1], vv[j][2], vv[j][3]), t, unused);
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    *reinterpret_cast<uint2 *>(v_lds + p * Tile::kPlane + at + ((p16 ^ vswz(key)) << 4)) = t[p];
+                continue;
+            }
             *reinterpret_cast<uint4 *>(k_lds + key * Tile::kKPitch + piece * 16) = *reinterpret_cast<const uint4 *>(kk[j]);
             if constexpr (!Tile::kTransposed)
                 *reinterpret_cast<uint4 *>(v_lds + key * Tile::kVPitch + piece * 16) = *reinterpret_cast<const uint4 *>(vv[j]);
@@ -397,32 +445,55 @@ score_attn_any_kernel(ScoreArgs a) {
             }
         }
         // A tile with keys that some row does not see, and values that are not finite.
-        again |= __syncthreads_or(odd && min(kt0 + kKeys, w.nk) > tile_all);
+        again |= odd && min(kt0 + kKeys, w.nk) > tile_all;
         if (kt0 + kKeys < kt_last * kKeys) load(kt0 + kKeys);
+        barrier_no_fence();  // the tile is written
         if (wave_row0 >= w.rows) continue;
 
         f32x16 s[KT];
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            s[kt] = f32x16{};
-            const char * krow = k_lds + (kt * 32 + r) * Tile::kKPitch;
-            if constexpr (sizeof(T) == 2) {
+        for (int kt = 0; kt < KT; ++kt) s[kt] = f32x16{};
+        if constexpr (SPLIT) {
 #pragma unroll
-                for (int st = 0; st < DP / 16; ++st) {
-                    const bf16x8 kf = *reinterpret_cast<const bf16x8 *>(krow + h * DP + st * 16);
-                    bf16x8 qf;
+            for (int st = 0; st < NST; ++st) {
+                bf16x8 kf[KT][3];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) qf[e] = __builtin_bit_cast(__bf16, qv[st * 8 + e]);
-                    s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf, s[kt], 0, 0, 0);
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int rw = kt * 32 + r;
+#pragma unroll
+                    for (int p = 0; p < 3; ++p)
+                        kf[kt][p] = *reinterpret_cast<const bf16x8 *>(k_lds + p * Tile::kPlane + (st / 4) * kHalf + rw * 128 +
+                                                                      (((4 * h + st % 4) ^ kswz(rw)) << 4));
                 }
-            } else {
 #pragma unroll
-                for (int u = 0; u < DP / 8; ++u) {
-                    const f32x4 kf = *reinterpret_cast<const f32x4 *>(krow + (h * (DP / 2) + 4 * u) * 4);
+                for (int n = 0; n < 6; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], __builtin_bit_cast(float, qv[4 * u + e]),
-                                                                     s[kt], 0, 0, 0);
+                    for (int kt = 0; kt < KT; ++kt)
+                        s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kt][kSplitTermA[n]], qf[kSplitTermB[n]][st],
+                                                                        s[kt], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const char * krow = k_lds + (kt * 32 + r) * Tile::kKPitch;
+                if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                    for (int st = 0; st < NST; ++st) {
+                        const bf16x8 kf = *reinterpret_cast<const bf16x8 *>(krow + h * DP + st * 16);
+                        bf16x8 qb;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) qb[e] = __builtin_bit_cast(__bf16, qv[st * 8 + e]);
+                        s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb, s[kt], 0, 0, 0);
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < DP / 8; ++u) {
+                        const f32x4 kf = *reinterpret_cast<const f32x4 *>(krow + (h * (DP / 2) + 4 * u) * 4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], __builtin_bit_cast(float, qv[4 * u + e]),
+                                                                         s[kt], 0, 0, 0);
+                    }
                 }
             }
         }
@@ -472,7 +543,46 @@ score_attn_any_kernel(ScoreArgs a) {
             for (int e = 0; e < 16; ++e) oacc[dt][e] *= keep;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-            if constexpr (sizeof(T) == 2) {
+            if constexpr (SPLIT) {
+                const int G = lane >> 4, jl = lane & 15;
+                const int key_off = 4 * (G >> 1) + (jl >> 2), dim_off = 16 * (G & 1) + 4 * (jl & 3);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    bf16x8 pf[3];
+                    uint2 lo4[3], hi4[3];
+                    split4(make_float4(s[kt][8 * u], s[kt][8 * u + 1], s[kt][8 * u + 2], s[kt][8 * u + 3]), lo4, unused);
+                    split4(make_float4(s[kt][8 * u + 4], s[kt][8 * u + 5], s[kt][8 * u + 6], s[kt][8 * u + 7]), hi4, unused);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p)
+                        pf[p] = __builtin_bit_cast(bf16x8, make_uint4(lo4[p].x, lo4[p].y, hi4[p].x, hi4[p].y));
+                    const int ka = kt * 32 + 16 * u + key_off, kb = ka + 8;
+#pragma unroll
+                    for (int d2 = 0; d2 < DT; d2 += 2) {
+                        bf16x8 vf[2][3];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int dbyte = (i * 32 + dim_off) * 2, p16 = dbyte >> 4, within = dbyte & 15;
+#pragma unroll
+                            for (int p = 0; p < 3; ++p) {
+                                const char * vh = v_lds + p * Tile::kPlane + (d2 / 2) * kHalf;
+                                const char * pa = vh + ka * 128 + ((p16 ^ vswz(ka)) << 4) + within;
+                                const char * pb = vh + kb * 128 + ((p16 ^ vswz(kb)) << 4) + within;
+                                const uint2 lo2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                                                (v4i16 __attribute__((address_space(3))) *)(pa)));
+                                const uint2 hi2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                                                (v4i16 __attribute__((address_space(3))) *)(pb)));
+                                vf[i][p] = __builtin_bit_cast(bf16x8, make_uint4(lo2.x, lo2.y, hi2.x, hi2.y));
+                            }
+                        }
+#pragma unroll
+                        for (int n = 0; n < 6; ++n)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                oacc[d2 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i][kSplitTermA[n]], pf[kSplitTermB[n]],
+                                                                                       oacc[d2 + i], 0, 0, 0);
+                    }
+                }
+            } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     bf16x8 p;  // weights round to bf16, as the values they multiply are
@@ -500,14 +610,16 @@ score_attn_any_kernel(ScoreArgs a) {
             }
         }
     }
-    if (again) {
+    if constexpr (SPLIT) {
+        if (__syncthreads_or(wild || hi_bits > kSplitHighBits)) return false;
+    } else if (__syncthreads_or(again)) {
         for (int i = 0; i < 32; ++i)
             if (wave_row0 + i < w.rows)
                 row_alone<T, DP / 64>(a, w, wave_row0 + i, kt_first * kKeys, kt_last * kKeys, lane, a.splits > 1,
                                       split_slot(a, w, split, wave_row0 + i));
-        return;
+        return true;
     }
-    if (!live) return;
+    if (!live) return true;
     const int64_t slot = split_slot(a, w, split, row);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T * o = static_cast<T *>(a.o) + (w.q0 + qi) * a.ldo + static_cast<int64_t>(head) * a.d;
@@ -521,6 +633,20 @@ score_attn_any_kernel(ScoreArgs a) {
             if (a.splits > 1) a.part[slot * a.d + dim] = oacc[dt][e];
             else store_f32(o + dim, oacc[dt][e] * inv);
         }
+    return true;
+}
+
+template <typename T, int DP, bool SPLIT>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 || (DP == 128 && !SPLIT) ? 2 : 1)))
+score_attn_any_kernel(ScoreArgs a) {
+    extern __shared__ __align__(16) char smem[];
+    Rows w;
+    int split;
+    if (!locate_work(a, 128, threadIdx.x & 63, w, split)) return;
+    if constexpr (SPLIT) {
+        if (any_pass<T, DP, true>(a, w, split, smem)) return;
+    }
+    any_pass<T, DP, false>(a, w, split, smem);
 }
 
 // ---- bf16, head sizes of whole 16-byte pieces up to 128 -----------------------------------------------------
@@ -1296,10 +1422,10 @@ int64_t few_part_rows(int64_t total_k, int nseg, int kv_heads) {
     return ((2 * static_cast<int64_t>(nseg) + 3) * kv_heads + std::min(total_k / kFewKeys * kv_heads, kFewItems)) * kFewRows;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool SPLIT = false>
 int launch_any(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
-    constexpr int smem = AnyTile<T, DP>::kBytes;
-    auto kernel = &score_attn_any_kernel<T, DP>;
+    constexpr int plain = AnyTile<T, DP, false>::kBytes, smem = SPLIT ? std::max(plain, AnyTile<T, DP, true>::kBytes) : plain;
+    auto kernel = &score_attn_any_kernel<T, DP, SPLIT>;
     if constexpr (smem > 64 * 1024) {
         static std::atomic<uint64_t> done{0};
         if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), smem, done, "hipFuncSetAttribute(score_attn)")) return rc;
@@ -1310,6 +1436,12 @@ int launch_any(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
 
 template <typename T>
 int run_any(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
+    if constexpr (sizeof(T) == 4) {
+        if (a.d <= 128 && a.scale_log2 <= 0x1p41f) {
+            if (a.d <= 64) return launch_any<T, 64, true>(a, blocks, s);
+            return launch_any<T, 128, true>(a, blocks, s);
+        }
+    }
     if (a.d <= 64) return launch_any<T, 64>(a, blocks, s);
     if (a.d <= 128) return launch_any<T, 128>(a, blocks, s);
     return launch_any<T, 256>(a, blocks, s);

@@ -263,3 +263,31 @@ def test_workspace_never_falls(px):
                 assert size(a, other, other, heads, kv, d) <= size(b, other, other, heads, kv, d)
                 assert size(other, a, other, heads, kv, d) <= size(other, b, other, heads, kv, d)
                 assert size(other, other, a, heads, kv, d) <= size(other, other, b, heads, kv, d)
+
+
+@pytest.mark.parametrize("d", [64, 100, 128])
+def test_fp32_values_of_every_magnitude(px, d):
+    """fp32 operands that three bf16 terms do not hold, in all rows, in some, and beside others:
+    values near the least normal number, keys and queries past 2^50, and ordinary ones."""
+    heads, kv, q_len, k_len = 4, 2, [150, 1, 40], [150, 600, 300]
+    for what in ("tiny values", "some tiny values", "large keys", "one large query", "values from 1e-30 to 1e30"):
+        q, k, v = inputs(q_len, k_len, heads, kv, d, torch.float32, 16)
+        scale = 1.0 / math.sqrt(d)
+        if what == "tiny values":
+            v *= 2.0 ** -118
+        elif what == "some tiny values":
+            v[::7] *= 2.0 ** -118
+            v[:, 5] *= 2.0 ** -118
+        elif what == "large keys":
+            k *= 2.0 ** 55
+            scale *= 2.0 ** -55
+        elif what == "one large query":
+            q[3] *= 2.0 ** 60
+        else:
+            v *= torch.logspace(-30, 30, d * kv, device="cuda")
+        print(f"[scores] fp32 {what} d={d}", flush=True)
+        o = px.varlen_attention_scores(q, k, v, bounds(q_len), bounds(k_len), heads, kv, d, scale, causal=True)
+        want, tol = formula(q, k, v, q_len, k_len, heads, kv, d, scale, causal=True)
+        # (a weight of a few 2^-126 less than the largest is 0: at most that much of the values)
+        check(o, want, tol + 2.0 ** -120 * float(v.abs().max()), what)
+    assert torch.isfinite(o).all()
