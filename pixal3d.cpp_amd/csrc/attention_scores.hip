@@ -67,7 +67,15 @@ struct Rows {
     int shift;            // position of query i: i + shift
     int prefix;           // keys that every row sees, 0..nk
     int chunk, chunks;    // of the segment's keys; 0 of 1 where they are not cut
+    int splits;           // of its keys where all of a call's are split alike: up to a.splits
 };
+
+constexpr int kSplitKeys = 256;  // keys that a split has at least
+
+// Splits that a segment of nk keys has of a call's.
+__device__ __forceinline__ int segment_splits(const ScoreArgs & a, int nk) {
+    return max(1, min(a.splits, (nk + kSplitKeys - 1) / kSplitKeys));
+}
 
 // Items of a segment: its row tiles, or where it has one and a.chunk is set the chunks of its keys.
 __device__ __forceinline__ int64_t segment_items(int64_t nq, int64_t nk, int group, int rows_per_tile, int chunk) {
@@ -113,6 +121,7 @@ __device__ __forceinline__ bool segment_rows(const ScoreArgs & a, const Segment 
     w.row0 = cut ? 0 : i * rows_per_tile;
     w.chunk = cut ? i : 0;
     w.chunks = !cut ? 1 : g.nk > 0 ? (g.nk - 1) / a.chunk + 1 : 0;
+    w.splits = segment_splits(a, g.nk);
     return w.row0 < w.rows;
 }
 
@@ -190,9 +199,10 @@ __device__ __forceinline__ bool locate_work(const ScoreArgs & a, int rows_per_ti
     const int t = static_cast<int>(blockIdx.x / per);
     w.kv = rest % a.kv_heads;
     split = rest / a.kv_heads;
-    if (a.causal && !a.tile_start && a.nseg > 1)
-        return locate_sorted(a, t, rows_per_tile, lane, w);
-    return locate_rows(a, static_cast<int>(a.tiles) - 1 - t, rows_per_tile, lane, w);
+    const bool found = a.causal && !a.tile_start && a.nseg > 1
+                           ? locate_sorted(a, t, rows_per_tile, lane, w)
+                           : locate_rows(a, static_cast<int>(a.tiles) - 1 - t, rows_per_tile, lane, w);
+    return found && split < w.splits;
 }
 
 // Query qi of the call: its segment, and the first of the segment's items; false for a row of no segment.
@@ -309,7 +319,7 @@ __device__ __forceinline__ int64_t split_slot(const ScoreArgs & a, const Rows & 
 //   laid out as the bf16 kernels' tiles are.  Bound by the vector instructions that split beside the
 //   matrix cores.  A workgroup that meets values the terms may not hold (above 2^50, not finite, or in V
 //   below 2^-110 and not zero) writes nothing and takes the next form.  (The scores' losses stay under
-//   128 x 2^50 x 2^-134 of the scale, at most 2^41.)  4,000 tokens, 16 heads of 64: SPLIT_US us against 644.
+//   128 x 2^50 x 2^-134 of the scale, at most 2^41.)  4,000 tokens, 16 heads of 64: 443 us against 644.
 // fp32 otherwise: v_mfma_f32_32x32x2_f32, V read as it lies, 32 dims of a key side by side.
 template <typename T, int DP, bool SPLIT> struct AnyTile {
     static constexpr bool kTransposed = sizeof(T) == 2;
@@ -337,8 +347,8 @@ __device__ __forceinline__ bool any_pass(const ScoreArgs & a, const Rows & w, in
 
     const int end = keys_end(a, w, w.row0 + 127);
     const int key_tiles = (end + kKeys - 1) / kKeys;
-    const int kt_first = static_cast<int>(static_cast<int64_t>(key_tiles) * split / a.splits);
-    const int kt_last = static_cast<int>(static_cast<int64_t>(key_tiles) * (split + 1) / a.splits);
+    const int kt_first = static_cast<int>(static_cast<int64_t>(key_tiles) * split / w.splits);
+    const int kt_last = static_cast<int>(static_cast<int64_t>(key_tiles) * (split + 1) / w.splits);
 
     const T * k = static_cast<const T *>(a.k) + w.k0 * a.ldk + static_cast<int64_t>(w.kv) * a.d;
     const T * v = static_cast<const T *>(a.v) + w.k0 * a.ldv + static_cast<int64_t>(w.kv) * a.d;
@@ -615,7 +625,7 @@ __device__ __forceinline__ bool any_pass(const ScoreArgs & a, const Rows & w, in
     } else if (__syncthreads_or(again)) {
         for (int i = 0; i < 32; ++i)
             if (wave_row0 + i < w.rows)
-                row_alone<T, DP / 64>(a, w, wave_row0 + i, kt_first * kKeys, kt_last * kKeys, lane, a.splits > 1,
+                row_alone<T, DP / 64>(a, w, wave_row0 + i, kt_first * kKeys, kt_last * kKeys, lane, w.splits > 1,
                                       split_slot(a, w, split, wave_row0 + i));
         return true;
     }
@@ -623,14 +633,14 @@ __device__ __forceinline__ bool any_pass(const ScoreArgs & a, const Rows & w, in
     const int64_t slot = split_slot(a, w, split, row);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T * o = static_cast<T *>(a.o) + (w.q0 + qi) * a.ldo + static_cast<int64_t>(head) * a.d;
-    if (a.splits > 1 && h == 0) a.part_ml[slot] = make_float2(m, l);
+    if (w.splits > 1 && h == 0) a.part_ml[slot] = make_float2(m, l);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int dim = dt * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
             if (dim >= a.d) continue;
-            if (a.splits > 1) a.part[slot * a.d + dim] = oacc[dt][e];
+            if (w.splits > 1) a.part[slot * a.d + dim] = oacc[dt][e];
             else store_f32(o + dim, oacc[dt][e] * inv);
         }
     return true;
@@ -960,8 +970,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
     if (!locate_work(a, 128, lane, w, split)) return;
     const int end = keys_end(a, w, w.row0 + 127);
     const int all = (end + F::kKeys - 1) / F::kKeys;
-    const int first = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
-    const int last = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits) - 1;
+    const int first = static_cast<int>(static_cast<int64_t>(all) * split / w.splits);
+    const int last = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / w.splits) - 1;
     const int n = last - first + 1;  // tiles, walked from `last` down: step i is tile last - i
 
     const int wave_row0 = w.row0 + wave * 32;
@@ -1077,13 +1087,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
         for (int j = 0; j < 32; ++j)
             if (wave_row0 + j < w.rows)
                 row_alone<uint16_t, DH / 64>(a, w, wave_row0 + j, first * F::kKeys, (last + 1) * F::kKeys, lane,
-                                             a.splits > 1, split_slot(a, w, split, wave_row0 + j));
+                                             w.splits > 1, split_slot(a, w, split, wave_row0 + j));
         return;
     }
     const float sum = lane_pair_sum(st.sum);
     if (!live) return;
     const int64_t part = split_slot(a, w, split, row);
-    if (a.splits > 1) {
+    if (w.splits > 1) {
         if (h == 0) a.part_ml[part] = make_float2(st.base, sum);
         float * o = a.part + part * a.d;
 #pragma unroll
@@ -1309,12 +1319,20 @@ __global__ void __launch_bounds__(256) score_join_kernel(ScoreArgs a) {
     const int quads = (a.d + 3) / 4;
     const int64_t rows = a.total_q * a.heads;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int64_t row = i / quads;
+    const int64_t row = i / quads, query = row / a.heads;
     const int dim = static_cast<int>(i % quads) * 4, dims = min(4, a.d - dim);
-    if (row >= rows || row < a.cu_q[0] * a.heads || row >= a.cu_q[a.nseg] * a.heads) return;  // (rows of no segment)
+    if (row >= rows || query < a.cu_q[0] || query >= a.cu_q[a.nseg]) return;  // (rows of no segment)
+    int seg = 0;  // the last that starts at or before the query
+    for (int left = a.nseg; left > 1;) {
+        const int half = left / 2;
+        if (a.cu_q[seg + half] <= query) seg += half;
+        left -= half;
+    }
+    const int splits = segment_splits(a, load_segment(a, seg).nk);
+    if (splits == 1) return;  // written whole
     float m = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int s = 0; s < a.splits; ++s) {
+    for (int s = 0; s < splits; ++s) {
         const int64_t at = s * rows + row;
         const float2 ml = a.part_ml[at];
         const float * o = a.part + at * a.d + dim;
@@ -1379,24 +1397,26 @@ constexpr int64_t kScoreMaxRows = INT32_MAX - 1023;  // rows and keys are counte
 constexpr int kWaveSegments = 64;   // segments that a wave's lanes hold; more take a table
 constexpr int kRowTile = 128;
 constexpr int64_t kSplitGrid = 512; // workgroups (two a CU) up to which a call's keys are split
-constexpr int64_t kSplitGridF32 = 1024;  // fp32: a workgroup keeps a CU's matrix cores busy, so finer
-constexpr int64_t kSplitKeys = 256; // keys that a split has at least, of the segments' mean
+// fp32: one and a half rounds of the two workgroups a CU (heads up to 64), or two of its one.  1,517 queries
+// over 2,887 keys, 16 heads of 64: 111 us, with 512 144, with 1024 129; 2,000 tokens, 16 heads of 128: 174 us,
+// with 384 250, with 768 197.
+constexpr int64_t kSplitGridF32 = 768, kSplitGridF32Wide = 512;
 
 int64_t row_tiles(int64_t total_q, int nseg, int group) { return total_q * group / kRowTile + nseg; }
 
-// Splits of the keys: as many as keep row tiles * key/value heads * splits within
-// kSplitGrid, and kSplitKeys keys each.
+// Splits of the longest segment's keys at most: as many as keep row tiles * key/value heads * splits
+// within `grid`.  (How long it is the host does not know: all the keys may be its.)
 int score_splits(int64_t grid, int nseg, int64_t total_q, int64_t total_k, int kv_heads, int group) {
     const int64_t fit = grid / (row_tiles(total_q, nseg, group) * kv_heads);
-    return static_cast<int>(std::max<int64_t>(1, std::min(fit, total_k / nseg / kSplitKeys)));
+    return static_cast<int>(std::max<int64_t>(1, std::min(fit, total_k / kSplitKeys)));
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Rows of partial results at most: a split call has at most kSplitGridF32 workgroups of
+// Rows of partial results at most: a split call has at most the largest split grid's workgroups of
 // kRowTile rows, whatever its other sizes; so the size never falls as a call grows.
 int64_t split_rows(int64_t total_q, int64_t total_k, int heads) {
-    constexpr int64_t kGrid = kSplitGridF32, kMost = kGrid * kRowTile;
+    constexpr int64_t kGrid = std::max({kSplitGrid, kSplitGridF32, kSplitGridF32Wide}), kMost = kGrid * kRowTile;
     const int64_t most = std::max<int64_t>(1, std::min(kGrid, total_k / kSplitKeys));
     if (most == 1) return 0;
     return std::min(kMost, total_q > kMost ? kMost : total_q * heads * most);
@@ -1420,6 +1440,16 @@ int64_t few_items(int64_t total_q, int64_t total_k, int nseg, int kv_heads, int 
 // most nseg tiles, and total_k / chunk is at most both total_k / kFewKeys and kFewItems / kv_heads.
 int64_t few_part_rows(int64_t total_k, int nseg, int kv_heads) {
     return ((2 * static_cast<int64_t>(nseg) + 3) * kv_heads + std::min(total_k / kFewKeys * kv_heads, kFewItems)) * kFewRows;
+}
+
+// Rows of partial results of any call of up to these sizes, and the workspace that holds them.
+int64_t score_part_rows(int nseg, int64_t total_q, int64_t total_k, int heads, int kv_heads) {
+    return std::max(split_rows(total_q, total_k, heads), few_part_rows(total_k, nseg, kv_heads));
+}
+size_t score_workspace(int nseg, int64_t part_rows, int head_dim) {
+    const size_t rows = static_cast<size_t>(part_rows);
+    return round256((static_cast<size_t>(nseg) + 1) * sizeof(int64_t)) + round256(rows * sizeof(float2)) +
+           round256(rows * head_dim * sizeof(float));
 }
 
 template <typename T, int DP, bool SPLIT = false>
@@ -1498,10 +1528,7 @@ extern "C" {
 size_t pxs_attention_scores_workspace_bytes(int nseg, int64_t total_q, int64_t total_k, int heads, int kv_heads,
                                             int head_dim) {
     if (nseg <= 0 || total_q <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 256;
-    total_k = std::max<int64_t>(total_k, 0);
-    const size_t rows = static_cast<size_t>(std::max(split_rows(total_q, total_k, heads), few_part_rows(total_k, nseg, kv_heads)));
-    return round256((static_cast<size_t>(nseg) + 1) * sizeof(int64_t)) + round256(rows * sizeof(float2)) +
-           round256(rows * head_dim * sizeof(float));
+    return score_workspace(nseg, score_part_rows(nseg, total_q, std::max<int64_t>(total_k, 0), heads, kv_heads), head_dim);
 }
 
 int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const void * k, int64_t ld_k, const void * v,
@@ -1556,12 +1583,16 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
         part_rows = blocks * kFewRows;
     } else {
         a.tiles = row_tiles(total_q, nseg, a.group);
-        a.splits = score_splits(dtype == PXS_F32 ? kSplitGridF32 : kSplitGrid, nseg, total_q, total_k, kv_heads, a.group);
+        const int64_t grid = dtype == PXS_BF16 ? kSplitGrid : head_dim <= 64 ? kSplitGridF32 : kSplitGridF32Wide;
+        a.splits = score_splits(grid, nseg, total_q, total_k, kv_heads, a.group);
         blocks = a.tiles * kv_heads * a.splits;
         if (a.splits > 1) part_rows = a.splits * total_q * heads;
     }
     PXS_CHECK(blocks <= UINT32_MAX / 256 && (!few || total_q * heads <= UINT32_MAX / 256), PXS_ERR_ARG,
               "attention grid too large");
+    // (The bounds that the workspace's size is made of hold for every rule above.)
+    PXS_CHECK(part_rows <= score_part_rows(nseg, total_q, total_k, heads, kv_heads), PXS_ERR_ARG,
+              "pxs_varlen_attention_scores: partial results past the workspace");
     char * ws = static_cast<char *>(workspace);
     if (nseg > kWaveSegments) {
         a.tile_start = reinterpret_cast<int64_t *>(ws);
