@@ -210,8 +210,10 @@ __device__ __forceinline__ bool locate_query(const ScoreArgs & a, int qi, int ro
     if (a.tile_start) {
         if (qi < a.cu_q[0] || qi >= a.cu_q[a.nseg]) return false;
         const int seg = find_segment(a.cu_q, a.nseg, qi, lane);
-        item = static_cast<int>(a.tile_start[seg]);
-        return segment_rows(a, load_segment(a, seg), 0, rows_per_tile, w);
+        const Segment g = load_segment(a, seg);
+        if (qi < g.q0 || qi >= g.q0 + g.nq) return false;  // (bounds that fall)
+        item = static_cast<int>(min(a.tile_start[seg], a.tiles));
+        return segment_rows(a, g, 0, rows_per_tile, w);
     }
     const Segment g = lane_segment(a, lane);
     const int items = static_cast<int>(segment_items(g.nq, g.nk, a.group, rows_per_tile, a.chunk));
@@ -1276,6 +1278,7 @@ __global__ void __launch_bounds__(256) score_join_few_kernel(ScoreArgs a) {
     w.kv = head / a.group;
     int item;
     if (!locate_query(a, qi, kFewRows, lane, w, item) || w.chunks <= 1) return;
+    if (item + w.chunks > a.tiles) return;  // (of segments that overlap: no such items)
     const int row = (qi - w.q0) * a.group + head % a.group;
     const int64_t at = (static_cast<int64_t>(item) * a.kv_heads + w.kv) * kFewRows + row;
     const int64_t step = static_cast<int64_t>(a.kv_heads) * kFewRows;
@@ -1359,17 +1362,18 @@ __global__ void __launch_bounds__(256) score_join_kernel(ScoreArgs a) {
 }
 
 // tile_start[s] = items of the segments before s, for more segments than a wave's lanes.
-__global__ void __launch_bounds__(1024) score_tiles_kernel(const int64_t * __restrict__ cu_q,
-                                                           const int64_t * __restrict__ cu_k, int nseg, int group,
-                                                           int rows_per_tile, int chunk,
+__global__ void __launch_bounds__(1024) score_tiles_kernel(ScoreArgs a, int rows_per_tile,
                                                            int64_t * __restrict__ tile_start) {
     __shared__ int64_t waves[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int64_t before = 0;
-    for (int s0 = 0; s0 < nseg; s0 += 1024) {
+    for (int s0 = 0; s0 < a.nseg; s0 += 1024) {
         const int s = s0 + tid;
         int64_t tiles = 0;
-        if (s < nseg) tiles = segment_items(cu_q[s + 1] - cu_q[s], cu_k[s + 1] - cu_k[s], group, rows_per_tile, chunk);
+        if (s < a.nseg) {
+            const Segment g = load_segment(a, s);
+            tiles = segment_items(g.nq, g.nk, a.group, rows_per_tile, a.chunk);
+        }
         int64_t sum = tiles;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -1383,11 +1387,11 @@ __global__ void __launch_bounds__(1024) score_tiles_kernel(const int64_t * __res
             if (i < wave) ahead += waves[i];
             all += waves[i];
         }
-        if (s < nseg) tile_start[s] = ahead + sum - tiles;
+        if (s < a.nseg) tile_start[s] = ahead + sum - tiles;
         before += all;
         __syncthreads();
     }
-    if (tid == 0) tile_start[nseg] = before;
+    if (tid == 0) tile_start[a.nseg] = before;
 }
 
 // ---- host -----------------------------------------------------------------------
@@ -1596,8 +1600,8 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
     char * ws = static_cast<char *>(workspace);
     if (nseg > kWaveSegments) {
         a.tile_start = reinterpret_cast<int64_t *>(ws);
-        hipLaunchKernelGGL(score_tiles_kernel, dim3(1), dim3(1024), 0, s, cu_q, cu_k, nseg, a.group,
-                           few ? kFewRows : kRowTile, a.chunk, reinterpret_cast<int64_t *>(ws));
+        hipLaunchKernelGGL(score_tiles_kernel, dim3(1), dim3(1024), 0, s, a, few ? kFewRows : kRowTile,
+                           reinterpret_cast<int64_t *>(ws));
         if (int rc = check_launch("scored attention tiles")) return rc;
     }
     ws += round256((static_cast<size_t>(nseg) + 1) * sizeof(int64_t));

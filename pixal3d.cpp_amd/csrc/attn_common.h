@@ -20,7 +20,7 @@ __device__ __forceinline__ int find_segment(const int64_t * __restrict__ tile_st
         const int stride = (len + 63) >> 6;
         const int off = lane * stride;
         const bool le = off < len && tile_start[lo + off] <= t;
-        const int cnt = __popcll(__ballot(le));  // >= 1: tile_start[lo] <= t
+        const int cnt = max(1, __popcll(__ballot(le)));  // (0 only where tile_start falls)
         lo += (cnt - 1) * stride;
         len = min(stride, len - (cnt - 1) * stride);
     }

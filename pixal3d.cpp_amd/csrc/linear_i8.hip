@@ -795,12 +795,7 @@ int launch_i8(I8Args a, hipStream_t s) {
         if (21.7 * rounds(192) < 12.6 * rounds(128)) return launch_i8_any<T, 192, 128, 8, 2, EPI>(a, s);
         return launch_i8_any<T, 128, 128, 8, 2, EPI>(a, s);
     }
-#ifndef PXS_I8_CFG
-    const int shape = i8_shape(a.m, a.n, a.k);
-#else
-    const int shape = PXS_I8_CFG;
-#endif
-    switch (shape) {
+    switch (i8_shape(a.m, a.n, a.k)) {
     case 0: return launch_i8_tiles<T, 256, 256, 16, 4, 2, 1, EPI>(a, s);
     case 1: return launch_i8_tiles<T, 192, 128, 8, 2, 2, 1, EPI>(a, s);
     case 2: return launch_i8_tiles<T, 128, 128, 8, 2, 2, 1, EPI>(a, s);
@@ -811,6 +806,7 @@ int launch_i8(I8Args a, hipStream_t s) {
 }
 
 constexpr int kI8MaxInputs = 131071;  // 131,071 products of -128 by -128 stay below 2^31
+constexpr int kI8MaxColumns = 1 << 30;  // columns are counted in 32 bits, a tile past their end
 
 // The checks that the 8-bit linears share; *run is false where there is nothing to do.
 int check_i8(const char * what, const int8_t * x, const float * x_scales, int64_t rows, int cin,
@@ -818,6 +814,7 @@ int check_i8(const char * what, const int8_t * x, const float * x_scales, int64_
     *run = false;
     if (rows < 0 || cin <= 0 || cout <= 0) return fail_call(what, "bad shape");
     if (cin > kI8MaxInputs) return fail_call(what, "more than 131071 inputs (their sum may not fit 32 bits)");
+    if (cout > kI8MaxColumns) return fail_call(what, "more than 2^30 outputs");
     if (rows == 0) return PXS_OK;
     if (!x || !x_scales || !weight || !w_scales || !out) return fail_call(what, "null pointer");
     *run = true;
@@ -835,6 +832,7 @@ int pxs_quantize_rows_i8(int dtype, const void * x, int64_t ld_x, int64_t rows, 
                          float * scales, void * stream) {
     PXS_CHECK(dtype == PXS_F32 || dtype == PXS_BF16, PXS_ERR_ARG, "pxs_quantize_rows_i8: bad dtype");
     PXS_CHECK(rows >= 0 && channels > 0 && ld_x >= channels, PXS_ERR_ARG, "pxs_quantize_rows_i8: bad shape");
+    PXS_CHECK(channels <= kI8MaxColumns, PXS_ERR_ARG, "pxs_quantize_rows_i8: more than 2^30 channels");
     if (rows == 0) return PXS_OK;
     PXS_CHECK(x && q && scales, PXS_ERR_ARG, "pxs_quantize_rows_i8: null pointer");
     QuantArgs a{x, ld_x, rows, channels, q, scales};

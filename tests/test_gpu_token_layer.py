@@ -231,6 +231,27 @@ def test_bounds_past_the_rows_stay_inside(px):
         assert torch.equal(px.varlen_attention_scores(q, k, v, cu, cu, 1, 1, 64, 0.1), good)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("segs", [3, 70])
+def test_bounds_that_fall_stay_inside(px, segs, dtype):
+    """Segments that overlap, or whose bounds fall: what they compute is undefined, but rows around the
+    tensors' stay as they were, and a call that follows is right."""
+    rows, keys, d = 48, 3000, 64
+    gen = torch.Generator("cuda").manual_seed(51)
+    q = torch.randn((rows, d), device="cuda", generator=gen).to(dtype)
+    k, v = (torch.randn((keys, d), device="cuda", generator=gen).to(dtype) for _ in range(2))
+    around = torch.full((rows + 64, d), 3.0, device="cuda").to(dtype)
+    o = around[32:32 + rows]
+    good = px.varlen_attention_scores(q, k, v, bounds([rows]), bounds([keys]), 1, 1, d, 0.1)
+    for cu_q, cu_k in (([0, 40, 8, rows], [0, keys, 100, keys]), ([0, 20, 48, 10], [0, keys, 0, keys]),
+                       ([5, 2, 48, 48], [7, 3, keys, 9]), ([0, -9, 60, 20], [-5, keys + 9, 0, keys])):
+        fill = [cu_q[-1]] * (segs - 3), [cu_k[-1]] * (segs - 3)
+        cq, ck = (torch.tensor(c + f, device="cuda") for c, f in zip((cu_q, cu_k), fill))
+        px.varlen_attention_scores(q, k, v, cq, ck, 1, 1, d, 0.1, causal=True, out=o)
+        assert (around[:32] == 3.0).all() and (around[32 + rows:] == 3.0).all()
+    assert torch.equal(px.varlen_attention_scores(q, k, v, bounds([rows]), bounds([keys]), 1, 1, d, 0.1), good)
+
+
 def test_wrong_tensors_are_refused(px):
     x = torch.zeros((4, 64), device="cuda", dtype=torch.bfloat16)
     q, s = px.quantize_rows(x)

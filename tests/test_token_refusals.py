@@ -30,7 +30,7 @@ QUANT = dict(dtype=0, x=P, ld=64, rows=4, channels=64, q=P, scales=P, stream=Non
 @pytest.mark.parametrize("change,text", [
     (dict(dtype=2), "bad dtype"), (dict(rows=-1), "bad shape"), (dict(channels=0), "bad shape"),
     (dict(ld=63), "bad shape"), (dict(x=None), "null pointer"), (dict(q=None), "null pointer"),
-    (dict(scales=None), "null pointer")])
+    (dict(scales=None), "null pointer"), (dict(channels=2 ** 30 + 1, ld=2 ** 31), "2^30 channels")])
 def test_quantize_refusals(lib, change, text):
     refused(lib, lib.pxs_quantize_rows_i8(*{**QUANT, **change}.values()), text)
 
@@ -42,7 +42,8 @@ LINEAR = dict(x=P, xs=P, rows=4, cin=64, w=P, ws=P, bias=None, cout=32, act=0, d
     (dict(dtype=7), "bad dtype"), (dict(act=9), "bad activation"), (dict(rows=-1), "bad shape"),
     (dict(cin=0), "bad shape"), (dict(cout=0), "bad shape"), (dict(cin=131072), "131071"), (dict(x=None), "null pointer"),
     (dict(xs=None), "null pointer"), (dict(w=None), "null pointer"), (dict(ws=None), "null pointer"),
-    (dict(y=None), "null pointer"), (dict(rows=2 ** 40, cin=1, cout=2 ** 20), "grid too large")])
+    (dict(y=None), "null pointer"), (dict(rows=2 ** 40, cin=1, cout=2 ** 20), "grid too large"),
+    (dict(cin=1, cout=2 ** 31 - 1), "2^30 outputs"), (dict(rows=0, cin=1, cout=2 ** 30 + 1), "2^30 outputs")])
 def test_linear_i8_refusals(lib, change, text):
     refused(lib, lib.pxs_linear_i8(*{**LINEAR, **change}.values()), text)
 
