@@ -394,7 +394,7 @@ int pxs_quantize_rows_i8(int dtype, const void * x, int64_t ld_x, int64_t rows, 
 
 /* y = act((x W^T) * x_scales[row] * w_scales[channel] + bias) in y_dtype, x
  * [rows, cin] and weight [cout, cin] 8-bit integers, summed exactly in 32 bits
- * (cin is at most 131071).  bias may be NULL; act is PXS_ACT_*.  A cin that is
+ * (cin is at most 131071, cout 2^30).  bias may be NULL; act is PXS_ACT_*.  A cin that is
  * a multiple of 16, with 16-byte-aligned x and weight, takes the fastest
  * kernels. */
 int pxs_linear_i8(const int8_t * x, const float * x_scales, int64_t rows, int cin,
@@ -544,8 +544,9 @@ int pxs_varlen_attention_noalloc(int dtype, const void * q, int64_t ld_q, const 
  *     included.  A query that sees no key gets zeros.
  * Row strides ld_* are in elements.  total_q = cu_q[nseg] and total_k =
  * cu_k[nseg], total_k and total_q * heads / kv_heads at most 2^31 - 1024; rows
- * of q and o behind the last segment are neither read nor written.  bf16 rows of 16-byte pieces with head_dim 64 or 128
- * take the fastest kernels.  The result depends on the whole call's sizes in its
+ * of q and o behind the last segment are neither read nor written.  bf16 with head_dim a
+ * multiple of 8 up to 128 (64 and 128 best), 16-byte-aligned q, k and v, and strides that
+ * are multiples of 8 takes the fastest kernels.  The result depends on the whole call's sizes in its
  * last bits (the keys of few rows are split and joined in a fixed order); the
  * same call gives the same bits.
  * workspace: pxs_attention_scores_workspace_bytes of the same sizes; calls that

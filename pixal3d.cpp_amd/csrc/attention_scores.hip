@@ -163,8 +163,9 @@ __device__ __forceinline__ int tiles_below(int x, int nq, int nk, int prefix, in
 
 // The t-th row tile of a call with a causal mask and 2 to 64 segments, those that see most keys
 // first: 64 classes of keys seen, counted by a lane each, then the tile within its class.  (In
-// the segments' order the last of a call's tiles may be its longest: prompts of 8192, 2903 and
-// 4739 tokens, 16 heads of 128, 524 us against 611.)
+// the segments' order, reversed, the last of a call's tiles may be long ones: eight prompts of 2,048
+// tokens, 16 heads of 128, 173 us against 189; ten of 100 to 5,000, 299 against 316; prompts of
+// 8192, 2903 and 4739, 445 against 453.  Two prompts whose first 1370 tokens all see lose 3%.)
 __device__ __forceinline__ bool locate_sorted(const ScoreArgs & a, int t, int rows_per_tile, int lane, Rows & w) {
     const int shift = 31 - __clz(rows_per_tile);
     const Segment g = lane_segment(a, lane);
@@ -321,7 +322,7 @@ __device__ __forceinline__ int64_t split_slot(const ScoreArgs & a, const Rows & 
 //   laid out as the bf16 kernels' tiles are.  Bound by the vector instructions that split beside the
 //   matrix cores.  A workgroup that meets values the terms may not hold (above 2^50, not finite, or in V
 //   below 2^-110 and not zero) writes nothing and takes the next form.  (The scores' losses stay under
-//   128 x 2^50 x 2^-134 of the scale, at most 2^41.)  4,000 tokens, 16 heads of 64: 443 us against 644.
+//   128 x 2^50 x 2^-134 of the scale, at most 2^41.)  4,000 tokens, 16 heads of 64: 400 us against 587.
 // fp32 otherwise: v_mfma_f32_32x32x2_f32, V read as it lies, 32 dims of a key side by side.
 template <typename T, int DP, bool SPLIT> struct AnyTile {
     static constexpr bool kTransposed = sizeof(T) == 2;
@@ -955,7 +956,9 @@ __device__ __forceinline__ TileSource<DH> tile_source(const ScoreArgs & a, const
 // its weights, O += V P of the tile before and S of the next, and takes its weights while
 // they run, without a maximum: a row's weights are redone with one where their sum passes
 // 2^40 (bf16 and fp32 hold 2^127).  With a bias that falls with the distance the nearest
-// keys come first, so that is rare.
+// keys come first, so that is rare.  Bound by the vector instructions of the weights beside the products,
+// and by the waits between the two: 8,192 tokens, 16 heads of 128, 0.60 ms (910 TFLOP/s; the matrix cores
+// busy in 45% of the cycles), of 64 0.32 ms (860), with a cap 0.42, with a bias of both sides 0.49.
 constexpr int kSlots = 4;
 constexpr float kSumLimit = 0x1p40f;
 
@@ -1402,8 +1405,8 @@ constexpr int kWaveSegments = 64;   // segments that a wave's lanes hold; more t
 constexpr int kRowTile = 128;
 constexpr int64_t kSplitGrid = 512; // workgroups (two a CU) up to which a call's keys are split
 // fp32: one and a half rounds of the two workgroups a CU (heads up to 64), or two of its one.  1,517 queries
-// over 2,887 keys, 16 heads of 64: 111 us, with 512 144, with 1024 129; 2,000 tokens, 16 heads of 128: 174 us,
-// with 384 250, with 768 197.
+// over 2,887 keys, 16 heads of 64: 107 us, with 512 136, with 1024 119; 2,000 tokens, 16 heads of 128: 175 us,
+// with 384 246, with 768 202.
 constexpr int64_t kSplitGridF32 = 768, kSplitGridF32Wide = 512;
 
 int64_t row_tiles(int64_t total_q, int nseg, int group) { return total_q * group / kRowTile + nseg; }
