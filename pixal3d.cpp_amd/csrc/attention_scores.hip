@@ -1032,7 +1032,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
             tile_pv<DH>(v_of(i), p, oacc, lane);
         }
     }
-    if (i < n) {
+    // (The step as a scalar: taken for a lane's, it kept a second copy of the output alive through the
+    // loop, and the compiler, out of registers, waited for every read of LDS: 475 us against 529 for the
+    // capped prompts above.)
+    i = __builtin_amdgcn_readfirstlane(i);
+    if (i < __builtin_amdgcn_readfirstlane(n)) {
         // Steps exact .. n - 1, one tile's products behind its weights.  Slot use: step i
         // reads V of i - 1 and K of i + 1 while i + 2 lands.
         auto weights = [&](int i, typename F::Scores & s) __attribute__((always_inline)) {
