@@ -165,7 +165,7 @@ __device__ __forceinline__ int tiles_below(int x, int nq, int nk, int prefix, in
 // first: 64 classes of keys seen, counted by a lane each, then the tile within its class.  (In
 // the segments' order, reversed, the last of a call's tiles may be long ones: eight prompts of 2,048
 // tokens, 16 heads of 128, 173 us against 189; ten of 100 to 5,000, 299 against 316; prompts of
-// 8192, 2903 and 4739, 445 against 453.  Two prompts whose first 1370 tokens all see lose 3%.)
+// 8192, 2903 and 4739, 445 against 453 (before the main loop's last gain, of 5 to 11%).  Two prompts whose first 1370 tokens all see lose 3%.)
 __device__ __forceinline__ bool locate_sorted(const ScoreArgs & a, int t, int rows_per_tile, int lane, Rows & w) {
     const int shift = 31 - __clz(rows_per_tile);
     const Segment g = lane_segment(a, lane);
@@ -957,8 +957,8 @@ __device__ __forceinline__ TileSource<DH> tile_source(const ScoreArgs & a, const
 // they run, without a maximum: a row's weights are redone with one where their sum passes
 // 2^40 (bf16 and fp32 hold 2^127).  With a bias that falls with the distance the nearest
 // keys come first, so that is rare.  Bound by the vector instructions of the weights beside the products,
-// and by the waits between the two: 8,192 tokens, 16 heads of 128, 0.60 ms (910 TFLOP/s; the matrix cores
-// busy in 45% of the cycles), of 64 0.32 ms (860), with a cap 0.42, with a bias of both sides 0.49.
+// and by the waits between the two: 8,192 tokens, 16 heads of 128, 0.53 to 0.56 ms (980 to 1,040 TFLOP/s; the
+// matrix cores busy in 55% of the cycles), of 64 0.30 to 0.32 ms, with a cap 0.41, with a bias of both sides 0.45.
 constexpr int kSlots = 4;
 constexpr float kSumLimit = 0x1p40f;
 
