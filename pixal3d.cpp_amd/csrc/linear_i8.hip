@@ -192,8 +192,8 @@ struct I8Args {
 // is v / (1 + e^-2u).  Within a few steps of the library's forms, which took a third of a
 // short product's time.
 __device__ __forceinline__ float i8_gelu(float v) {
-    const float u = 0.7978845608028654f * (v + 0.044715f * v * v * v);
-    return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.8853900817779268f * u));
+    const float e = v * __builtin_fmaf(v * v, -0.10294324f, -2.3022082f);  // -2 log2(e) u
+    return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(e));
 }
 __device__ __forceinline__ float i8_silu(float v) {
     return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
@@ -742,20 +742,21 @@ int launch_i8_few(const I8Args & a, hipStream_t s) {
 }
 
 // Tile shapes, their time alone on a CU and their share of a full CU's time, in us for
-// 1024 bytes of K more and without any (measured on 1 to 42,017 rows, 1024 to 4096 deep;
-// at the larger sizes the whole card runs slower than one tile alone):
-//   256 x 256, 16 waves of 64 x 64, one workgroup a CU:  42,017 x 4096 -> 1024 182 us (1,931 TOP/s)
-//   192 x 128 and 128 x 128, 8 waves, two workgroups:    212; 1,370 x 1024 -> 4096 14.3 on 128 rows
-//   128 x 64, 8 waves, two:                              1,370 x 4096 -> 1024 17.8 against 25.8
-//   64 x 64, 4 waves, two:                               1,000 x 1024 -> 1024 6.4 against 8.4
+// 1024 bytes of K more and without any: fitted to each shape's times at 68 sizes (65 to 206,980
+// rows, 256 to 8192 deep), where the shape picked takes 0.5% more than the best on average (at the larger
+// sizes the whole card runs slower than one tile alone):
+//   256 x 256, 16 waves of 64 x 64, one workgroup a CU:  8,192 x 8192 -> 4096 242 us (2,270 TOP/s)
+//   192 x 128 and 128 x 128, 8 waves, two workgroups:    287 and 289; 1,370 x 1024 -> 4096 13.1 and 13.6
+//   128 x 64, 8 waves, two:                              1,370 x 4096 -> 1024 17.8 against 20.3
+//   64 x 64, 4 waves, two:                               150 x 4096 -> 4096 15.1 against 17.0
 //   32 x 64, four groups of two waves over K, one:       300 x 4096 -> 1024 8.4 against 14.8
 struct I8Shape {
     int bm, bn;
     double alone0, alone1, each0, each1;
 };
 constexpr I8Shape kI8Shapes[] = {
-    {256, 256, 7.8, 8.4, 11.2, 12.4}, {192, 128, 5.0, 4.5, 4.0, 6.2}, {128, 128, 4.3, 3.4, 2.7, 4.1},
-    {128, 64, 3.2, 3.2, 1.3, 3.1},    {64, 64, 3.0, 2.9, 1.3, 1.9},   {32, 64, 3.9, 1.0, 2.7, 1.2},
+    {256, 256, 7.3, 8.9, 10.8, 13.4}, {192, 128, 4.9, 4.8, 4.2, 5.9}, {128, 128, 3.9, 4.0, 2.7, 4.4},
+    {128, 64, 3.6, 3.3, 2.0, 2.8},    {64, 64, 3.1, 2.9, 1.4, 2.0},   {32, 64, 3.7, 1.1, 2.7, 1.2},
 };
 
 int i8_shape(int64_t m, int n, int k) {
@@ -774,6 +775,8 @@ int i8_shape(int64_t m, int n, int k) {
     }
     return best;
 }
+
+constexpr int kI8DeepK = 1024;  // a longer K is worth a third stage (launch_i8)
 
 // Up to kI8FewRows rows: 16 output channels a workgroup, and as few of its 16-row blocks as
 // keep the workgroups near one a CU.
@@ -795,10 +798,20 @@ int launch_i8(I8Args a, hipStream_t s) {
         if (21.7 * rounds(192) < 12.6 * rounds(128)) return launch_i8_any<T, 192, 128, 8, 2, EPI>(a, s);
         return launch_i8_any<T, 128, 128, 8, 2, EPI>(a, s);
     }
+    // Three stages where a CU has one tile at most, so that no second tile's stages need fit, and K is
+    // longer than their start (1,500 x 4096 -> 2048 22 us against 27, 1,370 x 2048 -> 4096 19.6 against 20.4,
+    // but 1,000 x 1024 -> 4096 9.8 against 9.5; four stages the same as three).
+    auto deep = [&](int bm, int bn) {
+        return a.k > kI8DeepK && ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn) <= 256;
+    };
     switch (i8_shape(a.m, a.n, a.k)) {
     case 0: return launch_i8_tiles<T, 256, 256, 16, 4, 2, 1, EPI>(a, s);
-    case 1: return launch_i8_tiles<T, 192, 128, 8, 2, 2, 1, EPI>(a, s);
-    case 2: return launch_i8_tiles<T, 128, 128, 8, 2, 2, 1, EPI>(a, s);
+    case 1:
+        if (deep(192, 128)) return launch_i8_tiles<T, 192, 128, 8, 2, 3, 1, EPI>(a, s);
+        return launch_i8_tiles<T, 192, 128, 8, 2, 2, 1, EPI>(a, s);
+    case 2:
+        if (deep(128, 128)) return launch_i8_tiles<T, 128, 128, 8, 2, 3, 1, EPI>(a, s);
+        return launch_i8_tiles<T, 128, 128, 8, 2, 2, 1, EPI>(a, s);
     case 3: return launch_i8_tiles<T, 128, 64, 8, 4, 3, 1, EPI>(a, s);
     case 4: return launch_i8_tiles<T, 64, 64, 4, 2, 4, 1, EPI>(a, s);
     default: return launch_i8_tiles<T, 32, 64, 2, 1, 3, 4, EPI>(a, s);
