@@ -138,7 +138,7 @@ def test_quantize_strided_and_misaligned_rows(px, dtype):
 
 SHAPES = [(1, 1, 1), (1, 16, 8), (3, 15, 5), (2, 17, 33), (5, 127, 64), (16, 128, 16), (17, 144, 100), (64, 1024, 96),
           (65, 1370, 130), (130, 1008, 260), (1, 4096, 1024), (4, 1024, 4096), (33, 2000, 77), (257, 272, 513),
-          (700, 1040, 1021), (1370, 256, 1024), (2100, 512, 768)]
+          (700, 1040, 1021), (1370, 256, 1024), (2100, 512, 768), (1370, 1168, 4000), (1000, 1168, 4004)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -192,7 +192,8 @@ def test_linear_i8_misaligned_operands(px, rows, cin, cout):
             check(y, *bounds(v, bound, "none", "f32" if dtype == torch.float32 else "bf16"), what=f"shift {by}")
 
 
-@pytest.mark.parametrize("rows,cin,cout", [(1, 64, 32), (7, 1024, 1024), (250, 1024, 1024), (1237, 272, 320), (90, 33, 18)])
+@pytest.mark.parametrize("rows,cin,cout", [(1, 64, 32), (7, 1024, 1024), (250, 1024, 1024), (1237, 272, 320), (90, 33, 18), (1370, 1168, 4000),
+                                           (1000, 1168, 4004)])
 def test_linear_i8_residual_forms(px, rows, cin, cout):
     xq, wq = int_rows(84, rows, cin, 1), int_rows(84, cout, cin, 2)
     xs = np.exp(W.normal(84, rows, 3)).astype(np.float32) * np.float32(0.02)
