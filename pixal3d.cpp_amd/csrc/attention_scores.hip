@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 namespace pxs {
@@ -43,8 +44,11 @@ struct ScoreArgs {
     const int64_t * tile_start;  // [nseg + 1] items before each segment; null: at most 64 segments
     int chunk;                   // keys of an item of a segment with one row tile; 0: not cut
     int heads, kv_heads, group, d;
-    float scale_log2;            // scale * log2(e), or with a cap scale / cap
+    float scale_log2;            // scale * log2(e)
     float cap_log2;              // cap * log2(e); 0: no cap
+    float over_cap;              // scale / cap
+    float dot_mul, dot_over_cap; // their product is scale / cap, both in fp32's normal range
+    float exp_mul;               // 2 log2(e) scale / cap
     const float * slopes;        // [heads] or null
     int causal;
     const int64_t * prefix;      // [nseg] or null
@@ -240,7 +244,7 @@ __device__ __forceinline__ int keys_all(const ScoreArgs & a, const Rows & w, int
 // A score in log2 units, from a product q . k and the key's distance behind the query.
 __device__ __forceinline__ float score_log2(const ScoreArgs & a, float dot, float slope_log2, float away) {
     float z = dot * a.scale_log2;
-    if (a.cap_log2 > 0.0f) z = a.cap_log2 * tanhf(z);
+    if (a.cap_log2 > 0.0f) z = a.cap_log2 * tanhf(dot * a.dot_mul * a.dot_over_cap);
     return z - slope_log2 * fabsf(away);
 }
 
@@ -260,8 +264,9 @@ __device__ __forceinline__ bool is_finite_bits(float v) { return (__float_as_uin
 // A row again, one key after the other, keys that it does not see left out
 // altogether: for tiles where an unseen key's value is infinite or NaN, which
 // times a weight of zero is NaN.  One wave per row; lane l holds dims l, l + 64, ...
+// (Inlined: a call would take the arguments in memory, and with them every kernel's scalars.)
 template <typename T, int NC>
-__device__ void row_alone(const ScoreArgs & a, const Rows & w, int row, int key0, int key1, int lane, bool partial,
+__device__ __forceinline__ void row_alone(const ScoreArgs & a, const Rows & w, int row, int key0, int key1, int lane, bool partial,
                           int64_t slot) {
     const int i = row / a.group;
     const int head = w.kv * a.group + row % a.group;
@@ -669,9 +674,11 @@ score_attn_any_kernel(ScoreArgs a) {
 
 __device__ __align__(16) uint4 g_score_zero[8];  // what keys past a segment's end are read as
 
-// MODE bits: scores are capped, biased, and of a biased call that its mask lets queries see only keys at
-// or before them in the tiles taken without a maximum.
-constexpr int kCap = 1, kBias = 2, kBehind = 4;
+// MODE bits: scores are capped, biased, of a biased call that its mask lets queries see only keys at
+// or before them in the tiles taken without a maximum, and of a capped call that its cap is above kNearCap.
+constexpr int kCap = 1, kBias = 2, kBehind = 4, kFar = 8;
+constexpr float kNearCap = 256.0f;
+constexpr bool near_cap(int mode) { return (mode & (kCap | kFar)) == kCap; }
 
 // Head sizes that are multiples of 8 up to 128 run as the next of 64 and 128 (WHOLE false): the
 // missing pieces of a row come from a line of zeros.
@@ -692,24 +699,44 @@ template <int DH> struct Fast {
 //   z = raw * mul + add                              (no cap)
 //   z = add + top / (1 + 2^(raw * mul))              (cap: cap tanh(x) = cap - 2 cap / (1 + e^2x))
 //   with a bias, add - slope * |behind - key|.
+// That form of the cap is off by up to 2^-23 of the cap, whatever the score: 3e-5 at kNearCap, about what
+// the products' sums in fp32 are off by.  A larger cap (kFar) takes a form that is right relative to the
+// score, x = raw * over:
+//   z = add + raw * mul * (1 - x^2/3 + 2 x^4/15 - ...)        |x| < 1/4; the next term is 2^-26 there
+//   z = add + top - 2 top / (1 + e^2x)                        above, where the cap is at most 4.1 scores
+// Ten operations a score more than the near form: causal prompts of 8192, 2903 and 4739, 16 heads of 128 over
+// 4, 690 us against 485, 8,192 tokens without a mask, 16 heads of 64, 708 against 420; eight tokens over 170,161
+// keys 150 against 144.
 struct RowScore {
-    float mul, top, slope;
+    float mul, top, slope, over, part;
 };
 
 template <int MODE>
 __device__ __forceinline__ RowScore row_score(const ScoreArgs & a, int head) {
     RowScore s;
-    s.mul = MODE & kCap ? 2.0f * kLog2e * a.scale_log2 : a.scale_log2;
-    s.top = -2.0f * a.cap_log2;
+    s.mul = near_cap(MODE) ? a.exp_mul : a.scale_log2;
+    s.top = near_cap(MODE) ? -2.0f * a.cap_log2 : a.cap_log2;
+    s.over = a.over_cap;
+    s.part = -2.0f * a.cap_log2;
     s.slope = MODE & kBias ? -kLog2e * a.slopes[head] : 0.0f;
     return s;
 }
 
-// z - base of a product; key: behind - key is the distance.  add is cap_log2 - base, or -base.
+// z - base of a product; key: behind - key is the distance.  add is cap_log2 - base with a near cap, -base otherwise.
 template <int MODE>
 __device__ __forceinline__ float score_of(const RowScore & s, float raw, float add, float away) {
     float b = add;
     if constexpr (MODE & kBias) b = __builtin_fmaf(s.slope, fabsf(away), add);
+    if constexpr (MODE & kFar) {
+        const float x = raw * s.over, y = x * x;
+        const float series = __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, 0x1.664f48p-6f, -0x1.ba1ba2p-5f),
+                                                                                0x1.111112p-3f), -0x1.555556p-2f), 1.0f);
+        const float rest = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * (2.0f * kLog2e)));
+        // (Of the two forms' cheap parts one is taken: between their results the compiler branches.)
+        const bool near = fabsf(x) < 0.25f;
+        const float whole = near ? raw * s.mul * series : s.top, part = near ? 0.0f : s.part;
+        return __builtin_fmaf(part, rest, whole) + b;
+    }
     if constexpr (MODE & kCap)
         return __builtin_fmaf(s.top, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw * s.mul)), b);
     return __builtin_fmaf(raw, s.mul, b);
@@ -775,11 +802,11 @@ template <int DH, int MODE>
 __device__ __forceinline__ float tile_weights(const RowScore & rs, float cap_log2, const typename Fast<DH>::Scores & s,
                                               typename Fast<DH>::Weights & p, float base, float behind) {
     const bf16x2 ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
-    const float add = MODE & kCap ? cap_log2 - base : -base;
+    const float add = near_cap(MODE) ? cap_log2 - base : -base;
     const float start = MODE & kBehind ? __builtin_fmaf(rs.slope, behind, add) : 0.0f;
     auto weight = [&](int kt, int e) __attribute__((always_inline)) {
         const float key = static_cast<float>(key_of(kt, e));
-        const float z = MODE & kBehind ? score_of<MODE & kCap>(rs, s[kt][e], __builtin_fmaf(rs.slope, -key, start), 0.0f)
+        const float z = MODE & kBehind ? score_of<MODE & (kCap | kFar)>(rs, s[kt][e], __builtin_fmaf(rs.slope, -key, start), 0.0f)
                                        : score_of<MODE>(rs, s[kt][e], add, behind - key);
         return static_cast<__bf16>(__builtin_amdgcn_exp2f(z));
     };
@@ -805,7 +832,7 @@ __device__ __forceinline__ float tile_weights(const RowScore & rs, float cap_log
 template <int DH, int MODE>
 __device__ __forceinline__ float tile_max(const RowScore & rs, float cap_log2, const typename Fast<DH>::Scores & s,
                                           float behind) {
-    const float add = MODE & kCap ? cap_log2 : 0.0f;
+    const float add = near_cap(MODE) ? cap_log2 : 0.0f;
     float top = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < Fast<DH>::KT; ++kt)
@@ -822,7 +849,7 @@ __device__ __forceinline__ void tile_exact(const RowScore & rs, float cap_log2, 
                                            typename Fast<DH>::Weights & p, typename Fast<DH>::Out & oacc,
                                            RowState & st, float behind, int seen) {
     using F = Fast<DH>;
-    const float add = MODE & kCap ? cap_log2 : 0.0f;
+    const float add = near_cap(MODE) ? cap_log2 : 0.0f;
     float top = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < F::KT; ++kt)
@@ -1490,16 +1517,16 @@ int run_any(const ScoreArgs & a, int64_t blocks, hipStream_t s) {
 
 // kernel<mode of the call>
 template <bool BEHIND, typename F> int with_mode(const ScoreArgs & a, F && launch) {
-    if (BEHIND && a.slopes && a.causal) {
-        if (a.cap_log2 > 0.0f) return launch(std::integral_constant<int, kCap | kBias | kBehind>{});
-        return launch(std::integral_constant<int, kBias | kBehind>{});
-    }
-    if (a.cap_log2 > 0.0f) {
-        if (a.slopes) return launch(std::integral_constant<int, kCap | kBias>{});
-        return launch(std::integral_constant<int, kCap>{});
-    }
-    if (a.slopes) return launch(std::integral_constant<int, kBias>{});
-    return launch(std::integral_constant<int, 0>{});
+    auto capped = [&](auto rest) {
+        constexpr int kRest = decltype(rest)::value;
+        if (a.cap_log2 == 0.0f) return launch(rest);
+        if (a.cap_log2 <= kNearCap * kLog2e) return launch(std::integral_constant<int, kCap | kRest>{});
+        return launch(std::integral_constant<int, kCap | kFar | kRest>{});
+    };
+    if constexpr (BEHIND)
+        if (a.slopes && a.causal) return capped(std::integral_constant<int, kBias | kBehind>{});
+    if (a.slopes) return capped(std::integral_constant<int, kBias>{});
+    return capped(std::integral_constant<int, 0>{});
 }
 
 template <int DH, bool WHOLE>
@@ -1559,7 +1586,7 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
               "pxs_varlen_attention_scores: cap must be finite, and 0 for none");
     PXS_CHECK(causal == 0 || causal == 1, PXS_ERR_ARG, "pxs_varlen_attention_scores: causal must be 0 or 1");
     PXS_CHECK(causal || !prefix, PXS_ERR_ARG, "pxs_varlen_attention_scores: a prefix needs the causal mask");
-    PXS_CHECK(std::isfinite(scale * kLog2e) && (cap == 0.0f || (std::isfinite(scale / cap) && std::isfinite(cap * kLog2e))),
+    PXS_CHECK(std::isfinite(scale * kLog2e) && (cap == 0.0f || std::isfinite(scale / cap)),
               PXS_ERR_ARG, "pxs_varlen_attention_scores: scale and cap out of range");
     PXS_CHECK(nseg >= 0 && total_q >= 0 && total_k >= 0 && total_q <= kScoreMaxRows / (heads / kv_heads) &&
                   total_k <= kScoreMaxRows,
@@ -1575,8 +1602,16 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
     a.q = q; a.k = k; a.v = v; a.ldq = ld_q; a.ldk = ld_k; a.ldv = ld_v;
     a.cu_q = cu_q; a.cu_k = cu_k; a.nseg = nseg; a.total_q = total_q; a.total_k = total_k;
     a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.d = head_dim;
-    a.scale_log2 = cap > 0.0f ? scale / cap : scale * kLog2e;
+    // (Caps above a quarter of the largest number cap nothing that is not about to overflow; a multiplier past
+    // it is cut, so that a product of zero stays zero under it.)
+    constexpr float kLargest = std::numeric_limits<float>::max();
+    cap = std::min(cap, kLargest / 4);
+    a.scale_log2 = scale * kLog2e;
     a.cap_log2 = cap * kLog2e;
+    a.over_cap = cap > 0.0f ? scale / cap : 0.0f;
+    a.dot_mul = a.over_cap < 0x1p-126f ? 0x1p-64f : 1.0f;
+    a.dot_over_cap = cap > 0.0f ? static_cast<float>(static_cast<double>(scale) / cap / a.dot_mul) : 0.0f;
+    a.exp_mul = std::min(2.0f * kLog2e * a.over_cap, kLargest);
     a.slopes = slopes; a.causal = causal; a.prefix = prefix; a.o = o; a.ldo = ld_o;
     const int elem = dtype == PXS_BF16 ? 2 : 4;
     a.vec = rows_of_pieces(q, ld_q, head_dim, elem) && rows_of_pieces(k, ld_k, head_dim, elem) &&
