@@ -47,7 +47,6 @@ struct ScoreArgs {
     float scale_log2;            // scale * log2(e)
     float cap_log2;              // cap * log2(e); 0: no cap
     float over_cap;              // scale / cap
-    float dot_mul, dot_over_cap; // their product is scale / cap, both in fp32's normal range
     float exp_mul;               // 2 log2(e) scale / cap
     const float * slopes;        // [heads] or null
     int causal;
@@ -244,7 +243,7 @@ __device__ __forceinline__ int keys_all(const ScoreArgs & a, const Rows & w, int
 // A score in log2 units, from a product q . k and the key's distance behind the query.
 __device__ __forceinline__ float score_log2(const ScoreArgs & a, float dot, float slope_log2, float away) {
     float z = dot * a.scale_log2;
-    if (a.cap_log2 > 0.0f) z = a.cap_log2 * tanhf(dot * a.dot_mul * a.dot_over_cap);
+    if (a.cap_log2 > 0.0f) z = a.cap_log2 * tanhf(dot * a.over_cap);
     return z - slope_log2 * fabsf(away);
 }
 
@@ -1602,15 +1601,14 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
     a.q = q; a.k = k; a.v = v; a.ldq = ld_q; a.ldk = ld_k; a.ldv = ld_v;
     a.cu_q = cu_q; a.cu_k = cu_k; a.nseg = nseg; a.total_q = total_q; a.total_k = total_k;
     a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.d = head_dim;
-    // (Caps above a quarter of the largest number cap nothing that is not about to overflow; a multiplier past
-    // it is cut, so that a product of zero stays zero under it.)
+    // (Caps near the largest number, or that products of 2^113 at least are small against, cap nothing that
+    // fp32 holds: taken lower, so that scale / cap stays a normal number.  A multiplier past the largest
+    // number is cut, so that a product of zero stays zero under it.)
     constexpr float kLargest = std::numeric_limits<float>::max();
-    cap = std::min(cap, kLargest / 4);
+    cap = std::min({cap, kLargest / 4, scale * 0x1p126f});
     a.scale_log2 = scale * kLog2e;
     a.cap_log2 = cap * kLog2e;
     a.over_cap = cap > 0.0f ? scale / cap : 0.0f;
-    a.dot_mul = a.over_cap < 0x1p-126f ? 0x1p-64f : 1.0f;
-    a.dot_over_cap = cap > 0.0f ? static_cast<float>(static_cast<double>(scale) / cap / a.dot_mul) : 0.0f;
     a.exp_mul = std::min(2.0f * kLog2e * a.over_cap, kLargest);
     a.slopes = slopes; a.causal = causal; a.prefix = prefix; a.o = o; a.ldo = ld_o;
     const int elem = dtype == PXS_BF16 ? 2 : 4;
