@@ -981,12 +981,15 @@ __device__ __forceinline__ TileSource<DH> tile_source(const ScoreArgs & a, const
 // own scores set.  From there on tile j's step issues the products that do not depend on
 // its weights, O += V P of the tile before and S of the next, and takes its weights while
 // they run, without a maximum: a row's weights are redone with one where their sum passes
-// 2^40 (bf16 and fp32 hold 2^127).  With a bias that falls with the distance the nearest
-// keys come first, so that is rare.  Bound by the vector instructions of the weights beside the products,
+// 2^40.  With a bias that falls with the distance the nearest keys come first, so that is rare.
+// Weights past 1 may take large values past what fp32 holds: where outputs pass 2^118 (512 splits of
+// them can be joined) the tile is walked again with exact steps alone, whose weights are at most 1, as those
+// of the other kernels are.  Bound by the vector instructions of the weights beside the products,
 // and by the waits between the two: 8,192 tokens, 16 heads of 128, 0.53 to 0.56 ms (980 to 1,040 TFLOP/s; the
 // matrix cores busy in 55% of the cycles), of 64 0.30 to 0.32 ms, with a cap 0.41, with a bias of both sides 0.45.
 constexpr int kSlots = 4;
 constexpr float kSumLimit = 0x1p40f;
+constexpr float kOutLimit = 0x1p118f;
 
 template <int DH, int MODE, bool WHOLE>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) score_attn_rows_kernel(ScoreArgs a) {
@@ -1037,7 +1040,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
 #pragma unroll
     for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
     RowState st{-INFINITY, 0.0f};
-    bool odd = false;
+    bool odd = false, past = false;
     // Exact steps: tiles with hidden keys, and one of whole keys.
     const int exact = min(n, max(last + 1 - whole, 0) + 1);
     if (n > 0) issue(0);
@@ -1045,7 +1048,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
     typename F::Scores s_a, s_b;
     typename F::Weights p;
     int i = 0;
-    for (; i < exact; ++i) {
+    auto exact_step = [&]() __attribute__((always_inline)) {
         if (i + 1 < n) wait_vmcnt(kMine);
         else wait_vmcnt(0);
         barrier_no_fence();
@@ -1057,7 +1060,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
             tile_exact<DH, MODE>(rs, cap_log2, s_a, p, oacc, st, behind(i), seen - tile * F::kKeys);
             tile_pv<DH>(v_of(i), p, oacc, lane);
         }
-    }
+    };
+    for (; i < exact; ++i) exact_step();
     // (The step as a scalar: taken for a lane's, it kept a second copy of the output alive through the
     // loop, and the compiler, out of registers, waited for every read of LDS: 475 us against 529 for the
     // capped prompts above.)
@@ -1117,13 +1121,28 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) s
             weights(i, s_b);
             tile_pv<DH>(v_of(i), p, oacc, lane);
         }
+        // (A sum of magnitudes: infinities and NaN stay in it.)
+        float size[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) size[e & 3] += fabsf(oacc[dt][e]);
+        past = live && !((size[0] + size[1]) + (size[2] + size[3]) < kOutLimit) && is_finite_bits(st.sum);
     }
-    if (__syncthreads_or(odd)) {
-        for (int j = 0; j < 32; ++j)
-            if (wave_row0 + j < w.rows)
-                row_alone<uint16_t, DH / 64>(a, w, wave_row0 + j, first * F::kKeys, (last + 1) * F::kKeys, lane,
-                                             w.splits > 1, split_slot(a, w, split, wave_row0 + j));
-        return;
+    if (__builtin_expect(__syncthreads_or(odd || past), 0)) {
+        if (__syncthreads_or(odd)) {
+            for (int j = 0; j < 32; ++j)
+                if (wave_row0 + j < w.rows)
+                    row_alone<uint16_t, DH / 64>(a, w, wave_row0 + j, first * F::kKeys, (last + 1) * F::kKeys, lane,
+                                                 w.splits > 1, split_slot(a, w, split, wave_row0 + j));
+            return;
+        }
+        issue(0);  // (every wave is done with the slots)
+        if (n > 1) issue(1);
+#pragma unroll
+        for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
+        st = {-INFINITY, 0.0f};
+        for (i = 0; i < n; ++i) exact_step();
     }
     const float sum = lane_pair_sum(st.sum);
     if (!live) return;

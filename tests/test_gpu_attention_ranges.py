@@ -1,5 +1,5 @@
 """Scored attention at the ends of what its arguments may be, against the formula in 64 bits:
-caps far above and far below the scores.
+caps far above and far below the scores, and values near the largest number.
 
 Tolerances are those of test_gpu_attention_scores.py but for a capped score, whose error is
 relative to the score here and not to the cap.  u = 2^-24, x = s / cap before the cap:
@@ -127,3 +127,35 @@ def test_small_scale_under_a_large_cap(px):
                 o = px.varlen_attention_scores(big, k, v, bounds(q_len), bounds(k_len), 2, 2, d, scale, cap=cap)
                 want, tol = formula(big, k, v, q_len, k_len, 2, 2, d, scale)
                 check(o, want, tol, f"scale {scale}")
+
+
+def heads_of(px, q, k, v, q_len, k_len, heads, kv, d, scale, sample, what, cap=0.0, bias=False, causal=False, prefix=None):
+    """The call, and the sampled heads of its output against the formula."""
+    slopes = alibi(heads) if bias else None
+    o = px.varlen_attention_scores(q, k, v, bounds(q_len), bounds(k_len), heads, kv, d, scale, cap=cap, slopes=slopes,
+                                   causal=causal, prefix=None if prefix is None else torch.tensor(prefix, device="cuda"))
+    for h in sample:
+        cols, kv_cols = slice(h * d, (h + 1) * d), slice(h // (heads // kv) * d, (h // (heads // kv) + 1) * d)
+        want, tol = formula(q[:, cols], k[:, kv_cols], v[:, kv_cols], q_len, k_len, 1, 1, d, scale, cap,
+                            None if slopes is None else slopes[h:h + 1], causal, prefix)
+        check(o[:, cols], want, tol, f"{what}, head {h}")
+
+
+@pytest.mark.parametrize("heads", [2, 40])  # the keys split over workgroups, and walked by one
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("mode", [dict(), dict(causal=True), dict(causal=True, bias=True), dict(cap=100.0)])
+def test_large_values_under_rising_scores(px, d, heads, mode):
+    """Values near the largest number, and scores that rise by e^25 along the walk from the last key to the
+    first: no weight may carry the sums past what fp32 holds where the result is well within."""
+    n = 900
+    gen = torch.Generator("cuda").manual_seed(65)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
+    q, k = 0.02 * rand(n, heads, d), rand(n, heads, d)
+    q[:, :, 0], k[:, :, 0] = 1.0, 0.0
+    for at, score in ((10, 45.0), (300, 25.0), (480, 25.0), (700, 20.0)):
+        k[at, :, 0] = score
+    q, k = (t.reshape(n, heads * d).bfloat16() for t in (q, k))
+    for size in (1e30, 1e36):
+        v = (size * rand(n, heads * d)).bfloat16()
+        print(f"[scores] large values d={d} heads={heads} {mode} {size}", flush=True)
+        heads_of(px, q, k, v, [n], [n], heads, heads, d, 1.0, [0, heads - 1], f"values of {size}", **mode)
