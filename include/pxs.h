@@ -401,6 +401,12 @@ int pxs_linear_i8(const int8_t * x, const float * x_scales, int64_t rows, int ci
                   const int8_t * weight, const float * w_scales, const float * bias, int cout,
                   int act, int y_dtype, void * y, void * stream);
 
+/* On the host: what an 8-bit linear of these sizes runs on (any epilogue), for tests and
+ * profiles.  tile[0] rows by tile[1] channels a workgroup; tile[2] stages of K in shared
+ * memory, 1 where they pass through registers and 0 where operands are read as they lie;
+ * zeros for no rows.  whole_pieces: x and weight are 16-byte aligned. */
+int pxs_linear_i8_tile(int64_t rows, int cin, int cout, int whole_pieces, int * tile);
+
 /* residual (fp32) += the 8-bit linear, as pxs_linear_residual. */
 int pxs_linear_i8_residual(const int8_t * x, const float * x_scales, int64_t rows, int cin,
                            const int8_t * weight, const float * w_scales, const float * bias,

@@ -751,12 +751,12 @@ int launch_i8_few(const I8Args & a, hipStream_t s) {
 //   64 x 64, 4 waves, two:                               150 x 4096 -> 4096 15.1 against 17.0
 //   32 x 64, four groups of two waves over K, one:       300 x 4096 -> 1024 8.4 against 14.8
 struct I8Shape {
-    int bm, bn;
+    int bm, bn, stages;
     double alone0, alone1, each0, each1;
 };
 constexpr I8Shape kI8Shapes[] = {
-    {256, 256, 7.3, 8.9, 10.8, 13.4}, {192, 128, 4.9, 4.8, 4.2, 5.9}, {128, 128, 3.9, 4.0, 2.7, 4.4},
-    {128, 64, 3.6, 3.3, 2.0, 2.8},    {64, 64, 3.1, 2.9, 1.4, 2.0},   {32, 64, 3.7, 1.1, 2.7, 1.2},
+    {256, 256, 2, 7.3, 8.9, 10.8, 13.4}, {192, 128, 2, 4.9, 4.8, 4.2, 5.9}, {128, 128, 2, 3.9, 4.0, 2.7, 4.4},
+    {128, 64, 3, 3.6, 3.3, 2.0, 2.8},    {64, 64, 4, 3.1, 2.9, 1.4, 2.0},   {32, 64, 3, 3.7, 1.1, 2.7, 1.2},
 };
 
 int i8_shape(int64_t m, int n, int k) {
@@ -776,44 +776,61 @@ int i8_shape(int64_t m, int n, int k) {
     return best;
 }
 
-constexpr int kI8DeepK = 1024;  // a longer K is worth a third stage (launch_i8)
+constexpr int kI8DeepK = 1024;  // a longer K is worth a third stage (i8_plan)
 
 // Up to kI8FewRows rows: 16 output channels a workgroup, and as few of its 16-row blocks as
 // keep the workgroups near one a CU.
 constexpr int64_t kI8FewRows = 64;
 
-template <typename T, int EPI>
-int launch_i8(I8Args a, hipStream_t s) {
-    a.group_m = 8;
-    if (a.m <= kI8FewRows) {
-        const int64_t blocks = (a.n + 15) / 16 * ((a.m + 15) / 16);
-        if (blocks <= 256 || a.m <= 16) return launch_i8_few<T, 1, EPI>(a, s);
-        if (blocks <= 512 || a.m <= 32) return launch_i8_few<T, 2, EPI>(a, s);
-        return launch_i8_few<T, 4, EPI>(a, s);
+// What a call runs on: its tile of rows by output channels, and its stages of K in LDS by DMA; 1 through
+// registers (linear_i8_any_kernel), 0 straight from memory (linear_i8_few_kernel).
+struct I8Plan {
+    int bm, bn, stages;
+};
+
+// pieces: cin and the operands' addresses are multiples of 16.
+I8Plan i8_plan(int64_t m, int n, int k, bool pieces) {
+    if (m <= kI8FewRows) {
+        const int64_t blocks = (n + 15) / 16 * ((m + 15) / 16);
+        if (blocks <= 256 || m <= 16) return {16, 16, 0};
+        if (blocks <= 512 || m <= 32) return {32, 16, 0};
+        return {64, 16, 0};
     }
-    if (a.k % 16 != 0 || !aligned_to(a.x, 16) || !aligned_to(a.w, 16)) {
+    auto tiles = [&](int bm, int bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
+    if (!pieces) {
         // Rounds of tiles over the 256 CUs, 12.6 us each of 128 rows and 21.7 of 192 (4,739 x 1370 ->
         // 1021: 25.3 us in two rounds, 22.0 in one; 20,000 rows 60 and 66).
-        auto rounds = [&](int bm) { return (((a.m + bm - 1) / bm) * ((a.n + 127) / 128) + 255) / 256; };
-        if (21.7 * rounds(192) < 12.6 * rounds(128)) return launch_i8_any<T, 192, 128, 8, 2, EPI>(a, s);
-        return launch_i8_any<T, 128, 128, 8, 2, EPI>(a, s);
+        auto rounds = [&](int bm) { return (tiles(bm, 128) + 255) / 256; };
+        return {21.7 * rounds(192) < 12.6 * rounds(128) ? 192 : 128, 128, 1};
     }
+    const I8Shape & c = kI8Shapes[i8_shape(m, n, k)];
     // Three stages where a CU has one tile at most, so that no second tile's stages need fit, and K is
     // longer than their start (1,500 x 4096 -> 2048 22 us against 27, 1,370 x 2048 -> 4096 19.6 against 20.4,
     // but 1,000 x 1024 -> 4096 9.8 against 9.5; four stages the same as three).
-    auto deep = [&](int bm, int bn) {
-        return a.k > kI8DeepK && ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn) <= 256;
-    };
-    switch (i8_shape(a.m, a.n, a.k)) {
-    case 0: return launch_i8_tiles<T, 256, 256, 16, 4, 2, 1, EPI>(a, s);
-    case 1:
-        if (deep(192, 128)) return launch_i8_tiles<T, 192, 128, 8, 2, 3, 1, EPI>(a, s);
+    const bool deep = k > kI8DeepK && tiles(c.bm, c.bn) <= 256;
+    return {c.bm, c.bn, c.stages + (c.bn == 128 && deep ? 1 : 0)};
+}
+
+template <typename T, int EPI>
+int launch_i8(I8Args a, hipStream_t s) {
+    a.group_m = 8;
+    const I8Plan p = i8_plan(a.m, a.n, a.k, a.k % 16 == 0 && aligned_to(a.x, 16) && aligned_to(a.w, 16));
+    if (p.stages == 0) {
+        if (p.bm == 16) return launch_i8_few<T, 1, EPI>(a, s);
+        return p.bm == 32 ? launch_i8_few<T, 2, EPI>(a, s) : launch_i8_few<T, 4, EPI>(a, s);
+    }
+    if (p.stages == 1)
+        return p.bm == 192 ? launch_i8_any<T, 192, 128, 8, 2, EPI>(a, s) : launch_i8_any<T, 128, 128, 8, 2, EPI>(a, s);
+    switch (p.bm) {
+    case 256: return launch_i8_tiles<T, 256, 256, 16, 4, 2, 1, EPI>(a, s);
+    case 192:
+        if (p.stages == 3) return launch_i8_tiles<T, 192, 128, 8, 2, 3, 1, EPI>(a, s);
         return launch_i8_tiles<T, 192, 128, 8, 2, 2, 1, EPI>(a, s);
-    case 2:
-        if (deep(128, 128)) return launch_i8_tiles<T, 128, 128, 8, 2, 3, 1, EPI>(a, s);
+    case 128:
+        if (p.bn == 64) return launch_i8_tiles<T, 128, 64, 8, 4, 3, 1, EPI>(a, s);
+        if (p.stages == 3) return launch_i8_tiles<T, 128, 128, 8, 2, 3, 1, EPI>(a, s);
         return launch_i8_tiles<T, 128, 128, 8, 2, 2, 1, EPI>(a, s);
-    case 3: return launch_i8_tiles<T, 128, 64, 8, 4, 3, 1, EPI>(a, s);
-    case 4: return launch_i8_tiles<T, 64, 64, 4, 2, 4, 1, EPI>(a, s);
+    case 64: return launch_i8_tiles<T, 64, 64, 4, 2, 4, 1, EPI>(a, s);
     default: return launch_i8_tiles<T, 32, 64, 2, 1, 3, 4, EPI>(a, s);
     }
 }
@@ -870,6 +887,19 @@ int pxs_linear_i8(const int8_t * x, const float * x_scales, int64_t rows, int ci
     if (a.vec_out && cout % (y_dtype == PXS_BF16 ? 8 : 4) == 0 && aligned_to(y, 16)) a.vec_out = 2;
     return y_dtype == PXS_F32 ? launch_i8<float, kI8Store>(a, as_stream(stream))
                               : launch_i8<uint16_t, kI8Store>(a, as_stream(stream));
+}
+
+int pxs_linear_i8_tile(int64_t rows, int cin, int cout, int whole_pieces, int * tile) {
+    bool run;
+    const int8_t some = 0;
+    const float one = 1.0f;
+    if (int rc = check_i8("pxs_linear_i8_tile", &some, &one, rows, cin, &some, &one, cout, tile, &run)) return rc;
+    PXS_CHECK(tile, PXS_ERR_ARG, "pxs_linear_i8_tile: null pointer");
+    const I8Plan p = run ? i8_plan(rows, cout, cin, whole_pieces && cin % 16 == 0) : I8Plan{};
+    tile[0] = p.bm;
+    tile[1] = p.bn;
+    tile[2] = p.stages;
+    return PXS_OK;
 }
 
 int pxs_linear_i8_residual(const int8_t * x, const float * x_scales, int64_t rows, int cin, const int8_t * weight,

@@ -54,6 +54,7 @@ _SIGS = {
                                     _i32, _vp, C.c_uint32, _vp, _vp]),
     "pxs_quantize_rows_i8": (_i32, [_i32, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
     "pxs_linear_i8": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
+    "pxs_linear_i8_tile": (_i32, [_i64, _i32, _i32, _i32, C.POINTER(C.c_int)]),
     "pxs_linear_i8_residual": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp]),
     "pxs_linear_i8_gate_residual": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i32,
                                            _vp, _vp]),
