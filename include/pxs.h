@@ -556,7 +556,11 @@ int pxs_varlen_attention_noalloc(int dtype, const void * q, int64_t ld_q, const 
  * multiple of 8 up to 128 (64 and 128 best), 16-byte-aligned q, k and v, and strides that
  * are multiples of 8 takes the fastest kernels.  The result depends on the whole call's sizes in its
  * last bits (the keys of few rows are split and joined in a fixed order); the
- * same call gives the same bits.
+ * same call gives the same bits.  Whether keys are split is decided for the whole call: new
+ * tokens over long caches and long prompts run faster as two calls (a prompt of 4,000 and eight
+ * tokens over caches of 1 to 65,536 keys: 0.11 and 0.08 ms, 1.5 ms as one).   Calls of
+ * more than 2^24 - 1 workgroups are refused: one holds 128 (query, head) rows of a segment, or
+ * where segments have few rows (32 on average) one (query, head).
  * workspace: pxs_attention_scores_workspace_bytes of the same sizes; calls that
  * may overlap need one each. */
 size_t pxs_attention_scores_workspace_bytes(int nseg, int64_t total_q, int64_t total_k, int heads,

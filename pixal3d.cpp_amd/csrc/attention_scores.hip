@@ -166,9 +166,9 @@ __device__ __forceinline__ int tiles_below(int x, int nq, int nk, int prefix, in
 
 // The t-th row tile of a call with a causal mask and 2 to 64 segments, those that see most keys
 // first: 64 classes of keys seen, counted by a lane each, then the tile within its class.  (In
-// the segments' order, reversed, the last of a call's tiles may be long ones: eight prompts of 2,048
-// tokens, 16 heads of 128, 173 us against 189; ten of 100 to 5,000, 299 against 316; prompts of
-// 8192, 2903 and 4739, 445 against 453 (before the main loop's last gain, of 5 to 11%).  Two prompts whose first 1370 tokens all see lose 3%.)
+// the segments' order, reversed, the last of a call's tiles may be long ones: 16 heads of 128 over 4, eight prompts
+// of 2,048 tokens 172 us against 187; ten of 100 to 5,000, 295 against 306; five of 8,000 to 500, 365 against
+// 376; 8192, 2903 and 4739 with a cap, 483 against 495.  Two prompts whose first 1370 tokens all see lose 3%.)
 __device__ __forceinline__ bool locate_sorted(const ScoreArgs & a, int t, int rows_per_tile, int lane, Rows & w) {
     const int shift = 31 - __clz(rows_per_tile);
     const Segment g = lane_segment(a, lane);
@@ -263,6 +263,9 @@ __device__ __forceinline__ bool is_finite_bits(float v) { return (__float_as_uin
 // A row again, one key after the other, keys that it does not see left out
 // altogether: for tiles where an unseen key's value is infinite or NaN, which
 // times a weight of zero is NaN.  One wave per row; lane l holds dims l, l + 64, ...
+// Slow, a key a step: where a causal prompt's last value is NaN, 16 heads of 128, 1,024 tokens take 7.4 ms
+// (87 us without), 8,192 take 327 (0.33); 8 tokens over 8,192 keys 0.42 (0.09).  The last row sees such a value
+// and is NaN itself, so it is met in broken data alone.
 // (Inlined: a call would take the arguments in memory, and with them every kernel's scalars.)
 template <typename T, int NC>
 __device__ __forceinline__ void row_alone(const ScoreArgs & a, const Rows & w, int row, int key0, int key1, int lane, bool partial,
@@ -794,7 +797,11 @@ struct RowState {
     float base, sum;
 };
 
-// Weights of a tile relative to state.base: p = 2^(z - base), and their sum over this lane.
+// Weights of a tile relative to state.base: p = 2^(z - base), and their sum over this lane.  They are rounded to
+// bf16, as pxs_varlen_attention's are and as the values that they multiply are: the matrix cores take both operands
+// in one type, and a second term of each weight would be half as many products again.  The sum is of the rounded
+// weights, so their errors' mean cancels.  Relative L2 error against 64 bits 0.0017 to 0.0020, of which the
+// output's own rounding is 0.0017.
 // behind: the lane's query position minus the tile's first key and 4 h.
 // With kBehind the bias is a line over the keys, one operation a score and not two.
 template <int DH, int MODE>
@@ -1453,9 +1460,9 @@ constexpr int64_t kScoreMaxRows = INT32_MAX - 1023;  // rows and keys are counte
 constexpr int kWaveSegments = 64;   // segments that a wave's lanes hold; more take a table
 constexpr int kRowTile = 128;
 constexpr int64_t kSplitGrid = 512; // workgroups (two a CU) up to which a call's keys are split
-// fp32: one and a half rounds of the two workgroups a CU (heads up to 64), or two of its one.  1,517 queries
-// over 2,887 keys, 16 heads of 64: 107 us, with 512 136, with 1024 119; 2,000 tokens, 16 heads of 128: 175 us,
-// with 384 246, with 768 202.
+// fp32: one and a half rounds of the two workgroups a CU (heads up to 64), or two of its one.  Twelve calls of
+// 256 to 4,000 queries over 1,000 to 8,192 keys, 4 to 32 heads, geometric mean: heads of 64 the same with 512
+// (single calls 20% faster to 24% slower) and 2% slower with 1024; heads of 128 23% slower with 256, 7% with 768.
 constexpr int64_t kSplitGridF32 = 768, kSplitGridF32Wide = 512;
 
 int64_t row_tiles(int64_t total_q, int nseg, int group) { return total_q * group / kRowTile + nseg; }
@@ -1479,9 +1486,11 @@ int64_t split_rows(int64_t total_q, int64_t total_k, int heads) {
 }
 
 // Few rows a segment: keys of a chunk, so that a call has about kFewItems items, two rounds of two
-// workgroups a CU.  Eight tokens over 170,161 keys, 8 key/value heads of 128: 142 us (4.9 TB/s) with
-// 1,024 items, 153 with 1,536, 157 with 768, 170 with 512; at least 128 keys, a tile or two for each
-// wave: one token over 1,501 keys, 16 heads of 64, 10.1 us against 11.6 with 256.
+// workgroups a CU.  Ragged caches want them: eight tokens over 170,161 keys in caches of 1 to 65,536, 8 key/value
+// heads of 128: 138 us (5.05 TB/s), with 512 items 168, with 2,048 149.  Of twelve other calls (1 to 128
+// tokens, caches alike or one) five take the same with 512 and seven 3 to 24% less; 2,048 costs 6% on average.
+// At least 128 keys, a tile or two for each wave: one token over 1,501 keys, 16 heads of 64, 10.2 us against
+// 11.5 with 256; of the others four are 5 to 23% slower with 256 and two 21 to 23% faster.
 constexpr int64_t kFewItems = 1024;
 constexpr int64_t kFewKeys = 128;  // at least, and a multiple of
 int64_t few_chunk(int64_t total_k, int kv_heads) {

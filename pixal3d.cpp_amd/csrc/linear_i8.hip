@@ -799,7 +799,9 @@ I8Plan i8_plan(int64_t m, int n, int k, bool pieces) {
     auto tiles = [&](int bm, int bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
     if (!pieces) {
         // Rounds of tiles over the 256 CUs, 12.6 us each of 128 rows and 21.7 of 192 (4,739 x 1370 ->
-        // 1021: 25.3 us in two rounds, 22.0 in one; 20,000 rows 60 and 66).
+        // 1021: 23.7 us in two rounds, 20.5 in one; 20,000 rows 58 and 61).  At 43 of 55 sizes, 500 to 42,000 rows
+        // and 130 to 4090 deep, the pick is the faster form or within 5%; where 128 rows take three rounds
+        // or more it is up to 20% slower (42,000 x 1370 -> 1021 122 us, 108 with 192 rows).
         auto rounds = [&](int bm) { return (tiles(bm, 128) + 255) / 256; };
         return {21.7 * rounds(192) < 12.6 * rounds(128) ? 192 : 128, 128, 1};
     }
