@@ -420,6 +420,54 @@ int pxs_linear_i8_gate_residual(const int8_t * x, const float * x_scales, int64_
                                 const float * time_mod, int gate_offset, float * residual,
                                 void * stream);
 
+/* ---- linears in microscaled 4-bit floating point ------------------------------------
+ * Next to the linears in 8 bits (no counterpart in the reference): values in
+ * blocks of 32 of a row, each block under a power of two, a value as a sign,
+ * two bits of exponent and one of mantissa (0, 1/2, 1, 3/2, 2, 3, 4, 6).
+ *
+ * Layout.  codes: a row is pxs_mxfp4_code_bytes(channels) = 16 bytes a block,
+ * two values a byte, the earlier in its low half (sign, exponent, mantissa
+ * from the half's top bit down); codes past the row's end must be zero.
+ * scales: a row is pxs_mxfp4_scale_bytes(channels) bytes, the number of blocks
+ * rounded up to a multiple of 16: byte b scales block b's values by
+ * 2^(b - 127), 255 makes them NaN; what the bytes past the last block hold does
+ * not matter.  Rows follow one another; codes and scales are 16-byte aligned.
+ *
+ * pxs_quantize_mxfp4: a block's scale is 2^(floor(log2 max|x|) - 2), at
+ * least 2^-127, and each value the nearest of the eight magnitudes to
+ * |x| / scale, ties to the one with an even code, above 6 6.  A block that holds
+ * an infinity or a NaN gets scale 255 and zeros.  x has rows of any stride.
+ * Weights [cout, cin] are quantized by the same call, once.
+ * pxs_dequantize_mxfp4: the values back (rounded to bf16: exact but below
+ * 2^-126). */
+size_t pxs_mxfp4_code_bytes(int channels);
+size_t pxs_mxfp4_scale_bytes(int channels);
+int pxs_quantize_mxfp4(int dtype, const void * x, int64_t ld_x, int64_t rows, int channels,
+                       uint8_t * codes, uint8_t * scales, void * stream);
+int pxs_dequantize_mxfp4(const uint8_t * codes, const uint8_t * scales, int64_t rows, int channels,
+                         int dtype, void * y, int64_t ld_y, void * stream);
+
+/* y = act(x W^T + bias) in y_dtype, of the values that x's and weight's codes
+ * ([rows, cin], [cout, cin]) stand for: products exact, sums in fp32.  cin and
+ * cout are at most 2^30.  bias may be NULL; act is PXS_ACT_*.  The sums' order,
+ * and so their last bits, depends on the call's sizes. */
+int pxs_linear_mxfp4(const uint8_t * x, const uint8_t * x_scales, int64_t rows, int cin,
+                     const uint8_t * weight, const uint8_t * w_scales, const float * bias, int cout,
+                     int act, int y_dtype, void * y, void * stream);
+
+/* residual (fp32) += the 4-bit linear, as pxs_linear_residual. */
+int pxs_linear_mxfp4_residual(const uint8_t * x, const uint8_t * x_scales, int64_t rows, int cin,
+                              const uint8_t * weight, const uint8_t * w_scales, const float * bias,
+                              int cout, float * residual, void * stream);
+
+/* residual (fp32) += gate * the 4-bit linear, as pxs_linear_gate_residual
+ * (gate_offset 0..5 * cout). */
+int pxs_linear_mxfp4_gate_residual(const uint8_t * x, const uint8_t * x_scales, int64_t rows,
+                                   int cin, const uint8_t * weight, const uint8_t * w_scales,
+                                   const float * bias, int cout, const int32_t * coords,
+                                   const float * block_mod, const float * time_mod, int gate_offset,
+                                   float * residual, void * stream);
+
 /* ---- a10-a12: row-wise normalisation and position embedding ------------------- */
 
 /* sparse_layer_norm (src/sparse.cpp:490-534); gamma/beta both NULL or both set.
@@ -439,6 +487,27 @@ int pxs_layer_norm_modulate(int x_dtype, const void * x, int64_t rows, int chann
  * (src/sparse.cpp:919-997).  Rows have stride ld_x / ld_y elements. */
 int pxs_mh_rms_norm(int dtype, const void * x, int64_t ld_x, int64_t rows, int heads,
                     int head_dim, const float * gamma, void * y, int64_t ld_y, void * stream);
+
+/* The residual's addition and the root-mean-square norm of whole rows, for
+ * token models (no counterpart in the reference):
+ *   h = residual + x, rounded to the residual's type and stored in residual_out
+ *     (which may be residual; both [rows, channels], both NULL: h is x)
+ *   inv = 1 / sqrt(mean of h^2 + eps)
+ *   pxs_rms_norm: y = h * inv * gamma, [rows, channels] in y_dtype
+ *   pxs_rms_norm_i8: the rows h * gamma * inv in 8 bits, the input of
+ *     pxs_linear_i8: q and scales as pxs_quantize_rows_i8 makes them of the rows
+ *     t = h * gamma (each product rounded to fp32), its scales times inv.  A
+ *     row whose t are all below 2^-100 gets scale 0 and zeros, one whose t are not
+ *     all finite scale NaN and zeros.
+ * x has rows of stride ld_x, its type and the residual's are independent;
+ * gamma (fp32 [channels]) may be NULL: ones.  eps is positive.  y, q and scales
+ * must not overlap the inputs. */
+int pxs_rms_norm(int x_dtype, const void * x, int64_t ld_x, int residual_dtype,
+                 const void * residual, void * residual_out, int64_t rows, int channels, float eps,
+                 const float * gamma, int y_dtype, void * y, void * stream);
+int pxs_rms_norm_i8(int x_dtype, const void * x, int64_t ld_x, int residual_dtype,
+                    const void * residual, void * residual_out, int64_t rows, int channels,
+                    float eps, const float * gamma, int8_t * q, float * scales, void * stream);
 
 /* sparse_rotary_position_embedding (src/sparse.cpp:861-917). */
 int pxs_rope(int dtype, const int32_t * coords, const void * x, int64_t ld_x, int64_t rows,
@@ -571,6 +640,44 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
                                 int heads, int kv_heads, int head_dim, float scale, float cap,
                                 const float * slopes, int causal, const int64_t * prefix, void * o,
                                 int64_t ld_o, void * workspace, void * stream);
+
+/* Attention of drafted tokens over a cache, next to
+ * pxs_varlen_attention_scores (no counterpart in the reference).  The tokens of
+ * segment s, rows [cu_q[s], cu_q[s+1]) of q, k, v and o, continue a sequence
+ * whose keys and values are rows cache_start[s] .. + cache_len[s] - 1 of k_cache
+ * and v_cache (device int64 [nseg] each; sequences lie anywhere in the cache, with
+ * room between them, and several may share rows).
+ *   Tree: parents (device int32 [total_q]) holds for each token the one it
+ *     follows, counted from its segment's first, -1 for those that follow
+ *     the cache.  A token comes after its parent; a parent that is no
+ *     earlier token of the segment counts as -1.  A token sees the cached keys,
+ *     the tokens above it and itself; what the others hold does not matter, NaN
+ *     included.
+ *   Heads, head sizes, scale and cap: as pxs_varlen_attention_scores.
+ *   slopes (device fp32 [heads], may be NULL) lowers a score by slopes[head] *
+ *     |distance of the positions|: a cached key's is its place in the sequence, a
+ *     token's positions[row] (device int32 [total_q], needed with slopes).
+ * The cache is read only: rows of k and v that are accepted are appended by the
+ * caller.  total_q = cu_q[nseg]; rows of q and o behind the last segment are
+ * neither read nor written.  cache_rows is the cache's size in rows; total_q *
+ * heads / kv_heads and cache_rows are at most 2^31 - 1024.  Bounds past the rows
+ * are cut to them.  The lengths are read on the device alone: a captured call
+ * follows cache_start and cache_len as they change.  bf16 with head_dim a
+ * multiple of 8 up to 128 (64 and 128 best), 16-byte-aligned q, k, v and caches,
+ * and strides that are multiples of 8 takes the fastest kernels.  The same call
+ * gives the same bits; its last bits depend on all its lengths.
+ * workspace: pxs_tree_attention_workspace_bytes of the same sizes; calls that
+ * may overlap need one each. */
+size_t pxs_tree_attention_workspace_bytes(int nseg, int64_t total_q, int heads, int kv_heads,
+                                          int head_dim);
+int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, int64_t ld_k,
+                       const void * v, int64_t ld_v, const int64_t * cu_q, const int32_t * parents,
+                       const void * k_cache, int64_t ld_k_cache, const void * v_cache,
+                       int64_t ld_v_cache, const int64_t * cache_start, const int64_t * cache_len,
+                       int nseg, int64_t total_q, int64_t cache_rows, int heads, int kv_heads,
+                       int head_dim, float scale, float cap, const float * slopes,
+                       const int32_t * positions, void * o, int64_t ld_o, void * workspace,
+                       void * stream);
 
 /* Per-batch cu_seqlens from the batch column (src/sparse.cpp:731-737):
  * cu (device int64[batch_size + 1]). */

@@ -10,6 +10,7 @@
 // no order of it, and no tile, changes an output's bits.
 
 #include "pxs_common.h"
+#include "rows_i8.h"
 #include "tiles.h"
 
 #include <algorithm>
@@ -26,13 +27,7 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 // One pass: a row stays in registers between its maximum and its rounding, so
 // the bytes are those of x, q and the scales.  The maximum is taken of the bit
 // patterns of |x| as integers, which puts NaN above infinity above all numbers.
-// The product and the rounding are two roundings, as the formula says, never one
-// fused: adding 1.5 * 2^23 rounds the product to an integer, ties to even, and
-// leaves it in the sum's low byte.
-constexpr uint32_t kQuantFinite = 0x7F800000u;   // infinity's bits
-constexpr float kQuantLeast = 0x1p-100f;         // rows below count as zero: 127 / max stays finite
-constexpr float kRoundMagic = 12582912.0f;       // 1.5 * 2^23
-
+// (The rounding: rows_i8.h.)
 struct QuantArgs {
     const void * x;
     int64_t ldx;
@@ -61,31 +56,10 @@ __device__ __forceinline__ void load_elems8(const T * row, int c, int channels, 
     }
 }
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-
-// The scale of a row with this largest magnitude, and what its values are multiplied with.
-__device__ __forceinline__ void row_scale(uint32_t top_bits, float & scale, float & per) {
-    const float top = __uint_as_float(top_bits);
-    scale = 0.0f;
-    per = 0.0f;
-    if (top_bits >= kQuantFinite) {
-        scale = __uint_as_float(0x7FC00000u);  // NaN: the row's products are NaN
-    } else if (top >= kQuantLeast) {
-        scale = top / 127.0f;
-        per = 127.0f / top;
-    }
-}
-
 template <bool VEC>
 __device__ __forceinline__ void store_q8(int8_t * row, int c, int channels, const float (&v)[8], float per,
                                          bool finite) {
-#pragma clang fp contract(off)
-    uint32_t b[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(v[i] * per + kRoundMagic);
-    uint2 u;
-    u.x = (b[0] & 255u) | (b[1] & 255u) << 8 | (b[2] & 255u) << 16 | b[3] << 24;
-    u.y = (b[4] & 255u) | (b[5] & 255u) << 8 | (b[6] & 255u) << 16 | b[7] << 24;
+    uint2 u = q8_bytes(v, per);
     if (!finite) u = make_uint2(0u, 0u);
     if constexpr (VEC) {
         if (c < channels) __builtin_memcpy(row + min(c, channels - 8), &u, 8);

@@ -58,6 +58,19 @@ _SIGS = {
     "pxs_linear_i8_residual": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp]),
     "pxs_linear_i8_gate_residual": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i32,
                                            _vp, _vp]),
+    "pxs_mxfp4_code_bytes": (C.c_size_t, [_i32]),
+    "pxs_mxfp4_scale_bytes": (C.c_size_t, [_i32]),
+    "pxs_quantize_mxfp4": (_i32, [_i32, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "pxs_dequantize_mxfp4": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _i64, _vp]),
+    "pxs_linear_mxfp4": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
+    "pxs_linear_mxfp4_residual": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp]),
+    "pxs_linear_mxfp4_gate_residual": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i32,
+                                              _vp, _vp]),
+    "pxs_rms_norm": (_i32, [_i32, _vp, _i64, _i32, _vp, _vp, _i64, _i32, _f, _vp, _i32, _vp, _vp]),
+    "pxs_rms_norm_i8": (_i32, [_i32, _vp, _i64, _i32, _vp, _vp, _i64, _i32, _f, _vp, _vp, _vp, _vp]),
+    "pxs_tree_attention_workspace_bytes": (C.c_size_t, [_i32, _i64, _i32, _i32, _i32]),
+    "pxs_tree_attention": (_i32, [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp,
+                                  _i32, _i64, _i64, _i32, _i32, _i32, _f, _f, _vp, _vp, _vp, _i64, _vp, _vp]),
     "pxs_rope_frequencies": (_i32, [_i32] + [C.c_double] * 5 + [C.POINTER(C.c_double)]),
     "pxs_rope_positions": (_i32, [_i32, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _f, _vp, _i64, _vp]),
     "pxs_attention_scores_workspace_bytes": (C.c_size_t, [_i32, _i64, _i64, _i32, _i32, _i32]),
@@ -310,6 +323,12 @@ def _rows_ld(t, what, dev):
 def _expect(t, dtype, shape, what, dev):
     if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
         raise PxsError(f"{what} must be contiguous {dtype} {list(shape)} on the current device")
+
+
+def _mxfp4_bytes(channels):
+    """Bytes of a row's 4-bit codes and of its scales (pxs_mxfp4_code_bytes, pxs_mxfp4_scale_bytes)."""
+    blocks = -(-channels // 32)
+    return 16 * blocks, -(-blocks // 16) * 16
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -781,7 +800,137 @@ class Pxs:
             "pxs_linear_i8_gate_residual")
         return residual
 
+    # -- microscaled 4-bit linears ------------------------------------------------------
+    def quantize_mxfp4(self, x, out=None, scales=None):
+        """pxs_quantize_mxfp4 -> (codes uint8 [rows, 16 * blocks], scales uint8 [rows, blocks rounded up
+        to 16]); x may be a column slice (rows of any stride)."""
+        dev = _raw_device()
+        ld = _rows_ld(x, "quantize_mxfp4: x", dev)
+        rows, channels = x.shape
+        code_bytes, scale_bytes = _mxfp4_bytes(channels)
+        codes = torch.empty((rows, code_bytes), dtype=torch.uint8, device=x.device) if out is None else out
+        scales = torch.empty((rows, scale_bytes), dtype=torch.uint8, device=x.device) if scales is None else scales
+        _expect(codes, torch.uint8, (rows, code_bytes), "quantize_mxfp4: out", dev)
+        _expect(scales, torch.uint8, (rows, scale_bytes), "quantize_mxfp4: scales", dev)
+        self._check(self.lib.pxs_quantize_mxfp4(_dtype_code(x), x.data_ptr(), ld, rows, channels, codes.data_ptr(),
+                                                scales.data_ptr(), self.stream()), "pxs_quantize_mxfp4")
+        return codes, scales
+
+    def dequantize_mxfp4(self, codes, scales, channels, dtype=torch.float32, out=None):
+        """pxs_dequantize_mxfp4 -> [rows, channels] in `dtype` (or out, rows of any stride)."""
+        dev = _raw_device()
+        rows = codes.shape[0]
+        y = torch.empty((rows, channels), dtype=dtype, device=codes.device) if out is None else out
+        if y.shape != (rows, channels):
+            raise PxsError(f"dequantize_mxfp4: out must be {[rows, channels]}")
+        ld = _rows_ld(y, "dequantize_mxfp4: out", dev)
+        code_bytes, scale_bytes = _mxfp4_bytes(channels)
+        _expect(codes, torch.uint8, (rows, code_bytes), "dequantize_mxfp4: codes", dev)
+        _expect(scales, torch.uint8, (rows, scale_bytes), "dequantize_mxfp4: scales", dev)
+        self._check(self.lib.pxs_dequantize_mxfp4(codes.data_ptr(), scales.data_ptr(), rows, channels, _dtype_code(y),
+                                                  y.data_ptr(), ld, self.stream()), "pxs_dequantize_mxfp4")
+        return y
+
+    @staticmethod
+    def _mxfp4_operands(x, x_scales, weight, w_scales, cin, bias, out, what):
+        dev = _raw_device()
+        rows, cout = x.shape[0], weight.shape[0]
+        code_bytes, scale_bytes = _mxfp4_bytes(cin)
+        _expect(x, torch.uint8, (rows, code_bytes), what, dev)
+        _expect(x_scales, torch.uint8, (rows, scale_bytes), what, dev)
+        _expect(weight, torch.uint8, (cout, code_bytes), what, dev)
+        _expect(w_scales, torch.uint8, (cout, scale_bytes), what, dev)
+        if bias is not None:
+            _expect(bias, torch.float32, (cout,), what, dev)
+        _expect(out, out.dtype, (rows, cout), what, dev)
+        return rows, cout
+
+    def linear_mxfp4(self, x, x_scales, weight, w_scales, cin, bias=None, act=ACT_NONE, dtype=torch.bfloat16, out=None):
+        """pxs_linear_mxfp4: act(x W^T + bias) in `dtype` (or out's)."""
+        y = torch.empty((x.shape[0], weight.shape[0]), dtype=dtype, device=x.device) if out is None else out
+        rows, cout = self._mxfp4_operands(x, x_scales, weight, w_scales, cin, bias, y, "linear_mxfp4: an operand")
+        self._check(self.lib.pxs_linear_mxfp4(x.data_ptr(), x_scales.data_ptr(), rows, cin, weight.data_ptr(),
+                                              w_scales.data_ptr(), _ptr(bias), cout, act, _dtype_code(y),
+                                              y.data_ptr(), self.stream()),
+                    "pxs_linear_mxfp4")
+        return y
+
+    def linear_mxfp4_residual(self, x, x_scales, weight, w_scales, cin, bias, residual):
+        """pxs_linear_mxfp4_residual: residual (fp32) += the 4-bit linear."""
+        what = "linear_mxfp4_residual"
+        rows, cout = self._mxfp4_operands(x, x_scales, weight, w_scales, cin, bias, residual, what + ": an operand")
+        if residual.dtype != torch.float32:
+            raise PxsError(what + ": residual must be float32")
+        self._check(self.lib.pxs_linear_mxfp4_residual(_ptr(x), _ptr(x_scales), rows, cin, _ptr(weight), _ptr(w_scales),
+                                                       _ptr(bias), cout, _ptr(residual), self.stream()),
+                    "pxs_linear_mxfp4_residual")
+        return residual
+
+    def linear_mxfp4_gate_residual(self, x, x_scales, weight, w_scales, cin, bias, coords, block_mod, time_mod,
+                                   gate_offset, residual):
+        """pxs_linear_mxfp4_gate_residual: residual (fp32) += gate * the 4-bit linear; block_mod [6 cout],
+        time_mod [batch, 6 cout], coords int32 [rows, 4]."""
+        what = "linear_mxfp4_gate_residual"
+        rows, cout = self._mxfp4_operands(x, x_scales, weight, w_scales, cin, bias, residual, what + ": an operand")
+        dev = _raw_device()
+        if residual.dtype != torch.float32:
+            raise PxsError(what + ": residual must be float32")
+        _expect(coords, torch.int32, (rows, 4), what + ": coords", dev)
+        _expect(block_mod, torch.float32, block_mod.shape, what + ": block_mod", dev)
+        _expect(time_mod, torch.float32, time_mod.shape, what + ": time_mod", dev)
+        if block_mod.numel() != 6 * cout or time_mod.numel() % (6 * cout) != 0:
+            raise PxsError(what + ": block_mod must hold 6 * cout values, time_mod as many for each batch item")
+        self._check(self.lib.pxs_linear_mxfp4_gate_residual(
+            _ptr(x), _ptr(x_scales), rows, cin, _ptr(weight), _ptr(w_scales), _ptr(bias), cout, _ptr(coords),
+            _ptr(block_mod), _ptr(time_mod), gate_offset, _ptr(residual), self.stream()),
+            "pxs_linear_mxfp4_gate_residual")
+        return residual
+
     # -- row-wise ---------------------------------------------------------------------
+    @staticmethod
+    def _norm_operands(x, gamma, residual, residual_out, what):
+        dev = _raw_device()
+        ld = _rows_ld(x, what + ": x", dev)
+        rows, channels = x.shape
+        res_dtype = PXS_F32
+        if residual is not None:
+            res_dtype = _dtype_code(residual)
+            _expect(residual, residual.dtype, (rows, channels), what + ": residual", dev)
+            if residual_out is None:
+                residual_out = residual
+            else:
+                _expect(residual_out, residual.dtype, (rows, channels), what + ": residual_out", dev)
+        elif residual_out is not None:
+            raise PxsError(what + ": residual_out without residual")
+        if gamma is not None:
+            _expect(gamma, torch.float32, (channels,), what + ": gamma", dev)
+        return dev, ld, rows, channels, res_dtype, residual_out
+
+    def rms_norm(self, x, eps, gamma=None, residual=None, residual_out=None, out=None, out_dtype=None):
+        """pxs_rms_norm -> the normed rows in out_dtype (x's by default); residual += x first, in place or
+        to residual_out."""
+        dev, ld, rows, channels, res_dtype, res_out = self._norm_operands(x, gamma, residual, residual_out, "rms_norm")
+        y = torch.empty((rows, channels), dtype=out_dtype or x.dtype, device=x.device) if out is None else out
+        _expect(y, y.dtype, (rows, channels), "rms_norm: out", dev)
+        self._check(self.lib.pxs_rms_norm(_dtype_code(x), x.data_ptr(), ld, res_dtype, _ptr(residual), _ptr(res_out), rows,
+                                          channels, eps, _ptr(gamma), _dtype_code(y), y.data_ptr(), self.stream()),
+                    "pxs_rms_norm")
+        return y
+
+    def rms_norm_i8(self, x, eps, gamma=None, residual=None, residual_out=None, out=None, scales=None):
+        """pxs_rms_norm_i8 -> (int8 [rows, channels], fp32 scales [rows]), the input of linear_i8; residual
+        += x first, in place or to residual_out."""
+        dev, ld, rows, channels, res_dtype, res_out = self._norm_operands(x, gamma, residual, residual_out, "rms_norm_i8")
+        q = torch.empty((rows, channels), dtype=torch.int8, device=x.device) if out is None else out
+        scales = torch.empty(rows, dtype=torch.float32, device=x.device) if scales is None else scales
+        _expect(q, torch.int8, (rows, channels), "rms_norm_i8: out", dev)
+        _expect(scales, torch.float32, (rows,), "rms_norm_i8: scales", dev)
+        self._check(self.lib.pxs_rms_norm_i8(_dtype_code(x), x.data_ptr(), ld, res_dtype, _ptr(residual), _ptr(res_out),
+                                             rows, channels, eps, _ptr(gamma), q.data_ptr(), scales.data_ptr(),
+                                             self.stream()),
+                    "pxs_rms_norm_i8")
+        return q, scales
+
     def layer_norm(self, x, eps, gamma=None, beta=None, out_dtype=None):
         out_dtype = out_dtype or x.dtype
         y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
@@ -930,6 +1079,43 @@ class Pxs:
             _dtype_code(q), q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(), ld_v, cu_q.data_ptr(),
             cu_k.data_ptr(), nseg, total_q, total_k, heads, kv_heads, head_dim, scale, cap, _ptr(slopes), int(causal),
             _ptr(prefix), o.data_ptr(), ld_o, ws.data_ptr(), self.stream()), "pxs_varlen_attention_scores")
+        return o
+
+    def tree_attention_workspace(self, nseg, total_q, heads, kv_heads, head_dim, device="cuda"):
+        """A workspace for tree_attention calls of up to these sizes, whatever the caches' lengths."""
+        return self._ws(self.lib.pxs_tree_attention_workspace_bytes(nseg, total_q, heads, kv_heads, head_dim), device)
+
+    def tree_attention(self, q, k, v, cu_q, parents, k_cache, v_cache, cache_start, cache_len, heads, kv_heads, head_dim,
+                       scale, cap=0.0, slopes=None, positions=None, out=None, workspace=None):
+        """pxs_tree_attention: q [*, heads * head_dim], k, v and the caches [*, kv_heads * head_dim] (rows of
+        any stride), cu_q int64 [segments + 1], parents int32 [*], cache_start and cache_len int64 [segments]."""
+        dev = _raw_device()
+        what = "tree_attention"
+        nseg, total_q, cache_rows = cu_q.numel() - 1, q.shape[0], k_cache.shape[0]
+        o = torch.empty((total_q, heads * head_dim), dtype=q.dtype, device=q.device) if out is None else out
+        ld_q, ld_k, ld_v, ld_kc, ld_vc, ld_o = [_rows_ld(t, "tree_attention: q, k, v, caches and out", dev)
+                                                for t in (q, k, v, k_cache, v_cache, o)]
+        wide, narrow, cache = (total_q, heads * head_dim), (total_q, kv_heads * head_dim), (cache_rows, kv_heads * head_dim)
+        if q.shape != wide or o.shape != wide or k.shape != narrow or v.shape != narrow or k_cache.shape != cache or \
+                v_cache.shape != cache or not q.dtype is k.dtype is v.dtype is k_cache.dtype is v_cache.dtype is o.dtype:
+            raise PxsError(f"{what}: q and out must be {list(wide)}, k and v {list(narrow)}, the caches {list(cache)}, of one dtype")
+        _expect(cu_q, torch.int64, (nseg + 1,), what + ": cu_q", dev)
+        _expect(parents, torch.int32, (total_q,), what + ": parents", dev)
+        _expect(cache_start, torch.int64, (nseg,), what + ": cache_start", dev)
+        _expect(cache_len, torch.int64, (nseg,), what + ": cache_len", dev)
+        if slopes is not None:
+            _expect(slopes, torch.float32, (heads,), what + ": slopes", dev)
+        if positions is not None:
+            _expect(positions, torch.int32, (total_q,), what + ": positions", dev)
+        need = self.lib.pxs_tree_attention_workspace_bytes(nseg, total_q, heads, kv_heads, head_dim)
+        ws = self._ws(need, q.device) if workspace is None else workspace
+        if ws.numel() * ws.element_size() < need or ws.get_device() != dev:
+            raise PxsError(f"{what}: a workspace of {need} bytes on the current device needed")
+        self._check(self.lib.pxs_tree_attention(
+            _dtype_code(q), q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(), ld_v, cu_q.data_ptr(),
+            parents.data_ptr(), k_cache.data_ptr(), ld_kc, v_cache.data_ptr(), ld_vc, cache_start.data_ptr(),
+            cache_len.data_ptr(), nseg, total_q, cache_rows, heads, kv_heads, head_dim, scale, cap, _ptr(slopes),
+            _ptr(positions), o.data_ptr(), ld_o, ws.data_ptr(), self.stream()), "pxs_tree_attention")
         return o
 
     def transformer_block(self, cfg: BlockConfig, weights: BlockWeights, coords, batch_size, cu,
