@@ -213,6 +213,14 @@ template <> __device__ __forceinline__ void store_f32<uint16_t>(uint16_t * p, fl
     *p = f32_to_bf16(v);
 }
 
+// 16 bytes stored past the caches, from any element: for results that the L2s (32 MB) would not hold.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void store16_past(void * p, const void * v) {
+    u32x4_any w;
+    __builtin_memcpy(&w, v, 16);
+    __builtin_nontemporal_store(w, static_cast<u32x4_any *>(p));
+}
+
 // Device-coherent stores (sc1): written through to the level every XCD reads
 // with device-coherent loads, for data that other workgroups of the same
 // launch consume.  A wave that has issued them waits with release_stores()

@@ -86,7 +86,7 @@ def inputs(rows, channels, x_dtype, res_dtype, seed, gamma=True):
     return x, residual, torch.exp(0.3 * rand(channels)) * (rand(channels).sign()) if gamma else None
 
 
-@pytest.mark.parametrize("channels", [1, 7, 8, 9, 64, 500, 512, 513, 1021, 1024, 1370, 2040, 2048, 2049, 4096, 4100, 8192, 8200, 20001])
+@pytest.mark.parametrize("channels", [1, 7, 8, 9, 64, 500, 512, 513, 1021, 1024, 1370, 2040, 2048, 2049, 4096, 4100, 8192, 8200, 12290, 20001])
 @pytest.mark.parametrize("x_dtype,res_dtype", [(F32, None), (BF16, None), (F32, F32), (BF16, F32), (F32, BF16), (BF16, BF16)])
 def test_widths(px, x_dtype, res_dtype, channels):
     for rows in (1, 3, 70):
@@ -122,7 +122,7 @@ def test_strides_and_alignment(px, dtype, channels):
             assert (r[:1 + shift] == 77).all() and (r[1 + shift + rows * channels:] == 77).all()
 
 
-@pytest.mark.parametrize("channels", [24, 700, 1024, 4096, 8200])
+@pytest.mark.parametrize("channels", [24, 700, 1024, 4096, 8200, 17000])
 def test_special_rows(px, channels):
     """Zeros, rows below and above what fp32 can square, subnormals, ties, infinities and NaN."""
     x = torch.zeros((14, channels))
