@@ -448,12 +448,17 @@ int pxs_dequantize_mxfp4(const uint8_t * codes, const uint8_t * scales, int64_t 
                          int dtype, void * y, int64_t ld_y, void * stream);
 
 /* y = act(x W^T + bias) in y_dtype, of the values that x's and weight's codes
- * ([rows, cin], [cout, cin]) stand for: products exact, sums in fp32.  cin and
- * cout are at most 2^30.  bias may be NULL; act is PXS_ACT_*.  The sums' order,
+ * ([rows, cin], [cout, cin]) stand for: products exact, sums in fp32.  cin is
+ * at most 2^24, cout 2^30.  bias may be NULL; act is PXS_ACT_*.  The sums' order,
  * and so their last bits, depends on the call's sizes. */
 int pxs_linear_mxfp4(const uint8_t * x, const uint8_t * x_scales, int64_t rows, int cin,
                      const uint8_t * weight, const uint8_t * w_scales, const float * bias, int cout,
                      int act, int y_dtype, void * y, void * stream);
+
+/* On the host: what a 4-bit linear of these sizes runs on (any epilogue), for tests and
+ * profiles.  tile[0] rows by tile[1] channels a workgroup; tile[2] stages of K in shared
+ * memory, 0 where operands are read as they lie; zeros for no rows. */
+int pxs_linear_mxfp4_tile(int64_t rows, int cin, int cout, int * tile);
 
 /* residual (fp32) += the 4-bit linear, as pxs_linear_residual. */
 int pxs_linear_mxfp4_residual(const uint8_t * x, const uint8_t * x_scales, int64_t rows, int cin,

@@ -17,6 +17,7 @@
 #include "tiles.h"
 
 #include <algorithm>
+#include <iterator>
 #include <type_traits>
 
 namespace pxs {
@@ -190,6 +191,7 @@ struct MxArgs {
     const float * time_mod;    // [batch, 6 n]
     int gate_offset;
     int vec_out;               // 1: 4-channel vector accesses of all that the epilogue touches; 2: y in whole 16-byte pieces
+    int group_m;               // tile order (tile_of)
 };
 
 // The activations through one exponential and one reciprocal, as the 8-bit linears'.
@@ -358,6 +360,313 @@ __global__ void __launch_bounds__(kFewWaves * 64) linear_mxfp4_few_kernel(MxArgs
     mx_epilogue4<T, EPI>(a, mx_bias(a, col, a.vec_out && col + 3 < a.n), row, EPI == kMxGate ? a.coords[row * 4] : 0, col, sum);
 }
 
+// Row pitch in LDS of 32 rows of a wave's block, and 16 bytes against bank conflicts.
+template <typename T, int WN> constexpr int mx_pitch() { return WN * static_cast<int>(sizeof(T)) + 16; }
+
+// One wave's block of outputs: acc[i][j] holds 32 rows by 32 channels, lane (h, r) row r and
+// channels 8 g + 4 h + e.  Stores go through the wave's region of LDS (which no other wave uses
+// any more), 32 rows at a time, so that an instruction covers row segments of 64 bytes and more, and
+// past the caches: what reads y next runs on other XCDs (8,192 x 8192 -> 4096 155 -> 148 us, 1,370 x 1024 -> 4096
+// 12.6 -> 11.5).
+template <typename T, int TI, int TJ, int EPI>
+__device__ __forceinline__ void mx_tile_out(const MxArgs & a, const f32x16 (&acc)[TI][TJ], char * region, int64_t row0,
+                                            int col0, int h, int r, int lane) {
+    constexpr int WN = TJ * 32, kPitch = mx_pitch<T, WN>(), kElems = 16 / static_cast<int>(sizeof(T));
+    constexpr int kLanesPerRow = WN / kElems, kRowsPerPass = 64 / kLanesPerRow;
+    constexpr bool staged = EPI == kMxStore;
+    auto bias = [&](int j, int g) __attribute__((always_inline)) {
+        const int c = min(col0 + j * 32 + 8 * g + 4 * h, a.n - 1);
+        return mx_bias(a, c, a.vec_out && c + 3 < a.n);
+    };
+    MxBias held[TJ][4];  // every channel's, ahead of the first value
+#pragma unroll
+    for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) held[j][g] = bias(j, g);
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+        const int64_t row = row0 + i * 32 + r;
+        const int batch = EPI == kMxGate && row < a.m ? a.coords[row * 4] : 0;
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int cl = j * 32 + 8 * g + 4 * h, c = col0 + cl;
+                const float sum[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                const MxBias & b = held[j][g];
+                if constexpr (staged) {
+                    float v[4];
+                    mx_values4(a, b, sum, v);  // (past n: not stored)
+                    mx_put4(reinterpret_cast<T *>(region + r * kPitch + cl * static_cast<int>(sizeof(T))), v);
+                } else if (row < a.m && c < a.n) {
+                    mx_epilogue4<T, EPI>(a, b, row, batch, c, sum);
+                }
+            }
+        if constexpr (staged) {
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own writes
+            if (a.vec_out != 2) {  // an element a lane, in the order of their addresses
+#pragma unroll 2
+                for (int pass = 0; pass < 32 * WN / 64; ++pass) {
+                    const int rl = (pass * 64 + lane) / WN, cl = (pass * 64 + lane) % WN;
+                    const T v = *reinterpret_cast<const T *>(region + rl * kPitch + cl * static_cast<int>(sizeof(T)));
+                    const int64_t to = row0 + i * 32 + rl;
+                    if (to < a.m && col0 + cl < a.n) static_cast<T *>(a.y)[to * a.n + col0 + cl] = v;
+                }
+                continue;
+            }
+            const int lr = lane / kLanesPerRow, lc = lane % kLanesPerRow;
+#pragma unroll
+            for (int pass = 0; pass < 32 / kRowsPerPass; ++pass) {
+                const int rl = pass * kRowsPerPass + lr;
+                const uint4 v = *reinterpret_cast<const uint4 *>(region + rl * kPitch + lc * 16);
+                const int64_t to = row0 + i * 32 + rl;
+                const int c = col0 + lc * kElems;
+                if (to < a.m && c < a.n) store16_past(static_cast<T *>(a.y) + to * a.n + c, &v);
+            }
+        }
+    }
+}
+
+// As the 8-bit products (linear_i8.hip): BM rows of X and BN rows of W go 128 bytes of codes (8 blocks)
+// at a time from L2 to LDS by DMA, NSTAGE stages in flight, and a lane reads 16 contiguous bytes per
+// fragment, one block; the K order inside a stage is permuted alike for both operands, lane (h, r) of
+// step u taking block 4 h + u.  So the four steps' scales of a lane are one 32-bit word of the row's
+// scale bytes, and the instruction picks its byte.  Scale bytes come by DMA as well, 32 of a row (four
+// stages) at a time, ahead of the codes of the first of the four.
+// A 32 x 32 x 64 product takes the cycles of an 8-bit one of half its depth: bytes, stages and LDS
+// traffic are those of the 8-bit kernel and the rate is twice its.  Bound by no single unit: at 8,192 x 8192
+// -> 4096 (148 us, 3,720 TFLOP/s, 3.4 times the 16-bit library product's rate) the matrix cores are busy 46%
+// of the cycles, the return path of the DMA 53% and LDS about as much, in step with one another.  (64 x 64 a
+// wave and 16 waves 162 us, 128 x 128 and four waves 184.)
+//
+// KG groups of NW waves share a tile and take every KG-th stage each, in stages of their own (KG 4:
+// a group's stages are one of each four, and each loads its own scales); the groups' sums are added
+// through LDS in their order.  For calls of few tiles, whose time is the chain of stages.
+__device__ __align__(16) uint4 g_mx_zero[8];  // K pieces past the end
+
+constexpr int kMxKB = 128;           // bytes of codes of a row and stage
+constexpr int kMxScaleStages = 4;    // stages that a slot of scale bytes serves
+constexpr int kMxScaleRow = 32;      // its bytes of a row
+// (Those of stage s + nstage are loaded as stage s begins.)
+constexpr int mx_scale_slots(int nstage) { return (nstage + kMxScaleStages - 1) / kMxScaleStages + 1; }
+
+template <int U>
+__device__ __forceinline__ f32x16 mx_mfma(const uint4 & w, const uint4 & x, const f32x16 & acc, uint32_t ws, uint32_t xs) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(w), mx_operand(x), acc, kMxFp4, kMxFp4, U,
+                                                           static_cast<int>(ws), U, static_cast<int>(xs));
+}
+
+template <typename T, int BM, int BN, int NW, int WAVES_M, int NSTAGE, int KG, int EPI>
+__global__ void __launch_bounds__(NW * KG * 64) linear_mxfp4_kernel(MxArgs a) {
+    constexpr int KB = kMxKB, P = 8, RPI = 8;  // bytes, pieces per row of a stage; rows per DMA instruction
+    constexpr int WAVES_N = NW / WAVES_M, WM = BM / WAVES_M, WN = BN / WAVES_N, TI = WM / 32, TJ = WN / 32;
+    constexpr int kStage = (BM + BN) * KB;
+    constexpr int AI = BM / (RPI * NW), BI = BN / (RPI * NW), kPerStage = AI + BI;
+    static_assert(AI * RPI * NW == BM && BI * RPI * NW == BN, "tile rows must split over the waves");
+    // Scales: a DMA instruction takes 32 rows; slots of all rows behind the stages.
+    constexpr int kSlots = mx_scale_slots(KG > 1 ? 4 * NSTAGE : NSTAGE), kSlot = (BM + BN) * kMxScaleRow, kScaleInstr = (BM + BN) / 32;
+    constexpr int kScalePerWave = (kScaleInstr + NW - 1) / NW;
+    constexpr int kRing = NSTAGE * kStage + kSlots * kSlot;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int group = KG > 1 ? __builtin_amdgcn_readfirstlane(tid / (NW * 64)) : 0;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) - group * NW;  // in its group
+    char * ring = smem + group * kRing;
+    char * scale_ring = ring + NSTAGE * kStage;
+    const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+    const int h = lane >> 5, r = lane & 31;
+    const int tiles_n = (a.n + BN - 1) / BN, tiles_m = static_cast<int>((a.m + BM - 1) / BM);
+    int tm, tn;
+    tile_of(remap_xcd(blockIdx.x, gridDim.x), tiles_m, tiles_n, a.group_m, tm, tn);
+    const int64_t p0 = static_cast<int64_t>(tm) * BM;
+    const int n0 = tn * BN;
+    const int64_t row_bytes = static_cast<int64_t>(a.blocks) * 16;
+    const uint8_t * xs = a.x + p0 * row_bytes;
+    const uint8_t * wsb = a.w + static_cast<int64_t>(n0) * row_bytes;
+    const int all_stages = (a.blocks + P - 1) / P;
+    const int stages = (all_stages - group + KG - 1) / KG;       // of this group
+    const int steps = KG > 1 ? (all_stages + KG - 1) / KG : stages;  // of every group
+    const int lrow = lane / P, lslot = lane % P;
+    const int64_t last_x = a.m - 1 - p0;
+    const int last_w = a.n - 1 - n0;
+    uint32_t off[kPerStage];  // rows past the end are clamped; their outputs are not stored
+#pragma unroll
+    for (int j = 0; j < kPerStage; ++j) {
+        const bool is_x = j < AI;
+        const int row = (wave * (is_x ? AI : BI) + (is_x ? j : j - AI)) * RPI + lrow;
+        const int64_t at = is_x ? min(static_cast<int64_t>(row), last_x) : static_cast<int64_t>(min(row, last_w));
+        off[j] = static_cast<uint32_t>(at * row_bytes + (lslot ^ piece_swz<KB>(row)) * 16);
+    }
+    // This lane's row of each of the wave's scale instructions, two lanes a row.
+    const uint8_t * scale_row[kScalePerWave];
+#pragma unroll
+    for (int j = 0; j < kScalePerWave; ++j) {
+        const int row = (wave + j * NW) * 32 + (lane >> 1);
+        const bool is_x = row < BM;
+        const int64_t at = is_x ? p0 + min(static_cast<int64_t>(row), last_x) : n0 + static_cast<int64_t>(min(row - BM, last_w));
+        scale_row[j] = (is_x ? a.x_scales : a.w_scales) + at * a.pitch + (lane & 1) * 16;
+    }
+    // Stage s of this group is stage s * KG + group of the row; its scales lie in the 32 bytes of its four.
+    auto issue_scales = [&](int s) __attribute__((always_inline)) {
+        if (s % kMxScaleStages != 0 && KG == 1) return;
+        const int at = (s * KG + group) / kMxScaleStages;
+        const int slot = (KG == 1 ? s / kMxScaleStages : s) % kSlots;
+#pragma unroll
+        for (int j = 0; j < kScalePerWave; ++j) {
+            const int instr = wave + j * NW;
+            if (instr >= kScaleInstr) break;
+            const bool in = at * kMxScaleRow + (lane & 1) * 16 < a.pitch;
+            lds_dma16(in ? static_cast<const void *>(scale_row[j] + at * kMxScaleRow) : static_cast<const void *>(g_mx_zero),
+                      lds_offset(scale_ring + slot * kSlot + instr * 1024));
+        }
+    };
+    auto issue_one = [&](int s, int q, bool last) __attribute__((always_inline)) {
+        const bool is_x = q < AI;
+        const int row0 = (wave * (is_x ? AI : BI) + (is_x ? q : q - AI)) * RPI;
+        const uint32_t lds = lds_offset(ring + (s % NSTAGE) * kStage + ((is_x ? 0 : BM) + row0) * KB);
+        const int at = s * KG + group;
+        const uint8_t * src = (is_x ? xs : wsb) + static_cast<int64_t>(at) * KB;
+        if (last) {
+            const bool in = at * P + (lslot ^ piece_swz<KB>(row0 + lrow)) < a.blocks;  // (a last stage may hold pieces past the row)
+            lds_dma16(in ? static_cast<const void *>(src + off[q]) : static_cast<const void *>(g_mx_zero), lds);
+        } else {
+            lds_dma16_sbase(src, off[q], lds);
+        }
+    };
+    f32x16 acc[TI][TJ];
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) acc[i][j] = f32x16{};
+#pragma unroll
+    for (int s = 0; s < NSTAGE; ++s)
+        if (s < stages) {
+            issue_scales(s);
+#pragma unroll
+            for (int q = 0; q < kPerStage; ++q) issue_one(s, q, true);
+        }
+    // A step's fragments are read while the step before multiplies, those of a stage's first step beside the last
+    // products of the stage before: the wait for its DMA and the barrier lie ahead of those, when every wave holds
+    // the last fragments of its stage, whose slot is filled anew at once.
+    uint4 xf[2][TI], wf[2][TJ];
+    uint32_t xsc[TI], wsc[TJ], xnext[TI], wnext[TJ];
+    auto read_frags = [&](int s, int u, uint4 (&xo)[TI], uint4 (&wo)[TJ]) __attribute__((always_inline)) {
+        const char * sx = ring + (s % NSTAGE) * kStage;
+        const char * sw = sx + BM * KB;
+        const int piece = (P / 2) * h + u;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+            const int row = wm * WM + i * 32 + r;
+            xo[i] = *reinterpret_cast<const uint4 *>(sx + row * KB + ((piece ^ piece_swz<KB>(row)) << 4));
+        }
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) {
+            const int row = wn * WN + j * 32 + r;
+            wo[j] = *reinterpret_cast<const uint4 *>(sw + row * KB + ((piece ^ piece_swz<KB>(row)) << 4));
+        }
+    };
+    // The lanes' scale words.
+    auto read_scales = [&](int s, uint32_t (&xo)[TI], uint32_t (&wo)[TJ]) __attribute__((always_inline)) {
+        const int at = s * KG + group;
+        const char * sc = scale_ring + (KG == 1 ? s / kMxScaleStages : s) % kSlots * kSlot + at % kMxScaleStages * 8 + 4 * h;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) xo[i] = *reinterpret_cast<const uint32_t *>(sc + (wm * WM + i * 32 + r) * kMxScaleRow);
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) wo[j] = *reinterpret_cast<const uint32_t *>(sc + (BM + wn * WN + j * 32 + r) * kMxScaleRow);
+    };
+    // Stage s's, taken into use: those of blocks past the row's end, in its last stage, count as 1, whatever the
+    // bytes hold.
+    auto use_scales = [&](int s, bool ends) __attribute__((always_inline)) {
+        const int valid = a.blocks - ((s * KG + group) * P + 4 * h);
+        const uint32_t keep = !ends || valid >= 4 ? ~0u : valid <= 0 ? 0u : (1u << (8 * valid)) - 1u;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) xsc[i] = (xnext[i] & keep) | (~keep & 0x7F7F7F7Fu);
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) wsc[j] = (wnext[j] & keep) | (~keep & 0x7F7F7F7Fu);
+    };
+    // Stage s, whose first fragments and scales are read.  MORE: what is loaded beside its last products, 1 a stage
+    // that is not the group's last, 2 the last, 0 none; 3: there is no next stage.  (Bodies without branches
+    // between their products: the compiler moves the products past any to the stage's end, with all its
+    // fragments alive until there, and the large tiles spill.)
+    auto stage = [&](int s, auto what) __attribute__((always_inline)) {
+        constexpr int MORE = decltype(what)::value;
+        auto products = [&](auto which) __attribute__((always_inline)) {
+            constexpr int u = decltype(which)::value;
+            if constexpr (u + 1 < P / 2) read_frags(s, u + 1, xf[(u + 1) & 1], wf[(u + 1) & 1]);
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) {
+                    acc[i][j] = mx_mfma<u>(wf[u & 1][j], xf[u & 1][i], acc[i][j], wsc[j], xsc[i]);
+                    if constexpr (u == P / 2 - 1 && (MORE == 1 || MORE == 2)) {
+#pragma unroll
+                        for (int q = 0; q < kPerStage; ++q)
+                            if (q * (TI * TJ) / kPerStage == i * TJ + j) issue_one(s + NSTAGE, q, MORE == 2);
+                    }
+                }
+        };
+        if constexpr (MORE == 1 || MORE == 2) issue_scales(s + NSTAGE);
+        products(std::integral_constant<int, 0>{});
+        products(std::integral_constant<int, 1>{});
+        products(std::integral_constant<int, 2>{});
+        if constexpr (MORE != 3) {
+            // (Counts codes alone: with scales of a later stage in flight it waits for some of that stage too.)
+            wait_stages<NSTAGE - 2, kPerStage>(MORE > 0 ? NSTAGE : stages - 2 - s);
+            barrier_no_fence();
+            read_scales(s + 1, xnext, wnext);
+            read_frags(s + 1, 0, xf[0], wf[0]);
+        }
+        products(std::integral_constant<int, 3>{});
+        if constexpr (MORE != 3) use_scales(s + 1, MORE == 0);
+    };
+    if (KG == 1 || stages > 0) {
+        wait_stages<NSTAGE - 1, kPerStage>(stages - 1);
+        barrier_no_fence();
+        read_scales(0, xnext, wnext);
+        read_frags(0, 0, xf[0], wf[0]);
+        use_scales(0, true);
+        int s = 0;
+        for (; s + NSTAGE + 1 < stages; ++s) stage(s, std::integral_constant<int, 1>{});
+        if (s + NSTAGE + 1 == stages) stage(s++, std::integral_constant<int, 2>{});
+        for (; s + 1 < stages; ++s) stage(s, std::integral_constant<int, 0>{});
+        stage(s, std::integral_constant<int, 3>{});
+    }
+    // (Or the compiler moves the last products into the epilogue's branches, and spills.)
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) asm volatile("" : "+v"(acc[i][j]));
+    if constexpr (KG > 1)
+        for (int s = stages; s < steps; ++s) barrier_no_fence();  // (of groups with a stage more)
+    barrier_no_fence();  // every wave is done with the stages
+    constexpr int kOut = NW * 32 * mx_pitch<T, WN>();
+    if constexpr (KG > 1) {
+        // [group - 1][wave][register][lane], behind the first group's store regions
+        float * sums = reinterpret_cast<float *>(smem + kOut) + wave * TI * TJ * 16 * 64 + lane;
+        constexpr int kGroup = NW * TI * TJ * 16 * 64;
+        if (group > 0) {
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+#pragma unroll
+                for (int j = 0; j < TJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        sums[(group - 1) * kGroup + ((i * TJ + j) * 16 + e) * 64] = acc[i][j][e];
+        }
+        barrier_no_fence();
+        if (group > 0) return;
+#pragma unroll
+        for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+#pragma unroll
+                for (int j = 0; j < TJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[i][j][e] += sums[g * kGroup + ((i * TJ + j) * 16 + e) * 64];
+    }
+    mx_tile_out<T, TI, TJ, EPI>(a, acc, smem + wave * 32 * mx_pitch<T, WN>(), p0 + wm * WM, n0 + wn * WN, h, r, lane);
+}
+
 bool aligned_to(const void * p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 int check_mx_grid(int64_t blocks, int threads) {
@@ -375,20 +684,104 @@ int launch_mx_few(const MxArgs & a, hipStream_t s) {
     return check_launch("4-bit linear of few rows");
 }
 
+template <typename T, int BM, int BN, int NW, int WAVES_M, int NSTAGE, int KG, int EPI>
+int launch_mx_tiles(const MxArgs & a, hipStream_t s) {
+    constexpr int WN = BN / (NW / WAVES_M), kOut = NW * 32 * mx_pitch<T, WN>();
+    constexpr int kStages = KG * (NSTAGE * (BM + BN) * kMxKB + mx_scale_slots(KG > 1 ? 4 * NSTAGE : NSTAGE) * (BM + BN) * kMxScaleRow);
+    constexpr int kEnd = kOut + (KG - 1) * BM * BN * 4, smem = kStages > kEnd ? kStages : kEnd;
+    static_assert(smem <= 160 * 1024, "LDS");
+    const int64_t blocks = ((a.m + BM - 1) / BM) * ((a.n + BN - 1) / BN);
+    if (int rc = check_mx_grid(blocks, NW * KG * 64)) return rc;
+    auto kernel = &linear_mxfp4_kernel<T, BM, BN, NW, WAVES_M, NSTAGE, KG, EPI>;
+    if constexpr (smem > 64 * 1024) {
+        static std::atomic<uint64_t> done{0};
+        if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), smem, done, "hipFuncSetAttribute(linear_mxfp4)")) return rc;
+    }
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(NW * KG * 64), smem, s, a);
+    return check_launch("4-bit linear");
+}
+
+// Tile shapes, their time alone on a CU and their share of a full CU's time, in us for
+// 1024 bytes of codes a row more and without any: fitted to each shape's times at 64 sizes (66 to 42,017
+// rows, 256 to 8192 deep), where the shape picked takes 0.9% more than the best on average:
+//   256 x 256, 8 waves of 128 x 64, one workgroup a CU:  8,192 x 8192 -> 4096 148 us (3,720 TFLOP/s), next best 172
+//   128 x 128, 8 waves, two stages and two workgroups:   1,370 x 1024 -> 4096 11.6 against 15.4
+//   the same, three stages and one workgroup:            2,000 x 4096 -> 2048 18.0 against 19.6
+//   64 x 64, 4 waves, two:                               150 x 4096 -> 4096 10.8 against 15.6
+//   32 x 64, four groups of two waves over K, one:       87 x 8192 -> 1024 11.4 against 14.2
+struct MxShape {
+    int bm, bn, stages;
+    double alone0, alone1, each0, each1;
+};
+constexpr MxShape kMxShapes[] = {
+    {256, 256, 2, 11.4, 10.3, 8.5, 16.5}, {128, 128, 2, 6.1, 4.9, 3.3, 4.5}, {128, 128, 3, 6.5, 4.2, 4.3, 5.2},
+    {64, 64, 4, 6.0, 2.2, 1.9, 2.0},      {32, 64, 2, 6.1, 1.5, 3.0, 1.9},
+};
+
+int mx_shape(int64_t m, int n, int blocks) {
+    int best = 0;
+    double least = 0.0;
+    for (int i = 0; i < static_cast<int>(std::size(kMxShapes)); ++i) {
+        const MxShape & c = kMxShapes[i];
+        const double deep = blocks / 64.0, alone = c.alone0 + c.alone1 * deep, each = c.each0 + c.each1 * deep;
+        const int64_t tiles = ((m + c.bm - 1) / c.bm) * ((n + c.bn - 1) / c.bn);
+        const double time = tiles <= 256 ? alone + std::max(0.0, each - alone) * (tiles / 256.0)
+                                         : std::max(alone, ((tiles + 255) / 256) * each);
+        if (i == 0 || time < least) {
+            least = time;
+            best = i;
+        }
+    }
+    return best;
+}
+
+// Up to kMxFewRows rows: 16 output channels a workgroup, and as few of its 16-row blocks as
+// keep the workgroups near one a CU.
+constexpr int64_t kMxFewRows = 64;
+
+// What a call runs on: its tile of rows by output channels, and its stages of K in LDS by DMA; 0
+// straight from memory (linear_mxfp4_few_kernel).
+struct MxPlan {
+    int bm, bn, stages;
+};
+MxPlan mx_plan(int64_t m, int n, int blocks) {
+    if (m <= kMxFewRows) {
+        const int64_t groups = (n + 15) / 16 * ((m + 15) / 16);
+        if (groups <= 256 || m <= 16) return {16, 16, 0};
+        if (groups <= 512 || m <= 32) return {32, 16, 0};
+        return {64, 16, 0};
+    }
+    const MxShape & c = kMxShapes[mx_shape(m, n, blocks)];
+    return {c.bm, c.bn, c.stages};
+}
+
 template <typename T, int EPI>
-int launch_mx(const MxArgs & a, hipStream_t s) {
-    if (a.m <= 16) return launch_mx_few<T, 1, EPI>(a, s);
-    return launch_mx_few<T, 4, EPI>(a, s);
+int launch_mx(MxArgs a, hipStream_t s) {
+    a.group_m = 8;
+    const MxPlan p = mx_plan(a.m, a.n, a.blocks);
+    if (p.stages == 0) {
+        if (p.bm == 16) return launch_mx_few<T, 1, EPI>(a, s);
+        return p.bm == 32 ? launch_mx_few<T, 2, EPI>(a, s) : launch_mx_few<T, 4, EPI>(a, s);
+    }
+    switch (p.bm) {
+    case 256: return launch_mx_tiles<T, 256, 256, 8, 2, 2, 1, EPI>(a, s);
+    case 128:
+        if (p.stages == 3) return launch_mx_tiles<T, 128, 128, 8, 2, 3, 1, EPI>(a, s);
+        return launch_mx_tiles<T, 128, 128, 8, 2, 2, 1, EPI>(a, s);
+    case 64: return launch_mx_tiles<T, 64, 64, 4, 2, 4, 1, EPI>(a, s);
+    default: return launch_mx_tiles<T, 32, 64, 2, 1, 2, 4, EPI>(a, s);
+    }
 }
 
 constexpr int kMxMaxColumns = 1 << 30;  // columns are counted in 32 bits, a tile past their end
+constexpr int kMxMaxInputs = 1 << 24;   // a tile's 256 rows of codes are reached with 32-bit offsets
 
 // The checks that the 4-bit linears share; *run is false where there is nothing to do.
 int check_mx(const char * what, const uint8_t * x, const uint8_t * x_scales, int64_t rows, int cin, const uint8_t * weight,
              const uint8_t * w_scales, int cout, const void * out, bool * run) {
     *run = false;
     if (rows < 0 || cin <= 0 || cout <= 0) return fail_call(what, "bad shape");
-    if (cin > kMxMaxColumns) return fail_call(what, "more than 2^30 inputs");
+    if (cin > kMxMaxInputs) return fail_call(what, "more than 2^24 inputs");
     if (cout > kMxMaxColumns) return fail_call(what, "more than 2^30 outputs");
     if (rows == 0) return PXS_OK;
     if (!x || !x_scales || !weight || !w_scales || !out) return fail_call(what, "null pointer");
@@ -475,6 +868,17 @@ int pxs_linear_mxfp4(const uint8_t * x, const uint8_t * x_scales, int64_t rows, 
     a.act = act; a.y = y;
     return y_dtype == PXS_F32 ? launch_mx<float, kMxStore>(a, as_stream(stream))
                               : launch_mx<uint16_t, kMxStore>(a, as_stream(stream));
+}
+
+int pxs_linear_mxfp4_tile(int64_t rows, int cin, int cout, int * tile) {
+    PXS_CHECK(rows >= 0 && cin > 0 && cout > 0 && cin <= kMxMaxInputs && cout <= kMxMaxColumns, PXS_ERR_ARG,
+              "pxs_linear_mxfp4_tile: bad shape");
+    PXS_CHECK(tile, PXS_ERR_ARG, "pxs_linear_mxfp4_tile: null pointer");
+    const MxPlan p = rows > 0 ? mx_plan(rows, cout, mx_blocks(cin)) : MxPlan{};
+    tile[0] = p.bm;
+    tile[1] = p.bn;
+    tile[2] = p.stages;
+    return PXS_OK;
 }
 
 int pxs_linear_mxfp4_residual(const uint8_t * x, const uint8_t * x_scales, int64_t rows, int cin, const uint8_t * weight,

@@ -63,6 +63,7 @@ _SIGS = {
     "pxs_quantize_mxfp4": (_i32, [_i32, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
     "pxs_dequantize_mxfp4": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _i64, _vp]),
     "pxs_linear_mxfp4": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
+    "pxs_linear_mxfp4_tile": (_i32, [_i64, _i32, _i32, C.POINTER(C.c_int)]),
     "pxs_linear_mxfp4_residual": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp]),
     "pxs_linear_mxfp4_gate_residual": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i32,
                                               _vp, _vp]),

@@ -74,7 +74,7 @@ def test_mxfp4_conversion_refusals(lib, change, text):
 
 LINEAR = dict(x=P, xs=P, rows=4, cin=64, w=P, ws=P, bias=None, cout=32, act=0, dtype=0, y=P, stream=None)
 SHARED = [
-    (dict(rows=-1), "bad shape"), (dict(cin=0), "bad shape"), (dict(cout=0), "bad shape"), (dict(cin=2 ** 30 + 1), "2^30 inputs"),
+    (dict(rows=-1), "bad shape"), (dict(cin=0), "bad shape"), (dict(cout=0), "bad shape"), (dict(cin=2 ** 24 + 1), "2^24 inputs"),
     (dict(cout=2 ** 30 + 1), "2^30 outputs"), (dict(x=None), "null pointer"), (dict(xs=None), "null pointer"),
     (dict(w=None), "null pointer"), (dict(ws=None), "null pointer"), (dict(x=ODD), "16-byte"), (dict(xs=ODD), "16-byte"),
     (dict(w=ODD), "16-byte"), (dict(ws=ODD), "16-byte"), (dict(rows=2 ** 40, cin=1, cout=2 ** 20), "grid too large")]
@@ -100,6 +100,14 @@ def test_linear_mxfp4_gate_refusals(lib, change, text):
     gate = dict(x=P, xs=P, rows=4, cin=64, w=P, ws=P, bias=None, cout=32, coords=P, bmod=P, tmod=P, offset=0, residual=P,
                 stream=None)
     refused(lib, lib.pxs_linear_mxfp4_gate_residual(*{**gate, **change}.values()), text)
+
+
+def test_linear_mxfp4_tile(lib):
+    tile = (C.c_int * 3)(7, 7, 7)
+    assert lib.pxs_linear_mxfp4_tile(0, 64, 64, tile) == pxs.PXS_OK and list(tile) == [0, 0, 0]
+    for args in ((-1, 64, 64, tile), (1, 0, 64, tile), (1, 64, 0, tile), (1, 2 ** 24 + 1, 64, tile), (1, 64, 2 ** 30 + 1, tile)):
+        refused(lib, lib.pxs_linear_mxfp4_tile(*args), "bad shape")
+    refused(lib, lib.pxs_linear_mxfp4_tile(1, 64, 64, None), "null pointer")
 
 
 def test_mxfp4_of_nothing(lib):
