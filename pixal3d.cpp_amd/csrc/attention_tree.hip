@@ -9,7 +9,7 @@
 // as the scored attention's (attention_scores.hip).  The tokens' keys and values are rows of
 // their own, so that the cache is written only with those that are accepted.
 //
-// A row is a (query, head) of a key/value head's group, 32 rows a tile.  A tile's work is cut
+// A row is a (query, head) of a key/value head's group, 32 or 128 rows a tile.  A tile's work is cut
 // into chunks of the cached keys, an item each, the tree's keys with the first.  How long the
 // caches are only the device knows: every workgroup takes the chunk's size from the lengths
 // (segment_plan), so that a call has about `target` items, whatever the lengths, and a captured
@@ -20,11 +20,10 @@
 // taken from the last to the first: no mask is stored, whatever the tree's size.  A parent that
 // is no earlier token of the tree ends the walk.
 
-#include "attn_common.h"
+#include "attn_scores.h"
 
 #include <algorithm>
 #include <cmath>
-#include <limits>
 #include <type_traits>
 
 namespace pxs {
@@ -47,7 +46,7 @@ struct TreeArgs {
     int64_t total_q, cache_rows;
     const int64_t * table;     // null: at most 64 segments; or tree_table_kernel's
     int heads, kv_heads, group, d;
-    float scale_log2, cap_log2, over_cap;
+    float scale_log2, cap_log2, over_cap, exp_mul;
     const float * slopes;      // [heads] or null
     void * o;
     int64_t ldo;
@@ -55,11 +54,11 @@ struct TreeArgs {
     int64_t items;             // launched (bound)
     int64_t slots;             // items with partial results (bound)
     double per_target;         // 1 / items that the chunks add at most
-    float * part;              // [slots * kv_heads * kTreeRows][d] unnormalised outputs
+    int row_shift;             // log2 of a tile's rows
+    float * part;              // [slots * kv_heads << row_shift][d] unnormalised outputs
     float2 * part_ml;          // [..] maxima (log2 units) and sums
 };
 
-constexpr int kTreeRows = 32;
 constexpr int kTreeUnit = 128;  // keys that a chunk is a multiple of
 
 // A segment's queries and cached rows, kept within the call's whatever the bounds hold.
@@ -75,7 +74,7 @@ __device__ __forceinline__ Tree load_tree(const TreeArgs & a, int s) {
 }
 
 __device__ __forceinline__ int row_tiles_of(const TreeArgs & a, const Tree & g) {
-    return static_cast<int>((static_cast<int64_t>(g.nq) * a.group + kTreeRows - 1) / kTreeRows);
+    return static_cast<int>((static_cast<int64_t>(g.nq) * a.group + (1 << a.row_shift) - 1) >> a.row_shift);
 }
 // Keys of a chunk, from the sum of row tiles times cached keys: `work` of them over the
 // target's items, and one unit more, so that the chunks past a tile's first are at most the target.
@@ -84,6 +83,11 @@ __device__ __forceinline__ int chunk_of(const TreeArgs & a, double work) {
     return static_cast<int>(min(units * kTreeUnit, static_cast<double>(a.cache_rows + kTreeUnit)));
 }
 __device__ __forceinline__ int chunks_of(const Tree & g, int chunk) { return g.nk > chunk ? (g.nk - 1) / chunk + 1 : 1; }
+// First key of chunk i of a segment's: as even as whole units make them.
+__device__ __forceinline__ int chunk_start(const Tree & g, int i, int chunks) {
+    const int64_t units = (static_cast<int64_t>(g.nk) + kTreeUnit - 1) / kTreeUnit;
+    return static_cast<int>(min(units * i / chunks * kTreeUnit, static_cast<int64_t>(g.nk)));
+}
 
 // An item: a row tile and the chunk's keys.
 struct Item {
@@ -139,9 +143,9 @@ __device__ __forceinline__ bool item_of(const TreeArgs & a, const Tree & g, int 
     w.rows = g.nq * a.group;
     w.chunks = chunks_of(g, chunk);
     w.chunk = i / tiles;
-    w.row0 = i % tiles * kTreeRows;
-    w.key0 = static_cast<int>(min(static_cast<int64_t>(w.chunk) * chunk, static_cast<int64_t>(g.nk)));
-    w.key1 = static_cast<int>(min(static_cast<int64_t>(w.key0) + chunk, static_cast<int64_t>(g.nk)));
+    w.row0 = i % tiles << a.row_shift;
+    w.key0 = chunk_start(g, w.chunk, w.chunks);
+    w.key1 = chunk_start(g, w.chunk + 1, w.chunks);
     w.slot = slot0 + i;
     return w.chunk < w.chunks && (w.chunks == 1 || (w.slot >= 0 && w.slot < a.slots));
 }
@@ -178,6 +182,11 @@ __device__ __forceinline__ bool locate_query(const TreeArgs & a, int qi, int lan
     return item_of(a, tree_of(p.g, seg), 0, p.chunk, __builtin_amdgcn_readlane(p.slots_end - p.slots, seg), w);
 }
 
+// The item's rows of partial results.
+__device__ __forceinline__ int64_t item_rows(const TreeArgs & a, const Item & w) {
+    return (static_cast<int64_t>(w.slot) * a.kv_heads + w.kv) << a.row_shift;
+}
+
 // The token above token c of the tree whose first row is q0; -1 at the top.
 __device__ __forceinline__ int above(const TreeArgs & a, int q0, int c) {
     const int p = a.parents[q0 + c];
@@ -204,8 +213,6 @@ __device__ __forceinline__ void load_dims4(const T * row, int c, int d, bool vec
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = c + i < d ? load_f32(row + c + i) : 0.0f;
 }
-
-__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
 
 // A row of an item again, a key after the other, tokens that it does not see left out altogether: for
 // trees where a token's value is infinite or NaN, which times a weight of zero is NaN.  One wave;
@@ -355,14 +362,14 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 const float x = key < limit && dt * 32 + r < a.d ? load_f32(v + key * ldv + dt * 32 + r) : 0.0f;
-                odd |= tree && !finite(x);
+                odd |= tree && !is_finite_bits(x);
                 oacc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[e], oacc[dt], 0, 0, 0);
             }
         }
     }
-    const int64_t slot0 = (static_cast<int64_t>(w.slot) * a.kv_heads + w.kv) * kTreeRows;
+    const int64_t slot0 = item_rows(a, w);
     if (__syncthreads_or(odd)) {
-        for (int i = wave; i < kTreeRows; i += 4)
+        for (int i = wave; i < 32; i += 4)
             if (w.row0 + i < w.rows) tree_row_alone<T, (DP + 63) / 64>(a, w, w.row0 + i, lane, slot0 + i);
         return;
     }
@@ -399,6 +406,378 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
     }
 }
 
+// ---- bf16, head sizes of whole 16-byte pieces up to 128 -----------------------------------------------------
+// The tiles, products and weights of the scored attention's kernels (attn_scores.h).  An item's tiles are walked as
+// the tree's from the last to the first, each with the keys that a row sees as bits, then the cache's.
+
+// The tokens first .. first + keys - 1 (up to 64) that the lane's row sees, `at` its next from itself up.
+__device__ __forceinline__ uint64_t tree_bits(const TreeArgs & a, int q0, int & at, int first, int keys) {
+    uint64_t bits = 0;
+    while (at >= first + keys) at = above(a, q0, at);
+    for (; at >= first; at = above(a, q0, at)) bits |= uint64_t(1) << (at - first);
+    return bits;
+}
+// The first `seen` keys of a tile, as bits.
+__device__ __forceinline__ uint64_t first_bits(int seen) { return seen >= 64 ? ~uint64_t(0) : (uint64_t(1) << seen) - 1; }
+
+// One row's place: its query, head, constants and first fragments.
+template <int DH, int MODE> struct TreeRow {
+    RowScore rs;
+    bf16x8 qf[Fast<DH>::NST];
+    int row, qi, head, pos;
+    bool live;
+};
+template <int DH, int MODE>
+__device__ __forceinline__ void load_row(const TreeArgs & a, const Item & w, int row, int h, TreeRow<DH, MODE> & o) {
+    o.live = row < w.rows;
+    o.row = o.live ? row : w.rows - 1;
+    o.qi = o.row / a.group;
+    o.head = w.kv * a.group + o.row % a.group;
+    o.rs = row_score<MODE>(a, o.head);
+    o.pos = MODE & kBias ? a.positions[w.g.q0 + o.qi] : 0;
+    load_q_row<DH>(static_cast<const uint16_t *>(a.q) + (w.g.q0 + o.qi) * a.ldq + static_cast<int64_t>(o.head) * a.d, a.d, o.live, h,
+                   o.qf);
+}
+
+template <int DH> struct TreeSources {
+    TileSource<DH> tree, cache;
+};
+template <int DH>
+__device__ __forceinline__ TreeSources<DH> tree_sources(const TreeArgs & a, const Item & w) {
+    const int64_t col = static_cast<int64_t>(w.kv) * a.d;
+    const int64_t q0 = w.g.q0;
+    return {tile_source_of<DH>(static_cast<const uint16_t *>(a.k) + q0 * a.ldk + col,
+                               static_cast<const uint16_t *>(a.v) + q0 * a.ldv + col, a.ldk, a.ldv, w.g.nq),
+            tile_source_of<DH>(static_cast<const uint16_t *>(a.kc) + w.g.k0 * a.ldkc + col,
+                               static_cast<const uint16_t *>(a.vc) + w.g.k0 * a.ldvc + col, a.ldkc, a.ldvc, w.key1)};
+}
+
+// The exact step of a tile of the tree (its first token) or of the cache (its first key), whose keys the row
+// sees as bits.
+template <int DH, int MODE>
+__device__ __forceinline__ void tree_exact(const TreeArgs & a, const Item & w, const TreeRow<DH, MODE> & o, bool tree, int first,
+                                           uint64_t bits, int h, typename Fast<DH>::Scores & s, typename Fast<DH>::Weights & p,
+                                           typename Fast<DH>::Out & oacc, RowState & st) {
+    const uint32_t lo = static_cast<uint32_t>(bits) >> (4 * h), hi = static_cast<uint32_t>(bits >> 32) >> (4 * h);
+    auto seen = [&](int kt, int e) __attribute__((always_inline)) {  // (key_of is a constant)
+        return ((kt == 0 ? lo : hi) >> (key_of(0, e)) & 1u) != 0;
+    };
+    const float behind = static_cast<float>(o.pos - first - 4 * h);
+    if ((MODE & kBias) && tree) {
+        float at[Fast<DH>::KT][16];
+#pragma unroll
+        for (int kt = 0; kt < Fast<DH>::KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                at[kt][e] = static_cast<float>(o.pos - a.positions[w.g.q0 + min(first + key_of(kt, e) + 4 * h, w.g.nq - 1)]);
+        tile_exact_of<DH, MODE>(o.rs, a.cap_log2, s, p, oacc, st,
+                                [&](int kt, int e) __attribute__((always_inline)) { return at[kt][e]; }, seen);
+    } else {
+        tile_exact_of<DH, MODE>(o.rs, a.cap_log2, s, p, oacc, st,
+                                [&](int kt, int e) __attribute__((always_inline)) { return behind - static_cast<float>(key_of(kt, e)); },
+                                seen);
+    }
+}
+
+// Up to 32 rows a tile: a workgroup's two waves take every second key tile of an item each, through rings of
+// their own in LDS, with no barrier before the end, where their results are joined.
+constexpr int kTreeWaves = 2, kTreeStages = 2;  // 64 KB of LDS: two workgroups a CU
+template <int DH> constexpr int kTreeWaveBytes = kTreeStages * 2 * Fast<DH>::kTileBytes;
+template <int DH> constexpr int kTreeFewBytes = kTreeWaves * kTreeWaveBytes<DH> + kTreeWaves * 32 * static_cast<int>(sizeof(float2));
+
+template <int DH, int MODE, bool WHOLE>
+__global__ void __launch_bounds__(kTreeWaves * 64) tree_attn_few_kernel(TreeArgs a) {
+    using F = Fast<DH>;
+    constexpr int kInstr = 2 * F::kUnits;
+    extern __shared__ __align__(16) char tree_lds[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, r = lane & 31;
+    Item w;
+    w.kv = static_cast<int>(blockIdx.x % a.kv_heads);
+    if (!locate_item(a, static_cast<int>(blockIdx.x / a.kv_heads), lane, w)) return;
+    TreeSources<DH> src = tree_sources<DH>(a, w);
+    uint32_t off_tree[kInstr], off_cache[kInstr];
+    tile_offsets<DH>(src.tree, a.d, 0, lane, off_tree);
+    tile_offsets<DH>(src.cache, a.d, 0, lane, off_cache);
+    char * ring = tree_lds + wave * kTreeWaveBytes<DH>;
+    const uint32_t lds0 = lds_offset(ring);
+    const int tree_tiles = w.chunk == 0 ? (w.g.nq + F::kKeys - 1) / F::kKeys : 0;
+    const int cache0 = w.key0 / F::kKeys, all = tree_tiles + (w.key1 + F::kKeys - 1) / F::kKeys - cache0;
+    const int n = all > wave ? (all - wave + kTreeWaves - 1) / kTreeWaves : 0;
+    auto slot = [](int i) { return i % kTreeStages * 2 * F::kTileBytes; };
+    auto issue = [&](int i) __attribute__((always_inline)) {
+        const int t = wave + kTreeWaves * i;
+        if (t < tree_tiles) tile_issue<DH, WHOLE>(src.tree, tree_tiles - 1 - t, 0, off_tree, lds0 + slot(i), lane);
+        else tile_issue<DH, WHOLE>(src.cache, cache0 + t - tree_tiles, 0, off_cache, lds0 + slot(i), lane);
+    };
+    if (n > 0) issue(0);
+    TreeRow<DH, MODE> o;
+    load_row<DH, MODE>(a, w, w.row0 + r, h, o);
+    typename F::Out oacc;
+#pragma unroll
+    for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
+    RowState st{-INFINITY, 0.0f};
+    bool odd = false;
+    int walk = o.qi;
+#pragma unroll
+    for (int i = 1; i < kTreeStages; ++i)
+        if (i < n) issue(i);
+    for (int i = 0; i < n; ++i) {
+        const int t = wave + kTreeWaves * i;
+        const bool tree = t < tree_tiles;
+        const int first = (tree ? tree_tiles - 1 - t : cache0 + t - tree_tiles) * F::kKeys;
+        const uint64_t bits = tree ? tree_bits(a, w.g.q0, walk, first, F::kKeys) : first_bits(w.key1 - first);
+        wait_stages<kTreeStages - 1, kInstr>(n - 1 - i);
+        asm volatile("" ::: "memory");
+        const char * kl = ring + slot(i);
+        const char * vl = kl + F::kTileBytes;
+        if (tree) odd |= tile_odd<DH>(vl, lane, 64);
+        typename F::Scores s;
+        typename F::Weights p;
+        tile_qk<DH>(kl, o.qf, s, h, r);
+        tree_exact<DH, MODE>(a, w, o, tree, first, bits, h, s, p, oacc, st);
+        tile_pv<DH>(vl, p, oacc, lane);
+        wave_reads_done();
+        if (i + kTreeStages < n) issue(i + kTreeStages);
+    }
+    const int64_t part = item_rows(a, w);
+    if (__syncthreads_or(odd)) {
+        for (int j = wave; j < 32; j += kTreeWaves)
+            if (w.row0 + j < w.rows) tree_row_alone<uint16_t, DH / 64>(a, w, w.row0 + j, lane, part + j);
+        return;
+    }
+    // The waves' results: outputs in their own rings, bases and sums behind the rings.
+    float * mine = reinterpret_cast<float *>(ring);
+    float2 * ml = reinterpret_cast<float2 *>(tree_lds + kTreeWaves * kTreeWaveBytes<DH>);
+    const float sum = lane_pair_sum(st.sum);
+    if (h == 0) ml[wave * 32 + r] = make_float2(st.base, sum);
+#pragma unroll
+    for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float4 *>(mine + r * DH + dt * 32 + 8 * g + 4 * h) =
+                make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
+    __syncthreads();
+    const int jc = tid & 7;  // 8 threads a row
+#pragma unroll
+    for (int jr = tid >> 3; jr < 32; jr += kTreeWaves * 8) {
+        if (w.row0 + jr >= w.rows) return;
+        float base = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kTreeWaves; ++i) base = fmaxf(base, ml[i * 32 + jr].x);
+        const float ref = base == -INFINITY ? 0.0f : base;
+        float total = 0.0f, f[kTreeWaves];
+#pragma unroll
+        for (int i = 0; i < kTreeWaves; ++i) {
+            const float2 v = ml[i * 32 + jr];
+            f[i] = __builtin_amdgcn_exp2f(v.x - ref);
+            total += v.y * f[i];
+        }
+        const int token = (w.row0 + jr) / a.group;
+        const int to_head = w.kv * a.group + (w.row0 + jr) % a.group;
+        uint16_t * to = static_cast<uint16_t *>(a.o) + (w.g.q0 + token) * a.ldo + static_cast<int64_t>(to_head) * a.d;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        if (w.chunks > 1 && jc == 0) a.part_ml[part + jr] = make_float2(base, total);
+#pragma unroll
+        for (int c = jc * 4; c < DH; c += 32) {
+            if (!WHOLE && c >= a.d) break;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < kTreeWaves; ++i) {
+                const float4 x = *reinterpret_cast<const float4 *>(
+                    reinterpret_cast<const float *>(tree_lds + i * kTreeWaveBytes<DH>) + jr * DH + c);
+                v[0] += x.x * f[i]; v[1] += x.y * f[i]; v[2] += x.z * f[i]; v[3] += x.w * f[i];
+            }
+            if (w.chunks > 1)
+                *reinterpret_cast<float4 *>(a.part + (part + jr) * a.d + c) = make_float4(v[0], v[1], v[2], v[3]);
+            else
+                *reinterpret_cast<uint2 *>(to + c) =
+                    make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+        }
+    }
+}
+
+// More rows: four waves of 32 rows share the key tiles, a ring of four slots of K and V, as the scored attention's
+// kernel of many rows does.  The tree's tiles and the cache's last, which may end inside, are exact steps
+// (maximum, weights, product), and one whole tile after them, so that every row has a base that one of its own
+// scores set.  From there on a step issues the products that do not depend on its weights, O += V P of the tile before
+// and S of the next, and takes its weights while they run, without a maximum: a row's are redone with one
+// where their sum passes 2^40, and an item whose outputs pass 2^118 is walked again with exact steps alone.
+// Waves past the segment's rows only help to load.
+template <int DH, int MODE, bool WHOLE>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) tree_attn_rows_kernel(TreeArgs a) {
+    using F = Fast<DH>;
+    constexpr int kMine = 2 * F::kUnits / 4;  // DMA instructions of a wave and tile
+    __shared__ __align__(16) char lds[kSlots * 2 * F::kTileBytes];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, r = lane & 31;
+    Item w;
+    w.kv = static_cast<int>(blockIdx.x % a.kv_heads);
+    if (!locate_item(a, static_cast<int>(blockIdx.x / a.kv_heads), lane, w)) return;
+    const int tree_tiles = w.chunk == 0 ? (w.g.nq + F::kKeys - 1) / F::kKeys : 0;
+    const int cache0 = w.key0 / F::kKeys, cache1 = (w.key1 + F::kKeys - 1) / F::kKeys;
+    // Steps 0 .. n - 1: the tree's tiles from the last, then the cache's from the last.
+    const int n = __builtin_amdgcn_readfirstlane(tree_tiles + cache1 - cache0);
+    const int exact = __builtin_amdgcn_readfirstlane(min(n, tree_tiles + (w.key1 % F::kKeys != 0 ? 1 : 0) + 1));
+    const int wave_row0 = w.row0 + wave * 32;
+    const bool wave_live = wave_row0 < w.rows;
+
+    TreeSources<DH> src = tree_sources<DH>(a, w);
+    uint32_t off_tree[kMine], off_cache[kMine];
+    tile_offsets<DH>(src.tree, a.d, wave * kMine, lane, off_tree);
+    tile_offsets<DH>(src.cache, a.d, wave * kMine, lane, off_cache);
+    const uint32_t lds0 = lds_offset(&lds[0]);
+    auto slot = [](int i) { return (i % kSlots) * 2 * F::kTileBytes; };
+    auto cache_tile = [&](int i) { return cache1 - 1 - (i - tree_tiles); };
+    auto issue = [&](int i) __attribute__((always_inline)) {
+        if (i < tree_tiles) tile_issue<DH, WHOLE>(src.tree, tree_tiles - 1 - i, wave * kMine, off_tree, lds0 + slot(i), lane);
+        else tile_issue<DH, WHOLE>(src.cache, cache_tile(i), wave * kMine, off_cache, lds0 + slot(i), lane);
+    };
+    auto issue_cache = [&](int i) __attribute__((always_inline)) {
+        tile_issue<DH, WHOLE>(src.cache, cache_tile(i), wave * kMine, off_cache, lds0 + slot(i), lane);
+    };
+    auto k_of = [&](int i) { return lds + slot(i); };
+    auto v_of = [&](int i) { return lds + slot(i) + F::kTileBytes; };
+    issue(0);  // (an item has a tile: its segment's tokens, or keys)
+    if (n > 1) issue(1);
+    // (The steps' order of waits, barriers and loads is the same for all waves.)
+    auto await = [&](int i, bool more) __attribute__((always_inline)) {
+        if (more && i + 1 < n) wait_vmcnt(kMine);
+        else wait_vmcnt(0);
+        barrier_no_fence();
+    };
+    TreeRow<DH, MODE> o;
+    load_row<DH, MODE>(a, w, wave_row0 + r, h, o);
+    const float cap_log2 = a.cap_log2;
+    auto behind = [&](int i) { return static_cast<float>(o.pos - 4 * h - cache_tile(i) * F::kKeys); };
+    typename F::Out oacc;
+#pragma unroll
+    for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
+    RowState st{-INFINITY, 0.0f};
+    bool odd = false, past = false;
+    typename F::Scores s_a, s_b;
+    typename F::Weights p;
+    int i = 0, walk = o.qi;
+    auto exact_step = [&]() __attribute__((always_inline)) {
+        const bool tree = i < tree_tiles;
+        const int first = (tree ? tree_tiles - 1 - i : cache_tile(i)) * F::kKeys;
+        const uint64_t bits = tree ? tree_bits(a, w.g.q0, walk, first, F::kKeys) : first_bits(w.key1 - first);
+        await(i, true);
+        if (i + 2 < n) issue(i + 2);
+        if (tree) odd |= tile_odd<DH>(v_of(i), tid, 256);
+        if (wave_live) {
+            tile_qk<DH>(k_of(i), o.qf, s_a, h, r);
+            tree_exact<DH, MODE>(a, w, o, tree, first, bits, h, s_a, p, oacc, st);
+            tile_pv<DH>(v_of(i), p, oacc, lane);
+        }
+    };
+    for (; i < exact; ++i) exact_step();
+    i = __builtin_amdgcn_readfirstlane(i);
+    if (!wave_live) {
+        for (; i < n; ++i) {
+            await(i, i == exact);
+            if (i > exact && i + 1 < n) issue_cache(i + 1);
+        }
+    } else if (i < n) {
+        auto weights = [&](int i, typename F::Scores & s) __attribute__((always_inline)) {
+            float sum = tile_weights<DH, MODE>(o.rs, cap_log2, s, p, st.base, behind(i));
+            if (__builtin_expect(__ballot(!(sum <= kSumLimit)) != 0, 0)) {
+                const float top = fmaxf(st.base, tile_max<DH, MODE>(o.rs, cap_log2, s, behind(i)));
+                const float up = top == -INFINITY ? 0.0f : top;  // scores of minus infinity, or NaN, only
+                const float keep = __builtin_amdgcn_exp2f(st.base - up);
+                st.base = up;
+                st.sum *= keep;
+#pragma unroll
+                for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) oacc[dt][e] *= keep;
+                sum = tile_weights<DH, MODE>(o.rs, cap_log2, s, p, st.base, behind(i));
+            }
+            st.sum += sum;
+        };
+        await(i, true);
+        tile_qk<DH>(k_of(i), o.qf, s_a, h, r);
+        // The first: no product before it.
+        if (i + 1 < n) {
+            await(i + 1, false);
+            if (i + 2 < n) issue_cache(i + 2);
+            tile_qk<DH>(k_of(i + 1), o.qf, s_b, h, r);
+        }
+        weights(i, s_a);
+        ++i;
+        auto step = [&](typename F::Scores & now, typename F::Scores & next) __attribute__((always_inline)) {
+            await(i + 1, false);
+            if (i + 2 < n) issue_cache(i + 2);
+            tile_pv<DH>(v_of(i - 1), p, oacc, lane);
+            tile_qk<DH>(k_of(i + 1), o.qf, next, h, r);
+            weights(i, now);
+            ++i;
+        };
+        while (i + 2 < n) {
+            step(s_b, s_a);
+            step(s_a, s_b);
+        }
+        if (i + 1 < n) {
+            step(s_b, s_a);
+#pragma unroll
+            for (int kt = 0; kt < F::KT; ++kt) s_b[kt] = s_a[kt];
+        }
+        tile_pv<DH>(v_of(i - 1), p, oacc, lane);
+        if (i < n) {
+            weights(i, s_b);
+            tile_pv<DH>(v_of(i), p, oacc, lane);
+        }
+        // (A sum of magnitudes: infinities and NaN stay in it.)
+        float size[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) size[e & 3] += fabsf(oacc[dt][e]);
+        past = o.live && !((size[0] + size[1]) + (size[2] + size[3]) < kOutLimit) && is_finite_bits(st.sum);
+    }
+    const int64_t part = item_rows(a, w) + wave * 32;
+    if (__builtin_expect(__syncthreads_or(odd || past), 0)) {
+        if (__syncthreads_or(odd)) {
+            for (int j = 0; j < 32; ++j)
+                if (wave_row0 + j < w.rows) tree_row_alone<uint16_t, DH / 64>(a, w, wave_row0 + j, lane, part + j);
+            return;
+        }
+        issue(0);  // (every wave is done with the slots)
+        if (n > 1) issue(1);
+#pragma unroll
+        for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
+        st = {-INFINITY, 0.0f};
+        walk = o.qi;
+        for (i = 0; i < n; ++i) exact_step();
+    }
+    const float sum = lane_pair_sum(st.sum);
+    if (!o.live) return;
+    if (w.chunks > 1) {
+        if (h == 0) a.part_ml[part + r] = make_float2(st.base, sum);
+        float * to = a.part + (part + r) * a.d;
+#pragma unroll
+        for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (WHOLE || dt * 32 + 8 * g + 4 * h < a.d)
+                    *reinterpret_cast<float4 *>(to + dt * 32 + 8 * g + 4 * h) =
+                        make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
+        return;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t * to = static_cast<uint16_t *>(a.o) + (w.g.q0 + o.qi) * a.ldo + static_cast<int64_t>(o.head) * a.d;
+#pragma unroll
+    for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            if (WHOLE || dt * 32 + 8 * g + 4 * h < a.d)
+                *reinterpret_cast<uint2 *>(to + dt * 32 + 8 * g + 4 * h) =
+                    make_uint2(pack_bf16x2(oacc[dt][4 * g] * inv, oacc[dt][4 * g + 1] * inv),
+                               pack_bf16x2(oacc[dt][4 * g + 2] * inv, oacc[dt][4 * g + 3] * inv));
+}
+
 // Joins the chunks of a (query, head): eight groups of 32 lanes, each every eighth chunk, then
 // their results in order.
 template <typename T>
@@ -414,8 +793,9 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
     if (!locate_query(a, qi, lane, w) || w.chunks <= 1) return;
     const int tiles = row_tiles_of(a, w.g), row = (qi - w.g.q0) * a.group + head % a.group;
     if (w.slot + static_cast<int64_t>(tiles) * w.chunks > a.slots) return;  // (of bounds that fall: no such items)
-    const int64_t at = ((w.slot + row / kTreeRows) * static_cast<int64_t>(a.kv_heads) + w.kv) * kTreeRows + row % kTreeRows;
-    const int64_t step = static_cast<int64_t>(tiles) * a.kv_heads * kTreeRows;
+    w.slot += row >> a.row_shift;
+    const int64_t at = item_rows(a, w) + (row & ((1 << a.row_shift) - 1));
+    const int64_t step = static_cast<int64_t>(tiles) * a.kv_heads << a.row_shift;
     float m = -INFINITY, l = 0.0f, acc[kMost];
 #pragma unroll
     for (int c = 0; c < kMost; ++c) acc[c] = 0.0f;
@@ -515,19 +895,23 @@ __global__ void __launch_bounds__(1024) tree_table_kernel(TreeArgs a, int64_t * 
 constexpr int kTreeMaxDim = 256;
 constexpr int64_t kTreeMaxRows = INT32_MAX - 1023;  // rows and keys are counted in 32 bits, a tile past their end
 constexpr int kWaveSegments = 64;
-constexpr int64_t kTreeItems = 1024;  // workgroups that chunks past the first add at most
+constexpr int64_t kFewTreeRows = 32;  // rows a segment has on average in calls of tiles of 32
+// Workgroups that chunks past the first add at most, of tiles of 32 and of 128 rows.
+constexpr int64_t kTreeItems = 1024, kTreeItemsWide = 512;
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-int64_t tree_target(int kv_heads) { return std::max<int64_t>(1, kTreeItems / kv_heads); }
+int64_t tree_target(int kv_heads, int row_shift) {
+    return std::max<int64_t>(1, (row_shift == 5 ? kTreeItems : kTreeItemsWide) / kv_heads);
+}
 // Items a key/value head has at most: its row tiles, and the target of chunks past their first.
-int64_t tree_items(int nseg, int64_t total_q, int kv_heads, int group) {
-    return total_q * group / kTreeRows + nseg + tree_target(kv_heads);
+int64_t tree_items(int nseg, int64_t total_q, int kv_heads, int group, int row_shift) {
+    return (total_q * group >> row_shift) + nseg + tree_target(kv_heads, row_shift);
 }
 // Those with partial results: a segment of len keys in more chunks than one has at most 2 len / chunk.
-int64_t tree_slots(int kv_heads) { return 2 * tree_target(kv_heads); }
+int64_t tree_slots(int kv_heads, int row_shift) { return 2 * tree_target(kv_heads, row_shift); }
 size_t tree_table_bytes(int nseg) { return round256((2 * static_cast<size_t>(nseg) + 2) * sizeof(int64_t)); }
-size_t tree_part_rows(int kv_heads) { return static_cast<size_t>(tree_slots(kv_heads)) * kv_heads * kTreeRows; }
+size_t tree_part_rows(int kv_heads, int row_shift) { return static_cast<size_t>(tree_slots(kv_heads, row_shift)) * kv_heads << row_shift; }
 
 template <typename T, int DP>
 int launch_tree_any(const TreeArgs & a, hipStream_t s) {
@@ -541,9 +925,44 @@ int launch_tree_any(const TreeArgs & a, hipStream_t s) {
     return check_launch("tree attention");
 }
 
+// kernel<mode of the call>
+template <typename F> int with_tree_mode(const TreeArgs & a, F && launch) {
+    auto capped = [&](auto rest) {
+        constexpr int kRest = decltype(rest)::value;
+        if (a.cap_log2 == 0.0f) return launch(rest);
+        if (a.cap_log2 <= kNearCap * kLog2e) return launch(std::integral_constant<int, kCap | kRest>{});
+        return launch(std::integral_constant<int, kCap | kFar | kRest>{});
+    };
+    if (a.slopes) return capped(std::integral_constant<int, kBias>{});
+    return capped(std::integral_constant<int, 0>{});
+}
+
+template <int DH, bool WHOLE>
+int launch_tree_fast(const TreeArgs & a, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(a.items * a.kv_heads));
+    return with_tree_mode(a, [&](auto mode) {
+        constexpr int kMode = decltype(mode)::value;
+        if (a.row_shift == 7) {
+            hipLaunchKernelGGL((tree_attn_rows_kernel<DH, kMode, WHOLE>), grid, dim3(256), 0, s, a);
+            return check_launch("tree attention of many rows");
+        }
+        auto kernel = &tree_attn_few_kernel<DH, kMode, WHOLE>;
+        static std::atomic<uint64_t> done{0};
+        if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), kTreeFewBytes<DH>, done, "hipFuncSetAttribute(tree_attn_few)"))
+            return rc;
+        hipLaunchKernelGGL(kernel, grid, dim3(kTreeWaves * 64), kTreeFewBytes<DH>, s, a);
+        return check_launch("tree attention of few rows");
+    });
+}
+
 template <typename T>
-int run_tree(const TreeArgs & a, hipStream_t s) {
-    int rc = a.d <= 64 ? launch_tree_any<T, 64>(a, s) : a.d <= 128 ? launch_tree_any<T, 128>(a, s) : launch_tree_any<T, 256>(a, s);
+int run_tree(const TreeArgs & a, bool fast, hipStream_t s) {
+    int rc;
+    if (fast && a.d == 64) rc = launch_tree_fast<64, true>(a, s);
+    else if (fast && a.d == 128) rc = launch_tree_fast<128, true>(a, s);
+    else if (fast) rc = a.d < 64 ? launch_tree_fast<64, false>(a, s) : launch_tree_fast<128, false>(a, s);
+    else if (a.d <= 64) rc = launch_tree_any<T, 64>(a, s);
+    else rc = a.d <= 128 ? launch_tree_any<T, 128>(a, s) : launch_tree_any<T, 256>(a, s);
     if (rc || a.cache_rows <= kTreeUnit) return rc;  // (no chunk is shorter than a unit)
     hipLaunchKernelGGL(tree_join_kernel<T>, dim3(static_cast<unsigned>(a.total_q * a.heads)), dim3(256), 0, s, a);
     return check_launch("tree attention join");
@@ -562,7 +981,7 @@ extern "C" {
 
 size_t pxs_tree_attention_workspace_bytes(int nseg, int64_t total_q, int heads, int kv_heads, int head_dim) {
     if (nseg <= 0 || total_q <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 256;
-    const size_t rows = tree_part_rows(kv_heads);
+    const size_t rows = std::max(tree_part_rows(kv_heads, 5), tree_part_rows(kv_heads, 7));
     return tree_table_bytes(nseg) + round256(rows * sizeof(float2)) + round256(rows * head_dim * sizeof(float));
 }
 
@@ -599,19 +1018,20 @@ int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, 
     a.cu_q = cu_q; a.parents = parents; a.start = cache_start; a.len = cache_len; a.positions = positions;
     a.nseg = nseg; a.total_q = total_q; a.cache_rows = cache_rows;
     a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.d = head_dim;
-    // (Caps that cap nothing fp32 holds are taken lower, so that scale / cap stays a normal number.)
-    cap = std::min({cap, std::numeric_limits<float>::max() / 4, scale * 0x1p126f});
-    a.scale_log2 = scale * kLog2e;
-    a.cap_log2 = cap * kLog2e;
-    a.over_cap = cap > 0.0f ? scale / cap : 0.0f;
+    score_constants(a, scale, cap);
     a.slopes = slopes; a.o = o; a.ldo = ld_o;
     const int elem = dtype == PXS_BF16 ? 2 : 4;
     a.vec = whole_pieces(q, ld_q, head_dim, elem) && whole_pieces(k, ld_k, head_dim, elem) &&
             whole_pieces(v, ld_v, head_dim, elem) &&
             (cache_rows == 0 || (whole_pieces(k_cache, ld_k_cache, head_dim, elem) && whole_pieces(v_cache, ld_v_cache, head_dim, elem)));
-    a.items = tree_items(nseg, total_q, kv_heads, a.group);
-    a.slots = tree_slots(kv_heads);
-    a.per_target = 1.0 / static_cast<double>(tree_target(kv_heads));
+    // The fast kernels' 32-bit offsets within a key tile hold row strides below 2^24.
+    const bool fast = dtype == PXS_BF16 && head_dim <= 128 && a.vec && ld_k < (1 << 24) && ld_v < (1 << 24) &&
+                      (cache_rows == 0 || (ld_k_cache < (1 << 24) && ld_v_cache < (1 << 24))) &&
+                      reinterpret_cast<uintptr_t>(o) % 8 == 0 && ld_o % 4 == 0;
+    a.row_shift = fast && total_q * a.group > kFewTreeRows * nseg ? 7 : 5;
+    a.items = tree_items(nseg, total_q, kv_heads, a.group, a.row_shift);
+    a.slots = tree_slots(kv_heads, a.row_shift);
+    a.per_target = 1.0 / static_cast<double>(tree_target(kv_heads, a.row_shift));
     PXS_CHECK(a.items * kv_heads <= UINT32_MAX / 256 && total_q * heads <= UINT32_MAX / 256, PXS_ERR_ARG,
               "pxs_tree_attention: grid too large");
     char * ws = static_cast<char *>(workspace);
@@ -621,10 +1041,10 @@ int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, 
         if (int rc = check_launch("tree attention table")) return rc;
     }
     ws += tree_table_bytes(nseg);
-    const size_t rows = tree_part_rows(kv_heads);
+    const size_t rows = tree_part_rows(kv_heads, a.row_shift);
     a.part_ml = reinterpret_cast<float2 *>(ws);
     a.part = reinterpret_cast<float *>(ws + round256(rows * sizeof(float2)));
-    return dtype == PXS_F32 ? run_tree<float>(a, s) : run_tree<uint16_t>(a, s);
+    return dtype == PXS_F32 ? run_tree<float>(a, false, s) : run_tree<uint16_t>(a, fast, s);
 }
 
 } // extern "C"
