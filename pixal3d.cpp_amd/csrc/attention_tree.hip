@@ -410,11 +410,30 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
 // The tiles, products and weights of the scored attention's kernels (attn_scores.h).  An item's tiles are walked as
 // the tree's from the last to the first, each with the keys that a row sees as bits, then the cache's.
 
-// The tokens first .. first + keys - 1 (up to 64) that the lane's row sees, `at` its next from itself up.
-__device__ __forceinline__ uint64_t tree_bits(const TreeArgs & a, int q0, int & at, int first, int keys) {
+// A row's walk up the tree, a tile of tokens at a time from the last: `at` is the next token that the lane's row
+// sees, `done` the first token of the tile before.  A tile's parents are loaded by its lanes together, and the
+// steps of the walk go through them and not to memory.
+struct TreeWalk {
+    int at, done;
+};
+// The tokens first .. first + KEYS - 1 that the row sees, as bits; tiles between `done` and those are passed.
+template <int KEYS>
+__device__ __forceinline__ uint64_t tree_bits(const TreeArgs & a, const Tree & g, TreeWalk & walk, int first, int lane) {
+    static_assert(KEYS <= 64, "a lane a token");
     uint64_t bits = 0;
-    while (at >= first + keys) at = above(a, q0, at);
-    for (; at >= first; at = above(a, q0, at)) bits |= uint64_t(1) << (at - first);
+    while (walk.done > first) {
+        walk.done -= KEYS;
+        const int from = walk.done;
+        const int up = a.parents[g.q0 + min(from + (lane & (KEYS - 1)), g.nq - 1)];
+        while (__ballot(walk.at >= from)) {
+            const bool here = walk.at >= from;
+            const int k = here ? walk.at - from : 0;
+            if (here) bits |= uint64_t(1) << k;
+            const int next = __shfl(up, k, 64);
+            if (here) walk.at = next >= 0 && next < walk.at ? next : -1;
+        }
+        if (from > first) bits = 0;
+    }
     return bits;
 }
 // The first `seen` keys of a tile, as bits.
@@ -519,7 +538,7 @@ __global__ void __launch_bounds__(kTreeWaves * 64) tree_attn_few_kernel(TreeArgs
     for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
     RowState st{-INFINITY, 0.0f};
     bool odd = false;
-    int walk = o.qi;
+    TreeWalk walk{o.qi, tree_tiles * F::kKeys};
 #pragma unroll
     for (int i = 1; i < kTreeStages; ++i)
         if (i < n) issue(i);
@@ -527,7 +546,7 @@ __global__ void __launch_bounds__(kTreeWaves * 64) tree_attn_few_kernel(TreeArgs
         const int t = wave + kTreeWaves * i;
         const bool tree = t < tree_tiles;
         const int first = (tree ? tree_tiles - 1 - t : cache0 + t - tree_tiles) * F::kKeys;
-        const uint64_t bits = tree ? tree_bits(a, w.g.q0, walk, first, F::kKeys) : first_bits(w.key1 - first);
+        const uint64_t bits = tree ? tree_bits<F::kKeys>(a, w.g, walk, first, lane) : first_bits(w.key1 - first);
         wait_stages<kTreeStages - 1, kInstr>(n - 1 - i);
         asm volatile("" ::: "memory");
         const char * kl = ring + slot(i);
@@ -659,11 +678,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
     bool odd = false, past = false;
     typename F::Scores s_a, s_b;
     typename F::Weights p;
-    int i = 0, walk = o.qi;
+    int i = 0;
+    TreeWalk walk{o.qi, tree_tiles * F::kKeys};
     auto exact_step = [&]() __attribute__((always_inline)) {
         const bool tree = i < tree_tiles;
         const int first = (tree ? tree_tiles - 1 - i : cache_tile(i)) * F::kKeys;
-        const uint64_t bits = tree ? tree_bits(a, w.g.q0, walk, first, F::kKeys) : first_bits(w.key1 - first);
+        const uint64_t bits = tree ? tree_bits<F::kKeys>(a, w.g, walk, first, lane) : first_bits(w.key1 - first);
         await(i, true);
         if (i + 2 < n) issue(i + 2);
         if (tree) odd |= tile_odd<DH>(v_of(i), tid, 256);
@@ -749,7 +769,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
 #pragma unroll
         for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
         st = {-INFINITY, 0.0f};
-        walk = o.qi;
+        walk = {o.qi, tree_tiles * F::kKeys};
         for (i = 0; i < n; ++i) exact_step();
     }
     const float sum = lane_pair_sum(st.sum);
@@ -778,42 +798,63 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
                                pack_bf16x2(oacc[dt][4 * g + 2] * inv, oacc[dt][4 * g + 3] * inv));
 }
 
-// Joins the chunks of a (query, head): eight groups of 32 lanes, each every eighth chunk, then
-// their results in order.
-template <typename T>
+// Joins the chunks of (query, head) rows, in their order; 32 lanes a row and chunk, four dims a lane.
+// kRowsEach: a workgroup's eight groups of lanes have a row each, of eight heads of a query; otherwise they share one
+// row, each every eighth chunk, and their results are joined through LDS.  The first for calls of kJoinRows rows
+// and more, whose chunks are few.
+template <typename T, bool kRowsEach>
 __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
-    constexpr int kGroups = 8, kMost = 8;  // head sizes up to 32 kMost
+    constexpr int kGroups = 8, kParts = 2;  // head sizes up to 128 kParts
     __shared__ float2 ml[kGroups];
-    __shared__ float acc_of[kGroups][32 * kMost];
+    __shared__ __align__(16) float acc_of[kRowsEach ? 1 : kGroups][128 * kParts];
     const int lane = threadIdx.x & 63, l32 = threadIdx.x & 31, grp = threadIdx.x >> 5;
-    const int qi = static_cast<int>(blockIdx.x / a.heads);
-    const int head = static_cast<int>(blockIdx.x % a.heads);
+    const int per = kRowsEach ? (a.heads + kGroups - 1) / kGroups : a.heads;
+    const int qi = static_cast<int>(blockIdx.x / per);
+    int head = static_cast<int>(blockIdx.x % per);
     Item w;
-    w.kv = head / a.group;
+    w.kv = 0;
     if (!locate_query(a, qi, lane, w) || w.chunks <= 1) return;
+    if (kRowsEach) {
+        head = head * kGroups + grp;
+        if (head >= a.heads) return;
+    }
+    w.kv = head / a.group;
     const int tiles = row_tiles_of(a, w.g), row = (qi - w.g.q0) * a.group + head % a.group;
     if (w.slot + static_cast<int64_t>(tiles) * w.chunks > a.slots) return;  // (of bounds that fall: no such items)
     w.slot += row >> a.row_shift;
     const int64_t at = item_rows(a, w) + (row & ((1 << a.row_shift) - 1));
     const int64_t step = static_cast<int64_t>(tiles) * a.kv_heads << a.row_shift;
-    float m = -INFINITY, l = 0.0f, acc[kMost];
-#pragma unroll
-    for (int c = 0; c < kMost; ++c) acc[c] = 0.0f;
-    for (int i = grp; i < w.chunks; i += kGroups) {
+    const bool whole = (a.d & 3) == 0;
+    float m = -INFINITY, l = 0.0f, acc[kParts][4] = {};
+#pragma unroll 4
+    for (int i = kRowsEach ? 0 : grp; i < w.chunks; i += kRowsEach ? 1 : kGroups) {
         const float2 p = a.part_ml[at + i * step];
+        float o[kParts][4];
+#pragma unroll
+        for (int c = 0; c < kParts; ++c) load_dims4<float>(a.part + (at + i * step) * a.d, 128 * c + 4 * l32, a.d, whole, o[c]);
         const float up = fmaxf(m, p.x), ref = up == -INFINITY ? 0.0f : up;
-        const float keep = exp2f(m - ref), f = exp2f(p.x - ref);
+        const float keep = __builtin_amdgcn_exp2f(m - ref), f = __builtin_amdgcn_exp2f(p.x - ref);
         l = l * keep + p.y * f;
 #pragma unroll
-        for (int c = 0; c < kMost; ++c) {
-            const float o = l32 + 32 * c < a.d ? a.part[(at + i * step) * a.d + l32 + 32 * c] : 0.0f;
-            acc[c] = acc[c] * keep + o * f;
-        }
+        for (int c = 0; c < kParts; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[c][e] = acc[c][e] * keep + o[c][e] * f;
         m = up;
+    }
+    T * to = static_cast<T *>(a.o) + qi * a.ldo + static_cast<int64_t>(head) * a.d;
+    if constexpr (kRowsEach) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int c = 0; c < kParts; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (128 * c + 4 * l32 + e < a.d) store_f32(to + 128 * c + 4 * l32 + e, acc[c][e] * inv);
+        return;
     }
     if (l32 == 0) ml[grp] = make_float2(m, l);
 #pragma unroll
-    for (int c = 0; c < kMost; ++c) acc_of[grp][l32 + 32 * c] = acc[c];
+    for (int c = 0; c < kParts; ++c)
+        *reinterpret_cast<float4 *>(&acc_of[kRowsEach ? 0 : grp][128 * c + 4 * l32]) = make_float4(acc[c][0], acc[c][1], acc[c][2], acc[c][3]);
     __syncthreads();
     const int dim = threadIdx.x;
     if (dim >= a.d) return;
@@ -823,12 +864,12 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
     const float ref = base == -INFINITY ? 0.0f : base;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-        const float f = exp2f(ml[i].x - ref);
+        const float f = __builtin_amdgcn_exp2f(ml[i].x - ref);
         total += ml[i].y * f;
-        v += acc_of[i][dim] * f;
+        v += acc_of[kRowsEach ? 0 : i][dim] * f;
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    store_f32(static_cast<T *>(a.o) + qi * a.ldo + static_cast<int64_t>(head) * a.d + dim, v * inv);
+    store_f32(to + dim, v * inv);
 }
 
 // For more segments than a wave's lanes: items before each segment [nseg], all of them, the chunk,
@@ -895,23 +936,24 @@ __global__ void __launch_bounds__(1024) tree_table_kernel(TreeArgs a, int64_t * 
 constexpr int kTreeMaxDim = 256;
 constexpr int64_t kTreeMaxRows = INT32_MAX - 1023;  // rows and keys are counted in 32 bits, a tile past their end
 constexpr int kWaveSegments = 64;
+constexpr int64_t kJoinRows = 4096;     // (query, head) rows whose chunks a group of lanes joins alone
 constexpr int64_t kFewTreeRows = 32;  // rows a segment has on average in calls of tiles of 32
-// Workgroups that chunks past the first add at most, of tiles of 32 and of 128 rows.
-constexpr int64_t kTreeItems = 1024, kTreeItemsWide = 512;
+// Workgroups that chunks past the first add at most: one round of the fast kernels' two a CU (eight trees of
+// 64 over 8,192 keys 109 us, with 384 121, with 768 135; eight trees over caches of 0 to 40,001 98, with 320
+// 108, with 1,024 104; 64 of 8 over 4,096 207, 209 and 221).
+constexpr int64_t kTreeItems = 512;
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-int64_t tree_target(int kv_heads, int row_shift) {
-    return std::max<int64_t>(1, (row_shift == 5 ? kTreeItems : kTreeItemsWide) / kv_heads);
-}
+int64_t tree_target(int kv_heads) { return std::max<int64_t>(1, kTreeItems / kv_heads); }
 // Items a key/value head has at most: its row tiles, and the target of chunks past their first.
 int64_t tree_items(int nseg, int64_t total_q, int kv_heads, int group, int row_shift) {
-    return (total_q * group >> row_shift) + nseg + tree_target(kv_heads, row_shift);
+    return (total_q * group >> row_shift) + nseg + tree_target(kv_heads);
 }
 // Those with partial results: a segment of len keys in more chunks than one has at most 2 len / chunk.
-int64_t tree_slots(int kv_heads, int row_shift) { return 2 * tree_target(kv_heads, row_shift); }
+int64_t tree_slots(int kv_heads) { return 2 * tree_target(kv_heads); }
 size_t tree_table_bytes(int nseg) { return round256((2 * static_cast<size_t>(nseg) + 2) * sizeof(int64_t)); }
-size_t tree_part_rows(int kv_heads, int row_shift) { return static_cast<size_t>(tree_slots(kv_heads, row_shift)) * kv_heads << row_shift; }
+size_t tree_part_rows(int kv_heads, int row_shift) { return static_cast<size_t>(tree_slots(kv_heads)) * kv_heads << row_shift; }
 
 template <typename T, int DP>
 int launch_tree_any(const TreeArgs & a, hipStream_t s) {
@@ -964,7 +1006,10 @@ int run_tree(const TreeArgs & a, bool fast, hipStream_t s) {
     else if (a.d <= 64) rc = launch_tree_any<T, 64>(a, s);
     else rc = a.d <= 128 ? launch_tree_any<T, 128>(a, s) : launch_tree_any<T, 256>(a, s);
     if (rc || a.cache_rows <= kTreeUnit) return rc;  // (no chunk is shorter than a unit)
-    hipLaunchKernelGGL(tree_join_kernel<T>, dim3(static_cast<unsigned>(a.total_q * a.heads)), dim3(256), 0, s, a);
+    if (a.total_q * a.heads >= kJoinRows)
+        hipLaunchKernelGGL((tree_join_kernel<T, true>), dim3(static_cast<unsigned>(a.total_q * ((a.heads + 7) / 8))), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((tree_join_kernel<T, false>), dim3(static_cast<unsigned>(a.total_q * a.heads)), dim3(256), 0, s, a);
     return check_launch("tree attention join");
 }
 
@@ -981,7 +1026,7 @@ extern "C" {
 
 size_t pxs_tree_attention_workspace_bytes(int nseg, int64_t total_q, int heads, int kv_heads, int head_dim) {
     if (nseg <= 0 || total_q <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 256;
-    const size_t rows = std::max(tree_part_rows(kv_heads, 5), tree_part_rows(kv_heads, 7));
+    const size_t rows = tree_part_rows(kv_heads, 7);
     return tree_table_bytes(nseg) + round256(rows * sizeof(float2)) + round256(rows * head_dim * sizeof(float));
 }
 
@@ -1030,8 +1075,8 @@ int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, 
                       reinterpret_cast<uintptr_t>(o) % 8 == 0 && ld_o % 4 == 0;
     a.row_shift = fast && total_q * a.group > kFewTreeRows * nseg ? 7 : 5;
     a.items = tree_items(nseg, total_q, kv_heads, a.group, a.row_shift);
-    a.slots = tree_slots(kv_heads, a.row_shift);
-    a.per_target = 1.0 / static_cast<double>(tree_target(kv_heads, a.row_shift));
+    a.slots = tree_slots(kv_heads);
+    a.per_target = 1.0 / static_cast<double>(tree_target(kv_heads));
     PXS_CHECK(a.items * kv_heads <= UINT32_MAX / 256 && total_q * heads <= UINT32_MAX / 256, PXS_ERR_ARG,
               "pxs_tree_attention: grid too large");
     char * ws = static_cast<char *>(workspace);
