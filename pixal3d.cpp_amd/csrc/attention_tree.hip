@@ -53,7 +53,7 @@ struct TreeArgs {
     int vec;                   // rows of q, k and v in whole 16-byte pieces
     int64_t items;             // launched (bound)
     int64_t slots;             // items with partial results (bound)
-    double per_target;         // 1 / items that the chunks add at most
+    float per_target;          // 1 / (items that the chunks add at most * kTreeUnit)
     int row_shift;             // log2 of a tile's rows
     float * part;              // [slots * kv_heads << row_shift][d] unnormalised outputs
     float2 * part_ml;          // [..] maxima (log2 units) and sums
@@ -78,15 +78,17 @@ __device__ __forceinline__ int row_tiles_of(const TreeArgs & a, const Tree & g) 
 }
 // Keys of a chunk, from the sum of row tiles times cached keys: `work` of them over the
 // target's items, and one unit more, so that the chunks past a tile's first are at most the target.
-__device__ __forceinline__ int chunk_of(const TreeArgs & a, double work) {
-    const double units = floor(work * a.per_target * (1.0 / kTreeUnit)) + 1.0;
-    return static_cast<int>(min(units * kTreeUnit, static_cast<double>(a.cache_rows + kTreeUnit)));
+// (Rounded sums of it: they are the same in every wave, and off by so little that the target, at most 512, holds.)
+__device__ __forceinline__ int chunk_of(const TreeArgs & a, float work) {
+    const float units = floorf(work * a.per_target) + 1.0f, most = static_cast<float>(a.cache_rows / kTreeUnit + 1);
+    return static_cast<int>(fminf(units, most)) * kTreeUnit;
 }
 __device__ __forceinline__ int chunks_of(const Tree & g, int chunk) { return g.nk > chunk ? (g.nk - 1) / chunk + 1 : 1; }
 // First key of chunk i of a segment's: as even as whole units make them.
 __device__ __forceinline__ int chunk_start(const Tree & g, int i, int chunks) {
-    const int64_t units = (static_cast<int64_t>(g.nk) + kTreeUnit - 1) / kTreeUnit;
-    return static_cast<int>(min(units * i / chunks * kTreeUnit, static_cast<int64_t>(g.nk)));
+    const int units = static_cast<int>((static_cast<int64_t>(g.nk) + kTreeUnit - 1) / kTreeUnit);
+    const int each = units / chunks, more = units - each * chunks;  // (the first `more` have one more)
+    return static_cast<int>(min(static_cast<int64_t>(i * each + min(i, more)) * kTreeUnit, static_cast<int64_t>(g.nk)));
 }
 
 // An item: a row tile and the chunk's keys.
@@ -99,12 +101,18 @@ struct Item {
     int slot;             // of the item's partial results, where there are more chunks than one
 };
 
-__device__ __forceinline__ int tree_sums(int v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int below = __shfl_up(v, d, 64);
-        if (lane >= d) v += below;
-    }
+// v summed over the lanes up to each, through the lanes' own paths (a shuffle through LDS takes ten times as long).
+template <typename V> __device__ __forceinline__ V tree_sums(V v) {
+    auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        v += __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, decltype(rows)::value,
+                                                               0xF, false));
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});  // from 1, 2, 4, 8 lanes below in a row of 16
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // the last of row 0 to row 1, of 2 to 3
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // lane 31 to rows 2 and 3
     return v;
 }
 
@@ -118,14 +126,12 @@ __device__ __forceinline__ Plan segment_plan(const TreeArgs & a, int lane) {
     Plan p{};
     if (lane < a.nseg) p.g = load_tree(a, lane);
     const int tiles = row_tiles_of(a, p.g);
-    double work = static_cast<double>(tiles) * p.g.nk;
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) work += __shfl_xor(work, d, 64);
-    p.chunk = __builtin_amdgcn_readfirstlane(chunk_of(a, work));
+    const float work = tree_sums(static_cast<float>(tiles) * static_cast<float>(p.g.nk));
+    p.chunk = chunk_of(a, __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, work), 63)));
     p.items = tiles * chunks_of(p.g, p.chunk);
-    p.end = tree_sums(p.items, lane);
+    p.end = tree_sums(p.items);
     p.slots = p.items > tiles ? p.items : 0;
-    p.slots_end = tree_sums(p.slots, lane);
+    p.slots_end = tree_sums(p.slots);
     return p;
 }
 __device__ __forceinline__ Tree tree_of(const Tree & g, int from) {
@@ -266,13 +272,44 @@ __device__ __forceinline__ void tree_row_alone(const TreeArgs & a, const Item & 
     if (w.chunks > 1 && lane == 0) a.part_ml[slot] = make_float2(m, l);
 }
 
+// A row's walk up the tree, a tile of tokens at a time from the last: `at` is the next token that the lane's row
+// sees, `done` the first token of the tile before.  A tile's parents are loaded by its lanes together, and the
+// steps of the walk go through them and not to memory.
+struct TreeWalk {
+    int at, done;
+};
+// The tokens first .. first + KEYS - 1 that the row sees, as bits; tiles between `done` and those are passed.
+template <int KEYS>
+__device__ __forceinline__ uint64_t tree_bits(const TreeArgs & a, const Tree & g, TreeWalk & walk, int first, int lane) {
+    static_assert(KEYS <= 64, "a lane a token");
+    uint64_t bits = 0;
+    while (walk.done > first) {
+        walk.done -= KEYS;
+        const int from = walk.done;
+        const int up = a.parents[g.q0 + min(from + (lane & (KEYS - 1)), g.nq - 1)];
+        while (__ballot(walk.at >= from)) {
+            const bool here = walk.at >= from;
+            const int k = here ? walk.at - from : 0;
+            if (here) bits |= uint64_t(1) << k;
+            const int next = __shfl(up, k, 64);
+            if (here) walk.at = next >= 0 && next < walk.at ? next : -1;
+        }
+        if (from > first) bits = 0;
+    }
+    return bits;
+}
+// The first `seen` keys of a tile, as bits.
+__device__ __forceinline__ uint64_t first_bits(int seen) { return seen >= 64 ? ~uint64_t(0) : (uint64_t(1) << seen) - 1; }
+
 // Any type, head size up to DP, stride and alignment, in fp32 on v_mfma_f32_32x32x2_f32.  The four
 // waves of a workgroup have the same 32 rows and every fourth block of 32 keys each, straight from
 // memory; S^T = K Q^T, so that a lane owns one row and half of its scores, and O^T += V^T P^T.
-// Their results are joined through LDS.
-template <typename T, int DP>
+// Their results are joined through LDS.  WHOLE: head sizes of DP in rows of whole 16-byte pieces.
+// Where the registers hold them, a block's keys and values are loaded while the block before is multiplied.
+template <typename T, int DP, bool WHOLE>
 __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
     constexpr int DT = DP / 32;
+    constexpr bool kAhead = DP <= (WHOLE ? 128 : 64);
     extern __shared__ __align__(16) float tree_smem[];  // [4][32][DP] outputs, [4][32] maxima and sums
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -284,88 +321,125 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
     const bool live = w.row0 + r < w.rows;
     const int row = live ? w.row0 + r : w.rows - 1;
     const int qi = row / a.group, head = w.kv * a.group + row % a.group;
-    const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+    const RowScore rs = row_score<kCap | kFar>(a, head);
+    const bool capped = a.cap_log2 > 0.0f;
+    const float slope = a.slopes ? -kLog2e * a.slopes[head] : 0.0f;
     const int pos = a.slopes ? a.positions[w.g.q0 + qi] : 0;
     const int64_t col = static_cast<int64_t>(w.kv) * a.d;
-    const T * q = static_cast<const T *>(a.q) + (w.g.q0 + qi) * a.ldq + static_cast<int64_t>(head) * a.d;
-    float qv[DP / 2];  // dims h DP/2 .. h DP/2 + DP/2 - 1
+
+    const int tree_blocks = w.chunk == 0 ? (w.g.nq + 31) / 32 : 0;
+    const int all = tree_blocks + (w.key1 - w.key0 + 31) / 32;
+    struct Block {
+        bool tree;
+        int first, limit;  // its first key, and the keys there are from it on (32 or more: all of it)
+    };
+    auto block = [&](int b) {
+        Block o;
+        o.tree = b < tree_blocks;
+        o.first = o.tree ? (tree_blocks - 1 - b) * 32 : w.key0 + (b - tree_blocks) * 32;
+        o.limit = (o.tree ? w.g.nq : w.key1) - o.first;
+        return o;
+    };
+    // dims h DP/2 .. h DP/2 + DP/2 - 1 of a row; zeros past d
+    auto load_half = [&](const T * p, float (&out)[DP / 2]) __attribute__((always_inline)) {
+        if constexpr (WHOLE) {
+            constexpr int V = 16 / static_cast<int>(sizeof(T));
 #pragma unroll
-    for (int u = 0; u < DP / 8; ++u) {
-        float f[4];
-        load_dims4<T>(q, h * (DP / 2) + 4 * u, a.d, a.vec, f);
+            for (int u = 0; u < DP / 2 / V; ++u) {
+                T e[V];
+                __builtin_memcpy(e, __builtin_assume_aligned(p + h * (DP / 2) + V * u, 16), 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) qv[4 * u + e] = f[e];
+                for (int i = 0; i < V; ++i) out[V * u + i] = load_f32(e + i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < DP / 2; ++i) {
+                const int dim = h * (DP / 2) + i;
+                const float x = load_f32(p + min(dim, a.d - 1));
+                out[i] = dim < a.d ? x : 0.0f;
+            }
+        }
+    };
+    auto load_k = [&](const Block & o, float (&kk)[DP / 2]) __attribute__((always_inline)) {
+        const int key = o.first + min(r, o.limit - 1);
+        load_half(o.tree ? static_cast<const T *>(a.k) + static_cast<int64_t>(w.g.q0 + key) * a.ldk + col
+                         : static_cast<const T *>(a.kc) + (w.g.k0 + key) * a.ldkc + col, kk);
+    };
+    // Register e of dims dt: key 8 (e / 4) + 4 h + e % 4 of the block, dim 32 dt + r.  (Those of dims past d
+    // make outputs that are not stored.)
+    auto load_v = [&](const Block & o, float (&vv)[16][DT]) __attribute__((always_inline)) {
+        const int64_t ldv = o.tree ? a.ldv : a.ldvc;
+        const T * v = (o.tree ? static_cast<const T *>(a.v) + static_cast<int64_t>(w.g.q0 + o.first) * ldv
+                              : static_cast<const T *>(a.vc) + (w.g.k0 + o.first) * ldv) + col;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int key = 8 * (e >> 2) + 4 * h + (e & 3);
+            const T * p = v + min(key, o.limit - 1) * ldv;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) vv[e][dt] = load_f32(p + (WHOLE ? dt * 32 + r : min(dt * 32 + r, a.d - 1)));
+        }
+    };
+    float kk[DP / 2], vv[16][DT];
+    if (kAhead && wave < all) {
+        load_k(block(wave), kk);
+        load_v(block(wave), vv);
     }
+    float qv[DP / 2];
+    load_half(static_cast<const T *>(a.q) + (w.g.q0 + qi) * a.ldq + static_cast<int64_t>(head) * a.d, qv);
     f32x16 oacc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
     float m = -INFINITY, l = 0.0f;
     bool odd = false;
-    int walk = qi;  // the next of the row's tokens, from itself up
-
-    const int tree_blocks = w.chunk == 0 ? (w.g.nq + 31) / 32 : 0;
-    const int all = tree_blocks + (w.key1 - w.key0 + 31) / 32;
+    TreeWalk walk{qi, tree_blocks * 32};
     for (int b = wave; b < all; b += 4) {
-        const bool tree = b < tree_blocks;
-        const int first = tree ? (tree_blocks - 1 - b) * 32 : w.key0 + (b - tree_blocks) * 32;
-        const int limit = (tree ? w.g.nq : w.key1) - first;  // keys of the block, 32 or more: all
-        const int64_t ldk = tree ? a.ldk : a.ldkc, ldv = tree ? a.ldv : a.ldvc;
-        const int64_t at = (tree ? w.g.q0 : w.g.k0) + first;
-        const T * k = static_cast<const T *>(tree ? a.k : a.kc) + at * ldk + col;
-        const T * v = static_cast<const T *>(tree ? a.v : a.vc) + at * ldv + col;
-        uint32_t seen = limit >= 32 ? ~0u : (1u << limit) - 1u;
-        if (tree) {
-            seen = 0;
-            while (walk >= first + 32) walk = above(a, w.g.q0, walk);
-            for (; walk >= first; walk = above(a, w.g.q0, walk)) seen |= 1u << (walk - first);
-        }
+        const Block o = block(b);
+        if (!kAhead) load_k(o, kk);
+        const uint32_t seen = o.tree ? static_cast<uint32_t>(tree_bits<32>(a, w.g, walk, o.first, lane))
+                                     : static_cast<uint32_t>(first_bits(min(o.limit, 32)));
         f32x16 s = {};
-        const T * krow = k + min(r, limit - 1) * ldk;
 #pragma unroll
-        for (int u = 0; u < DP / 8; ++u) {
-            float f[4];
-            load_dims4<T>(krow, h * (DP / 2) + 4 * u, a.d, a.vec, f);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(f[e], qv[4 * u + e], s, 0, 0, 0);
-        }
-        // Register e holds key 8 (e / 4) + 4 h + e % 4 of the block.
+        for (int i = 0; i < DP / 2; ++i) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk[i], qv[i], s, 0, 0, 0);
+        if (kAhead && b + 4 < all) load_k(block(b + 4), kk);
         float top = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int key = 8 * (e >> 2) + 4 * h + (e & 3);
-            float away = 0.0f;
-            if (a.slopes) away = static_cast<float>(pos - (tree ? a.positions[w.g.q0 + first + min(key, limit - 1)] : first + key));
-            const float z = tree_score(a, s[e], slope, away);
+            float z = capped ? score_of<kCap | kFar>(rs, s[e], 0.0f, 0.0f) : s[e] * a.scale_log2;
+            if (a.slopes) {
+                const int at = o.tree ? a.positions[w.g.q0 + o.first + min(key, o.limit - 1)] : o.first + key;
+                z = __builtin_fmaf(slope, fabsf(static_cast<float>(pos - at)), z);
+            }
             s[e] = seen >> key & 1u ? z : -INFINITY;
             top = fmaxf(top, s[e]);
         }
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float up = fmaxf(m, top);
+        const float up = fmaxf(m, lane_pair_max(top));
         const float base = up == -INFINITY ? 0.0f : up;  // nothing seen yet: every weight is 0
-        const float keep = exp2f(m - base);
+        const float keep = __builtin_amdgcn_exp2f(m - base);
         float sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            s[e] = exp2f(s[e] - base);
+            s[e] = __builtin_amdgcn_exp2f(s[e] - base);
             sum += s[e];
         }
-        sum += __shfl_xor(sum, 32, 64);
-        l = l * keep + sum;
+        l = l * keep + lane_pair_sum(sum);
         m = up;
+        if (!kAhead) load_v(o, vv);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) oacc[dt][e] *= keep;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int key = 8 * (e >> 2) + 4 * h + (e & 3);
+            const bool in = 8 * (e >> 2) + 4 * h + (e & 3) < o.limit;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const float x = key < limit && dt * 32 + r < a.d ? load_f32(v + key * ldv + dt * 32 + r) : 0.0f;
-                odd |= tree && !is_finite_bits(x);
+                const float x = in ? vv[e][dt] : 0.0f;
+                odd |= o.tree && !is_finite_bits(x);
                 oacc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[e], oacc[dt], 0, 0, 0);
             }
         }
+        if (kAhead && b + 4 < all) load_v(block(b + 4), vv);
     }
     const int64_t slot0 = item_rows(a, w);
     if (__syncthreads_or(odd)) {
@@ -409,35 +483,6 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
 // ---- bf16, head sizes of whole 16-byte pieces up to 128 -----------------------------------------------------
 // The tiles, products and weights of the scored attention's kernels (attn_scores.h).  An item's tiles are walked as
 // the tree's from the last to the first, each with the keys that a row sees as bits, then the cache's.
-
-// A row's walk up the tree, a tile of tokens at a time from the last: `at` is the next token that the lane's row
-// sees, `done` the first token of the tile before.  A tile's parents are loaded by its lanes together, and the
-// steps of the walk go through them and not to memory.
-struct TreeWalk {
-    int at, done;
-};
-// The tokens first .. first + KEYS - 1 that the row sees, as bits; tiles between `done` and those are passed.
-template <int KEYS>
-__device__ __forceinline__ uint64_t tree_bits(const TreeArgs & a, const Tree & g, TreeWalk & walk, int first, int lane) {
-    static_assert(KEYS <= 64, "a lane a token");
-    uint64_t bits = 0;
-    while (walk.done > first) {
-        walk.done -= KEYS;
-        const int from = walk.done;
-        const int up = a.parents[g.q0 + min(from + (lane & (KEYS - 1)), g.nq - 1)];
-        while (__ballot(walk.at >= from)) {
-            const bool here = walk.at >= from;
-            const int k = here ? walk.at - from : 0;
-            if (here) bits |= uint64_t(1) << k;
-            const int next = __shfl(up, k, 64);
-            if (here) walk.at = next >= 0 && next < walk.at ? next : -1;
-        }
-        if (from > first) bits = 0;
-    }
-    return bits;
-}
-// The first `seen` keys of a tile, as bits.
-__device__ __forceinline__ uint64_t first_bits(int seen) { return seen >= 64 ? ~uint64_t(0) : (uint64_t(1) << seen) - 1; }
 
 // One row's place: its query, head, constants and first fragments.
 template <int DH, int MODE> struct TreeRow {
@@ -889,7 +934,7 @@ __global__ void __launch_bounds__(1024) tree_table_kernel(TreeArgs a, int64_t * 
     __syncthreads();
     work = 0.0;
     for (int i = 0; i < 16; ++i) work += works[i];
-    const int chunk = chunk_of(a, work);
+    const int chunk = chunk_of(a, static_cast<float>(work));
     int64_t before[2] = {0, 0};
     for (int s0 = 0; s0 < a.nseg; s0 += 1024) {
         const int s = s0 + tid;
@@ -955,10 +1000,10 @@ int64_t tree_slots(int kv_heads) { return 2 * tree_target(kv_heads); }
 size_t tree_table_bytes(int nseg) { return round256((2 * static_cast<size_t>(nseg) + 2) * sizeof(int64_t)); }
 size_t tree_part_rows(int kv_heads, int row_shift) { return static_cast<size_t>(tree_slots(kv_heads)) * kv_heads << row_shift; }
 
-template <typename T, int DP>
+template <typename T, int DP, bool WHOLE>
 int launch_tree_any(const TreeArgs & a, hipStream_t s) {
     constexpr int smem = 4 * 32 * DP * 4 + 4 * 32 * 8;
-    auto kernel = &tree_attn_any_kernel<T, DP>;
+    auto kernel = &tree_attn_any_kernel<T, DP, WHOLE>;
     if constexpr (smem > 64 * 1024) {
         static std::atomic<uint64_t> done{0};
         if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), smem, done, "hipFuncSetAttribute(tree_attn)")) return rc;
@@ -1003,8 +1048,14 @@ int run_tree(const TreeArgs & a, bool fast, hipStream_t s) {
     if (fast && a.d == 64) rc = launch_tree_fast<64, true>(a, s);
     else if (fast && a.d == 128) rc = launch_tree_fast<128, true>(a, s);
     else if (fast) rc = a.d < 64 ? launch_tree_fast<64, false>(a, s) : launch_tree_fast<128, false>(a, s);
-    else if (a.d <= 64) rc = launch_tree_any<T, 64>(a, s);
-    else rc = a.d <= 128 ? launch_tree_any<T, 128>(a, s) : launch_tree_any<T, 256>(a, s);
+    else if (a.vec && (a.d == 64 || a.d == 128 || a.d == 256))
+        rc = a.d == 64    ? launch_tree_any<T, 64, true>(a, s)
+             : a.d == 128 ? launch_tree_any<T, 128, true>(a, s)
+                          : launch_tree_any<T, 256, true>(a, s);
+    else
+        rc = a.d <= 64    ? launch_tree_any<T, 64, false>(a, s)
+             : a.d <= 128 ? launch_tree_any<T, 128, false>(a, s)
+                          : launch_tree_any<T, 256, false>(a, s);
     if (rc || a.cache_rows <= kTreeUnit) return rc;  // (no chunk is shorter than a unit)
     if (a.total_q * a.heads >= kJoinRows)
         hipLaunchKernelGGL((tree_join_kernel<T, true>), dim3(static_cast<unsigned>(a.total_q * ((a.heads + 7) / 8))), dim3(256), 0, s, a);
@@ -1076,7 +1127,7 @@ int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, 
     a.row_shift = fast && total_q * a.group > kFewTreeRows * nseg ? 7 : 5;
     a.items = tree_items(nseg, total_q, kv_heads, a.group, a.row_shift);
     a.slots = tree_slots(kv_heads);
-    a.per_target = 1.0 / static_cast<double>(tree_target(kv_heads));
+    a.per_target = 1.0f / static_cast<float>(tree_target(kv_heads) * kTreeUnit);
     PXS_CHECK(a.items * kv_heads <= UINT32_MAX / 256 && total_q * heads <= UINT32_MAX / 256, PXS_ERR_ARG,
               "pxs_tree_attention: grid too large");
     char * ws = static_cast<char *>(workspace);
