@@ -84,11 +84,13 @@ __device__ __forceinline__ int chunk_of(const TreeArgs & a, float work) {
     return static_cast<int>(fminf(units, most)) * kTreeUnit;
 }
 __device__ __forceinline__ int chunks_of(const Tree & g, int chunk) { return g.nk > chunk ? (g.nk - 1) / chunk + 1 : 1; }
-// First key of chunk i of a segment's: as even as whole units make them.
+// First key of chunk i of a segment's: as even as whole units make them, where the first chunk has the tree's too.
 __device__ __forceinline__ int chunk_start(const Tree & g, int i, int chunks) {
-    const int units = static_cast<int>((static_cast<int64_t>(g.nk) + kTreeUnit - 1) / kTreeUnit);
-    const int each = units / chunks, more = units - each * chunks;  // (the first `more` have one more)
-    return static_cast<int>(min(static_cast<int64_t>(i * each + min(i, more)) * kTreeUnit, static_cast<int64_t>(g.nk)));
+    if (i == 0) return 0;
+    const int cached = static_cast<int>((static_cast<int64_t>(g.nk) + kTreeUnit - 1) / kTreeUnit);
+    const int tree = min((g.nq - 1) / kTreeUnit + 1, cached / chunks);  // (no chunk but the first is left without keys)
+    const int units = cached + tree, each = units / chunks, more = units - each * chunks;  // (the first `more` have one more)
+    return static_cast<int>(min(static_cast<int64_t>(i * each + min(i, more) - tree) * kTreeUnit, static_cast<int64_t>(g.nk)));
 }
 
 // An item: a row tile and the chunk's keys.
@@ -301,6 +303,9 @@ __device__ __forceinline__ uint64_t tree_bits(const TreeArgs & a, const Tree & g
 // The first `seen` keys of a tile, as bits.
 __device__ __forceinline__ uint64_t first_bits(int seen) { return seen >= 64 ? ~uint64_t(0) : (uint64_t(1) << seen) - 1; }
 
+// A row's floats in LDS: four more than its values, which spreads 32 rows' pieces over the banks.
+constexpr int tree_any_pitch(int dp) { return dp + 4; }
+
 // Any type, head size up to DP, stride and alignment, in fp32 on v_mfma_f32_32x32x2_f32.  The four
 // waves of a workgroup have the same 32 rows and every fourth block of 32 keys each, straight from
 // memory; S^T = K Q^T, so that a lane owns one row and half of its scores, and O^T += V^T P^T.
@@ -310,7 +315,8 @@ template <typename T, int DP, bool WHOLE>
 __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
     constexpr int DT = DP / 32;
     constexpr bool kAhead = DP <= (WHOLE ? 128 : 64);
-    extern __shared__ __align__(16) float tree_smem[];  // [4][32][DP] outputs, [4][32] maxima and sums
+    constexpr int P = tree_any_pitch(DP);
+    extern __shared__ __align__(16) float tree_smem[];  // [4][32][P] outputs, [4][32] maxima and sums
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, r = lane & 31;
@@ -447,13 +453,13 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
             if (w.row0 + i < w.rows) tree_row_alone<T, (DP + 63) / 64>(a, w, w.row0 + i, lane, slot0 + i);
         return;
     }
-    float2 * ml = reinterpret_cast<float2 *>(tree_smem + 4 * 32 * DP);
+    float2 * ml = reinterpret_cast<float2 *>(tree_smem + 4 * 32 * P);
     if (h == 0) ml[wave * 32 + r] = make_float2(m, l);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4 *>(tree_smem + (wave * 32 + r) * DP + dt * 32 + 8 * g + 4 * h) =
+            *reinterpret_cast<float4 *>(tree_smem + (wave * 32 + r) * P + dt * 32 + 8 * g + 4 * h) =
                 make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
     __syncthreads();
     const int jr = tid >> 3;  // 8 threads a row
@@ -474,7 +480,7 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
     for (int c = tid & 7; c < a.d; c += 8) {
         float x = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x += tree_smem[(i * 32 + jr) * DP + c] * f[i];
+        for (int i = 0; i < 4; ++i) x += tree_smem[(i * 32 + jr) * P + c] * f[i];
         if (w.chunks > 1) a.part[(slot0 + jr) * a.d + c] = x;
         else store_f32(o + c, x * inv);
     }
@@ -1002,7 +1008,7 @@ size_t tree_part_rows(int kv_heads, int row_shift) { return static_cast<size_t>(
 
 template <typename T, int DP, bool WHOLE>
 int launch_tree_any(const TreeArgs & a, hipStream_t s) {
-    constexpr int smem = 4 * 32 * DP * 4 + 4 * 32 * 8;
+    constexpr int smem = 4 * 32 * tree_any_pitch(DP) * 4 + 4 * 32 * 8;
     auto kernel = &tree_attn_any_kernel<T, DP, WHOLE>;
     if constexpr (smem > 64 * 1024) {
         static std::atomic<uint64_t> done{0};
