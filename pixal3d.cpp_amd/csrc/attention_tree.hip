@@ -303,18 +303,21 @@ __device__ __forceinline__ uint64_t tree_bits(const TreeArgs & a, const Tree & g
 // The first `seen` keys of a tile, as bits.
 __device__ __forceinline__ uint64_t first_bits(int seen) { return seen >= 64 ? ~uint64_t(0) : (uint64_t(1) << seen) - 1; }
 
+// How heads lie in memory: anywhere, in whole 16-byte pieces, or as such of DP values.
+enum { kAnyRows, kPieceRows, kWholeRows };
 // A row's floats in LDS: four more than its values, which spreads 32 rows' pieces over the banks.
 constexpr int tree_any_pitch(int dp) { return dp + 4; }
 
 // Any type, head size up to DP, stride and alignment, in fp32 on v_mfma_f32_32x32x2_f32.  The four
 // waves of a workgroup have the same 32 rows and every fourth block of 32 keys each, straight from
 // memory; S^T = K Q^T, so that a lane owns one row and half of its scores, and O^T += V^T P^T.
-// Their results are joined through LDS.  WHOLE: head sizes of DP in rows of whole 16-byte pieces.
-// Where the registers hold them, a block's keys and values are loaded while the block before is multiplied.
-template <typename T, int DP, bool WHOLE>
+// Their results are joined through LDS.
+// Where the registers hold them, a block's keys and values are loaded while the block before is multiplied;
+// otherwise q is in LDS and keys and values come a piece ahead of the products.
+template <typename T, int DP, int FORM>
 __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
     constexpr int DT = DP / 32;
-    constexpr bool kAhead = DP <= (WHOLE ? 128 : 64);
+    constexpr bool kAhead = DP <= (FORM == kAnyRows ? 64 : 128);
     constexpr int P = tree_any_pitch(DP);
     extern __shared__ __align__(16) float tree_smem[];  // [4][32][P] outputs, [4][32] maxima and sums
     const int tid = threadIdx.x, lane = tid & 63;
@@ -346,52 +349,69 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
         o.limit = (o.tree ? w.g.nq : w.key1) - o.first;
         return o;
     };
-    // dims h DP/2 .. h DP/2 + DP/2 - 1 of a row; zeros past d
-    auto load_half = [&](const T * p, float (&out)[DP / 2]) __attribute__((always_inline)) {
-        if constexpr (WHOLE) {
+    // Dims h DP/2 + at .. of a row, N of them; zeros past d
+    auto load_part = [&](const T * p, int at, auto & out) __attribute__((always_inline)) {
+        constexpr int N = sizeof(out) / sizeof(float);
+        if constexpr (FORM != kAnyRows) {
             constexpr int V = 16 / static_cast<int>(sizeof(T));
 #pragma unroll
-            for (int u = 0; u < DP / 2 / V; ++u) {
+            for (int u = 0; u < N / V; ++u) {
+                const int dim = h * (DP / 2) + at + V * u;
                 T e[V];
-                __builtin_memcpy(e, __builtin_assume_aligned(p + h * (DP / 2) + V * u, 16), 16);
+                __builtin_memcpy(e, __builtin_assume_aligned(p + (FORM == kWholeRows ? dim : min(dim, a.d - V)), 16), 16);
 #pragma unroll
-                for (int i = 0; i < V; ++i) out[V * u + i] = load_f32(e + i);
+                for (int i = 0; i < V; ++i) out[V * u + i] = FORM == kWholeRows || dim < a.d ? load_f32(e + i) : 0.0f;
             }
         } else {
+            int d = a.d;
+            asm volatile("" : "+s"(d));  // (the comparisons stay here: kept over the loop they cost more registers than there are)
 #pragma unroll
-            for (int i = 0; i < DP / 2; ++i) {
-                const int dim = h * (DP / 2) + i;
-                const float x = load_f32(p + min(dim, a.d - 1));
-                out[i] = dim < a.d ? x : 0.0f;
+            for (int i = 0; i < N; ++i) {
+                const int dim = h * (DP / 2) + at + i;
+                const float x = load_f32(p + min(dim, d - 1));
+                out[i] = dim < d ? x : 0.0f;
             }
         }
     };
-    auto load_k = [&](const Block & o, float (&kk)[DP / 2]) __attribute__((always_inline)) {
+    auto load_k = [&](const Block & o, int at, auto & kk) __attribute__((always_inline)) {
         const int key = o.first + min(r, o.limit - 1);
-        load_half(o.tree ? static_cast<const T *>(a.k) + static_cast<int64_t>(w.g.q0 + key) * a.ldk + col
-                         : static_cast<const T *>(a.kc) + (w.g.k0 + key) * a.ldkc + col, kk);
+        load_part(o.tree ? static_cast<const T *>(a.k) + static_cast<int64_t>(w.g.q0 + key) * a.ldk + col
+                         : static_cast<const T *>(a.kc) + (w.g.k0 + key) * a.ldkc + col, at, kk);
     };
     // Register e of dims dt: key 8 (e / 4) + 4 h + e % 4 of the block, dim 32 dt + r.  (Those of dims past d
     // make outputs that are not stored.)
-    auto load_v = [&](const Block & o, float (&vv)[16][DT]) __attribute__((always_inline)) {
+    auto load_v = [&](const Block & o, int from, auto & vv) __attribute__((always_inline)) {
+        constexpr int N = sizeof(vv) / sizeof(vv[0]);
         const int64_t ldv = o.tree ? a.ldv : a.ldvc;
         const T * v = (o.tree ? static_cast<const T *>(a.v) + static_cast<int64_t>(w.g.q0 + o.first) * ldv
                               : static_cast<const T *>(a.vc) + (w.g.k0 + o.first) * ldv) + col;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int key = 8 * (e >> 2) + 4 * h + (e & 3);
+        for (int e = 0; e < N; ++e) {
+            const int key = 8 * ((from + e) >> 2) + 4 * h + (e & 3);
             const T * p = v + min(key, o.limit - 1) * ldv;
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) vv[e][dt] = load_f32(p + (WHOLE ? dt * 32 + r : min(dt * 32 + r, a.d - 1)));
+            for (int dt = 0; dt < DT; ++dt) vv[e][dt] = load_f32(p + (FORM == kWholeRows ? dt * 32 + r : min(dt * 32 + r, a.d - 1)));
         }
     };
-    float kk[DP / 2], vv[16][DT];
-    if (kAhead && wave < all) {
-        load_k(block(wave), kk);
-        load_v(block(wave), vv);
+    constexpr int KN = kAhead ? DP / 2 : 32, KP = DP / 2 / KN, VN = kAhead ? 16 : 16 / static_cast<int>(sizeof(T)), VP = 16 / VN;
+    float kk[2][KN], vv[2][VN][DT];
+    const T * qrow = static_cast<const T *>(a.q) + (w.g.q0 + qi) * a.ldq + static_cast<int64_t>(head) * a.d;
+    if (wave < all) {
+        load_k(block(wave), 0, kk[0]);
+        if (kAhead) load_v(block(wave), 0, vv[0]);
     }
-    float qv[DP / 2];
-    load_half(static_cast<const T *>(a.q) + (w.g.q0 + qi) * a.ldq + static_cast<int64_t>(head) * a.d, qv);
+    float qv[KN];
+    float * qs = tree_smem + r * P + h * (DP / 2);
+    if (kAhead) {
+        load_part(qrow, 0, qv);
+    } else {
+        for (int u = wave; u < KP; u += 4) {
+            load_part(qrow, KN * u, qv);
+#pragma unroll
+            for (int i = 0; i < KN; i += 4) *reinterpret_cast<float4 *>(qs + KN * u + i) = make_float4(qv[i], qv[i + 1], qv[i + 2], qv[i + 3]);
+        }
+        __syncthreads();
+    }
     f32x16 oacc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
@@ -400,13 +420,25 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
     TreeWalk walk{qi, tree_blocks * 32};
     for (int b = wave; b < all; b += 4) {
         const Block o = block(b);
-        if (!kAhead) load_k(o, kk);
         const uint32_t seen = o.tree ? static_cast<uint32_t>(tree_bits<32>(a, w.g, walk, o.first, lane))
                                      : static_cast<uint32_t>(first_bits(min(o.limit, 32)));
         f32x16 s = {};
 #pragma unroll
-        for (int i = 0; i < DP / 2; ++i) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk[i], qv[i], s, 0, 0, 0);
-        if (kAhead && b + 4 < all) load_k(block(b + 4), kk);
+        for (int u = 0; u < KP; ++u) {
+            if (!kAhead) {
+                if (u + 1 < KP) load_k(o, KN * (u + 1), kk[(u + 1) & 1]);
+                else load_v(o, 0, vv[0]);
+#pragma unroll
+                for (int i = 0; i < KN; i += 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(qs + KN * u + i);
+                    qv[i] = x.x, qv[i + 1] = x.y, qv[i + 2] = x.z, qv[i + 3] = x.w;
+                }
+                asm volatile("" ::: "memory");  // (keeps the pieces' loads from being moved to one place)
+            }
+#pragma unroll
+            for (int i = 0; i < KN; ++i) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk[u & 1][i], qv[i], s, 0, 0, 0);
+        }
+        if (b + 4 < all) load_k(block(b + 4), 0, kk[0]);
         float top = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -430,22 +462,28 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
         }
         l = l * keep + lane_pair_sum(sum);
         m = up;
-        if (!kAhead) load_v(o, vv);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) oacc[dt][e] *= keep;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const bool in = 8 * (e >> 2) + 4 * h + (e & 3) < o.limit;
+        for (int u = 0; u < VP; ++u) {
+            if (u + 1 < VP) {
+                load_v(o, VN * (u + 1), vv[(u + 1) & 1]);
+                asm volatile("" ::: "memory");
+            }
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const float x = in ? vv[e][dt] : 0.0f;
-                odd |= o.tree && !is_finite_bits(x);
-                oacc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[e], oacc[dt], 0, 0, 0);
+            for (int e = VN * u; e < VN * (u + 1); ++e) {
+                const bool in = 8 * (e >> 2) + 4 * h + (e & 3) < o.limit;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const float x = in ? vv[u & 1][e - VN * u][dt] : 0.0f;
+                    odd |= o.tree && !is_finite_bits(x);
+                    oacc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[e], oacc[dt], 0, 0, 0);
+                }
             }
         }
-        if (kAhead && b + 4 < all) load_v(block(b + 4), vv);
+        if (kAhead && b + 4 < all) load_v(block(b + 4), 0, vv[0]);
     }
     const int64_t slot0 = item_rows(a, w);
     if (__syncthreads_or(odd)) {
@@ -1006,16 +1044,23 @@ int64_t tree_slots(int kv_heads) { return 2 * tree_target(kv_heads); }
 size_t tree_table_bytes(int nseg) { return round256((2 * static_cast<size_t>(nseg) + 2) * sizeof(int64_t)); }
 size_t tree_part_rows(int kv_heads, int row_shift) { return static_cast<size_t>(tree_slots(kv_heads)) * kv_heads << row_shift; }
 
-template <typename T, int DP, bool WHOLE>
+template <typename T, int DP, int FORM>
 int launch_tree_any(const TreeArgs & a, hipStream_t s) {
     constexpr int smem = 4 * 32 * tree_any_pitch(DP) * 4 + 4 * 32 * 8;
-    auto kernel = &tree_attn_any_kernel<T, DP, WHOLE>;
+    auto kernel = &tree_attn_any_kernel<T, DP, FORM>;
     if constexpr (smem > 64 * 1024) {
         static std::atomic<uint64_t> done{0};
         if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), smem, done, "hipFuncSetAttribute(tree_attn)")) return rc;
     }
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.items * a.kv_heads)), dim3(256), smem, s, a);
     return check_launch("tree attention");
+}
+
+template <typename T, int FORM>
+int launch_tree_any(const TreeArgs & a, hipStream_t s) {
+    return a.d <= 64    ? launch_tree_any<T, 64, FORM>(a, s)
+           : a.d <= 128 ? launch_tree_any<T, 128, FORM>(a, s)
+                        : launch_tree_any<T, 256, FORM>(a, s);
 }
 
 // kernel<mode of the call>
@@ -1054,14 +1099,8 @@ int run_tree(const TreeArgs & a, bool fast, hipStream_t s) {
     if (fast && a.d == 64) rc = launch_tree_fast<64, true>(a, s);
     else if (fast && a.d == 128) rc = launch_tree_fast<128, true>(a, s);
     else if (fast) rc = a.d < 64 ? launch_tree_fast<64, false>(a, s) : launch_tree_fast<128, false>(a, s);
-    else if (a.vec && (a.d == 64 || a.d == 128 || a.d == 256))
-        rc = a.d == 64    ? launch_tree_any<T, 64, true>(a, s)
-             : a.d == 128 ? launch_tree_any<T, 128, true>(a, s)
-                          : launch_tree_any<T, 256, true>(a, s);
-    else
-        rc = a.d <= 64    ? launch_tree_any<T, 64, false>(a, s)
-             : a.d <= 128 ? launch_tree_any<T, 128, false>(a, s)
-                          : launch_tree_any<T, 256, false>(a, s);
+    else if (a.vec && (a.d == 64 || a.d == 128 || a.d == 256)) rc = launch_tree_any<T, kWholeRows>(a, s);
+    else rc = a.vec ? launch_tree_any<T, kPieceRows>(a, s) : launch_tree_any<T, kAnyRows>(a, s);
     if (rc || a.cache_rows <= kTreeUnit) return rc;  // (no chunk is shorter than a unit)
     if (a.total_q * a.heads >= kJoinRows)
         hipLaunchKernelGGL((tree_join_kernel<T, true>), dim3(static_cast<unsigned>(a.total_q * ((a.heads + 7) / 8))), dim3(256), 0, s, a);
