@@ -55,7 +55,8 @@ struct TreeArgs {
     int64_t slots;             // items with partial results (bound)
     float per_target;          // 1 / (items that the chunks add at most * kTreeUnit)
     int row_shift;             // log2 of a tile's rows
-    float * part;              // [slots * kv_heads << row_shift][d] unnormalised outputs
+    int slot_rows;             // those that one of the call's can have
+    float * part;              // [slots * kv_heads * slot_rows][d] unnormalised outputs
     float2 * part_ml;          // [..] maxima (log2 units) and sums
 };
 
@@ -192,7 +193,7 @@ __device__ __forceinline__ bool locate_query(const TreeArgs & a, int qi, int lan
 
 // The item's rows of partial results.
 __device__ __forceinline__ int64_t item_rows(const TreeArgs & a, const Item & w) {
-    return (static_cast<int64_t>(w.slot) * a.kv_heads + w.kv) << a.row_shift;
+    return (static_cast<int64_t>(w.slot) * a.kv_heads + w.kv) * a.slot_rows;
 }
 
 // The token above token c of the tree whose first row is q0; -1 at the top.
@@ -587,127 +588,8 @@ __device__ __forceinline__ void tree_exact(const TreeArgs & a, const Item & w, c
     }
 }
 
-// Up to 32 rows a tile: a workgroup's two waves take every second key tile of an item each, through rings of
-// their own in LDS, with no barrier before the end, where their results are joined.
-constexpr int kTreeWaves = 2, kTreeStages = 2;  // 64 KB of LDS: two workgroups a CU
-template <int DH> constexpr int kTreeWaveBytes = kTreeStages * 2 * Fast<DH>::kTileBytes;
-template <int DH> constexpr int kTreeFewBytes = kTreeWaves * kTreeWaveBytes<DH> + kTreeWaves * 32 * static_cast<int>(sizeof(float2));
-
-template <int DH, int MODE, bool WHOLE>
-__global__ void __launch_bounds__(kTreeWaves * 64) tree_attn_few_kernel(TreeArgs a) {
-    using F = Fast<DH>;
-    constexpr int kInstr = 2 * F::kUnits;
-    extern __shared__ __align__(16) char tree_lds[];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = lane >> 5, r = lane & 31;
-    Item w;
-    w.kv = static_cast<int>(blockIdx.x % a.kv_heads);
-    if (!locate_item(a, static_cast<int>(blockIdx.x / a.kv_heads), lane, w)) return;
-    TreeSources<DH> src = tree_sources<DH>(a, w);
-    uint32_t off_tree[kInstr], off_cache[kInstr];
-    tile_offsets<DH>(src.tree, a.d, 0, lane, off_tree);
-    tile_offsets<DH>(src.cache, a.d, 0, lane, off_cache);
-    char * ring = tree_lds + wave * kTreeWaveBytes<DH>;
-    const uint32_t lds0 = lds_offset(ring);
-    const int tree_tiles = w.chunk == 0 ? (w.g.nq + F::kKeys - 1) / F::kKeys : 0;
-    const int cache0 = w.key0 / F::kKeys, all = tree_tiles + (w.key1 + F::kKeys - 1) / F::kKeys - cache0;
-    const int n = all > wave ? (all - wave + kTreeWaves - 1) / kTreeWaves : 0;
-    auto slot = [](int i) { return i % kTreeStages * 2 * F::kTileBytes; };
-    auto issue = [&](int i) __attribute__((always_inline)) {
-        const int t = wave + kTreeWaves * i;
-        if (t < tree_tiles) tile_issue<DH, WHOLE>(src.tree, tree_tiles - 1 - t, 0, off_tree, lds0 + slot(i), lane);
-        else tile_issue<DH, WHOLE>(src.cache, cache0 + t - tree_tiles, 0, off_cache, lds0 + slot(i), lane);
-    };
-    if (n > 0) issue(0);
-    TreeRow<DH, MODE> o;
-    load_row<DH, MODE>(a, w, w.row0 + r, h, o);
-    typename F::Out oacc;
-#pragma unroll
-    for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
-    RowState st{-INFINITY, 0.0f};
-    bool odd = false;
-    TreeWalk walk{o.qi, tree_tiles * F::kKeys};
-#pragma unroll
-    for (int i = 1; i < kTreeStages; ++i)
-        if (i < n) issue(i);
-    for (int i = 0; i < n; ++i) {
-        const int t = wave + kTreeWaves * i;
-        const bool tree = t < tree_tiles;
-        const int first = (tree ? tree_tiles - 1 - t : cache0 + t - tree_tiles) * F::kKeys;
-        const uint64_t bits = tree ? tree_bits<F::kKeys>(a, w.g, walk, first, lane) : first_bits(w.key1 - first);
-        wait_stages<kTreeStages - 1, kInstr>(n - 1 - i);
-        asm volatile("" ::: "memory");
-        const char * kl = ring + slot(i);
-        const char * vl = kl + F::kTileBytes;
-        if (tree) odd |= tile_odd<DH>(vl, lane, 64);
-        typename F::Scores s;
-        typename F::Weights p;
-        tile_qk<DH>(kl, o.qf, s, h, r);
-        tree_exact<DH, MODE>(a, w, o, tree, first, bits, h, s, p, oacc, st);
-        tile_pv<DH>(vl, p, oacc, lane);
-        wave_reads_done();
-        if (i + kTreeStages < n) issue(i + kTreeStages);
-    }
-    const int64_t part = item_rows(a, w);
-    if (__syncthreads_or(odd)) {
-        for (int j = wave; j < 32; j += kTreeWaves)
-            if (w.row0 + j < w.rows) tree_row_alone<uint16_t, DH / 64>(a, w, w.row0 + j, lane, part + j);
-        return;
-    }
-    // The waves' results: outputs in their own rings, bases and sums behind the rings.
-    float * mine = reinterpret_cast<float *>(ring);
-    float2 * ml = reinterpret_cast<float2 *>(tree_lds + kTreeWaves * kTreeWaveBytes<DH>);
-    const float sum = lane_pair_sum(st.sum);
-    if (h == 0) ml[wave * 32 + r] = make_float2(st.base, sum);
-#pragma unroll
-    for (int dt = 0; dt < F::NDT; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4 *>(mine + r * DH + dt * 32 + 8 * g + 4 * h) =
-                make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
-    __syncthreads();
-    const int jc = tid & 7;  // 8 threads a row
-#pragma unroll
-    for (int jr = tid >> 3; jr < 32; jr += kTreeWaves * 8) {
-        if (w.row0 + jr >= w.rows) return;
-        float base = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kTreeWaves; ++i) base = fmaxf(base, ml[i * 32 + jr].x);
-        const float ref = base == -INFINITY ? 0.0f : base;
-        float total = 0.0f, f[kTreeWaves];
-#pragma unroll
-        for (int i = 0; i < kTreeWaves; ++i) {
-            const float2 v = ml[i * 32 + jr];
-            f[i] = __builtin_amdgcn_exp2f(v.x - ref);
-            total += v.y * f[i];
-        }
-        const int token = (w.row0 + jr) / a.group;
-        const int to_head = w.kv * a.group + (w.row0 + jr) % a.group;
-        uint16_t * to = static_cast<uint16_t *>(a.o) + (w.g.q0 + token) * a.ldo + static_cast<int64_t>(to_head) * a.d;
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        if (w.chunks > 1 && jc == 0) a.part_ml[part + jr] = make_float2(base, total);
-#pragma unroll
-        for (int c = jc * 4; c < DH; c += 32) {
-            if (!WHOLE && c >= a.d) break;
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < kTreeWaves; ++i) {
-                const float4 x = *reinterpret_cast<const float4 *>(
-                    reinterpret_cast<const float *>(tree_lds + i * kTreeWaveBytes<DH>) + jr * DH + c);
-                v[0] += x.x * f[i]; v[1] += x.y * f[i]; v[2] += x.z * f[i]; v[3] += x.w * f[i];
-            }
-            if (w.chunks > 1)
-                *reinterpret_cast<float4 *>(a.part + (part + jr) * a.d + c) = make_float4(v[0], v[1], v[2], v[3]);
-            else
-                *reinterpret_cast<uint2 *>(to + c) =
-                    make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
-        }
-    }
-}
-
-// More rows: four waves of 32 rows share the key tiles, a ring of four slots of K and V, as the scored attention's
-// kernel of many rows does.  The tree's tiles and the cache's last, which may end inside, are exact steps
+// Four waves of 32 rows share the key tiles, a ring of four slots of K and V, as the scored attention's kernel of many
+// rows does.  The tree's tiles and the cache's last, which may end inside, are exact steps
 // (maximum, weights, product), and one whole tile after them, so that every row has a base that one of its own
 // scores set.  From there on a step issues the products that do not depend on its weights, O += V P of the tile before
 // and S of the next, and takes its weights while they run, without a maximum: a row's are redone with one
@@ -912,7 +794,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a) {
     if (w.slot + static_cast<int64_t>(tiles) * w.chunks > a.slots) return;  // (of bounds that fall: no such items)
     w.slot += row >> a.row_shift;
     const int64_t at = item_rows(a, w) + (row & ((1 << a.row_shift) - 1));
-    const int64_t step = static_cast<int64_t>(tiles) * a.kv_heads << a.row_shift;
+    const int64_t step = static_cast<int64_t>(tiles) * a.kv_heads * a.slot_rows;
     const bool whole = (a.d & 3) == 0;
     float m = -INFINITY, l = 0.0f, acc[kParts][4] = {};
 #pragma unroll 4
@@ -1026,7 +908,6 @@ constexpr int kTreeMaxDim = 256;
 constexpr int64_t kTreeMaxRows = INT32_MAX - 1023;  // rows and keys are counted in 32 bits, a tile past their end
 constexpr int kWaveSegments = 64;
 constexpr int64_t kJoinRows = 4096;     // (query, head) rows whose chunks a group of lanes joins alone
-constexpr int64_t kFewTreeRows = 32;  // rows a segment has on average in calls of tiles of 32
 // Workgroups that chunks past the first add at most: one round of the fast kernels' two a CU (eight trees of
 // 64 over 8,192 keys 109 us, with 384 121, with 768 135; eight trees over caches of 0 to 40,001 98, with 320
 // 108, with 1,024 104; 64 of 8 over 4,096 207, 209 and 221).
@@ -1042,7 +923,8 @@ int64_t tree_items(int nseg, int64_t total_q, int kv_heads, int group, int row_s
 // Those with partial results: a segment of len keys in more chunks than one has at most 2 len / chunk.
 int64_t tree_slots(int kv_heads) { return 2 * tree_target(kv_heads); }
 size_t tree_table_bytes(int nseg) { return round256((2 * static_cast<size_t>(nseg) + 2) * sizeof(int64_t)); }
-size_t tree_part_rows(int kv_heads, int row_shift) { return static_cast<size_t>(tree_slots(kv_heads)) * kv_heads << row_shift; }
+int tree_slot_rows(int64_t rows, int row_shift) { return static_cast<int>(std::min<int64_t>(rows, int64_t(1) << row_shift)); }
+size_t tree_part_rows(int kv_heads, int slot_rows) { return static_cast<size_t>(tree_slots(kv_heads)) * kv_heads * slot_rows; }
 
 template <typename T, int DP, int FORM>
 int launch_tree_any(const TreeArgs & a, hipStream_t s) {
@@ -1080,16 +962,8 @@ int launch_tree_fast(const TreeArgs & a, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(a.items * a.kv_heads));
     return with_tree_mode(a, [&](auto mode) {
         constexpr int kMode = decltype(mode)::value;
-        if (a.row_shift == 7) {
-            hipLaunchKernelGGL((tree_attn_rows_kernel<DH, kMode, WHOLE>), grid, dim3(256), 0, s, a);
-            return check_launch("tree attention of many rows");
-        }
-        auto kernel = &tree_attn_few_kernel<DH, kMode, WHOLE>;
-        static std::atomic<uint64_t> done{0};
-        if (int rc = allow_lds(reinterpret_cast<const void *>(kernel), kTreeFewBytes<DH>, done, "hipFuncSetAttribute(tree_attn_few)"))
-            return rc;
-        hipLaunchKernelGGL(kernel, grid, dim3(kTreeWaves * 64), kTreeFewBytes<DH>, s, a);
-        return check_launch("tree attention of few rows");
+        hipLaunchKernelGGL((tree_attn_rows_kernel<DH, kMode, WHOLE>), grid, dim3(256), 0, s, a);
+        return check_launch("tree attention");
     });
 }
 
@@ -1122,7 +996,8 @@ extern "C" {
 
 size_t pxs_tree_attention_workspace_bytes(int nseg, int64_t total_q, int heads, int kv_heads, int head_dim) {
     if (nseg <= 0 || total_q <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 256;
-    const size_t rows = tree_part_rows(kv_heads, 7);
+    const int64_t group = (heads - 1) / kv_heads + 1;
+    const size_t rows = tree_part_rows(kv_heads, tree_slot_rows(std::min<int64_t>(total_q, 128) * group, 7));  // (fp32's are fewer)
     return tree_table_bytes(nseg) + round256(rows * sizeof(float2)) + round256(rows * head_dim * sizeof(float));
 }
 
@@ -1169,8 +1044,9 @@ int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, 
     const bool fast = dtype == PXS_BF16 && head_dim <= 128 && a.vec && ld_k < (1 << 24) && ld_v < (1 << 24) &&
                       (cache_rows == 0 || (ld_k_cache < (1 << 24) && ld_v_cache < (1 << 24))) &&
                       reinterpret_cast<uintptr_t>(o) % 8 == 0 && ld_o % 4 == 0;
-    a.row_shift = fast && total_q * a.group > kFewTreeRows * nseg ? 7 : 5;
+    a.row_shift = fast ? 7 : 5;
     a.items = tree_items(nseg, total_q, kv_heads, a.group, a.row_shift);
+    a.slot_rows = tree_slot_rows(total_q * a.group, a.row_shift);
     a.slots = tree_slots(kv_heads);
     a.per_target = 1.0f / static_cast<float>(tree_target(kv_heads) * kTreeUnit);
     PXS_CHECK(a.items * kv_heads <= UINT32_MAX / 256 && total_q * heads <= UINT32_MAX / 256, PXS_ERR_ARG,
@@ -1182,7 +1058,7 @@ int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, 
         if (int rc = check_launch("tree attention table")) return rc;
     }
     ws += tree_table_bytes(nseg);
-    const size_t rows = tree_part_rows(kv_heads, a.row_shift);
+    const size_t rows = tree_part_rows(kv_heads, a.slot_rows);
     a.part_ml = reinterpret_cast<float2 *>(ws);
     a.part = reinterpret_cast<float *>(ws + round256(rows * sizeof(float2)));
     return dtype == PXS_F32 ? run_tree<float>(a, false, s) : run_tree<uint16_t>(a, fast, s);
