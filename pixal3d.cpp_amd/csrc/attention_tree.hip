@@ -312,7 +312,9 @@ constexpr int tree_any_pitch(int dp) { return dp + 4; }
 // Any type, head size up to DP, stride and alignment, in fp32 on v_mfma_f32_32x32x2_f32.  The four
 // waves of a workgroup have the same 32 rows and every fourth block of 32 keys each, straight from
 // memory; S^T = K Q^T, so that a lane owns one row and half of its scores, and O^T += V^T P^T.
-// Their results are joined through LDS.
+// Their results are joined through LDS.  The products bound it where rows are many (32,000 keys for 128 tokens of 16
+// heads of 64 in 44 us, 2.9 TB/s; a block of 32 keys is 1.75 us of a wave's products), the way from the
+// lengths to the first loads, and the joins, where they are few (37 and 100 tokens over 2,370 and 517 keys 26 us).
 // Where the registers hold them, a block's keys and values are loaded while the block before is multiplied;
 // otherwise q is in LDS and keys and values come a piece ahead of the products.
 template <typename T, int DP, int FORM>
@@ -594,7 +596,9 @@ __device__ __forceinline__ void tree_exact(const TreeArgs & a, const Item & w, c
 // scores set.  From there on a step issues the products that do not depend on its weights, O += V P of the tile before
 // and S of the next, and takes its weights while they run, without a maximum: a row's are redone with one
 // where their sum passes 2^40, and an item whose outputs pass 2^118 is walked again with exact steps alone.
-// Waves past the segment's rows only help to load.
+// Waves past the segment's rows only help to load: with one row or 32 the cache's bytes bound it (eight caches of
+// 32,768 keys, one token each, 5.2 TB/s; two waves a workgroup with a ring of their own were 2 to 9% slower from
+// one row to 64), with 256 a segment the products and the weights' exponentials (620 TFLOP/s, 515 with a cap).
 template <int DH, int MODE, bool WHOLE>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) tree_attn_rows_kernel(TreeArgs a) {
     using F = Fast<DH>;
@@ -907,10 +911,13 @@ __global__ void __launch_bounds__(1024) tree_table_kernel(TreeArgs a, int64_t * 
 constexpr int kTreeMaxDim = 256;
 constexpr int64_t kTreeMaxRows = INT32_MAX - 1023;  // rows and keys are counted in 32 bits, a tile past their end
 constexpr int kWaveSegments = 64;
-constexpr int64_t kJoinRows = 4096;     // (query, head) rows whose chunks a group of lanes joins alone
-// Workgroups that chunks past the first add at most: one round of the fast kernels' two a CU (eight trees of
-// 64 over 8,192 keys 109 us, with 384 121, with 768 135; eight trees over caches of 0 to 40,001 98, with 320
-// 108, with 1,024 104; 64 of 8 over 4,096 207, 209 and 221).
+// (query, head) rows from which a group of lanes joins one alone: many rows have few chunks each.  16,384 rows of 4
+// chunks 110 us with the attention, a workgroup a row 125; 4,096 of 8 68 and 71; 192 of 12 17.7 and 15.0; 1,024 of
+// 64 55 and 49.
+constexpr int64_t kJoinRows = 4096;
+// Workgroups that chunks past the first add at most: one round of the kernels' two a CU (eight trees of 64 over
+// 8,192 keys 112 us, with 384 119, with 768 133, with 1,024 126; eight trees over caches of 0 to 40,001 keys 93, 97,
+// 106 and 100; 64 of 8 over 4,096 198, 198, 220 and 221; in fp32 eight of 16 over 4,000 51, 57, 63 and 58).
 constexpr int64_t kTreeItems = 512;
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
