@@ -718,9 +718,8 @@ constexpr MxShape kMxShapes[] = {
     {64, 64, 4, 6.0, 2.2, 1.9, 2.0},      {32, 64, 2, 6.1, 1.5, 3.0, 1.9},
 };
 
-int mx_shape(int64_t m, int n, int blocks) {
+int mx_shape(int64_t m, int n, int blocks, double & least) {
     int best = 0;
-    double least = 0.0;
     for (int i = 0; i < static_cast<int>(std::size(kMxShapes)); ++i) {
         const MxShape & c = kMxShapes[i];
         const double deep = blocks / 64.0, alone = c.alone0 + c.alone1 * deep, each = c.each0 + c.each1 * deep;
@@ -735,8 +734,11 @@ int mx_shape(int64_t m, int n, int blocks) {
     return best;
 }
 
-// Up to kMxFewRows rows: 16 output channels a workgroup, and as few of its 16-row blocks as
-// keep the workgroups near one a CU.
+// Up to kMxFewRows rows a workgroup may have 16 output channels and as few of the rows' 16-row blocks as keep the
+// workgroups near one a CU, straight from memory.  Its time is its launch's and that of the codes that a CU
+// loads, 24 KB a us (within 10% of the measured at 32 sizes of 1 to 64 rows), and it is taken where that is
+// less than the tiles': 1 x 1024 -> 4096 4.8 us against 6.2, 16 x 4096 -> 4096 7.0 and 9.1, 16 x 4096 -> 14336 15.2
+// and 10.9, 64 x 8192 -> 1024 9.5 and 12.1, 64 x 4096 -> 4096 11.5 and 9.4.
 constexpr int64_t kMxFewRows = 64;
 
 // What a call runs on: its tile of rows by output channels, and its stages of K in LDS by DMA; 0
@@ -745,13 +747,16 @@ struct MxPlan {
     int bm, bn, stages;
 };
 MxPlan mx_plan(int64_t m, int n, int blocks) {
+    double tiles = 0.0;
+    const MxShape & c = kMxShapes[mx_shape(m, n, blocks, tiles)];
     if (m <= kMxFewRows) {
-        const int64_t groups = (n + 15) / 16 * ((m + 15) / 16);
-        if (groups <= 256 || m <= 16) return {16, 16, 0};
-        if (groups <= 512 || m <= 32) return {32, 16, 0};
-        return {64, 16, 0};
+        const int64_t columns = (n + 15) / 16, row_blocks = (m + 15) / 16;
+        const int rb = columns * row_blocks <= 256 || m <= 16 ? 1 : columns * row_blocks <= 512 || m <= 32 ? 2 : 4;
+        const int64_t workgroups = columns * ((row_blocks + rb - 1) / rb);
+        const int64_t rows = 16 + std::min<int64_t>(16 * rb, m);  // of codes that one loads, its channels' and its rows'
+        const double few = 4.3 + 0.042 * static_cast<double>((workgroups + 255) / 256 * rows) * blocks / 64.0;
+        if (few < tiles) return {16 * rb, 16, 0};
     }
-    const MxShape & c = kMxShapes[mx_shape(m, n, blocks)];
     return {c.bm, c.bn, c.stages};
 }
 

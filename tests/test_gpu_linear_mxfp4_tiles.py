@@ -17,7 +17,10 @@ from test_gpu_linear_mxfp4 import BF16, F32, gpu, random_codes, values
 
 # rows, cin, cout, (tile rows, channels, stages of K)
 SIZES = [
-    (5, 4240, 33, (16, 16, 0)), (32, 144, 4100, (32, 16, 0)), (40, 400, 2810, (64, 16, 0)), (64, 2000, 5000, (64, 16, 0)),
+    (5, 4240, 33, (16, 16, 0)), (32, 144, 4100, (32, 16, 0)), (40, 400, 2810, (64, 16, 0)), (64, 1400, 2810, (64, 16, 0)),
+    # few rows of many channels
+    (1, 4096, 14336, (32, 64, 2)), (16, 2000, 16000, (32, 64, 2)), (16, 1025, 20000, (64, 64, 4)),
+    (33, 2000, 5001, (32, 64, 2)), (64, 2000, 5000, (32, 64, 2)),
     # four groups take every fourth 256 of K
     (66, 305, 100, (32, 64, 2)), (65, 544, 100, (32, 64, 2)), (65, 774, 100, (32, 64, 2)), (67, 1025, 100, (32, 64, 2)),
     (66, 1281, 100, (32, 64, 2)), (65, 1589, 100, (32, 64, 2)), (67, 1808, 260, (32, 64, 2)), (67, 2116, 101, (32, 64, 2)),
