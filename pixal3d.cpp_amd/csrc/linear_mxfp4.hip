@@ -363,17 +363,35 @@ __global__ void __launch_bounds__(kFewWaves * 64) linear_mxfp4_few_kernel(MxArgs
 // Row pitch in LDS of 32 rows of a wave's block, and 16 bytes against bank conflicts.
 template <typename T, int WN> constexpr int mx_pitch() { return WN * static_cast<int>(sizeof(T)) + 16; }
 
+// The gates of K channels from c, kept from a row to the next of its batch item.
+template <int K> struct MxGates {
+    int batch = -1;
+    float g[K];
+    __device__ __forceinline__ void to(const MxArgs & a, int item, int c) {
+        if (item == batch) return;
+        batch = item;
+        const float * bm = a.block_mod + a.gate_offset;
+        const float * tm = a.time_mod + static_cast<int64_t>(item) * 6 * a.n + a.gate_offset;
+#pragma unroll
+        for (int e = 0; e < K; ++e) {
+            const int ce = min(c + e, a.n - 1);
+            g[e] = bm[ce] + tm[ce];
+        }
+    }
+};
+
 // One wave's block of outputs: acc[i][j] holds 32 rows by 32 channels, lane (h, r) row r and
-// channels 8 g + 4 h + e.  Stores go through the wave's region of LDS (which no other wave uses
-// any more), 32 rows at a time, so that an instruction covers row segments of 64 bytes and more, and
-// past the caches: what reads y next runs on other XCDs (8,192 x 8192 -> 4096 155 -> 148 us, 1,370 x 1024 -> 4096
-// 12.6 -> 11.5).
+// channels 8 g + 4 h + e.  Values go through the wave's region of LDS (which no other wave uses
+// any more), 32 rows at a time, so that an instruction covers row segments of 64 bytes and more.  Stores
+// pass the caches by: what reads y next runs on other XCDs (8,192 x 8192 -> 4096 155 -> 148 us, 1,370 x 1024 -> 4096
+// 12.6 -> 11.5).  A residual's values are loaded ahead of the block's (into one, 42,017 x 4096 -> 1024 214 -> 166 us).
 template <typename T, int TI, int TJ, int EPI>
 __device__ __forceinline__ void mx_tile_out(const MxArgs & a, const f32x16 (&acc)[TI][TJ], char * region, int64_t row0,
                                             int col0, int h, int r, int lane) {
     constexpr int WN = TJ * 32, kPitch = mx_pitch<T, WN>(), kElems = 16 / static_cast<int>(sizeof(T));
-    constexpr int kLanesPerRow = WN / kElems, kRowsPerPass = 64 / kLanesPerRow;
-    constexpr bool staged = EPI == kMxStore;
+    constexpr int kLanesPerRow = WN / kElems, kRowsPerPass = 64 / kLanesPerRow, kPasses = 32 / kRowsPerPass;
+    constexpr bool kAdds = EPI != kMxStore;
+    static_assert(!kAdds || sizeof(T) == 4, "residuals are fp32");
     auto bias = [&](int j, int g) __attribute__((always_inline)) {
         const int c = min(col0 + j * 32 + 8 * g + 4 * h, a.n - 1);
         return mx_bias(a, c, a.vec_out && c + 3 < a.n);
@@ -383,45 +401,68 @@ __device__ __forceinline__ void mx_tile_out(const MxArgs & a, const f32x16 (&acc
     for (int j = 0; j < TJ; ++j)
 #pragma unroll
         for (int g = 0; g < 4; ++g) held[j][g] = bias(j, g);
+    const int lr = lane / kLanesPerRow, lc = lane % kLanesPerRow, c16 = col0 + lc * kElems;
+    static_assert(64 % WN == 0, "a lane's elements are of one channel");
+    MxGates<4> gates;
+    MxGates<1> gate;
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
-        const int64_t row = row0 + i * 32 + r;
-        const int batch = EPI == kMxGate && row < a.m ? a.coords[row * 4] : 0;
+        const int64_t block = row0 + i * 32;
+        float4 old[kAdds ? kPasses : 1];
+        int batch[EPI == kMxGate ? kPasses : 1];
+        if (kAdds && a.vec_out == 2) {
+#pragma unroll
+            for (int pass = 0; pass < kPasses; ++pass) {
+                const int64_t to = min(block + pass * kRowsPerPass + lr, a.m - 1);
+                old[kAdds ? pass : 0] = *reinterpret_cast<const float4 *>(a.residual + to * a.n + min(c16, a.n - 4));
+                if (EPI == kMxGate) batch[EPI == kMxGate ? pass : 0] = a.coords[to * 4];
+            }
+        }
 #pragma unroll
         for (int j = 0; j < TJ; ++j)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int cl = j * 32 + 8 * g + 4 * h, c = col0 + cl;
                 const float sum[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                const MxBias & b = held[j][g];
-                if constexpr (staged) {
-                    float v[4];
-                    mx_values4(a, b, sum, v);  // (past n: not stored)
-                    mx_put4(reinterpret_cast<T *>(region + r * kPitch + cl * static_cast<int>(sizeof(T))), v);
-                } else if (row < a.m && c < a.n) {
-                    mx_epilogue4<T, EPI>(a, b, row, batch, c, sum);
+                float v[4];
+                mx_values4(a, held[j][g], sum, v);  // (past n: not stored)
+                mx_put4(reinterpret_cast<T *>(region + r * kPitch + (j * 32 + 8 * g + 4 * h) * static_cast<int>(sizeof(T))), v);
+            }
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own writes
+        if (a.vec_out != 2) {  // an element a lane, in the order of their addresses
+#pragma unroll 8
+            for (int pass = 0; pass < 32 * WN / 64; ++pass) {
+                const int rl = (pass * 64 + lane) / WN, cl = (pass * 64 + lane) % WN;
+                const T v = *reinterpret_cast<const T *>(region + rl * kPitch + cl * static_cast<int>(sizeof(T)));
+                const int64_t to = block + rl;
+                const int c = col0 + cl;
+                if (to < a.m && c < a.n) {
+                    if constexpr (kAdds) {
+                        if constexpr (EPI == kMxGate) gate.to(a, a.coords[to * 4], c);
+                        a.residual[to * a.n + c] += EPI == kMxGate ? v * gate.g[0] : v;
+                    } else {
+                        static_cast<T *>(a.y)[to * a.n + c] = v;
+                    }
                 }
             }
-        if constexpr (staged) {
-            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own writes
-            if (a.vec_out != 2) {  // an element a lane, in the order of their addresses
-#pragma unroll 2
-                for (int pass = 0; pass < 32 * WN / 64; ++pass) {
-                    const int rl = (pass * 64 + lane) / WN, cl = (pass * 64 + lane) % WN;
-                    const T v = *reinterpret_cast<const T *>(region + rl * kPitch + cl * static_cast<int>(sizeof(T)));
-                    const int64_t to = row0 + i * 32 + rl;
-                    if (to < a.m && col0 + cl < a.n) static_cast<T *>(a.y)[to * a.n + col0 + cl] = v;
-                }
-                continue;
-            }
-            const int lr = lane / kLanesPerRow, lc = lane % kLanesPerRow;
+            continue;
+        }
 #pragma unroll
-            for (int pass = 0; pass < 32 / kRowsPerPass; ++pass) {
-                const int rl = pass * kRowsPerPass + lr;
-                const uint4 v = *reinterpret_cast<const uint4 *>(region + rl * kPitch + lc * 16);
-                const int64_t to = row0 + i * 32 + rl;
-                const int c = col0 + lc * kElems;
-                if (to < a.m && c < a.n) store16_past(static_cast<T *>(a.y) + to * a.n + c, &v);
+        for (int pass = 0; pass < kPasses; ++pass) {
+            const int rl = pass * kRowsPerPass + lr;
+            uint4 v = *reinterpret_cast<const uint4 *>(region + rl * kPitch + lc * 16);
+            const int64_t to = block + rl;
+            if (to < a.m && c16 < a.n) {
+                if constexpr (kAdds) {
+                    float4 f = __builtin_bit_cast(float4, v), & o = old[pass];
+                    if constexpr (EPI == kMxGate) {
+                        gates.to(a, batch[pass], c16);
+                        f.x *= gates.g[0]; f.y *= gates.g[1]; f.z *= gates.g[2]; f.w *= gates.g[3];
+                    }
+                    o.x += f.x; o.y += f.y; o.z += f.z; o.w += f.w;
+                    *reinterpret_cast<float4 *>(a.residual + to * a.n + c16) = o;
+                } else {
+                    store16_past(static_cast<T *>(a.y) + to * a.n + c16, &v);
+                }
             }
         }
     }
