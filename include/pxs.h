@@ -506,7 +506,7 @@ int pxs_mh_rms_norm(int dtype, const void * x, int64_t ld_x, int64_t rows, int h
  *     all finite scale NaN and zeros.
  * x has rows of stride ld_x, its type and the residual's are independent;
  * gamma (fp32 [channels]) may be NULL: ones.  eps is positive.  y, q and scales
- * must not overlap the inputs. */
+ * must not overlap the inputs, nor residual_out x, nor a residual that it is not. */
 int pxs_rms_norm(int x_dtype, const void * x, int64_t ld_x, int residual_dtype,
                  const void * residual, void * residual_out, int64_t rows, int channels, float eps,
                  const float * gamma, int y_dtype, void * y, void * stream);
@@ -663,13 +663,13 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
  *     |distance of the positions|: a cached key's is its place in the sequence, a
  *     token's positions[row] (device int32 [total_q], needed with slopes).
  * The cache is read only: rows of k and v that are accepted are appended by the
- * caller.  total_q = cu_q[nseg]; rows of q and o behind the last segment are
- * neither read nor written.  cache_rows is the cache's size in rows; total_q *
+ * caller, and o overlaps no input.  total_q is at least cu_q[nseg]; rows of q
+ * and o behind the last segment are neither read nor written.  cache_rows is the cache's size in rows; total_q *
  * heads / kv_heads and cache_rows are at most 2^31 - 1024.  Bounds past the rows
  * are cut to them.  The lengths are read on the device alone: a captured call
  * follows cache_start and cache_len as they change.  bf16 with head_dim a
  * multiple of 8 up to 128 (64 and 128 best), 16-byte-aligned q, k, v and caches,
- * and strides that are multiples of 8 takes the fastest kernels.  The same call
+ * and strides that are multiples of 8 below 2^24 takes the fastest kernels.  The same call
  * gives the same bits; its last bits depend on all its lengths.
  * workspace: pxs_tree_attention_workspace_bytes of the same sizes; calls that
  * may overlap need one each. */

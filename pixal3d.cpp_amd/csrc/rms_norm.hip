@@ -252,6 +252,10 @@ __global__ void __launch_bounds__(norm_threads(WPR)) rms_norm_rows_kernel(NormAr
     }
 }
 
+// Waves a row: as few as hold it in 16 values a lane or less, one up to 1024 channels (42,017 x 512 48 us, with four
+// 65; 1 x 1024 4.7 and 7.4), four to 2048 (4,739 x 1370 17.2, with one 21.7), eight to 8192 (10,000 x 4096 86, with
+// four 88, with sixteen 127; 15,000 x 2600 88, 94 and 182; 5,000 x 8192 89, 91 and 88), sixteen to 16,384
+// (2,500 x 16,384 102, a value at a time 197).
 template <typename XT, typename RT, bool Q>
 int launch_norm(const NormArgs & a, hipStream_t s) {
     const int64_t one = (a.rows + 3) / 4;
@@ -261,8 +265,8 @@ int launch_norm(const NormArgs & a, hipStream_t s) {
     if (a.channels <= 512) launch(rms_norm_rows_kernel<XT, RT, Q, 1, 1>, one);
     else if (a.channels <= 1024) launch(rms_norm_rows_kernel<XT, RT, Q, 1, 2>, one);
     else if (a.channels <= 2048) launch(rms_norm_rows_kernel<XT, RT, Q, 4, 1>, a.rows);
-    else if (a.channels <= 4096) launch(rms_norm_rows_kernel<XT, RT, Q, 4, 2>, a.rows);
-    else if (a.channels <= 8192) launch(rms_norm_rows_kernel<XT, RT, Q, 4, 4>, a.rows);
+    else if (a.channels <= 4096) launch(rms_norm_rows_kernel<XT, RT, Q, 8, 1>, a.rows, norm_threads(8));
+    else if (a.channels <= 8192) launch(rms_norm_rows_kernel<XT, RT, Q, 8, 2>, a.rows, norm_threads(8));
     else if (a.channels <= 16384) launch(rms_norm_rows_kernel<XT, RT, Q, 16, 2>, a.rows, norm_threads(16));
     else launch(rms_norm_any_kernel<XT, RT, Q>, a.rows);
     return check_launch("RMS norm");
