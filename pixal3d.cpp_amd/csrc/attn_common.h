@@ -1,5 +1,5 @@
-// Shared by the attention kernels (attention.hip, attention_scores.hip): the
-// segment of a tile, the LDS layouts of K and V tiles, and sums and maxima over
+// Shared by the attention kernels (attention.hip, attention_scores.hip,
+// attention_tree.hip): the segment of a tile, the LDS layouts of K and V tiles, and sums and maxima over
 // the two lanes that share a query.
 #pragma once
 

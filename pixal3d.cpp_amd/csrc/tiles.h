@@ -1,4 +1,4 @@
-// Shared by the dense products (dense.hip, linear_i8.hip): the order of output
+// Shared by the dense products (dense.hip, linear_i8.hip, linear_mxfp4.hip): the order of output
 // tiles, the swizzle of K chunks in LDS, and the wait for their stages.
 #pragma once
 
