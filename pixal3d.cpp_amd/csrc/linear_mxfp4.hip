@@ -429,20 +429,38 @@ __device__ __forceinline__ void mx_tile_out(const MxArgs & a, const f32x16 (&acc
             }
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own writes
         if (a.vec_out != 2) {  // an element a lane, in the order of their addresses
-#pragma unroll 8
-            for (int pass = 0; pass < 32 * WN / 64; ++pass) {
-                const int rl = (pass * 64 + lane) / WN, cl = (pass * 64 + lane) % WN;
-                const T v = *reinterpret_cast<const T *>(region + rl * kPitch + cl * static_cast<int>(sizeof(T)));
-                const int64_t to = block + rl;
-                const int c = col0 + cl;
-                if (to < a.m && c < a.n) {
-                    if constexpr (kAdds) {
-                        if constexpr (EPI == kMxGate) gate.to(a, a.coords[to * 4], c);
-                        a.residual[to * a.n + c] += EPI == kMxGate ? v * gate.g[0] : v;
-                    } else {
-                        static_cast<T *>(a.y)[to * a.n + c] = v;
-                    }
+            constexpr int kStep = 64 / WN;  // rows of a pass
+            const int rl = lane / WN, cl = lane % WN, c = col0 + cl;
+            const int64_t left = c < a.n ? a.m - block - rl : 0;
+            const char * from = region + rl * kPitch + cl * static_cast<int>(sizeof(T));
+            T * to = static_cast<T *>(kAdds ? static_cast<void *>(a.residual) : a.y) + (block + rl) * a.n + c;
+            const int64_t step = static_cast<int64_t>(kStep) * a.n;
+#pragma unroll
+            for (int first = 0; first < 32; first += 8 * kStep) {
+                T v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const T *>(from + (first + u * kStep) * kPitch);
+                if constexpr (kAdds) {
+                    float o[8];
+                    int item[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        if (first + u * kStep < left) {
+                            o[u] = to[u * step];
+                            item[u] = EPI == kMxGate ? a.coords[(block + rl + first + u * kStep) * 4] : 0;
+                        }
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        if (first + u * kStep < left) {
+                            if constexpr (EPI == kMxGate) gate.to(a, item[u], c);
+                            to[u * step] = o[u] + (EPI == kMxGate ? v[u] * gate.g[0] : v[u]);
+                        }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        if (first + u * kStep < left) to[u * step] = v[u];
                 }
+                to += 8 * step;
             }
             continue;
         }
