@@ -661,7 +661,8 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
  *   Heads, head sizes, scale and cap: as pxs_varlen_attention_scores.
  *   slopes (device fp32 [heads], may be NULL) lowers a score by slopes[head] *
  *     |distance of the positions|: a cached key's is its place in the sequence, a
- *     token's positions[row] (device int32 [total_q], needed with slopes).
+ *     token's positions[row] (device int32 [total_q], 0 or more, needed with
+ *     slopes).
  * The cache is read only: rows of k and v that are accepted are appended by the
  * caller, and o overlaps no input.  total_q is at least cu_q[nseg]; rows of q
  * and o behind the last segment are neither read nor written.  cache_rows is the cache's size in rows; total_q *

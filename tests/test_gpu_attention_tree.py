@@ -174,6 +174,14 @@ def test_one_token(px, dtype, heads, kv):
         run_case(px, [1], [n], heads, kv, 64, dtype, 4 + n)
 
 
+@pytest.mark.parametrize("dtype,d", [(F32, 64), (F32, 130), (BF16, 64), (BF16, 128), (BF16, 72), (BF16, 33)])
+def test_no_cache_at_all(px, dtype, d):
+    """Caches of no rows (null pointers), and trees of no tokens between others."""
+    b = Batch([3, 0, 70], [0, 0, 0], 4, 2, d, dtype, 11)
+    b.kc, b.vc = (torch.empty((0, b.kv * d), dtype=dtype, device="cuda") for _ in range(2))
+    check(b.run(px), *b.want(), "no cache")
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_many_sequences(px, dtype):
     """More than a wave holds: the items come from a table."""
@@ -299,6 +307,13 @@ def test_rows_past_2_31_elements(px):
     one = lambda c, s: px.tree_attention(q, k, v, cu, par, c[:, :kv * d], c[:, kv * d:], torch.tensor([s], device="cuda"),  # noqa: E731
                                          torch.tensor([n], device="cuda"), 32, kv, d, 0.05)
     assert torch.equal(one(cache, at), one(cache[at:].clone(), 0))
+
+
+@pytest.mark.parametrize("dtype,d", [(F32, 64), (F32, 96), (F32, 160), (F32, 256), (F32, 99), (F32, 201), (BF16, 64), (BF16, 120),
+                                     (BF16, 256), (BF16, 99), (BF16, 131)])
+def test_long_trees_beside_short_caches(px, dtype, d):
+    """Trees of more tokens than a chunk has keys; chunks of unequal shares, rows of several tiles."""
+    run_case(px, [400, 1, 140], [1300, 2600, 257], 2, 1, d, dtype, 12, cap=30.0, bias=True)
 
 
 def test_same_call_same_bits_and_single_tokens_meet_the_scored_attention(px):
