@@ -53,14 +53,14 @@ struct TreeArgs {
     int vec;                   // rows of q, k and v in whole 16-byte pieces
     int64_t items;             // launched (bound)
     int64_t slots;             // items with partial results (bound)
-    float per_target;          // 1 / (items that the chunks add at most * kTreeUnit)
+    float per_target;          // 1 / (items that the chunks add at most * 2 kTreeUnit)
     int row_shift;             // log2 of a tile's rows
     int slot_rows;             // those that one of the call's can have
     float * part;              // [slots * kv_heads * slot_rows][d] unnormalised outputs
     float2 * part_ml;          // [..] maxima (log2 units) and sums
 };
 
-constexpr int kTreeUnit = 128;  // keys that a chunk is a multiple of
+constexpr int kTreeUnit = 64;  // keys that a chunk starts at a multiple of, a tile's
 
 // A segment's queries and cached rows, kept within the call's whatever the bounds hold.
 struct Tree {
@@ -77,12 +77,14 @@ __device__ __forceinline__ Tree load_tree(const TreeArgs & a, int s) {
 __device__ __forceinline__ int row_tiles_of(const TreeArgs & a, const Tree & g) {
     return static_cast<int>((static_cast<int64_t>(g.nq) * a.group + (1 << a.row_shift) - 1) >> a.row_shift);
 }
-// Keys of a chunk, from the sum of row tiles times cached keys: `work` of them over the
-// target's items, and one unit more, so that the chunks past a tile's first are at most the target.
+// Keys of a chunk, from the sum of row tiles times cached keys: `work` of them over the target's items, and
+// so much more that the chunks past a tile's first are at most the target: to the next multiple of two units (of
+// one: eight caches of 0 to 40,001 keys 126 us, 92 so), or one unit where that is enough (12 tokens over 1,501
+// keys 13.7 us, with two 14.3; one over 300 12.0 and 13.1).
 // (Rounded sums of it: they are the same in every wave, and off by so little that the target, at most 512, holds.)
 __device__ __forceinline__ int chunk_of(const TreeArgs & a, float work) {
-    const float units = floorf(work * a.per_target) + 1.0f, most = static_cast<float>(a.cache_rows / kTreeUnit + 1);
-    return static_cast<int>(fminf(units, most)) * kTreeUnit;
+    const float pairs = floorf(work * a.per_target) + 1.0f, most = static_cast<float>(a.cache_rows / (2 * kTreeUnit) + 1);
+    return work * a.per_target <= 0.5f ? kTreeUnit : static_cast<int>(fminf(pairs, most)) * (2 * kTreeUnit);
 }
 __device__ __forceinline__ int chunks_of(const Tree & g, int chunk) { return g.nk > chunk ? (g.nk - 1) / chunk + 1 : 1; }
 // First key of chunk i of a segment's: as even as whole units make them, where the first chunk has the tree's too.
@@ -1055,7 +1057,7 @@ int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, 
     a.items = tree_items(nseg, total_q, kv_heads, a.group, a.row_shift);
     a.slot_rows = tree_slot_rows(total_q * a.group, a.row_shift);
     a.slots = tree_slots(kv_heads);
-    a.per_target = 1.0f / static_cast<float>(tree_target(kv_heads) * kTreeUnit);
+    a.per_target = 1.0f / static_cast<float>(tree_target(kv_heads) * 2 * kTreeUnit);
     PXS_CHECK(a.items * kv_heads <= UINT32_MAX / 256 && total_q * heads <= UINT32_MAX / 256, PXS_ERR_ARG,
               "pxs_tree_attention: grid too large");
     char * ws = static_cast<char *>(workspace);
