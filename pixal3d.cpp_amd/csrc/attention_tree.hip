@@ -315,7 +315,7 @@ constexpr int tree_any_pitch(int dp) { return dp + 4; }
 // waves of a workgroup have the same 32 rows and every fourth block of 32 keys each, straight from
 // memory; S^T = K Q^T, so that a lane owns one row and half of its scores, and O^T += V^T P^T.
 // Their results are joined through LDS.  The products bound it where rows are many (32,000 keys for 128 tokens of 16
-// heads of 64 in 44 us, 2.9 TB/s; a block of 32 keys is 1.75 us of a wave's products), the way from the
+// heads of 64 in 42 us, 3.1 TB/s; a block of 32 keys is 1.75 us of a wave's products), the way from the
 // lengths to the first loads, and the joins, where they are few (37 and 100 tokens over 2,370 and 517 keys 26 us).
 // Where the registers hold them, a block's keys and values are loaded while the block before is multiplied;
 // otherwise q is in LDS and keys and values come a piece ahead of the products.

@@ -321,6 +321,16 @@ def _rows_ld(t, what, dev):
     raise PxsError(f"{what} must be rows of contiguous columns on the current device")
 
 
+def _rows_of(t, dtype, shape, what, dev):
+    """_rows_ld of rows of this type and shape (rows, columns)."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == dev:
+        row_stride, column_stride = t.stride()
+        if column_stride == 1 and row_stride >= shape[1]:
+            return row_stride
+        return _rows_ld(t, what, dev)
+    raise PxsError(f"{what} must be {dtype} {list(shape)} on the current device")
+
+
 def _expect(t, dtype, shape, what, dev):
     if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
         raise PxsError(f"{what} must be contiguous {dtype} {list(shape)} on the current device")
@@ -1090,28 +1100,27 @@ class Pxs:
                        scale, cap=0.0, slopes=None, positions=None, out=None, workspace=None):
         """pxs_tree_attention: q [*, heads * head_dim], k, v and the caches [*, kv_heads * head_dim] (rows of
         any stride), cu_q int64 [segments + 1], parents int32 [*], cache_start and cache_len int64 [segments]."""
-        dev = _raw_device()
-        what = "tree_attention"
+        dev, dtype = _raw_device(), q.dtype
         nseg, total_q, cache_rows = cu_q.numel() - 1, q.shape[0], k_cache.shape[0]
-        o = torch.empty((total_q, heads * head_dim), dtype=q.dtype, device=q.device) if out is None else out
-        ld_q, ld_k, ld_v, ld_kc, ld_vc, ld_o = [_rows_ld(t, "tree_attention: q, k, v, caches and out", dev)
-                                                for t in (q, k, v, k_cache, v_cache, o)]
-        wide, narrow, cache = (total_q, heads * head_dim), (total_q, kv_heads * head_dim), (cache_rows, kv_heads * head_dim)
-        if q.shape != wide or o.shape != wide or k.shape != narrow or v.shape != narrow or k_cache.shape != cache or \
-                v_cache.shape != cache or not q.dtype is k.dtype is v.dtype is k_cache.dtype is v_cache.dtype is o.dtype:
-            raise PxsError(f"{what}: q and out must be {list(wide)}, k and v {list(narrow)}, the caches {list(cache)}, of one dtype")
-        _expect(cu_q, torch.int64, (nseg + 1,), what + ": cu_q", dev)
-        _expect(parents, torch.int32, (total_q,), what + ": parents", dev)
-        _expect(cache_start, torch.int64, (nseg,), what + ": cache_start", dev)
-        _expect(cache_len, torch.int64, (nseg,), what + ": cache_len", dev)
+        width, kv_width = heads * head_dim, kv_heads * head_dim
+        o = torch.empty((total_q, width), dtype=dtype, device=q.device) if out is None else out
+        what = "tree_attention: q, k, v, caches and out"
+        wide, narrow, cached = (total_q, width), (total_q, kv_width), (cache_rows, kv_width)
+        ld_q, ld_o = _rows_of(q, dtype, wide, what, dev), _rows_of(o, dtype, wide, what, dev)
+        ld_k, ld_v = _rows_of(k, dtype, narrow, what, dev), _rows_of(v, dtype, narrow, what, dev)
+        ld_kc, ld_vc = _rows_of(k_cache, dtype, cached, what, dev), _rows_of(v_cache, dtype, cached, what, dev)
+        _expect(cu_q, torch.int64, (nseg + 1,), "tree_attention: cu_q", dev)
+        _expect(parents, torch.int32, (total_q,), "tree_attention: parents", dev)
+        _expect(cache_start, torch.int64, (nseg,), "tree_attention: cache_start", dev)
+        _expect(cache_len, torch.int64, (nseg,), "tree_attention: cache_len", dev)
         if slopes is not None:
-            _expect(slopes, torch.float32, (heads,), what + ": slopes", dev)
+            _expect(slopes, torch.float32, (heads,), "tree_attention: slopes", dev)
         if positions is not None:
-            _expect(positions, torch.int32, (total_q,), what + ": positions", dev)
+            _expect(positions, torch.int32, (total_q,), "tree_attention: positions", dev)
         need = self.lib.pxs_tree_attention_workspace_bytes(nseg, total_q, heads, kv_heads, head_dim)
         ws = self._ws(need, q.device) if workspace is None else workspace
-        if ws.numel() * ws.element_size() < need or ws.get_device() != dev:
-            raise PxsError(f"{what}: a workspace of {need} bytes on the current device needed")
+        if ws.nbytes < need or ws.get_device() != dev:
+            raise PxsError(f"tree_attention: a workspace of {need} bytes on the current device needed")
         self._check(self.lib.pxs_tree_attention(
             _dtype_code(q), q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(), ld_v, cu_q.data_ptr(),
             parents.data_ptr(), k_cache.data_ptr(), ld_kc, v_cache.data_ptr(), ld_vc, cache_start.data_ptr(),
