@@ -342,12 +342,14 @@ def _mxfp4_bytes(channels):
     return 16 * blocks, -(-blocks // 16) * 16
 
 
+_DTYPE_CODES = {torch.float32: PXS_F32, torch.bfloat16: PXS_BF16}
+
+
 def _dtype_code(t: torch.Tensor) -> int:
-    if t.dtype == torch.float32:
-        return PXS_F32
-    if t.dtype == torch.bfloat16:
-        return PXS_BF16
-    raise PxsError(f"unsupported dtype {t.dtype}")
+    code = _DTYPE_CODES.get(t.dtype)
+    if code is None:
+        raise PxsError(f"unsupported dtype {t.dtype}")
+    return code
 
 
 class Pxs:
