@@ -672,8 +672,9 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
  * multiple of 8 up to 128 (64 and 128 best), 16-byte-aligned q, k, v and caches,
  * and strides that are multiples of 8 below 2^24 takes the fastest kernels.  The same call
  * gives the same bits; its last bits depend on all its lengths.
- * workspace: pxs_tree_attention_workspace_bytes of the same sizes; calls that
- * may overlap need one each. */
+ * workspace: pxs_tree_attention_workspace_bytes of the same heads and of nseg and
+ * total_q no less than the call's, whatever it holds; calls that may overlap
+ * need one each. */
 size_t pxs_tree_attention_workspace_bytes(int nseg, int64_t total_q, int heads, int kv_heads,
                                           int head_dim);
 int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, int64_t ld_k,
