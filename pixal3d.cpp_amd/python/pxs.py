@@ -342,6 +342,7 @@ def _mxfp4_bytes(channels):
     return 16 * blocks, -(-blocks // 16) * 16
 
 
+_U8 = torch.uint8
 _DTYPE_CODES = {torch.float32: PXS_F32, torch.bfloat16: PXS_BF16}
 
 
@@ -361,10 +362,10 @@ class Pxs:
 
     # -- plumbing ---------------------------------------------------------------
     @staticmethod
-    def stream():
+    def stream(dev=None):
         if _raw_stream is None:
             return torch.cuda.current_stream().cuda_stream
-        return _raw_stream(_raw_device())
+        return _raw_stream(_raw_device() if dev is None else dev)
 
     def _check(self, rc: int, what: str):
         if rc != 0:
@@ -823,10 +824,10 @@ class Pxs:
         code_bytes, scale_bytes = _mxfp4_bytes(channels)
         codes = torch.empty((rows, code_bytes), dtype=torch.uint8, device=x.device) if out is None else out
         scales = torch.empty((rows, scale_bytes), dtype=torch.uint8, device=x.device) if scales is None else scales
-        _expect(codes, torch.uint8, (rows, code_bytes), "quantize_mxfp4: out", dev)
-        _expect(scales, torch.uint8, (rows, scale_bytes), "quantize_mxfp4: scales", dev)
+        _expect(codes, _U8, (rows, code_bytes), "quantize_mxfp4: out", dev)
+        _expect(scales, _U8, (rows, scale_bytes), "quantize_mxfp4: scales", dev)
         self._check(self.lib.pxs_quantize_mxfp4(_dtype_code(x), x.data_ptr(), ld, rows, channels, codes.data_ptr(),
-                                                scales.data_ptr(), self.stream()), "pxs_quantize_mxfp4")
+                                                scales.data_ptr(), self.stream(dev)), "pxs_quantize_mxfp4")
         return codes, scales
 
     def dequantize_mxfp4(self, codes, scales, channels, dtype=torch.float32, out=None):
@@ -849,10 +850,13 @@ class Pxs:
         dev = _raw_device()
         rows, cout = x.shape[0], weight.shape[0]
         code_bytes, scale_bytes = _mxfp4_bytes(cin)
-        _expect(x, torch.uint8, (rows, code_bytes), what, dev)
-        _expect(x_scales, torch.uint8, (rows, scale_bytes), what, dev)
-        _expect(weight, torch.uint8, (cout, code_bytes), what, dev)
-        _expect(w_scales, torch.uint8, (cout, scale_bytes), what, dev)
+        # (one condition: _expect of each takes longer)
+        if not (x.dtype is x_scales.dtype is weight.dtype is w_scales.dtype is _U8 and x.shape == (rows, code_bytes)
+                and x_scales.shape == (rows, scale_bytes) and weight.shape == (cout, code_bytes)
+                and w_scales.shape == (cout, scale_bytes) and x.is_contiguous() and x_scales.is_contiguous()
+                and weight.is_contiguous() and w_scales.is_contiguous()
+                and dev == x.get_device() == x_scales.get_device() == weight.get_device() == w_scales.get_device()):
+            raise PxsError(f"{what} must be contiguous torch.uint8 on the current device, {code_bytes} and {scale_bytes} bytes a row")
         if bias is not None:
             _expect(bias, torch.float32, (cout,), what, dev)
         _expect(out, out.dtype, (rows, cout), what, dev)
@@ -926,7 +930,7 @@ class Pxs:
         y = torch.empty((rows, channels), dtype=out_dtype or x.dtype, device=x.device) if out is None else out
         _expect(y, y.dtype, (rows, channels), "rms_norm: out", dev)
         self._check(self.lib.pxs_rms_norm(_dtype_code(x), x.data_ptr(), ld, res_dtype, _ptr(residual), _ptr(res_out), rows,
-                                          channels, eps, _ptr(gamma), _dtype_code(y), y.data_ptr(), self.stream()),
+                                          channels, eps, _ptr(gamma), _dtype_code(y), y.data_ptr(), self.stream(dev)),
                     "pxs_rms_norm")
         return y
 
@@ -940,7 +944,7 @@ class Pxs:
         _expect(scales, torch.float32, (rows,), "rms_norm_i8: scales", dev)
         self._check(self.lib.pxs_rms_norm_i8(_dtype_code(x), x.data_ptr(), ld, res_dtype, _ptr(residual), _ptr(res_out),
                                              rows, channels, eps, _ptr(gamma), q.data_ptr(), scales.data_ptr(),
-                                             self.stream()),
+                                             self.stream(dev)),
                     "pxs_rms_norm_i8")
         return q, scales
 
@@ -1127,7 +1131,7 @@ class Pxs:
             _dtype_code(q), q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(), ld_v, cu_q.data_ptr(),
             parents.data_ptr(), k_cache.data_ptr(), ld_kc, v_cache.data_ptr(), ld_vc, cache_start.data_ptr(),
             cache_len.data_ptr(), nseg, total_q, cache_rows, heads, kv_heads, head_dim, scale, cap, _ptr(slopes),
-            _ptr(positions), o.data_ptr(), ld_o, ws.data_ptr(), self.stream()), "pxs_tree_attention")
+            _ptr(positions), o.data_ptr(), ld_o, ws.data_ptr(), self.stream(dev)), "pxs_tree_attention")
         return o
 
     def transformer_block(self, cfg: BlockConfig, weights: BlockWeights, coords, batch_size, cu,
