@@ -686,6 +686,15 @@ int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, 
                        const int32_t * positions, void * o, int64_t ld_o, void * workspace,
                        void * stream);
 
+/* On the host: how a tree attention call of these lengths (host int64 [nseg] each) is
+ * cut, where its rows lie in whole 16-byte pieces, for tests and profiles.  plan[0] rows a
+ * tile; plan[1] keys a step; plan[2] cached keys a chunk; plan[3] the most steps that an
+ * item has after those that take a maximum, of items where they are even in number (of the
+ * fastest kernels; 0 for the others), plan[4] where they are odd; plan[5] how chunks are
+ * joined: 0 there is one, 1 a workgroup a row, 2 a group of lanes a row. */
+int pxs_tree_attention_plan(int dtype, const int64_t * q_len, const int64_t * cache_len, int nseg,
+                            int64_t cache_rows, int heads, int kv_heads, int head_dim, int * plan);
+
 /* Per-batch cu_seqlens from the batch column (src/sparse.cpp:731-737):
  * cu (device int64[batch_size + 1]). */
 int pxs_batch_cu_seqlens(const int32_t * coords, int64_t n, int batch_size, int64_t * cu,

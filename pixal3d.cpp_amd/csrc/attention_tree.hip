@@ -74,7 +74,7 @@ __device__ __forceinline__ Tree load_tree(const TreeArgs & a, int s) {
     return {static_cast<int>(q0), static_cast<int>(q1 - q0), static_cast<int>(nk), k0};
 }
 
-__device__ __forceinline__ int row_tiles_of(const TreeArgs & a, const Tree & g) {
+__host__ __device__ __forceinline__ int row_tiles_of(const TreeArgs & a, const Tree & g) {
     return static_cast<int>((static_cast<int64_t>(g.nq) * a.group + (1 << a.row_shift) - 1) >> a.row_shift);
 }
 // Keys of a chunk, from the sum of row tiles times cached keys: `work` of them over the target's items, and
@@ -82,18 +82,28 @@ __device__ __forceinline__ int row_tiles_of(const TreeArgs & a, const Tree & g) 
 // one: eight caches of 0 to 40,001 keys 126 us, 92 so), or one unit where that is enough (12 tokens over 1,501
 // keys 13.7 us, with two 14.3; one over 300 12.0 and 13.1).
 // (Rounded sums of it: they are the same in every wave, and off by so little that the target, at most 512, holds.)
-__device__ __forceinline__ int chunk_of(const TreeArgs & a, float work) {
+__host__ __device__ __forceinline__ int chunk_of(const TreeArgs & a, float work) {
     const float pairs = floorf(work * a.per_target) + 1.0f, most = static_cast<float>(a.cache_rows / (2 * kTreeUnit) + 1);
     return work * a.per_target <= 0.5f ? kTreeUnit : static_cast<int>(fminf(pairs, most)) * (2 * kTreeUnit);
 }
-__device__ __forceinline__ int chunks_of(const Tree & g, int chunk) { return g.nk > chunk ? (g.nk - 1) / chunk + 1 : 1; }
+__host__ __device__ __forceinline__ int chunks_of(const Tree & g, int chunk) { return g.nk > chunk ? (g.nk - 1) / chunk + 1 : 1; }
 // First key of chunk i of a segment's: as even as whole units make them, where the first chunk has the tree's too.
-__device__ __forceinline__ int chunk_start(const Tree & g, int i, int chunks) {
+__host__ __device__ __forceinline__ int chunk_start(const Tree & g, int i, int chunks) {
     if (i == 0) return 0;
     const int cached = static_cast<int>((static_cast<int64_t>(g.nk) + kTreeUnit - 1) / kTreeUnit);
     const int tree = min((g.nq - 1) / kTreeUnit + 1, cached / chunks);  // (no chunk but the first is left without keys)
     const int units = cached + tree, each = units / chunks, more = units - each * chunks;  // (the first `more` have one more)
     return static_cast<int>(min(static_cast<int64_t>(i * each + min(i, more) - tree) * kTreeUnit, static_cast<int64_t>(g.nk)));
+}
+
+// The fast kernel's steps for an item, a tile of `keys` keys each: the tree's tiles (with the first chunk), all of
+// them, and those that take a maximum: the tree's, the cache's last where it ends inside, and one whole tile.
+struct TreeSteps {
+    int tree, all, exact;
+};
+__host__ __device__ __forceinline__ TreeSteps tree_steps(int nq, int chunk, int key0, int key1, int keys) {
+    const int tree = chunk == 0 ? (nq + keys - 1) / keys : 0, all = tree + (key1 + keys - 1) / keys - key0 / keys;
+    return {tree, all, std::min(all, tree + (key1 % keys != 0 ? 1 : 0) + 1)};
 }
 
 // An item: a row tile and the chunk's keys.
@@ -612,11 +622,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
     Item w;
     w.kv = static_cast<int>(blockIdx.x % a.kv_heads);
     if (!locate_item(a, static_cast<int>(blockIdx.x / a.kv_heads), lane, w)) return;
-    const int tree_tiles = w.chunk == 0 ? (w.g.nq + F::kKeys - 1) / F::kKeys : 0;
-    const int cache0 = w.key0 / F::kKeys, cache1 = (w.key1 + F::kKeys - 1) / F::kKeys;
+    const TreeSteps steps = tree_steps(w.g.nq, w.chunk, w.key0, w.key1, F::kKeys);
+    const int tree_tiles = steps.tree, cache1 = (w.key1 + F::kKeys - 1) / F::kKeys;
     // Steps 0 .. n - 1: the tree's tiles from the last, then the cache's from the last.
-    const int n = __builtin_amdgcn_readfirstlane(tree_tiles + cache1 - cache0);
-    const int exact = __builtin_amdgcn_readfirstlane(min(n, tree_tiles + (w.key1 % F::kKeys != 0 ? 1 : 0) + 1));
+    const int n = __builtin_amdgcn_readfirstlane(steps.all);
+    const int exact = __builtin_amdgcn_readfirstlane(steps.exact);
     const int wave_row0 = w.row0 + wave * 32;
     const bool wave_live = wave_row0 < w.rows;
 
@@ -917,6 +927,7 @@ constexpr int kWaveSegments = 64;
 // chunks 110 us with the attention, a workgroup a row 125; 4,096 of 8 68 and 71; 192 of 12 17.7 and 15.0; 1,024 of
 // 64 55 and 49.
 constexpr int64_t kJoinRows = 4096;
+bool joins_rows_each(int64_t total_q, int heads) { return total_q * heads >= kJoinRows; }
 // Workgroups that chunks past the first add at most: one round of the kernels' two a CU (eight trees of 64 over
 // 8,192 keys 112 us, with 384 119, with 768 133, with 1,024 126; eight trees over caches of 0 to 40,001 keys 93, 97,
 // 106 and 100; 64 of 8 over 4,096 198, 198, 220 and 221; in fp32 eight of 16 over 4,000 51, 57, 63 and 58).
@@ -934,6 +945,11 @@ int64_t tree_slots(int kv_heads) { return 2 * tree_target(kv_heads); }
 size_t tree_table_bytes(int nseg) { return round256((2 * static_cast<size_t>(nseg) + 2) * sizeof(int64_t)); }
 int tree_slot_rows(int64_t rows, int row_shift) { return static_cast<int>(std::min<int64_t>(rows, int64_t(1) << row_shift)); }
 size_t tree_part_rows(int kv_heads, int slot_rows) { return static_cast<size_t>(tree_slots(kv_heads)) * kv_heads * slot_rows; }
+
+void set_tree_cuts(TreeArgs & a, bool fast) {
+    a.row_shift = fast ? 7 : 5;
+    a.per_target = 1.0f / static_cast<float>(tree_target(a.kv_heads) * 2 * kTreeUnit);
+}
 
 template <typename T, int DP, int FORM>
 int launch_tree_any(const TreeArgs & a, hipStream_t s) {
@@ -985,7 +1001,7 @@ int run_tree(const TreeArgs & a, bool fast, hipStream_t s) {
     else if (a.vec && (a.d == 64 || a.d == 128 || a.d == 256)) rc = launch_tree_any<T, kWholeRows>(a, s);
     else rc = a.vec ? launch_tree_any<T, kPieceRows>(a, s) : launch_tree_any<T, kAnyRows>(a, s);
     if (rc || a.cache_rows <= kTreeUnit) return rc;  // (no chunk is shorter than a unit)
-    if (a.total_q * a.heads >= kJoinRows)
+    if (joins_rows_each(a.total_q, a.heads))
         hipLaunchKernelGGL((tree_join_kernel<T, true>), dim3(static_cast<unsigned>(a.total_q * ((a.heads + 7) / 8))), dim3(256), 0, s, a);
     else
         hipLaunchKernelGGL((tree_join_kernel<T, false>), dim3(static_cast<unsigned>(a.total_q * a.heads)), dim3(256), 0, s, a);
@@ -1008,6 +1024,47 @@ size_t pxs_tree_attention_workspace_bytes(int nseg, int64_t total_q, int heads, 
     const int64_t group = (heads - 1) / kv_heads + 1;
     const size_t rows = tree_part_rows(kv_heads, tree_slot_rows(std::min<int64_t>(total_q, 128) * group, 7));  // (fp32's are fewer)
     return tree_table_bytes(nseg) + round256(rows * sizeof(float2)) + round256(rows * head_dim * sizeof(float));
+}
+
+int pxs_tree_attention_plan(int dtype, const int64_t * q_len, const int64_t * cache_len, int nseg, int64_t cache_rows,
+                            int heads, int kv_heads, int head_dim, int * plan) {
+    PXS_CHECK(dtype == PXS_F32 || dtype == PXS_BF16, PXS_ERR_ARG, "pxs_tree_attention_plan: bad dtype");
+    PXS_CHECK(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads <= 65535 && head_dim > 0 && head_dim <= kTreeMaxDim,
+              PXS_ERR_ARG, "pxs_tree_attention_plan: bad heads");
+    PXS_CHECK(nseg > 0 && q_len && cache_len && plan, PXS_ERR_ARG, "pxs_tree_attention_plan: null pointer");
+    PXS_CHECK(cache_rows >= 0 && cache_rows <= kTreeMaxRows, PXS_ERR_ARG, "pxs_tree_attention_plan: bad cache");
+    TreeArgs a{};
+    a.cache_rows = cache_rows; a.kv_heads = kv_heads; a.group = heads / kv_heads;
+    const bool fast = dtype == PXS_BF16 && head_dim <= 128 && head_dim % 8 == 0;
+    set_tree_cuts(a, fast);
+    const int keys = !fast || head_dim > 64 ? 32 : 64;
+    double work = 0.0;
+    int64_t total_q = 0;
+    for (int s = 0; s < nseg; ++s) {
+        PXS_CHECK(q_len[s] >= 0 && q_len[s] <= kTreeMaxRows / a.group - total_q && cache_len[s] >= 0 && cache_len[s] <= cache_rows,
+                  PXS_ERR_ARG, "pxs_tree_attention_plan: bad length");
+        total_q += q_len[s];
+        work += static_cast<double>(row_tiles_of(a, {0, static_cast<int>(q_len[s]), 0, 0})) * static_cast<double>(cache_len[s]);
+    }
+    const int chunk = chunk_of(a, static_cast<float>(work));
+    int most[2] = {0, 0}, joined = 0;  // (of an even and of an odd number)
+    for (int s = 0; s < nseg; ++s) {
+        const Tree g{0, static_cast<int>(q_len[s]), static_cast<int>(cache_len[s]), 0};
+        const int chunks = chunks_of(g, chunk);
+        for (int i = 0; g.nq > 0 && i < chunks; ++i) {
+            const TreeSteps t = tree_steps(g.nq, i, chunk_start(g, i, chunks), chunk_start(g, i + 1, chunks), keys);
+            int & of = most[(t.all - t.exact) % 2];
+            if (fast) of = std::max(of, t.all - t.exact);
+        }
+        if (g.nq > 0 && chunks > 1) joined = joins_rows_each(total_q, heads) ? 2 : 1;
+    }
+    plan[0] = 1 << a.row_shift;
+    plan[1] = keys;
+    plan[2] = chunk;
+    plan[3] = most[0];
+    plan[4] = most[1];
+    plan[5] = joined;
+    return PXS_OK;
 }
 
 int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, int64_t ld_k, const void * v, int64_t ld_v,
@@ -1053,11 +1110,10 @@ int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, 
     const bool fast = dtype == PXS_BF16 && head_dim <= 128 && a.vec && ld_k < (1 << 24) && ld_v < (1 << 24) &&
                       (cache_rows == 0 || (ld_k_cache < (1 << 24) && ld_v_cache < (1 << 24))) &&
                       reinterpret_cast<uintptr_t>(o) % 8 == 0 && ld_o % 4 == 0;
-    a.row_shift = fast ? 7 : 5;
+    set_tree_cuts(a, fast);
     a.items = tree_items(nseg, total_q, kv_heads, a.group, a.row_shift);
     a.slot_rows = tree_slot_rows(total_q * a.group, a.row_shift);
     a.slots = tree_slots(kv_heads);
-    a.per_target = 1.0f / static_cast<float>(tree_target(kv_heads) * 2 * kTreeUnit);
     PXS_CHECK(a.items * kv_heads <= UINT32_MAX / 256 && total_q * heads <= UINT32_MAX / 256, PXS_ERR_ARG,
               "pxs_tree_attention: grid too large");
     char * ws = static_cast<char *>(workspace);

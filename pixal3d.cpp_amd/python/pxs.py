@@ -72,6 +72,8 @@ _SIGS = {
     "pxs_tree_attention_workspace_bytes": (C.c_size_t, [_i32, _i64, _i32, _i32, _i32]),
     "pxs_tree_attention": (_i32, [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp,
                                   _i32, _i64, _i64, _i32, _i32, _i32, _f, _f, _vp, _vp, _vp, _i64, _vp, _vp]),
+    "pxs_tree_attention_plan": (_i32, [_i32, C.POINTER(C.c_int64), C.POINTER(C.c_int64), _i32, _i64, _i32, _i32, _i32,
+                                       C.POINTER(C.c_int)]),
     "pxs_rope_frequencies": (_i32, [_i32] + [C.c_double] * 5 + [C.POINTER(C.c_double)]),
     "pxs_rope_positions": (_i32, [_i32, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _f, _vp, _i64, _vp]),
     "pxs_attention_scores_workspace_bytes": (C.c_size_t, [_i32, _i64, _i64, _i32, _i32, _i32]),
