@@ -449,7 +449,8 @@ int pxs_dequantize_mxfp4(const uint8_t * codes, const uint8_t * scales, int64_t 
 
 /* y = act(x W^T + bias) in y_dtype, of the values that x's and weight's codes
  * ([rows, cin], [cout, cin]) stand for: products exact, sums in fp32.  cin is
- * at most 2^24, cout 2^30.  bias may be NULL; act is PXS_ACT_*.  The sums' order,
+ * at most 2^24, cout 2^30, and rows * cout, each rounded up to a multiple of 256,
+ * less than 2^39.  bias may be NULL; act is PXS_ACT_*.  The sums' order,
  * and so their last bits, depends on the call's sizes. */
 int pxs_linear_mxfp4(const uint8_t * x, const uint8_t * x_scales, int64_t rows, int cin,
                      const uint8_t * weight, const uint8_t * w_scales, const float * bias, int cout,

@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <iterator>
+#include <limits>
 #include <type_traits>
 
 namespace pxs {
@@ -728,8 +729,10 @@ __global__ void __launch_bounds__(NW * KG * 64) linear_mxfp4_kernel(MxArgs a) {
 
 bool aligned_to(const void * p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-int check_mx_grid(int64_t blocks, int threads) {
-    PXS_CHECK(blocks <= UINT32_MAX / threads, PXS_ERR_ARG, "4-bit linear grid too large");
+// A launch counts its threads in 32 bits.
+bool mx_grid_fits(int64_t workgroups, int threads) { return workgroups <= UINT32_MAX / threads; }
+int check_mx_grid(int64_t workgroups, int threads) {
+    PXS_CHECK(mx_grid_fits(workgroups, threads), PXS_ERR_ARG, "4-bit linear grid too large");
     return PXS_OK;
 }
 
@@ -738,7 +741,7 @@ int launch_mx_few(const MxArgs & a, hipStream_t s) {
     const int64_t rows = (a.m + 16 * RB - 1) / (16 * RB);
     PXS_CHECK(rows <= 65535, PXS_ERR_ARG, "4-bit linear grid too large");
     const dim3 grid(grid_for(a.n, 16), static_cast<unsigned>(rows));
-    if (int rc = check_mx_grid(grid.x, kFewWaves * 64)) return rc;
+    if (int rc = check_mx_grid(grid.x * rows, kFewWaves * 64)) return rc;
     hipLaunchKernelGGL((linear_mxfp4_few_kernel<T, RB, EPI>), grid, dim3(kFewWaves * 64), 0, s, a);
     return check_launch("4-bit linear of few rows");
 }
@@ -769,23 +772,25 @@ int launch_mx_tiles(const MxArgs & a, hipStream_t s) {
 //   64 x 64, 4 waves, two:                               150 x 4096 -> 4096 10.8 against 15.6
 //   32 x 64, four groups of two waves over K, one:       87 x 8192 -> 1024 11.4 against 14.2
 struct MxShape {
-    int bm, bn, stages;
+    int bm, bn, stages, threads;
     double alone0, alone1, each0, each1;
 };
 constexpr MxShape kMxShapes[] = {
-    {256, 256, 2, 11.4, 10.3, 8.5, 16.5}, {128, 128, 2, 6.1, 4.9, 3.3, 4.5}, {128, 128, 3, 6.5, 4.2, 4.3, 5.2},
-    {64, 64, 4, 6.0, 2.2, 1.9, 2.0},      {32, 64, 2, 6.1, 1.5, 3.0, 1.9},
+    {256, 256, 2, 512, 11.4, 10.3, 8.5, 16.5}, {128, 128, 2, 512, 6.1, 4.9, 3.3, 4.5}, {128, 128, 3, 512, 6.5, 4.2, 4.3, 5.2},
+    {64, 64, 4, 256, 6.0, 2.2, 1.9, 2.0},      {32, 64, 2, 512, 6.1, 1.5, 3.0, 1.9},
 };
 
+// Of the shapes whose grid can be launched, the one of the least time (the largest, if there is none: refused).
 int mx_shape(int64_t m, int n, int blocks, double & least) {
     int best = 0;
+    least = std::numeric_limits<double>::infinity();
     for (int i = 0; i < static_cast<int>(std::size(kMxShapes)); ++i) {
         const MxShape & c = kMxShapes[i];
         const double deep = blocks / 64.0, alone = c.alone0 + c.alone1 * deep, each = c.each0 + c.each1 * deep;
         const int64_t tiles = ((m + c.bm - 1) / c.bm) * ((n + c.bn - 1) / c.bn);
         const double time = tiles <= 256 ? alone + std::max(0.0, each - alone) * (tiles / 256.0)
                                          : std::max(alone, ((tiles + 255) / 256) * each);
-        if (i == 0 || time < least) {
+        if (time < least && mx_grid_fits(tiles, c.threads)) {
             least = time;
             best = i;
         }
@@ -806,7 +811,7 @@ struct MxPlan {
     int bm, bn, stages;
 };
 MxPlan mx_plan(int64_t m, int n, int blocks) {
-    double tiles = 0.0;
+    double tiles;
     const MxShape & c = kMxShapes[mx_shape(m, n, blocks, tiles)];
     if (m <= kMxFewRows) {
         const int64_t columns = (n + 15) / 16, row_blocks = (m + 15) / 16;
@@ -814,7 +819,7 @@ MxPlan mx_plan(int64_t m, int n, int blocks) {
         const int64_t workgroups = columns * ((row_blocks + rb - 1) / rb);
         const int64_t rows = 16 + std::min<int64_t>(16 * rb, m);  // of codes that one loads, its channels' and its rows'
         const double few = 4.3 + 0.042 * static_cast<double>((workgroups + 255) / 256 * rows) * blocks / 64.0;
-        if (few < tiles) return {16 * rb, 16, 0};
+        if (few < tiles && mx_grid_fits(workgroups, kFewWaves * 64)) return {16 * rb, 16, 0};
     }
     return {c.bm, c.bn, c.stages};
 }
