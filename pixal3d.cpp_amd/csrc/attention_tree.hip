@@ -235,9 +235,17 @@ __device__ __forceinline__ void load_dims4(const T * row, int c, int d, bool vec
     for (int i = 0; i < 4; ++i) out[i] = c + i < d ? load_f32(row + c + i) : 0.0f;
 }
 
+// Outputs are sums of weights up to 1 times values until the last division, and a mean of values below the largest
+// number may be a sum above it.  So sums past kTreeOutLimit (512 chunks' of those below it are joined inside fp32)
+// are taken again with weights that are lower by this power of two: all keys' together are then at most 1/2.
+constexpr float kTreeOutLimit = 0x1p117f;
+__device__ __forceinline__ float tree_lift(const Tree & g) {
+    return static_cast<float>(33 - __clz(static_cast<int>(static_cast<uint32_t>(g.nk) + static_cast<uint32_t>(g.nq))));
+}
+
 // A row of an item again, a key after the other, tokens that it does not see left out altogether: for
-// trees where a token's value is infinite or NaN, which times a weight of zero is NaN.  One wave;
-// lane l holds dims l, l + 64, ...  Broken data alone comes here.
+// trees where a token's value is infinite or NaN, which times a weight of zero is NaN, and for sums past
+// kTreeOutLimit.  One wave; lane l holds dims l, l + 64, ...  Broken or enormous data alone comes here.
 template <typename T, int NC>
 __device__ __forceinline__ void tree_row_alone(const TreeArgs & a, const Item & w, int row, int lane, int64_t slot) {
     const int i = row / a.group;
@@ -251,6 +259,7 @@ __device__ __forceinline__ void tree_row_alone(const TreeArgs & a, const Item & 
         qv[c] = lane + 64 * c < a.d ? load_f32(q + lane + 64 * c) : 0.0f;
         acc[c] = 0.0f;
     }
+    const float lift = tree_lift(w.g);
     float m = -INFINITY, l = 0.0f;
     auto step = [&](const T * k, const T * v, int at) {
         float dot = 0.0f;
@@ -260,7 +269,7 @@ __device__ __forceinline__ void tree_row_alone(const TreeArgs & a, const Item & 
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) dot += __shfl_xor(dot, off, 64);
         const float z = tree_score(a, dot, slope, static_cast<float>(pos - at));
-        const float up = fmaxf(m, z);
+        const float up = fmaxf(m, z + lift);
         const float base = up == -INFINITY ? 0.0f : up;
         const float p = exp2f(z - base), keep = exp2f(m - base);
         l = l * keep + p;
@@ -501,23 +510,21 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
         if (kAhead && b + 4 < all) load_v(block(b + 4), 0, vv[0]);
     }
     const int64_t slot0 = item_rows(a, w);
-    if (__syncthreads_or(odd)) {
-        for (int i = wave; i < 32; i += 4)
-            if (w.row0 + i < w.rows) tree_row_alone<T, (DP + 63) / 64>(a, w, w.row0 + i, lane, slot0 + i);
-        return;
-    }
+    if (!kAhead) __syncthreads();  // (q's place is the outputs')
     float2 * ml = reinterpret_cast<float2 *>(tree_smem + 4 * 32 * P);
-    if (h == 0) ml[wave * 32 + r] = make_float2(m, l);
+    int again = lane;
+    asm volatile("" : "+v"(again));  // (h and r taken anew: kept over the loop they cost more registers than there are)
+    const int to_h = again >> 5, to_r = again & 31;
+    if (to_h == 0) ml[wave * 32 + to_r] = make_float2(m, l);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4 *>(tree_smem + (wave * 32 + r) * P + dt * 32 + 8 * g + 4 * h) =
+            *reinterpret_cast<float4 *>(tree_smem + (wave * 32 + to_r) * P + dt * 32 + 8 * g + 4 * to_h) =
                 make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
     __syncthreads();
     const int jr = tid >> 3;  // 8 threads a row
-    if (w.row0 + jr >= w.rows) return;
-    float base = -INFINITY, total = 0.0f, f[4];
+    float base = -INFINITY, total = 0.0f, f[4], x[DP / 8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) base = fmaxf(base, ml[i * 32 + jr].x);
     const float ref = base == -INFINITY ? 0.0f : base;
@@ -526,16 +533,30 @@ __global__ void __launch_bounds__(256) tree_attn_any_kernel(TreeArgs a) {
         f[i] = exp2f(ml[i * 32 + jr].x - ref);
         total += ml[i * 32 + jr].y * f[i];
     }
+    bool past = false;
+#pragma unroll
+    for (int u = 0; u < DP / 8; ++u) {
+        x[u] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[u] += tree_smem[(i * 32 + jr) * P + u * 8 + (tid & 7)] * f[i];
+        past |= !(fabsf(x[u]) < kTreeOutLimit);  // (a row of no query repeats the last, dims past d its last one's)
+    }
+    if (__builtin_expect(__syncthreads_or(odd || (past && is_finite_bits(total))), 0)) {
+        for (int i = wave; i < 32; i += 4)
+            if (w.row0 + i < w.rows) tree_row_alone<T, (DP + 63) / 64>(a, w, w.row0 + i, lane, slot0 + i);
+        return;
+    }
+    if (w.row0 + jr >= w.rows) return;
     const int to = (w.row0 + jr) / a.group, to_head = w.kv * a.group + (w.row0 + jr) % a.group;
     T * o = static_cast<T *>(a.o) + (w.g.q0 + to) * a.ldo + static_cast<int64_t>(to_head) * a.d;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     if (w.chunks > 1 && (tid & 7) == 0) a.part_ml[slot0 + jr] = make_float2(base, total);
-    for (int c = tid & 7; c < a.d; c += 8) {
-        float x = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x += tree_smem[(i * 32 + jr) * P + c] * f[i];
-        if (w.chunks > 1) a.part[(slot0 + jr) * a.d + c] = x;
-        else store_f32(o + c, x * inv);
+    for (int u = 0; u < DP / 8; ++u) {
+        const int c = u * 8 + (tid & 7);
+        if (c >= a.d) continue;
+        if (w.chunks > 1) a.part[(slot0 + jr) * a.d + c] = x[u];
+        else store_f32(o + c, x[u] * inv);
     }
 }
 
@@ -580,7 +601,7 @@ __device__ __forceinline__ TreeSources<DH> tree_sources(const TreeArgs & a, cons
 template <int DH, int MODE>
 __device__ __forceinline__ void tree_exact(const TreeArgs & a, const Item & w, const TreeRow<DH, MODE> & o, bool tree, int first,
                                            uint64_t bits, int h, typename Fast<DH>::Scores & s, typename Fast<DH>::Weights & p,
-                                           typename Fast<DH>::Out & oacc, RowState & st) {
+                                           typename Fast<DH>::Out & oacc, RowState & st, float lift) {
     const uint32_t lo = static_cast<uint32_t>(bits) >> (4 * h), hi = static_cast<uint32_t>(bits >> 32) >> (4 * h);
     auto seen = [&](int kt, int e) __attribute__((always_inline)) {  // (key_of is a constant)
         return ((kt == 0 ? lo : hi) >> (key_of(0, e)) & 1u) != 0;
@@ -594,11 +615,11 @@ __device__ __forceinline__ void tree_exact(const TreeArgs & a, const Item & w, c
             for (int e = 0; e < 16; ++e)
                 at[kt][e] = static_cast<float>(o.pos - a.positions[w.g.q0 + min(first + key_of(kt, e) + 4 * h, w.g.nq - 1)]);
         tile_exact_of<DH, MODE>(o.rs, a.cap_log2, s, p, oacc, st,
-                                [&](int kt, int e) __attribute__((always_inline)) { return at[kt][e]; }, seen);
+                                [&](int kt, int e) __attribute__((always_inline)) { return at[kt][e]; }, seen, lift);
     } else {
         tile_exact_of<DH, MODE>(o.rs, a.cap_log2, s, p, oacc, st,
                                 [&](int kt, int e) __attribute__((always_inline)) { return behind - static_cast<float>(key_of(kt, e)); },
-                                seen);
+                                seen, lift);
     }
 }
 
@@ -607,7 +628,7 @@ __device__ __forceinline__ void tree_exact(const TreeArgs & a, const Item & w, c
 // (maximum, weights, product), and one whole tile after them, so that every row has a base that one of its own
 // scores set.  From there on a step issues the products that do not depend on its weights, O += V P of the tile before
 // and S of the next, and takes its weights while they run, without a maximum: a row's are redone with one
-// where their sum passes 2^40, and an item whose outputs pass 2^118 is walked again with exact steps alone.
+// where their sum passes 2^40, and an item whose outputs pass kTreeOutLimit is walked again with exact steps alone.
 // Waves past the segment's rows only help to load: with one row or 32 the cache's bytes bound it (eight caches of
 // 32,768 keys, one token each, 5.2 TB/s; two waves a workgroup with a ring of their own were 2 to 9% slower from
 // one row to 64), with 256 a segment the products and the weights' exponentials (620 TFLOP/s, 515 with a cap).
@@ -667,7 +688,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
     typename F::Weights p;
     int i = 0;
     TreeWalk walk{o.qi, tree_tiles * F::kKeys};
-    auto exact_step = [&]() __attribute__((always_inline)) {
+    auto exact_step = [&](float lift) __attribute__((always_inline)) {
         const bool tree = i < tree_tiles;
         const int first = (tree ? tree_tiles - 1 - i : cache_tile(i)) * F::kKeys;
         const uint64_t bits = tree ? tree_bits<F::kKeys>(a, w.g, walk, first, lane) : first_bits(w.key1 - first);
@@ -676,11 +697,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
         if (tree) odd |= tile_odd<DH>(v_of(i), tid, 256);
         if (wave_live) {
             tile_qk<DH>(k_of(i), o.qf, s_a, h, r);
-            tree_exact<DH, MODE>(a, w, o, tree, first, bits, h, s_a, p, oacc, st);
+            tree_exact<DH, MODE>(a, w, o, tree, first, bits, h, s_a, p, oacc, st, lift);
             tile_pv<DH>(v_of(i), p, oacc, lane);
         }
     };
-    for (; i < exact; ++i) exact_step();
+    for (; i < exact; ++i) exact_step(-0.0f);
     i = __builtin_amdgcn_readfirstlane(i);
     if (!wave_live) {
         for (; i < n; ++i) {
@@ -736,14 +757,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
             weights(i, s_b);
             tile_pv<DH>(v_of(i), p, oacc, lane);
         }
-        // (A sum of magnitudes: infinities and NaN stay in it.)
-        float size[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int dt = 0; dt < F::NDT; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) size[e & 3] += fabsf(oacc[dt][e]);
-        past = o.live && !((size[0] + size[1]) + (size[2] + size[3]) < kOutLimit) && is_finite_bits(st.sum);
     }
+    // (A sum of magnitudes: infinities and NaN stay in it.)
+    float size[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int dt = 0; dt < F::NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) size[e & 3] += fabsf(oacc[dt][e]);
+    past = o.live && !((size[0] + size[1]) + (size[2] + size[3]) < kTreeOutLimit) && is_finite_bits(st.sum);
     const int64_t part = item_rows(a, w) + wave * 32;
     if (__builtin_expect(__syncthreads_or(odd || past), 0)) {
         if (__syncthreads_or(odd)) {
@@ -757,7 +778,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) t
         for (int dt = 0; dt < F::NDT; ++dt) oacc[dt] = f32x16{};
         st = {-INFINITY, 0.0f};
         walk = {o.qi, tree_tiles * F::kKeys};
-        for (i = 0; i < n; ++i) exact_step();
+        const float lift = tree_lift(w.g);
+        for (i = 0; i < n; ++i) exact_step(lift);
     }
     const float sum = lane_pair_sum(st.sum);
     if (!o.live) return;

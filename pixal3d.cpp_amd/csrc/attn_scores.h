@@ -207,11 +207,12 @@ __device__ __forceinline__ float tile_max(const RowScore & rs, float cap_log2, c
 }
 
 // The exact step of a tile: hidden keys get weight 0, the base rises to the maximum and the output
-// with it.  away(kt, e) and seen(kt, e) of the lane's keys.
+// with it.  away(kt, e) and seen(kt, e) of the lane's keys.  lift: how far above the maximum the base is kept, so
+// that weights are at most 2^-lift (-0, which adds nothing to any number).
 template <int DH, int MODE, typename Away, typename Seen>
 __device__ __forceinline__ void tile_exact_of(const RowScore & rs, float cap_log2, typename Fast<DH>::Scores & s,
                                               typename Fast<DH>::Weights & p, typename Fast<DH>::Out & oacc,
-                                              RowState & st, Away away, Seen seen) {
+                                              RowState & st, Away away, Seen seen, float lift = -0.0f) {
     using F = Fast<DH>;
     const float add = near_cap(MODE) ? cap_log2 : 0.0f;
     float top = -INFINITY;
@@ -223,7 +224,7 @@ __device__ __forceinline__ void tile_exact_of(const RowScore & rs, float cap_log
             s[kt][e] = seen(kt, e) ? z : -INFINITY;
             top = fmaxf(top, s[kt][e]);
         }
-    const float up = fmaxf(st.base, lane_pair_max(top));
+    const float up = fmaxf(st.base, lane_pair_max(top) + lift);
     const float base = up == -INFINITY ? 0.0f : up;  // nothing seen yet: every weight is 0
     const float keep = __builtin_amdgcn_exp2f(st.base - base);
     const bf16x2 ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
