@@ -667,8 +667,8 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
  * The cache is read only: rows of k and v that are accepted are appended by the
  * caller, and o overlaps no input.  total_q is at least cu_q[nseg]; rows of q
  * and o behind the last segment are neither read nor written.  cache_rows is the cache's size in rows; total_q *
- * heads / kv_heads and cache_rows are at most 2^31 - 1024.  Bounds past the rows
- * are cut to them.  The lengths are read on the device alone: a captured call
+ * heads / kv_heads and cache_rows are at most 2^31 - 1024, nseg * kv_heads and total_q *
+ * heads / 8 (eighths rounded up) 2^23.  Bounds past the rows are cut to them.  The lengths are read on the device alone: a captured call
  * follows cache_start and cache_len as they change.  bf16 with head_dim a
  * multiple of 8 up to 128 (64 and 128 best), 16-byte-aligned q, k, v and caches,
  * and strides that are multiples of 8 below 2^24 takes the fastest kernels.  The same call

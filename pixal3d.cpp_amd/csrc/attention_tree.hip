@@ -950,6 +950,11 @@ constexpr int kWaveSegments = 64;
 // 64 55 and 49.
 constexpr int64_t kJoinRows = 4096;
 bool joins_rows_each(int64_t total_q, int heads) { return total_q * heads >= kJoinRows; }
+// Workgroups of the join; none where no chunk is shorter than the cache.
+int64_t join_groups(const TreeArgs & a) {
+    if (a.cache_rows <= kTreeUnit) return 0;
+    return a.total_q * (joins_rows_each(a.total_q, a.heads) ? (a.heads + 7) / 8 : a.heads);
+}
 // Workgroups that chunks past the first add at most: one round of the kernels' two a CU (eight trees of 64 over
 // 8,192 keys 112 us, with 384 119, with 768 133, with 1,024 126; eight trees over caches of 0 to 40,001 keys 93, 97,
 // 106 and 100; 64 of 8 over 4,096 198, 198, 220 and 221; in fp32 eight of 16 over 4,000 51, 57, 63 and 58).
@@ -1022,11 +1027,10 @@ int run_tree(const TreeArgs & a, bool fast, hipStream_t s) {
     else if (fast) rc = a.d < 64 ? launch_tree_fast<64, false>(a, s) : launch_tree_fast<128, false>(a, s);
     else if (a.vec && (a.d == 64 || a.d == 128 || a.d == 256)) rc = launch_tree_any<T, kWholeRows>(a, s);
     else rc = a.vec ? launch_tree_any<T, kPieceRows>(a, s) : launch_tree_any<T, kAnyRows>(a, s);
-    if (rc || a.cache_rows <= kTreeUnit) return rc;  // (no chunk is shorter than a unit)
-    if (joins_rows_each(a.total_q, a.heads))
-        hipLaunchKernelGGL((tree_join_kernel<T, true>), dim3(static_cast<unsigned>(a.total_q * ((a.heads + 7) / 8))), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL((tree_join_kernel<T, false>), dim3(static_cast<unsigned>(a.total_q * a.heads)), dim3(256), 0, s, a);
+    const dim3 groups(static_cast<unsigned>(join_groups(a)));
+    if (rc || groups.x == 0) return rc;
+    if (joins_rows_each(a.total_q, a.heads)) hipLaunchKernelGGL((tree_join_kernel<T, true>), groups, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((tree_join_kernel<T, false>), groups, dim3(256), 0, s, a);
     return check_launch("tree attention join");
 }
 
@@ -1136,7 +1140,7 @@ int pxs_tree_attention(int dtype, const void * q, int64_t ld_q, const void * k, 
     a.items = tree_items(nseg, total_q, kv_heads, a.group, a.row_shift);
     a.slot_rows = tree_slot_rows(total_q * a.group, a.row_shift);
     a.slots = tree_slots(kv_heads);
-    PXS_CHECK(a.items * kv_heads <= UINT32_MAX / 256 && total_q * heads <= UINT32_MAX / 256, PXS_ERR_ARG,
+    PXS_CHECK(a.items * kv_heads <= UINT32_MAX / 256 && join_groups(a) <= UINT32_MAX / 256, PXS_ERR_ARG,
               "pxs_tree_attention: grid too large");
     char * ws = static_cast<char *>(workspace);
     if (nseg > kWaveSegments) {
