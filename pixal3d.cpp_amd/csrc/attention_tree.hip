@@ -132,12 +132,14 @@ template <typename V> __device__ __forceinline__ V tree_sums(V v) {
 }
 
 // Of up to 64 segments, one a lane: its bounds, its items and those up to it, the same of
-// items with partial results, and the chunk.
+// items with partial results, and the chunk.  The attention's kernels and the joins' each make it and need the
+// same: a product and an addition of the sum are two roundings, and no compiler's choice of one fused.
 struct Plan {
     Tree g;
     int items, end, slots, slots_end, chunk;
 };
 __device__ __forceinline__ Plan segment_plan(const TreeArgs & a, int lane) {
+#pragma clang fp contract(off)
     Plan p{};
     if (lane < a.nseg) p.g = load_tree(a, lane);
     const int tiles = row_tiles_of(a, p.g);
