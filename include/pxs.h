@@ -394,7 +394,8 @@ int pxs_quantize_rows_i8(int dtype, const void * x, int64_t ld_x, int64_t rows, 
 
 /* y = act((x W^T) * x_scales[row] * w_scales[channel] + bias) in y_dtype, x
  * [rows, cin] and weight [cout, cin] 8-bit integers, summed exactly in 32 bits
- * (cin is at most 131071, cout 2^30).  bias may be NULL; act is PXS_ACT_*.  A cin that is
+ * (cin is at most 131071, cout 2^29, and rows * cout, each rounded up to a
+ * multiple of 128, less than 2^37).  bias may be NULL; act is PXS_ACT_*.  A cin that is
  * a multiple of 16, with 16-byte-aligned x and weight, takes the fastest
  * kernels. */
 int pxs_linear_i8(const int8_t * x, const float * x_scales, int64_t rows, int cin,

@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <iterator>
+#include <limits>
 #include <type_traits>
 
 namespace pxs {
@@ -671,8 +672,10 @@ __global__ void __launch_bounds__(NW * KG * 64) linear_i8_kernel(I8Args a) {
 
 bool aligned_to(const void * p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-int check_i8_grid(int64_t blocks, int threads) {
-    PXS_CHECK(blocks <= UINT32_MAX / threads, PXS_ERR_ARG, "8-bit linear grid too large");
+// A launch counts its threads in 32 bits.
+bool i8_grid_fits(int64_t workgroups, int threads) { return workgroups <= UINT32_MAX / threads; }
+int check_i8_grid(int64_t workgroups, int threads) {
+    PXS_CHECK(i8_grid_fits(workgroups, threads), PXS_ERR_ARG, "8-bit linear grid too large");
     return PXS_OK;
 }
 
@@ -725,24 +728,25 @@ int launch_i8_few(const I8Args & a, hipStream_t s) {
 //   64 x 64, 4 waves, two:                               150 x 4096 -> 4096 15.1 against 17.0
 //   32 x 64, four groups of two waves over K, one:       300 x 4096 -> 1024 8.4 against 14.8
 struct I8Shape {
-    int bm, bn, stages;
+    int bm, bn, stages, threads;
     double alone0, alone1, each0, each1;
 };
 constexpr I8Shape kI8Shapes[] = {
-    {256, 256, 2, 7.3, 8.9, 10.8, 13.4}, {192, 128, 2, 4.9, 4.8, 4.2, 5.9}, {128, 128, 2, 3.9, 4.0, 2.7, 4.4},
-    {128, 64, 3, 3.6, 3.3, 2.0, 2.8},    {64, 64, 4, 3.1, 2.9, 1.4, 2.0},   {32, 64, 3, 3.7, 1.1, 2.7, 1.2},
+    {256, 256, 2, 1024, 7.3, 8.9, 10.8, 13.4}, {192, 128, 2, 512, 4.9, 4.8, 4.2, 5.9}, {128, 128, 2, 512, 3.9, 4.0, 2.7, 4.4},
+    {128, 64, 3, 512, 3.6, 3.3, 2.0, 2.8},     {64, 64, 4, 256, 3.1, 2.9, 1.4, 2.0},   {32, 64, 3, 512, 3.7, 1.1, 2.7, 1.2},
 };
 
+// Of the shapes whose grid can be launched, the one of the least time (the largest, if there is none: refused).
 int i8_shape(int64_t m, int n, int k) {
     int best = 0;
-    double least = 0.0;
+    double least = std::numeric_limits<double>::infinity();
     for (int i = 0; i < static_cast<int>(std::size(kI8Shapes)); ++i) {
         const I8Shape & c = kI8Shapes[i];
         const double deep = k / 1024.0, alone = c.alone0 + c.alone1 * deep, each = c.each0 + c.each1 * deep;
         const int64_t tiles = ((m + c.bm - 1) / c.bm) * ((n + c.bn - 1) / c.bn);
         const double time = tiles <= 256 ? alone + std::max(0.0, each - alone) * (tiles / 256.0)
                                          : std::max(alone, ((tiles + 255) / 256) * each);
-        if (i == 0 || time < least) {
+        if (time < least && i8_grid_fits(tiles, c.threads)) {
             least = time;
             best = i;
         }
@@ -765,10 +769,9 @@ struct I8Plan {
 // pieces: cin and the operands' addresses are multiples of 16.
 I8Plan i8_plan(int64_t m, int n, int k, bool pieces) {
     if (m <= kI8FewRows) {
-        const int64_t blocks = (n + 15) / 16 * ((m + 15) / 16);
-        if (blocks <= 256 || m <= 16) return {16, 16, 0};
-        if (blocks <= 512 || m <= 32) return {32, 16, 0};
-        return {64, 16, 0};
+        const int64_t columns = (static_cast<int64_t>(n) + 15) / 16, row_blocks = (m + 15) / 16, blocks = columns * row_blocks;
+        const int rb = blocks <= 256 || m <= 16 ? 1 : blocks <= 512 || m <= 32 ? 2 : 4;
+        if (i8_grid_fits(columns * ((row_blocks + rb - 1) / rb), kFewWaves * 64)) return {16 * rb, 16, 0};
     }
     auto tiles = [&](int bm, int bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
     if (!pieces) {
@@ -777,7 +780,8 @@ I8Plan i8_plan(int64_t m, int n, int k, bool pieces) {
         // and 130 to 4090 deep, the pick is the faster form or within 5%; where 128 rows take three rounds
         // or more it is up to 20% slower (42,000 x 1370 -> 1021 122 us, 108 with 192 rows).
         auto rounds = [&](int bm) { return (tiles(bm, 128) + 255) / 256; };
-        return {21.7 * rounds(192) < 12.6 * rounds(128) ? 192 : 128, 128, 1};
+        const bool tall = 21.7 * rounds(192) < 12.6 * rounds(128) || !i8_grid_fits(tiles(128, 128), 512);
+        return {tall ? 192 : 128, 128, 1};
     }
     const I8Shape & c = kI8Shapes[i8_shape(m, n, k)];
     // Three stages where a CU has one tile at most, so that no second tile's stages need fit, and K is
