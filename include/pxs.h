@@ -626,6 +626,8 @@ int pxs_varlen_attention_noalloc(int dtype, const void * q, int64_t ld_q, const 
  *     prefix[s] (device int64 [nseg], may be NULL), which all queries of the
  *     segment see.  What hidden keys and values hold does not matter, NaN
  *     included.  A query that sees no key gets zeros.
+ *   Values: weighted sums are held in fp32 until they are divided by the weights'
+ *     sum, so a value times the keys that a query sees must stay below 2^127.
  * Row strides ld_* are in elements.  total_q = cu_q[nseg] and total_k =
  * cu_k[nseg], total_k and total_q * heads / kv_heads at most 2^31 - 1024; rows
  * of q and o behind the last segment are neither read nor written.  bf16 with head_dim a
@@ -660,7 +662,8 @@ int pxs_varlen_attention_scores(int dtype, const void * q, int64_t ld_q, const v
  *     earlier token of the segment counts as -1.  A token sees the cached keys,
  *     the tokens above it and itself; what the others hold does not matter, NaN
  *     included.
- *   Heads, head sizes, scale and cap: as pxs_varlen_attention_scores.
+ *   Heads, head sizes, scale and cap: as pxs_varlen_attention_scores.  Values may have any
+ *     size, whatever the number of keys.
  *   slopes (device fp32 [heads], may be NULL) lowers a score by slopes[head] *
  *     |distance of the positions|: a cached key's is its place in the sequence, a
  *     token's positions[row] (device int32 [total_q], 0 or more, needed with

@@ -495,9 +495,9 @@ __device__ __forceinline__ void mx_tile_out(const MxArgs & a, const f32x16 (&acc
 // stages) at a time, ahead of the codes of the first of the four.
 // A 32 x 32 x 64 product takes the cycles of an 8-bit one of half its depth: bytes, stages and LDS
 // traffic are those of the 8-bit kernel and the rate is twice its.  Bound by no single unit: at 8,192 x 8192
-// -> 4096 (148 us, 3,720 TFLOP/s, 3.4 times the 16-bit library product's rate) the matrix cores are busy 46%
-// of the cycles, the return path of the DMA 53% and LDS about as much, in step with one another.  (64 x 64 a
-// wave and 16 waves 162 us, 128 x 128 and four waves 184.)
+// -> 4096 (144 us, 3,830 TFLOP/s, 3.6 times the 16-bit library product's rate) the matrix cores are busy 48%
+// of the cycles, the return path of the DMA 56% and LDS 56% (17 of them bank conflicts), in step with one
+// another.  (Beside 148 us on another card, 64 x 64 a wave and 16 waves 162, 128 x 128 and four waves 184.)
 //
 // KG groups of NW waves share a tile and take every KG-th stage each, in stages of their own (KG 4:
 // a group's stages are one of each four, and each loads its own scales); the groups' sums are added
@@ -765,12 +765,14 @@ int launch_mx_tiles(const MxArgs & a, hipStream_t s) {
 
 // Tile shapes, their time alone on a CU and their share of a full CU's time, in us for
 // 1024 bytes of codes a row more and without any: fitted to each shape's times at 64 sizes (66 to 42,017
-// rows, 256 to 8192 deep), where the shape picked takes 0.9% more than the best on average:
-//   256 x 256, 8 waves of 128 x 64, one workgroup a CU:  8,192 x 8192 -> 4096 148 us (3,720 TFLOP/s), next best 172
-//   128 x 128, 8 waves, two stages and two workgroups:   1,370 x 1024 -> 4096 11.6 against 15.4
-//   the same, three stages and one workgroup:            2,000 x 4096 -> 2048 18.0 against 19.6
-//   64 x 64, 4 waves, two:                               150 x 4096 -> 4096 10.8 against 15.6
-//   32 x 64, four groups of two waves over K, one:       87 x 8192 -> 1024 11.4 against 14.2
+// rows, 256 to 8192 deep), where the shape picked takes 0.6% more than the best on average, 17% at most (2,873 x
+// 256 -> 1024):
+//   256 x 256, 8 waves of 128 x 64, one workgroup a CU:  8,192 x 8192 -> 4096 144 us (3,830 TFLOP/s), next best 192
+//   128 x 128, 8 waves, two stages and two workgroups:   1,370 x 1024 -> 4096 11.6 against 14.6
+//   the same, three stages and one workgroup:            2,000 x 4096 -> 2048 17.9 against 19.5
+//   64 x 64, 4 waves, two:                               150 x 4096 -> 4096 10.6 against 15.5
+//   32 x 64, four groups of two waves over K, one:       87 x 8192 -> 1024 11.3 against 14.2
+// (bf16 outputs; another output's bytes, or a residual's, change no choice.)
 struct MxShape {
     int bm, bn, stages, threads;
     double alone0, alone1, each0, each1;

@@ -54,9 +54,10 @@ __device__ __forceinline__ void norm_store(const NormArgs & a, int64_t at, float
     else static_cast<float *>(a.y)[at] = v;
 }
 
-// Workgroups launched at most: each then takes several rows, with the gains loaded once (42,017 x 1024
-// bf16 on an fp32 residual, 8-bit rows: 91 us with 4,096, 94 with 2,048, 90 with one for every four rows; 4,739 x
-// 1370 in bf16 15.1, 14.2 and 16.5; 8,192 x 4096 48.8, 52.6 and 50.7).
+// Workgroups launched at most: each then takes several rows, with the gains loaded once.  Of three rules the one
+// that is nowhere more than 2.5% behind the best: 42,017 x 1024 bf16 on an fp32 residual into 8-bit rows 90 us with
+// 4,096, 94 with 2,048, 89 with one for every four rows; 8,192 x 4096 of the same 49.9, 48.7 and 49.0; 4,739 x 1370
+// in bf16 throughout 14.5, 14.3 and 15.8.
 constexpr int64_t kNormGrid = 4096;
 
 // A workgroup a row, a value at a time, the row read again for its output: rows of more than 16,384 channels.
@@ -148,7 +149,7 @@ constexpr int norm_threads(int wpr) { return wpr > 4 ? wpr * 64 : 256; }
 // WPR waves share a row of up to WPR * 64 * 8 * NV channels, which they hold in registers between
 // the sums and the rounding: every value is read and written once.  Rows start at any element.  The
 // gains are loaded once for all the rows that a wave takes.  Bound by HBM: 42,017 x 1024, bf16 on an fp32
-// residual, 90 us, 5.2 TB/s (the kernel above, a value at a time, 183); one row of 1024 3.5 us, its launch, loads and
+// residual, 90 us, 5.2 TB/s (the kernel above, a value at a time, 175); one row of 1024 3.4 us, its launch, loads and
 // two reductions.
 template <typename XT, typename RT, bool Q, int WPR, int NV>
 __global__ void __launch_bounds__(norm_threads(WPR)) rms_norm_rows_kernel(NormArgs a) {
@@ -252,10 +253,11 @@ __global__ void __launch_bounds__(norm_threads(WPR)) rms_norm_rows_kernel(NormAr
     }
 }
 
-// Waves a row: as few as hold it in 16 values a lane or less, one up to 1024 channels (42,017 x 512 48 us, with four
-// 65; 1 x 1024 4.7 and 7.4), four to 2048 (4,739 x 1370 17.2, with one 21.7), eight to 8192 (10,000 x 4096 86, with
-// four 88, with sixteen 127; 15,000 x 2600 88, 94 and 182; 5,000 x 8192 89, 91 and 88), sixteen to 16,384
-// (2,500 x 16,384 102, a value at a time 197).
+// Waves a row: as few as hold it in 16 values a lane or less, one up to 1024 channels (42,017 x 512 47 us, with four
+// 61; at 1024 channels they meet: 42,017 rows 90 and 88 to 92, 2,000 7.1 and 7.1, one 3.4 and 3.3), four to 2048
+// (4,739 x 1370 14.5, with one 16.1), eight to 8192 (10,000 x 4096 84, with four 87, with sixteen 123; 15,000 x 2600 85, 92
+// and 179; 5,000 x 8192 88, 90 and 89), sixteen to 16,384 (2,500 x 16,384 101, a value at a time 197).
+// (4,739 x 1370 in bf16 throughout, the others bf16 on an fp32 residual into 8-bit rows.)
 template <typename XT, typename RT, bool Q>
 int launch_norm(const NormArgs & a, hipStream_t s) {
     const int64_t one = (a.rows + 3) / 4;
